@@ -2,7 +2,8 @@
 
 ``ElasticBuffer``, ``EPHandle``, ``EventHandle`` and ``EventOverlap`` keep the reference's names and
 signatures (deep_ep/__init__.py:11-16).  The V1 ``Buffer`` and ``Config`` classes are outside this
-build.  ``install_as_deep_ep()`` registers this package under the name ``deep_ep`` for callers that
+build.  ``Router`` chooses the experts that ``ElasticBuffer`` dispatches to, with the balance loss and both gradients; ``w4`` holds
+the products of few tokens with 4-bit weights; the reference has neither.  ``install_as_deep_ep()`` registers this package under the name ``deep_ep`` for callers that
 import the reference's module path.
 """
 
@@ -18,10 +19,14 @@ _LAZY = {
     "EPHandle": ("deepep_amd.elastic", "EPHandle"),
     "EventHandle": ("deepep_amd.event", "EventHandle"),
     "EventOverlap": ("deepep_amd.event", "EventOverlap"),
+    "Router": ("deepep_amd.router", "Router"),
+    "BalanceLoss": ("deepep_amd.router", "BalanceLoss"),
 }
 
 
 def __getattr__(name):
+    if name == "w4":
+        return importlib.import_module("deepep_amd.w4")
     target = _LAZY.get(name)
     if target is None:
         raise AttributeError(name)

@@ -542,3 +542,195 @@ def megamoe_forward(ws, x_codes, x_scales, topk_idx, topk_weights, w1, s1, w2, s
         )
     _lib.check(status, "megamoe_forward")
     return y, expert_token_nums
+
+
+# ---------------------------------------------------------------------------------------------
+# Router, balance loss and 4-bit products
+# ---------------------------------------------------------------------------------------------
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DPEP_TYPE_*
+SCORES = ("softmax", "sigmoid")  # DPEP_SCORE_*
+
+
+class RouterSpec(ctypes.Structure):
+    """``dpep_router`` of include/deepep_amd.h."""
+
+    _fields_ = [("num_experts", ctypes.c_int32), ("num_topk", ctypes.c_int32), ("num_groups", ctypes.c_int32),
+                ("num_topk_groups", ctypes.c_int32), ("score", ctypes.c_int32), ("normalize", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("logits_type", ctypes.c_int32), ("index_bytes", ctypes.c_int32)]
+
+
+class _RouterGradients(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("logits", "topk_idx", "topk_weights", "grad_weights", "sequence_offsets", "counts",
+                                                     "tokens", "grad_losses", "grad_logits")] + [("num_sequences", ctypes.c_int32)]
+
+
+class _W4(ctypes.Structure):
+    _fields_ = [("packed", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
+                ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("group", ctypes.c_int32)]
+
+
+def _require_logits(spec: RouterSpec, logits):
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _TYPES:
+        raise ValueError("logits must be an FP32, BF16 or FP16 tensor")
+    _require("logits", logits, logits.dtype)
+    if logits.ndim != 2 or logits.shape[1] != spec.num_experts:
+        raise ValueError(f"logits must be [T, {spec.num_experts}] (got {tuple(logits.shape)})")
+    spec.logits_type = _TYPES[logits.dtype]
+    return logits.shape[0], logits.device
+
+
+def _require_routes(spec: RouterSpec, topk_idx, tokens, device):
+    if not isinstance(topk_idx, torch.Tensor) or topk_idx.dtype not in (torch.int64, torch.int32):
+        raise ValueError("topk_idx must be an int64 or int32 tensor")
+    _require("topk_idx", topk_idx, topk_idx.dtype, (tokens, spec.num_topk), device)
+    spec.index_bytes = topk_idx.element_size()
+
+
+def _require_sequences(sequence_offsets, device):
+    if sequence_offsets is None:
+        return 1
+    _require("sequence_offsets", sequence_offsets, torch.int32, device=device)
+    if sequence_offsets.ndim != 1 or sequence_offsets.shape[0] < 2:
+        raise ValueError("sequence_offsets must be [B + 1] with B >= 1")
+    return sequence_offsets.shape[0] - 1
+
+
+def route(spec: RouterSpec, logits, bias=None, token_mask=None, index_dtype=torch.int64):
+    """``(topk_idx [T,K], topk_weights FP32 [T,K])`` of logits [T,E]; ``bias`` FP32 [E], ``token_mask`` bool [T] (False: padding)."""
+    tokens, dev = _require_logits(spec, logits)
+    if index_dtype not in (torch.int64, torch.int32):
+        raise ValueError("index_dtype must be torch.int64 or torch.int32")
+    if bias is not None:
+        _require("bias", bias, torch.float32, (spec.num_experts,), dev)
+    if token_mask is not None:
+        _require("token_mask", token_mask, torch.bool, (tokens,), dev)
+    spec.index_bytes = 8 if index_dtype == torch.int64 else 4
+    topk_idx = torch.empty((tokens, spec.num_topk), dtype=index_dtype, device=dev)
+    topk_weights = torch.empty((tokens, spec.num_topk), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        status = _lib.load().dpep_route(ctypes.byref(spec), _ptr(logits), _ptr(bias), _ptr(token_mask), tokens, _ptr(topk_idx),
+                                        _ptr(topk_weights), _stream(dev))
+    _lib.check(status, "route")
+    return topk_idx, topk_weights
+
+
+def balance_loss(spec: RouterSpec, logits, topk_idx, sequence_offsets=None):
+    """``(losses FP32 [B], counts int32 [B,E], tokens int32 [B])`` of the sequences that ``sequence_offsets`` int32 [B+1] cuts the
+    batch into (None: one)."""
+    tokens, dev = _require_logits(spec, logits)
+    _require_routes(spec, topk_idx, tokens, dev)
+    sequences = _require_sequences(sequence_offsets, dev)
+    lib = _lib.load()
+    losses = torch.empty((sequences,), dtype=torch.float32, device=dev)
+    counts = torch.empty((sequences, spec.num_experts), dtype=torch.int32, device=dev)
+    members = torch.empty((sequences,), dtype=torch.int32, device=dev)
+    scratch = torch.empty((lib.dpep_balance_scratch_bytes(spec.num_experts, tokens, sequences),), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        status = lib.dpep_balance_loss(ctypes.byref(spec), _ptr(logits), _ptr(topk_idx), tokens, _ptr(sequence_offsets), sequences,
+                                       _ptr(losses), _ptr(counts), _ptr(members), _ptr(scratch), _stream(dev))
+    _lib.check(status, "balance_loss")
+    return losses, counts, members
+
+
+def router_backward(spec: RouterSpec, logits, topk_idx, topk_weights=None, grad_weights=None, sequence_offsets=None, counts=None,
+                    tokens=None, grad_losses=None):
+    """Gradient of ``logits`` in their type, from ``grad_weights`` FP32 [T,K], from ``grad_losses`` FP32 [B] with what
+    ``balance_loss`` was given and returned, or from both."""
+    num_tokens, dev = _require_logits(spec, logits)
+    _require_routes(spec, topk_idx, num_tokens, dev)
+    if grad_weights is None and grad_losses is None:
+        raise ValueError("router_backward needs grad_weights, grad_losses or both")
+    sequences = 1
+    if grad_weights is not None:
+        _require("grad_weights", grad_weights, torch.float32, (num_tokens, spec.num_topk), dev)
+        if spec.normalize:
+            _require("topk_weights", topk_weights, torch.float32, (num_tokens, spec.num_topk), dev)
+    if grad_losses is not None:
+        sequences = _require_sequences(sequence_offsets, dev)
+        _require("grad_losses", grad_losses, torch.float32, (sequences,), dev)
+        _require("counts", counts, torch.int32, (sequences, spec.num_experts), dev)
+        _require("tokens", tokens, torch.int32, (sequences,), dev)
+    grad_logits = torch.empty_like(logits)
+    address = [None if t is None else t.data_ptr() for t in (logits, topk_idx, topk_weights, grad_weights, sequence_offsets, counts, tokens,
+                                                             grad_losses, grad_logits)]
+    call = _RouterGradients(*address, sequences)
+    with _on_device(dev):
+        status = _lib.load().dpep_router_backward(ctypes.byref(spec), ctypes.byref(call), num_tokens, _stream(dev))
+    _lib.check(status, "router_backward")
+    return grad_logits
+
+
+def _w4(name, packed, scales, zeros, dtype, device, ndim):
+    """The C struct of a matrix ([N,K/2]) or of experts' matrices ([L,N,K/2])."""
+    _require(f"{name} packed", packed, torch.uint8, device=device)
+    if packed.ndim != ndim or packed.shape[-1] == 0 or packed.shape[-2] == 0:
+        raise ValueError(f"{name} packed must be [{'L, ' if ndim == 3 else ''}N, K/2]")
+    _require(f"{name} scales", scales, dtype, device=device)
+    k, groups = 2 * packed.shape[-1], scales.shape[-1] if scales.ndim == ndim else 0
+    if scales.ndim != ndim or scales.shape[:-1] != packed.shape[:-1] or groups == 0 or k % groups:
+        raise ValueError(f"{name} scales must be {tuple(packed.shape[:-1])} + (K / group,) (got {tuple(scales.shape)})")
+    if zeros is not None:
+        _require(f"{name} zeros", zeros, torch.uint8, tuple(scales.shape), device)
+    return _W4(packed.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), packed.shape[-2], k, k // groups)
+
+
+def _aligned(x):
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def w4_matvec(x, packed, scales, zeros=None, out=None):
+    """x [M,K] (BF16 or FP16) times a matrix of 4-bit values: packed uint8 [N,K/2], scales [N,K/group] in x's type, zeros uint8
+    [N,K/group] (None: 8).  Returns [M,N] in x's type."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("x must be a BF16 or FP16 tensor")
+    _require("x", x, x.dtype)
+    dev = x.device
+    weights = _w4("w4_matvec", packed, scales, zeros, x.dtype, dev, 2)
+    if x.ndim != 2 or x.shape[1] != weights.k:
+        raise ValueError(f"x must be [M, {weights.k}] (got {tuple(x.shape)})")
+    rows = x.shape[0]
+    if out is None:
+        out = torch.empty((rows, weights.n), dtype=x.dtype, device=dev)
+    else:
+        _require("out", out, x.dtype, (rows, weights.n), dev)
+    x = _aligned(x)
+    with _on_device(dev):
+        status = _lib.load().dpep_w4_matvec(ctypes.byref(weights), _TYPES[x.dtype], _ptr(x), rows, _ptr(out), _stream(dev))
+    _lib.check(status, "w4_matvec")
+    return out
+
+
+def w4_experts(x, topk_idx, topk_weights, gate_up, down, expert_begin: int = 0, out=None):
+    """The expert layer of a few tokens over 4-bit weights: gate_up = (packed [L,2I,H/2], scales, zeros), down = (packed [L,H,I/2],
+    scales, zeros).  Returns [T,H] in x's type; slots whose expert is not local do not count."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("x must be a BF16 or FP16 tensor")
+    _require("x", x, x.dtype)
+    dev = x.device
+    first = _w4("gate_up", *gate_up, x.dtype, dev, 3)
+    second = _w4("down", *down, x.dtype, dev, 3)
+    local = gate_up[0].shape[0]
+    if down[0].shape[0] != local or first.n != 2 * second.k or first.k != second.n:
+        raise ValueError("gate_up [L, 2I, H/2] and down [L, H, I/2] do not belong together")
+    if x.ndim != 2 or x.shape[1] != first.k:
+        raise ValueError(f"x must be [T, {first.k}] (got {tuple(x.shape)})")
+    tokens = x.shape[0]
+    if not isinstance(topk_idx, torch.Tensor) or topk_idx.dtype not in (torch.int64, torch.int32):
+        raise ValueError("topk_idx must be an int64 or int32 tensor")
+    _require("topk_idx", topk_idx, topk_idx.dtype, device=dev)
+    if topk_idx.ndim != 2 or topk_idx.shape[0] != tokens or topk_idx.shape[1] == 0:
+        raise ValueError("topk_idx must be [T, K]")
+    topk = topk_idx.shape[1]
+    _require("topk_weights", topk_weights, torch.float32, (tokens, topk), dev)
+    if out is None:
+        out = torch.empty((tokens, first.k), dtype=x.dtype, device=dev)
+    else:
+        _require("out", out, x.dtype, (tokens, first.k), dev)
+    lib = _lib.load()
+    x = _aligned(x)
+    scratch = torch.empty((lib.dpep_w4_experts_scratch_bytes(tokens, topk, first.k, second.k),), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        status = lib.dpep_w4_experts(ctypes.byref(first), ctypes.byref(second), _TYPES[x.dtype], _ptr(x), _ptr(topk_idx), topk_idx.element_size(),
+                                     _ptr(topk_weights), tokens, topk, int(expert_begin), local, _ptr(out), _ptr(scratch), _stream(dev))
+    _lib.check(status, "w4_experts")
+    return out

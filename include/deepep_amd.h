@@ -355,6 +355,82 @@ typedef struct dpep_megamoe_call {
 } dpep_megamoe_call;
 int dpep_megamoe_run(void* ws, const dpep_megamoe_call* call, void* stream);
 
+/* ---- Operators around dispatch and combine: router, balance loss, 4-bit products.  The reference takes routes and experts as given, so
+ * these have no counterpart there. ---- */
+#define DPEP_TYPE_F32 0
+#define DPEP_TYPE_BF16 1
+#define DPEP_TYPE_F16 2
+#define DPEP_SCORE_SOFTMAX 0
+#define DPEP_SCORE_SIGMOID 1
+
+/* A layer's router.  Scores: softmax over the row, or each logit's sigmoid.  Experts are chosen by key: the logit (softmax), or the
+ * sigmoid plus the expert's bias, rounded to fp32; an expert whose logit is -inf is never chosen, a NaN ranks with +inf.  With
+ * num_groups > 1 the num_experts / num_groups experts of a group stand together: the num_topk_groups groups of the largest key
+ * (softmax), or of the largest sum of two keys (sigmoid), stay in the choice.  Ties go to the lowest index.
+ *   num_experts  1..1024;  num_topk  1..DPEP_MAX_TOPK, at most the experts of num_topk_groups groups
+ *   normalize    != 0: the chosen experts' scores are divided by their sum (sigmoid: plus 1e-20)
+ *   scale        factor of the weights, finite and not 0
+ *   logits_type  DPEP_TYPE_*;  index_bytes  of an expert id: 8, or 4 */
+typedef struct dpep_router {
+    int32_t num_experts, num_topk, num_groups, num_topk_groups;
+    int32_t score, normalize;
+    float scale;
+    int32_t logits_type, index_bytes;
+} dpep_router;
+/* Expert ids and weights of every token, best first; -1 and 0 where fewer than num_topk experts are left.
+ *   logits [T,E];  bias optional fp32 [E] (sigmoid only);  token_mask optional bytes [T], 0: padding, which gets no route
+ *   topk_idx int64 or int32 [T,K];  topk_weights fp32 [T,K] */
+int dpep_route(const dpep_router* r, const void* logits, const float* bias, const uint8_t* token_mask, int num_tokens, void* topk_idx,
+               float* topk_weights, void* stream);
+
+/* Balance loss of every sequence, and its counts.  A token without a route (ids outside 0..E-1) is padding.  In a sequence of N other
+ * tokens with R routes, c_e of them to expert e: loss = sum_e (E c_e / R) (sum_t p_te / N), p a token's softmax, or its sigmoids over
+ * (their sum + 1e-20); 0 for a sequence without tokens.  Sums are taken in an order that depends on the sizes alone.
+ *   sequence_offsets  int32 [B+1] ascending from 0 to T, or NULL: one sequence
+ *   losses fp32 [B];  counts int32 [B,E];  tokens int32 [B] (N);  scratch  dpep_balance_scratch_bytes, 4-byte aligned */
+size_t dpep_balance_scratch_bytes(int num_experts, int num_tokens, int num_sequences);
+int dpep_balance_loss(const dpep_router* r, const void* logits, const void* topk_idx, int num_tokens, const int32_t* sequence_offsets, int num_sequences,
+                      float* losses, int32_t* counts, int32_t* tokens, void* scratch, void* stream);
+
+/* Gradient of the logits, in their type, from the gradient of the route weights (grad_weights, as dpep_combine's return channel gives
+ * it; entries without a route are not read into it), of the balance losses (grad_losses, with what dpep_balance_loss was given and
+ * returned), or of both.  The choice itself and the counts have no gradient.  Ids of a token are taken for distinct.
+ *   topk_weights  dpep_route's, needed where they are normalised */
+typedef struct dpep_router_gradients {
+    const void* logits;
+    const void* topk_idx;
+    const float* topk_weights;
+    const float* grad_weights;
+    const int32_t* sequence_offsets;
+    const int32_t* counts;
+    const int32_t* tokens;
+    const float* grad_losses;
+    void* grad_logits;
+    int32_t num_sequences;
+} dpep_router_gradients;
+int dpep_router_backward(const dpep_router* r, const dpep_router_gradients* g, int num_tokens, void* stream);
+
+/* Matrices [L,N,K] in 4 bits: value (q - zero) * scale, q two to a byte along K (low nibble: even k), one scale and zero point for each
+ * `group` values of a row.
+ *   packed [L,N,K/2], 16-byte aligned;  scales [L,N,K/group] in the type of the rows multiplied;  zeros bytes [L,N,K/group] (0..15), or
+ *   NULL: 8;  group 32, 64 or a multiple of 128, a divisor of K */
+typedef struct dpep_w4 {
+    const uint8_t* packed;
+    const void* scales;
+    const uint8_t* zeros;
+    int32_t n, k, group;
+} dpep_w4;
+/* y[m] = W x[m]: x, y of `type` (BF16 or FP16), x [M,K] 16-byte aligned, y [M,N], sums in fp32, rounded once. */
+int dpep_w4_matvec(const dpep_w4* w, int type, const void* x, int num_rows, void* y, void* stream);
+/* An expert layer for few tokens (T*K <= 2048 routes): y[t] = sum over the slots s of topk_weights[t,s] * W2[e] (silu(g) * u) with
+ * (g, u) = W1[e] x[t], e = topk_idx[t,s] - expert_begin; slots whose expert is not one of the num_local do not count, a token without
+ * a slot that does gets zeros.  The rows between the products keep 16 bits of mantissa.
+ *   gate_up [L,2I,H]: gate rows, then up rows;  down [L,H,I];  x [T,H] 16-byte aligned;  topk_idx [T,K] of index_bytes 8 or 4;  y [T,H]
+ *   scratch  dpep_w4_experts_scratch_bytes, 16-byte aligned */
+size_t dpep_w4_experts_scratch_bytes(int num_tokens, int num_topk, int hidden, int intermediate);
+int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const void* x, const void* topk_idx, int index_bytes, const float* topk_weights,
+                    int num_tokens, int num_topk, int expert_begin, int num_local, void* y, void* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,91 @@
+"""What the router and the 4-bit products refuse before anything is launched; runs without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from deepep_amd import Router, _lib, ops, w4
+
+
+@pytest.mark.parametrize("arguments", [
+    dict(num_experts=0, num_topk=1), dict(num_experts=1025, num_topk=1), dict(num_experts=8, num_topk=9), dict(num_experts=64, num_topk=33),
+    dict(num_experts=8, num_topk=0), dict(num_experts=8, num_topk=2, num_groups=3), dict(num_experts=8, num_topk=2, num_groups=4, num_topk_groups=5),
+    dict(num_experts=8, num_topk=5, num_groups=4, num_topk_groups=2), dict(num_experts=8, num_topk=2, score="relu"),
+    dict(num_experts=8, num_topk=2, scale=0.0), dict(num_experts=8, num_topk=2, scale=float("nan")), dict(num_experts=8, num_topk=2, scale=float("inf")),
+    dict(num_experts=8, num_topk=2, index_dtype=torch.int16), dict(num_experts=8.0, num_topk=2), dict(num_experts=True, num_topk=1),
+])
+def test_router_arguments(arguments):
+    with pytest.raises(ValueError):
+        Router(**arguments)
+
+
+def test_c_abi_refuses_before_it_launches():
+    lib = _lib.load()
+    spec = ops.RouterSpec(16, 4, 1, 1, 0, 1, 1.0, 0, 8)
+
+    def message():
+        return lib.dpep_last_error().decode()
+
+    assert lib.dpep_route(None, None, None, None, 1, None, None, None) == -1 and "NULL" in message()
+    assert lib.dpep_route(ctypes.byref(spec), None, None, None, 1, None, None, None) == -1 and "NULL" in message()
+    assert lib.dpep_route(ctypes.byref(spec), None, None, None, -1, None, None, None) == -1 and "num_tokens" in message()
+    assert lib.dpep_route(ctypes.byref(spec), None, None, None, 0, None, None, None) == 0
+    assert lib.dpep_route(ctypes.byref(spec), None, ctypes.c_void_p(64), None, 0, None, None, None) == -1 and "bias" in message()
+    for field, value, word in (("num_experts", 2000, "num_experts"), ("num_topk", 17, "num_topk"), ("num_groups", 3, "num_groups"), ("num_topk_groups", 2, "num_topk_groups"),
+                               ("score", 2, "score"), ("logits_type", 3, "logits_type"), ("index_bytes", 2, "index_bytes"), ("scale", 0.0, "scale")):
+        wrong = ops.RouterSpec(16, 4, 1, 1, 0, 1, 1.0, 0, 8)
+        setattr(wrong, field, value)
+        assert lib.dpep_route(ctypes.byref(wrong), None, None, None, 0, None, None, None) == -1 and word in message(), field
+    assert lib.dpep_balance_loss(ctypes.byref(spec), None, None, 0, None, 2, None, None, None, None, None) == -1 and "num_sequences" in message()
+    assert lib.dpep_balance_scratch_bytes(0, 4, 1) == 0 and lib.dpep_balance_scratch_bytes(16, 4, 0) == 0 and lib.dpep_balance_scratch_bytes(16, 0, 1) > 0
+    assert lib.dpep_router_backward(ctypes.byref(spec), None, 0, None) == -1 and "NULL" in message()
+    assert lib.dpep_router_backward(ctypes.byref(spec), ctypes.byref(ops._RouterGradients()), 0, None) == -1 and "neither" in message()
+
+
+def test_w4_refuses_before_it_launches():
+    lib = _lib.load()
+
+    def message():
+        return lib.dpep_last_error().decode()
+
+    def matrix(n=64, k=128, group=32, packed=256, scales=256):
+        return ctypes.byref(ops._W4(packed, scales, None, n, k, group))
+
+    assert lib.dpep_w4_matvec(None, 1, None, 1, None, None) == -1 and "NULL" in message()
+    assert lib.dpep_w4_matvec(matrix(), 0, None, 1, None, None) == -1 and "type" in message()
+    assert lib.dpep_w4_matvec(matrix(group=48), 1, None, 1, None, None) == -1 and "group" in message()
+    assert lib.dpep_w4_matvec(matrix(group=192, k=384), 1, None, 1, None, None) == -1 and "group" in message()
+    assert lib.dpep_w4_matvec(matrix(k=96, group=64), 1, None, 1, None, None) == -1 and "group" in message()
+    assert lib.dpep_w4_matvec(matrix(packed=264), 1, None, 1, None, None) == -1 and "aligned" in message()
+    assert lib.dpep_w4_matvec(matrix(), 1, None, -1, None, None) == -1 and "num_rows" in message()
+    assert lib.dpep_w4_matvec(matrix(), 1, None, 0, None, None) == 0
+    assert lib.dpep_w4_matvec(matrix(), 1, None, 1, None, None) == -1 and "NULL" in message()
+
+    def experts(gate_up, down, tokens=4, topk=2, index_bytes=8, local=4):
+        return lib.dpep_w4_experts(gate_up, down, 1, None, None, index_bytes, None, tokens, topk, 0, local, None, None, None)
+
+    assert experts(matrix(n=128, k=64), matrix(n=64, k=96)) == -1 and "belong" in message()
+    assert experts(matrix(n=128, k=64), matrix(n=64, k=64), tokens=1025) == -1 and "routes" in message()
+    assert experts(matrix(n=128, k=64), matrix(n=64, k=64), topk=33) == -1 and "slots" in message()
+    assert experts(matrix(n=128, k=64), matrix(n=64, k=64), local=1025) == -1 and "num_local" in message()
+    assert experts(matrix(n=128, k=64), matrix(n=64, k=64), index_bytes=2) == -1 and "index_bytes" in message()
+    assert experts(matrix(n=128, k=64), matrix(n=64, k=64), tokens=0) == 0
+    assert experts(matrix(n=128, k=64), matrix(n=64, k=64)) == -1 and "NULL" in message()
+    assert lib.dpep_w4_experts_scratch_bytes(-1, 2, 64, 64) == 0 and lib.dpep_w4_experts_scratch_bytes(4, 2, 64, 64) > 0
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+def test_quantize_rounds_to_half_a_step(symmetric, group):
+    gen = torch.Generator().manual_seed(group)
+    weight = torch.randn((3, 5, 256), generator=gen)
+    held = w4.quantize(weight, group, symmetric=symmetric, dtype=torch.float16)
+    assert held.packed.shape == (3, 5, 128) and held.scales.shape == (3, 5, 256 // group) and (held.zeros is None) == symmetric
+    step = held.scales.float().repeat_interleave(group, dim=-1)
+    # half a step; a zero point that is rounded, and a scale that is (2^-11 of 15 steps), may cut the ends by another half
+    assert ((w4.dequantize(held) - weight).abs() <= step * (0.51 if symmetric else 1.02)).all()
+    with pytest.raises(ValueError):
+        w4.quantize(weight, 48)
+    with pytest.raises(ValueError):
+        w4.quantize(weight[..., :250], 128)
