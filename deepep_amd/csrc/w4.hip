@@ -2,6 +2,9 @@
 //
 //   W[n,k] = (q[n,k] - zero[n,k/G]) * scale[n,k/G],  y[m,n] = sum_k x[m,k] W[n,k]
 //   experts: h = silu(W1g[e] x_t) * (W1u[e] x_t),  y_t = sum_s w_ts W2[e] h
+#include <algorithm>
+#include <type_traits>
+
 #include "common.h"
 
 #pragma clang fp contract(off)
@@ -10,6 +13,7 @@ namespace dpep {
 namespace {
 
 constexpr int kMaxRoutes = 2048;
+constexpr int kMaxK = 16384;
 
 // Expert ids of 8 or 4 bytes.
 struct Ids {
@@ -27,74 +31,417 @@ struct Ids {
 __device__ __forceinline__ float widen(uint32_t bits, bool half) { return half ? f16_to_f32(bits) : bf16_to_f32(bits); }
 __device__ __forceinline__ uint16_t narrow(float v, bool half) { return static_cast<uint16_t>((half ? pack_f16x2(v, 0.0f) : pack_bf16x2(v, 0.0f)) & 0xffffu); }
 
-// One row of a matrix times a vector, by a wave: every lane takes 32 values of k at a time.
-template <class X>
-__device__ float row_product(const dpep_w4& w, bool half, size_t row, const X* x, int lane)
+// The products run on the matrix cores (16 x 16 x 32): rows of x against 16 rows of W, whose codes become numbers without arithmetic: a
+// code's bits under the exponent of 16 are the 16-bit number 16 + q.  Over a group, with X = sum of x,
+//   sum x W = scale (sum x (16 + q) - (16 + zero) X)
+// where the accumulator starts at -(16 + zero) X, so a group ends with one multiply-add for every result.
+//
+// A wave streams pairs of 16-byte loads that cover 8 rows of whole 128-byte lines each (16 rows x 256 of k, a "unit"), which HBM serves as fast
+// as contiguous kilobytes (6.9 TB/s; 16 rows of 64 bytes: 5.5).  Lane l loads row l % 8 of each half, chunk (32 values) l / 16 + 4 (l / 8 % 2); swapping
+// between lanes 8 apart makes of the two loads the two operands X and Y, in which lane l holds row l % 16 and chunk l / 16 of the
+// unit's first and second 128 values.
+//
+// An MFMA adds up the four chunks of its operand.  Where a group is shorter than 128 values these belong to kDiag = 2 or 4 groups: the rows of the
+// other operand are then (group, token) with zeros outside the row's own group, so that every group has accumulators of its own, at 16 / kDiag
+// tokens an MFMA; in all cases a lane's results belong to the group of the chunk that the lane loaded.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kUnit = 256;  // values of k
+constexpr int kAhead = 2;   // units in flight, a pair of tiles each
+
+enum Kind { kMatvec, kGateUp, kDown };
+
+// One launch's matrices and how they are walked.
+struct Product {
+    const uint8_t* packed;
+    const uint16_t* scales;
+    const uint8_t* zeros;
+    int n, k, group;    // of one matrix
+    int units, groups;  // of a row
+    int group_inverse;  // ceil(2^20 / (group / 128)), for groups of 128 and more
+    int split;          // waves that share a tile's k, a power of two
+    int tile_groups;    // pairs of tiles of a matrix
+    int per;            // of them to a workgroup and wave group, one after the other
+    int row_cap;        // rows of x held in LDS
+    // rows: matvec: x [rows, k]; gate_up: x [token, k]; down: the routes' (high, low) rows [route][2][k]
+    const uint16_t* x;
+    int rows;
+    Ids ids;
+    int routes, topk;
+    const float* route_weights;
+    void* out;  // matvec: y; gate_up: the down product's x; down: [route][n] fp32
+};
+
+template <bool kHalf>
+__device__ __forceinline__ u32x4 unpack(uint32_t w)
 {
-    const uint8_t* const q = w.packed + row * (w.k / 2);
-    const size_t groups = w.k / w.group;
-    float sum = 0.0f;
-    for (int k = lane * 32; k < w.k; k += kWave * 32) {
-        const size_t g = row * groups + k / w.group;
-        const float scale = widen(static_cast<const uint16_t*>(w.scales)[g], half), zero = w.zeros == nullptr ? 8.0f : static_cast<float>(w.zeros[g]);
-        float part = 0.0f;
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t both = q[k / 2 + i];
-            float a, b;
-            if constexpr (sizeof(X) == 4) {
-                a = x[k + 2 * i];
-                b = x[k + 2 * i + 1];
-            } else {
-                a = widen(x[k + 2 * i], half);
-                b = widen(x[k + 2 * i + 1], half);
+    constexpr uint32_t mask = kHalf ? 0x03C003C0u : 0x00780078u, sixteen = kHalf ? 0x4C004C00u : 0x41804180u;
+    if constexpr (kHalf) return u32x4{((w << 6) & mask) | sixteen, ((w << 2) & mask) | sixteen, ((w >> 2) & mask) | sixteen, ((w >> 6) & mask) | sixteen};
+    return u32x4{((w << 3) & mask) | sixteen, ((w >> 1) & mask) | sixteen, ((w >> 5) & mask) | sixteen, ((w >> 9) & mask) | sixteen};
+}
+template <bool kHalf>
+__device__ __forceinline__ f32x4 multiply(u32x4 x, u32x4 w, f32x4 c)
+{
+    if constexpr (kHalf) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, w), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, w), c, 0, 0, 0);
+}
+
+// Waits for LDS alone: the loads in flight stay in flight.
+__device__ __forceinline__ void lds_barrier()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Sizes of a launch's LDS: the rows in the MFMA's order, their groups' sums, the waves' results.
+__host__ __device__ inline int x_bytes(int units, int rows, int padded) { return (units * 32 * rows + padded) * 16; }  // (a short block of rows reads on)
+__host__ __device__ inline int sum_bytes(int units, int diag, int padded) { return units * 2 * diag * padded * 4; }
+
+template <Kind kKind, bool kHalf, bool kZeros, int kDiag, int kBlocks>
+__global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel(const Product p)
+{
+    constexpr bool kHalfRows = kHalf && kKind != kDown;      // the down product's rows are BF16 pairs whatever the type
+    constexpr int kTiles = 2;                                // tiles of 16 rows of W to a tile group
+    constexpr int kTokens = 16 / kDiag, kRows = kTokens * kBlocks;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ uint32_t experts_hit[DPEP_MAX_LOCAL_EXPERTS / 32];
+    __shared__ uint16_t my_routes[kKind == kMatvec ? 1 : kMaxRoutes];
+    __shared__ float my_weights[kKind == kGateUp ? kMaxRoutes : 1];
+    __shared__ int my_count;
+    __shared__ __attribute__((aligned(16))) uint32_t zero16[4];
+    __shared__ float results[kWaves][kTiles][kBlocks][4][kWave];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, chunk = lane >> 4;
+    int expert = 0, count = p.rows;
+    if (tid < 4) zero16[tid] = 0;
+    if constexpr (kKind != kMatvec) {
+        // The slot-th of the experts that any route goes to, and its routes in order.
+        for (int i = tid; i < DPEP_MAX_LOCAL_EXPERTS / 32; i += kThreads) experts_hit[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < p.routes; i += kThreads)
+            if (const int e = p.ids[i]; e >= 0) atomicOr(&experts_hit[e >> 5], 1u << (e & 31));
+        __syncthreads();
+        uint32_t word = lane < DPEP_MAX_LOCAL_EXPERTS / 32 ? experts_hit[lane] : 0;
+        const int inclusive = wave_scan(__popc(word)), exclusive = inclusive - __popc(word), slot = blockIdx.y;
+        const unsigned long long found = __ballot(slot >= exclusive && slot < inclusive);
+        if (found == 0) return;
+        const int at = __ffsll(found) - 1;
+        word = __builtin_amdgcn_readlane(word, at);
+        for (int skip = slot - __builtin_amdgcn_readlane(exclusive, at); skip > 0; --skip) word &= word - 1;
+        expert = __builtin_amdgcn_readfirstlane(at * 32 + __ffs(word) - 1);
+        if (wave == 0) {
+            int held = 0;
+            for (int base = 0; base < p.routes; base += kWave) {
+                const bool hit = base + lane < p.routes && p.ids[base + lane] == expert;
+                const unsigned long long mask = __ballot(hit);
+                if (hit) {
+                    const int to = held + __popcll(mask & ((1ull << lane) - 1));
+                    my_routes[to] = static_cast<uint16_t>(base + lane);
+                    if constexpr (kKind == kGateUp) my_weights[to] = p.route_weights[base + lane];
+                }
+                held += __popcll(mask);
             }
-            part = fmaf(static_cast<float>(both & 15u) - zero, a, part);
-            part = fmaf(static_cast<float>(both >> 4) - zero, b, part);
+            if (lane == 0) my_count = held;
         }
-        sum = fmaf(part, scale, sum);
+        __syncthreads();
+        count = __builtin_amdgcn_readfirstlane(my_count) * (kKind == kDown ? 2 : 1);
     }
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    return sum;
-}
 
-__global__ __launch_bounds__(256) void matvec_kernel(const dpep_w4 w, bool half, const uint16_t* x, uint16_t* y)
-{
-    const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6), m = blockIdx.y;
-    if (n >= w.n) return;
-    const float sum = row_product(w, half, n, x + static_cast<size_t>(m) * w.k, lane);
-    if (lane == 0) y[static_cast<size_t>(m) * w.n + n] = narrow(sum, half);
-}
+    // What this wave streams: units first_unit .. last_unit - 1 of its tile groups.
+    const int split = p.split, lanes_of_groups = kWaves / split;
+    const int share = wave & (split - 1), mine = wave / split;
+    const int first_unit = p.units * share / split, last_unit = p.units * (share + 1) / split;
+    const int matrix_rows = kKind == kGateUp ? p.n / 2 : p.n;  // among which tiles are counted
+    const int first_group = blockIdx.x * p.per * lanes_of_groups + mine;
+    const int half_k = p.k / 2;
+    const uint8_t* const packed = p.packed + static_cast<size_t>(expert) * p.n * half_k;
+    const uint16_t* const scales = p.scales + static_cast<size_t>(expert) * p.n * p.groups;
+    const uint8_t* const zeros = kZeros ? p.zeros + static_cast<size_t>(expert) * p.n * p.groups : nullptr;
+    // (a matrix of fewer than 16 rows: lanes past its end load its last row; the last tile of others is moved up to end with the matrix)
+    const int loaded_chunk = chunk + 4 * ((lane >> 3) & 1);
+    const uint32_t row_low = min(lane & 7, matrix_rows - 1) * half_k, row_high = min((lane & 7) + 8, matrix_rows - 1) * half_k;
+    const int tail_chunk = (p.units - 1) * 8 + loaded_chunk < p.k / 32 ? loaded_chunk : 0;  // chunks behind k: any that exist (x is zero there)
+    const uint32_t scale_row = min(col, matrix_rows - 1) * p.groups;
 
-__global__ __launch_bounds__(256) void gate_up_kernel(const dpep_w4 w, bool half, const uint16_t* x, const Ids ids, int topk, float* h)
-{
-    const int lane = threadIdx.x & 63, inter = w.n / 2, n = blockIdx.x * 4 + (threadIdx.x >> 6), route = blockIdx.y;
-    const int e = ids[route];
-    if (n >= inter || e < 0) return;
-    const uint16_t* const row = x + static_cast<size_t>(route / topk) * w.k;
-    const float gate = row_product(w, half, static_cast<size_t>(e) * w.n + n, row, lane);
-    const float up = row_product(w, half, static_cast<size_t>(e) * w.n + inter + n, row, lane);
-    if (lane == 0) h[static_cast<size_t>(route) * inter + n] = gate / (1.0f + expf(-gate)) * up;
-}
+    auto tile_row = [&](int g, int tile) {  // of the matrix: first row of one of a tile group's two tiles
+        g = min(g, p.tile_groups - 1);
+        if constexpr (kKind == kGateUp) return min(g * 16, max(matrix_rows - 16, 0)) + tile * matrix_rows;
+        return min((g * 2 + tile) * 16, max(matrix_rows - 16, 0));
+    };
 
-__global__ __launch_bounds__(256) void down_kernel(const dpep_w4 w, bool half, const float* h, const Ids ids, const float* weights, int topk, uint16_t* y)
-{
-    const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6), token = blockIdx.y;
-    if (n >= w.n) return;
-    float sum = 0.0f;
-    for (int s = 0; s < topk; ++s) {
-        const int route = token * topk + s;
-        const int e = ids[route];
-        if (e < 0) continue;
-        sum = fmaf(weights[route], row_product(w, half, static_cast<size_t>(e) * w.n + n, h + static_cast<size_t>(route) * w.k, lane), sum);
+    struct Slot {
+        u32x4 low[kTiles], high[kTiles];
+        uint32_t scale[kTiles][2], zero[kTiles][2];
+    };
+    auto load = [&](Slot& s, int g, int u) {
+        const uint32_t at = (u == p.units - 1 ? tail_chunk : loaded_chunk) * 16;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int row = tile_row(g, t);
+            const uint8_t* const base = packed + static_cast<size_t>(row) * half_k + u * (kUnit / 2);
+            s.low[t] = load16_nt(base + (row_low + at));
+            s.high[t] = load16_nt(base + (row_high + at));
+            const size_t first_scale = static_cast<size_t>(row) * p.groups;
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int part = u * 2 + f;
+                int of = kDiag == 1 ? (part * p.group_inverse) >> 20 : part * kDiag + chunk / (4 / kDiag);
+                of = min(of, p.groups - 1);
+                const uint32_t index = scale_row + of;
+                s.scale[t][f] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(scales + first_scale) + 2 * index);
+                if constexpr (kZeros) s.zero[t][f] = (zeros + first_scale)[index];
+            }
+        }
+    };
+
+    // Where a lane reads x: token lane % 16 (of its group's rows), chunk lane / 16; zeros outside the row's own group.
+    const int token_of_lane = col % kTokens;
+    const bool own = kDiag == 1 || chunk / (4 / kDiag) == col / kTokens;
+
+    for (int first_row = 0; first_row < count; first_row += p.row_cap) {
+        const int rows = min(count - first_row, p.row_cap), padded = (rows + kRows - 1) / kRows * kRows;
+        unsigned char* const x_lds = lds;
+        float* const sums_lds = reinterpret_cast<float*>(lds + x_bytes(p.units, p.row_cap, kRows));
+        if (first_row > 0) lds_barrier();
+
+        Slot ring[kAhead];
+        int load_group = 0, load_unit = first_unit;
+        auto load_next = [&](Slot& s) {
+            load(s, first_group + load_group * lanes_of_groups, load_unit);
+            if (++load_unit == last_unit) {
+                load_unit = first_unit;
+                load_group = min(load_group + 1, p.per - 1);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
+
+        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.
+        for (int i = tid; i < rows * p.units * 8; i += kThreads) {
+            const int m = i / (p.units * 8), c32 = i - m * (p.units * 8);
+            const int which = first_row + m;
+            const uint16_t* from;
+            if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
+            else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
+            else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
+            float sum = 0.0f;
+            const bool real = c32 < p.k / 32;
+            unsigned char* const to = x_lds + static_cast<size_t>((((c32 >> 2) * 4) * 4 + (c32 & 3)) * rows + m) * 16;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u32x4 v = {0u, 0u, 0u, 0u};
+                if (real) v = load16(from + c32 * 32 + j * 8);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) sum += widen(v[d] & 0xffffu, kHalfRows) + widen(v[d] >> 16, kHalfRows);
+                const u32x4 pairs = {(v[0] & 0xffffu) | (v[2] << 16), (v[0] >> 16) | (v[2] & 0xffff0000u), (v[1] & 0xffffu) | (v[3] << 16),
+                                     (v[1] >> 16) | (v[3] & 0xffff0000u)};
+                *reinterpret_cast<u32x4*>(to + static_cast<size_t>(j * 4 * rows) * 16) = pairs;
+            }
+            if constexpr (kDiag < 4) sum += __shfl_xor(sum, 1);
+            if constexpr (kDiag < 2) sum += __shfl_xor(sum, 2);
+            if ((c32 & (4 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(c32 / (4 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
+        }
+        lds_barrier();
+
+        f32x4 acc[kTiles][kBlocks] = {};
+        const int x_lane = own ? (chunk * rows + min(token_of_lane, rows - 1)) * 16 : 0;
+        auto consume = [&](const Slot& s, int u) {
+            u32x4 w[2][kTiles];
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    w[0][t][d] = __builtin_amdgcn_update_dpp(s.low[t][d], s.high[t][d], 0x128, 0xf, 0xc, false);
+                    w[1][t][d] = __builtin_amdgcn_update_dpp(s.high[t][d], s.low[t][d], 0x128, 0xf, 0x3, false);
+                }
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int part = u * 2 + f;
+                f32x4 c[kTiles][kBlocks];
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    const int sub = kDiag == 1 ? 0 : chunk / (4 / kDiag), token = (kDiag == 1 ? chunk * 4 : kDiag == 2 ? (chunk & 1) * 4 : 0) + b * kTokens;
+                    const f32x4 start = *reinterpret_cast<const f32x4*>(sums_lds + static_cast<size_t>(part * kDiag + sub) * padded + token);
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        c[t][b] = start;
+                        if constexpr (kZeros) {
+                            const float zero = 16.0f + static_cast<float>(s.zero[t][f]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) c[t][b][i] *= zero;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned char* const from = own ? x_lds + (part * 4 + j) * 4 * rows * 16 + x_lane : reinterpret_cast<const unsigned char*>(zero16);
+                    u32x4 q[kTiles];
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) q[t] = unpack<kHalfRows>(w[f][t][j]);
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        const u32x4 a = *reinterpret_cast<const u32x4*>(from + (own ? b * kTokens * 16 : 0));
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) c[t][b] = multiply<kHalfRows>(a, q[t], c[t][b]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    const float scale = widen(s.scale[t][f], kHalf);
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[t][b][i] = fmaf(scale, c[t][b][i], acc[t][b][i]);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (the other half's operands would be fetched here, and cost registers)
+            }
+        };
+
+        // Sum of a result over the waves that share its tile and, for short groups, over the lanes that hold its groups.
+        auto result = [&](int group, int tile, int m, int n) {
+            const int b = m / kTokens, token = m % kTokens;
+            float sum = 0.0f;
+            for (int w = 0; w < split; ++w)
+#pragma unroll
+                for (int d = 0; d < kDiag; ++d) {
+                    const int from = kDiag == 1 ? token / 4 : kDiag == 2 ? token / 4 + 2 * d : d;
+                    sum += results[group * split + w][tile][b][token % 4][from * 16 + n];
+                }
+            return sum;
+        };
+        auto finish = [&](int done) {  // tile groups number `done` of this workgroup's waves
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        results[wave][t][b][i][lane] = acc[t][b][i];
+                        acc[t][b][i] = 0.0f;
+                    }
+            lds_barrier();
+            constexpr int kOut = kKind == kGateUp ? 1 : kTiles;  // result tiles of a tile group
+            const int outputs = lanes_of_groups * kOut * 16 * (kKind == kDown ? rows / 2 : rows);
+            for (int o = tid; o < outputs; o += kThreads) {
+                const int n = o & 15, tile = (o >> 4) % kOut, rest = (o >> 4) / kOut, group = rest % lanes_of_groups, m = rest / lanes_of_groups;
+                const int g = blockIdx.x * p.per * lanes_of_groups + done * lanes_of_groups + group;
+                const int to = tile_row(g, tile) + n;
+                if (g >= p.tile_groups || to >= matrix_rows) continue;
+                if constexpr (kKind == kMatvec) {
+                    static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(result(group, tile, m, n), kHalf);
+                } else if constexpr (kKind == kGateUp) {
+                    const float gate = result(group, 0, m, n), up = result(group, 1, m, n);
+                    const int route = my_routes[first_row + m];
+                    // The route's weight is folded in here.  Two BF16 numbers hold the product's high and low part, together 16 bits of mantissa.
+                    const float h = gate / (1.0f + expf(-gate)) * up * my_weights[first_row + m];
+                    const uint32_t high = f32_to_bf16(h);
+                    uint16_t* const row = static_cast<uint16_t*>(p.out) + static_cast<size_t>(route) * 2 * matrix_rows + to;
+                    row[0] = static_cast<uint16_t>(high);
+                    row[matrix_rows] = static_cast<uint16_t>(f32_to_bf16(h - bf16_to_f32(high)));
+                } else {
+                    const int route = my_routes[(first_row >> 1) + m];
+                    static_cast<float*>(p.out)[static_cast<size_t>(route) * p.n + to] = result(group, tile, 2 * m, n) + result(group, tile, 2 * m + 1, n);
+                }
+            }
+            lds_barrier();
+        };
+
+        int unit = first_unit, done = 0;
+        while (done < p.per) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (done >= p.per) break;
+                consume(ring[i], unit);
+                load_next(ring[i]);
+                if (++unit == last_unit) {
+                    unit = first_unit;
+                    finish(done++);
+                }
+            }
+        }
     }
-    if (lane == 0) y[static_cast<size_t>(token) * w.n + n] = narrow(sum, half);
+}
+
+// y[t] = sum of its routes' rows, in the order of the slots.
+__global__ __launch_bounds__(256) void sum_routes_kernel(const float* rows, const Ids ids, int tokens, int topk, int hidden, bool half, uint16_t* y)
+{
+    const int per_row = hidden / 4, i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= tokens * per_row) return;
+    const int token = i / per_row, at = (i - token * per_row) * 4;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < topk; ++s)
+        if (const int route = token * topk + s; ids[route] >= 0) sum += *reinterpret_cast<const f32x4*>(rows + static_cast<size_t>(route) * hidden + at);
+    uint16_t* const to = y + static_cast<size_t>(token) * hidden + at;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) to[d] = narrow(sum[d], half);
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------------------------------
+constexpr int kLdsBytes = 48 << 10;  // of a workgroup's rows and sums, so that two share a CU
+
+template <Kind kKind>
+int launch_product(Product p, int type, int slots, int rows_expected, int rows_most, hipStream_t stream)
+{
+    p.units = (p.k + kUnit - 1) / kUnit;
+    p.groups = p.k / p.group;
+    const int diag = p.group >= 128 ? 1 : 128 / p.group;
+    p.group_inverse = diag == 1 ? ((1 << 20) + p.group / 128 - 1) / (p.group / 128) : 0;
+    p.split = 1;
+    while (p.split < kWaves && p.split * 2 * 3 <= p.units) p.split *= 2;
+    const int counted = kKind == kGateUp ? p.n / 2 : (p.n + 1) / 2;
+    p.tile_groups = (counted + 15) / 16;
+    const int at_once = kWaves / p.split, steps = (p.tile_groups + at_once - 1) / at_once;
+    p.per = std::max(1, std::min(8, steps * slots / 1024));
+    const int tokens = 16 / diag, blocks = std::min(4, std::max(1, (rows_expected + tokens - 1) / tokens));
+    const int by_blocks = blocks <= 1 ? 1 : 4, most = tokens * by_blocks;
+    int rows = std::min(rows_most, most);
+    while (rows > (kKind == kDown ? 2 : 1) && x_bytes(p.units, rows, most) + sum_bytes(p.units, diag, most) > kLdsBytes) --rows;
+    if (kKind == kDown) rows &= ~1;
+    p.row_cap = rows;
+    const int bytes = x_bytes(p.units, rows, most) + sum_bytes(p.units, diag, most);
+    const dim3 grid((steps + p.per - 1) / p.per, slots);
+    int status = DPEP_OK;
+    auto go = [&](auto half, auto zeros, auto d, auto b) {
+        const auto kernel = product_kernel<kKind, half(), zeros(), d(), b()>;
+        if (bytes > 32 << 10) {
+            const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (err != hipSuccess) {
+                status = fail(DPEP_ERUNTIME, "w4: %s", hipGetErrorString(err));
+                return;
+            }
+        }
+        kernel<<<grid, kThreads, bytes, stream>>>(p);
+        status = launch_status("w4 product");
+    };
+    auto by_block = [&](auto half, auto zeros, auto d) {
+        if (by_blocks == 1) go(half, zeros, d, std::integral_constant<int, 1>{});
+        else go(half, zeros, d, std::integral_constant<int, 4>{});
+    };
+    auto by_group = [&](auto half, auto zeros) {
+        if (diag == 1) by_block(half, zeros, std::integral_constant<int, 1>{});
+        else if (diag == 2) by_block(half, zeros, std::integral_constant<int, 2>{});
+        else by_block(half, zeros, std::integral_constant<int, 4>{});
+    };
+    auto by_zeros = [&](auto half) {
+        if (p.zeros != nullptr) by_group(half, std::true_type{});
+        else by_group(half, std::false_type{});
+    };
+    if (type == DPEP_TYPE_F16) by_zeros(std::true_type{});
+    else by_zeros(std::false_type{});
+    return status;
 }
 
 int check_w4(const dpep_w4* w, int type, const char* what)
 {
     DPEP_REQUIRE(w != nullptr, "%s: weights is NULL", what);
     DPEP_REQUIRE(type == DPEP_TYPE_BF16 || type == DPEP_TYPE_F16, "%s: type=%d is neither BF16 nor FP16", what, type);
-    DPEP_REQUIRE(w->n >= 1 && w->k >= 32, "%s: N=%d K=%d", what, w->n, w->k);
+    DPEP_REQUIRE(w->n >= 1 && w->k >= 32 && w->k <= kMaxK, "%s: N=%d K=%d: K is at most %d", what, w->n, w->k, kMaxK);
     DPEP_REQUIRE((w->group == 32 || w->group == 64 || (w->group >= 128 && w->group % 128 == 0)) && w->k % w->group == 0,
                  "%s: group=%d is not 32, 64 or a multiple of 128 that divides K=%d", what, w->group, w->k);
     DPEP_REQUIRE(w->packed != nullptr && w->scales != nullptr, "%s: a NULL buffer", what);
@@ -115,15 +462,23 @@ int dpep_w4_matvec(const dpep_w4* w, int type, const void* x, int num_rows, void
     DPEP_REQUIRE(num_rows >= 0 && num_rows <= 65535, "w4_matvec: num_rows=%d is not in [0, 65535]", num_rows);
     if (num_rows == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && y != nullptr && aligned16(x), "w4_matvec: a NULL or misaligned buffer");
-    matvec_kernel<<<dim3((w->n + 3) / 4, num_rows), 256, 0, static_cast<hipStream_t>(stream)>>>(*w, type == DPEP_TYPE_F16, static_cast<const uint16_t*>(x),
-                                                                                               static_cast<uint16_t*>(y));
-    return launch_status("w4_matvec");
+    Product p = {};
+    p.packed = w->packed;
+    p.scales = static_cast<const uint16_t*>(w->scales);
+    p.zeros = w->zeros;
+    p.n = w->n;
+    p.k = w->k;
+    p.group = w->group;
+    p.x = static_cast<const uint16_t*>(x);
+    p.rows = num_rows;
+    p.out = y;
+    return launch_product<kMatvec>(p, type, 1, num_rows, num_rows, static_cast<hipStream_t>(stream));
 }
 
 size_t dpep_w4_experts_scratch_bytes(int num_tokens, int num_topk, int hidden, int intermediate)
 {
     if (num_tokens < 0 || num_topk < 1 || hidden < 1 || intermediate < 1) return 0;
-    return static_cast<size_t>(num_tokens) * num_topk * intermediate * 4;
+    return static_cast<size_t>(num_tokens) * num_topk * (static_cast<size_t>(intermediate) + hidden) * 4;
 }
 
 int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const void* x, const void* topk_idx, int index_bytes, const float* topk_weights,
@@ -141,11 +496,35 @@ int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const
     DPEP_REQUIRE(x != nullptr && topk_idx != nullptr && topk_weights != nullptr && y != nullptr && scratch != nullptr && aligned16(x) && aligned16(scratch),
                  "w4_experts: a NULL or misaligned buffer");
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool half = type == DPEP_TYPE_F16;
-    float* const h = static_cast<float*>(scratch);
-    const Ids ids = {topk_idx, index_bytes == 8, expert_begin, num_local};
-    gate_up_kernel<<<dim3((down->k + 3) / 4, num_tokens * num_topk), 256, 0, s>>>(*gate_up, half, static_cast<const uint16_t*>(x), ids, num_topk, h);
-    down_kernel<<<dim3((down->n + 3) / 4, num_tokens), 256, 0, s>>>(*down, half, h, ids, topk_weights, num_topk, static_cast<uint16_t*>(y));
+    const int routes = num_tokens * num_topk, slots = std::min(routes, num_local);
+    // rows of an expert: about routes / experts, at most all of them (a token may name an expert twice)
+    const int expected = 2 * routes / num_local + 1;
+    Product p = {};
+    p.packed = gate_up->packed;
+    p.scales = static_cast<const uint16_t*>(gate_up->scales);
+    p.zeros = gate_up->zeros;
+    p.n = gate_up->n;
+    p.k = gate_up->k;
+    p.group = gate_up->group;
+    p.x = static_cast<const uint16_t*>(x);
+    p.ids = {topk_idx, index_bytes == 8, expert_begin, num_local};
+    p.routes = routes;
+    p.topk = num_topk;
+    p.route_weights = topk_weights;
+    p.out = scratch;
+    if (int rc = launch_product<kGateUp>(p, type, slots, expected, routes, s); rc != DPEP_OK) return rc;
+    float* const rows = static_cast<float*>(scratch) + static_cast<size_t>(routes) * down->k;
+    p.packed = down->packed;
+    p.scales = static_cast<const uint16_t*>(down->scales);
+    p.zeros = down->zeros;
+    p.n = down->n;
+    p.k = down->k;
+    p.group = down->group;
+    p.x = static_cast<const uint16_t*>(scratch);
+    p.out = rows;
+    if (int rc = launch_product<kDown>(p, type, slots, 2 * expected, 2 * routes, s); rc != DPEP_OK) return rc;
+    const int pieces = num_tokens * (down->n / 4);
+    sum_routes_kernel<<<(pieces + 255) / 256, 256, 0, s>>>(rows, p.ids, num_tokens, num_topk, down->n, type == DPEP_TYPE_F16, static_cast<uint16_t*>(y));
     return launch_status("w4_experts");
 }
 
