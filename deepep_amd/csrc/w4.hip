@@ -51,7 +51,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kUnit = 256;  // values of k
-constexpr int kAhead = 2;   // units in flight, a pair of tiles each
 
 enum Kind { kMatvec, kGateUp, kDown };
 
@@ -64,8 +63,8 @@ struct Product {
     int units, groups;  // of a row
     int group_inverse;  // ceil(2^20 / (group / 128)), for groups of 128 and more
     int split;          // waves that share a tile's k, a power of two
-    int tile_groups;    // pairs of tiles of a matrix
-    int per;            // of them to a workgroup and wave group, one after the other
+    int tile_groups;    // of a matrix, kTiles tiles each
+    int steps;          // a matrix in steps of a workgroup: kWaves / split tile groups at a time
     int row_cap;        // rows of x held in LDS
     // rows: matvec: x [rows, k]; gate_up: x [token, k]; down: the routes' (high, low) rows [route][2][k]
     const uint16_t* x;
@@ -76,13 +75,22 @@ struct Product {
     void* out;  // matvec: y; gate_up: the down product's x; down: [route][n] fp32
 };
 
+// The constants that make numbers of codes, in registers (an instruction that masks and inserts takes no literals).
 template <bool kHalf>
-__device__ __forceinline__ u32x4 unpack(uint32_t w)
-{
-    constexpr uint32_t mask = kHalf ? 0x03C003C0u : 0x00780078u, sixteen = kHalf ? 0x4C004C00u : 0x41804180u;
-    if constexpr (kHalf) return u32x4{((w << 6) & mask) | sixteen, ((w << 2) & mask) | sixteen, ((w >> 2) & mask) | sixteen, ((w >> 6) & mask) | sixteen};
-    return u32x4{((w << 3) & mask) | sixteen, ((w >> 1) & mask) | sixteen, ((w >> 5) & mask) | sixteen, ((w >> 9) & mask) | sixteen};
-}
+struct Codes {
+    uint32_t mask, sixteen;
+    __device__ __forceinline__ Codes()
+    {
+        asm("s_mov_b32 %0, %1" : "=s"(mask) : "i"(kHalf ? 0x03C003C0u : 0x00780078u));
+        asm("v_mov_b32 %0, %1" : "=v"(sixteen) : "i"(kHalf ? 0x4C004C00u : 0x41804180u));
+    }
+    // Eight codes, values (0, 4), (1, 5), (2, 6) and (3, 7), each 16 + q.
+    __device__ __forceinline__ u32x4 unpack(uint32_t w) const
+    {
+        if constexpr (kHalf) return u32x4{((w << 6) & mask) | sixteen, ((w << 2) & mask) | sixteen, ((w >> 2) & mask) | sixteen, ((w >> 6) & mask) | sixteen};
+        return u32x4{((w << 3) & mask) | sixteen, ((w >> 1) & mask) | sixteen, ((w >> 5) & mask) | sixteen, ((w >> 9) & mask) | sixteen};
+    }
+};
 template <bool kHalf>
 __device__ __forceinline__ f32x4 multiply(u32x4 x, u32x4 w, f32x4 c)
 {
@@ -102,269 +110,296 @@ __device__ __forceinline__ void lds_barrier()
 __host__ __device__ inline int x_bytes(int units, int rows, int padded) { return (units * 32 * rows + padded) * 16; }  // (a short block of rows reads on)
 __host__ __device__ inline int sum_bytes(int units, int diag, int padded) { return units * 2 * diag * padded * 4; }
 
+// A workgroup takes an even share of all steps: of the matrices that have rows one after the other (matvec: of the passes over the rows), each
+// with the rows it multiplies in LDS.
 template <Kind kKind, bool kHalf, bool kZeros, int kDiag, int kBlocks>
 __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel(const Product p)
 {
-    constexpr bool kHalfRows = kHalf && kKind != kDown;      // the down product's rows are BF16 pairs whatever the type
-    constexpr int kTiles = 2;                                // tiles of 16 rows of W to a tile group
+    constexpr bool kHalfRows = kHalf && kKind != kDown;  // the down product's rows are BF16 pairs whatever the type
+    constexpr int kTiles = kKind == kMatvec ? 1 : 2;     // tiles of 16 rows of W to a tile group; gate_up: a gate tile and its up tile
+    constexpr int kAhead = kKind == kMatvec ? 4 : 2;     // units in flight
     constexpr int kTokens = 16 / kDiag, kRows = kTokens * kBlocks;
+    constexpr int kRouteSlots = kKind == kMatvec ? 1 : kMaxRoutes;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ uint32_t experts_hit[DPEP_MAX_LOCAL_EXPERTS / 32];
-    __shared__ uint16_t my_routes[kKind == kMatvec ? 1 : kMaxRoutes];
-    __shared__ float my_weights[kKind == kGateUp ? kMaxRoutes : 1];
+    __shared__ int16_t expert_of[kRouteSlots];
+    __shared__ uint16_t my_routes[kRouteSlots];
+    __shared__ float route_weights[kKind == kGateUp ? kMaxRoutes : 1];
     __shared__ int my_count;
     __shared__ __attribute__((aligned(16))) uint32_t zero16[4];
     __shared__ float results[kWaves][kTiles][kBlocks][4][kWave];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, chunk = lane >> 4;
-    int expert = 0, count = p.rows;
     if (tid < 4) zero16[tid] = 0;
-    if constexpr (kKind != kMatvec) {
-        // The slot-th of the experts that any route goes to, and its routes in order.
-        for (int i = tid; i < DPEP_MAX_LOCAL_EXPERTS / 32; i += kThreads) experts_hit[i] = 0;
+    uint32_t hit_word = 0;  // lane l: which of experts 32 l .. 32 l + 31 have a route
+    int hit_before = 0, matrices = 0;
+    if constexpr (kKind == kMatvec) {
+        matrices = (p.rows + p.row_cap - 1) / p.row_cap;
+    } else {
+        if (tid < DPEP_MAX_LOCAL_EXPERTS / 32) experts_hit[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < p.routes; i += kThreads)
-            if (const int e = p.ids[i]; e >= 0) atomicOr(&experts_hit[e >> 5], 1u << (e & 31));
-        __syncthreads();
-        uint32_t word = lane < DPEP_MAX_LOCAL_EXPERTS / 32 ? experts_hit[lane] : 0;
-        const int inclusive = wave_scan(__popc(word)), exclusive = inclusive - __popc(word), slot = blockIdx.y;
-        const unsigned long long found = __ballot(slot >= exclusive && slot < inclusive);
-        if (found == 0) return;
-        const int at = __ffsll(found) - 1;
-        word = __builtin_amdgcn_readlane(word, at);
-        for (int skip = slot - __builtin_amdgcn_readlane(exclusive, at); skip > 0; --skip) word &= word - 1;
-        expert = __builtin_amdgcn_readfirstlane(at * 32 + __ffs(word) - 1);
-        if (wave == 0) {
-            int held = 0;
-            for (int base = 0; base < p.routes; base += kWave) {
-                const bool hit = base + lane < p.routes && p.ids[base + lane] == expert;
-                const unsigned long long mask = __ballot(hit);
-                if (hit) {
-                    const int to = held + __popcll(mask & ((1ull << lane) - 1));
-                    my_routes[to] = static_cast<uint16_t>(base + lane);
-                    if constexpr (kKind == kGateUp) my_weights[to] = p.route_weights[base + lane];
-                }
-                held += __popcll(mask);
-            }
-            if (lane == 0) my_count = held;
+        for (int i = tid; i < p.routes; i += kThreads) {
+            const int e = p.ids[i];
+            if constexpr (kKind == kGateUp) route_weights[i] = p.route_weights[i];
+            expert_of[i] = static_cast<int16_t>(e);
+            if (e >= 0) atomicOr(&experts_hit[e >> 5], 1u << (e & 31));
         }
         __syncthreads();
-        count = __builtin_amdgcn_readfirstlane(my_count) * (kKind == kDown ? 2 : 1);
+        hit_word = lane < DPEP_MAX_LOCAL_EXPERTS / 32 ? experts_hit[lane] : 0;
+        const int until = wave_scan(__popc(hit_word));
+        hit_before = until - __popc(hit_word);
+        matrices = __builtin_amdgcn_readlane(until, 63);
     }
+    const int all_steps = matrices * p.steps;
+    int step = static_cast<int>(static_cast<long long>(all_steps) * blockIdx.x / gridDim.x);
+    const int end_step = static_cast<int>(static_cast<long long>(all_steps) * (blockIdx.x + 1) / gridDim.x);
 
     // What this wave streams: units first_unit .. last_unit - 1 of its tile groups.
     const int split = p.split, lanes_of_groups = kWaves / split;
     const int share = wave & (split - 1), mine = wave / split;
     const int first_unit = p.units * share / split, last_unit = p.units * (share + 1) / split;
     const int matrix_rows = kKind == kGateUp ? p.n / 2 : p.n;  // among which tiles are counted
-    const int first_group = blockIdx.x * p.per * lanes_of_groups + mine;
     const int half_k = p.k / 2;
-    const uint8_t* const packed = p.packed + static_cast<size_t>(expert) * p.n * half_k;
-    const uint16_t* const scales = p.scales + static_cast<size_t>(expert) * p.n * p.groups;
-    const uint8_t* const zeros = kZeros ? p.zeros + static_cast<size_t>(expert) * p.n * p.groups : nullptr;
     // (a matrix of fewer than 16 rows: lanes past its end load its last row; the last tile of others is moved up to end with the matrix)
     const int loaded_chunk = chunk + 4 * ((lane >> 3) & 1);
     const uint32_t row_low = min(lane & 7, matrix_rows - 1) * half_k, row_high = min((lane & 7) + 8, matrix_rows - 1) * half_k;
     const int tail_chunk = (p.units - 1) * 8 + loaded_chunk < p.k / 32 ? loaded_chunk : 0;  // chunks behind k: any that exist (x is zero there)
     const uint32_t scale_row = min(col, matrix_rows - 1) * p.groups;
-
-    auto tile_row = [&](int g, int tile) {  // of the matrix: first row of one of a tile group's two tiles
+    auto tile_row = [&](int g, int tile) {  // of the matrix: first row of one of a tile group's tiles
         g = min(g, p.tile_groups - 1);
         if constexpr (kKind == kGateUp) return min(g * 16, max(matrix_rows - 16, 0)) + tile * matrix_rows;
-        return min((g * 2 + tile) * 16, max(matrix_rows - 16, 0));
+        return min((g * kTiles + tile) * 16, max(matrix_rows - 16, 0));
     };
-
-    struct Slot {
-        u32x4 low[kTiles], high[kTiles];
-        uint32_t scale[kTiles][2], zero[kTiles][2];
-    };
-    auto load = [&](Slot& s, int g, int u) {
-        const uint32_t at = (u == p.units - 1 ? tail_chunk : loaded_chunk) * 16;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            const int row = tile_row(g, t);
-            const uint8_t* const base = packed + static_cast<size_t>(row) * half_k + u * (kUnit / 2);
-            s.low[t] = load16_nt(base + (row_low + at));
-            s.high[t] = load16_nt(base + (row_high + at));
-            const size_t first_scale = static_cast<size_t>(row) * p.groups;
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                const int part = u * 2 + f;
-                int of = kDiag == 1 ? (part * p.group_inverse) >> 20 : part * kDiag + chunk / (4 / kDiag);
-                of = min(of, p.groups - 1);
-                const uint32_t index = scale_row + of;
-                s.scale[t][f] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(scales + first_scale) + 2 * index);
-                if constexpr (kZeros) s.zero[t][f] = (zeros + first_scale)[index];
-            }
-        }
-    };
-
+    const Codes<kHalfRows> codes;
     // Where a lane reads x: token lane % 16 (of its group's rows), chunk lane / 16; zeros outside the row's own group.
-    const int token_of_lane = col % kTokens;
     const bool own = kDiag == 1 || chunk / (4 / kDiag) == col / kTokens;
 
-    for (int first_row = 0; first_row < count; first_row += p.row_cap) {
-        const int rows = min(count - first_row, p.row_cap), padded = (rows + kRows - 1) / kRows * kRows;
-        unsigned char* const x_lds = lds;
-        float* const sums_lds = reinterpret_cast<float*>(lds + x_bytes(p.units, p.row_cap, kRows));
-        if (first_row > 0) lds_barrier();
+    while (step < end_step) {
+        const int matrix = step / p.steps, first_step = step - matrix * p.steps, steps = min(p.steps - first_step, end_step - step);
+        step += steps;
+        int expert = 0, count = p.rows, first_row = 0;
+        if constexpr (kKind == kMatvec) {
+            first_row = matrix * p.row_cap;
+            count = min(p.rows, first_row + p.row_cap);
+        } else {
+            // The matrix-th of the experts that have a route, and its routes in order.
+            const int at = __ffsll(__ballot(matrix >= hit_before && matrix < hit_before + __popc(hit_word))) - 1;
+            uint32_t word = __builtin_amdgcn_readlane(hit_word, at);
+            for (int skip = matrix - __builtin_amdgcn_readlane(hit_before, at); skip > 0; --skip) word &= word - 1;
+            expert = __builtin_amdgcn_readfirstlane(at * 32 + __ffs(word) - 1);
+        }
+        const uint8_t* const packed = p.packed + static_cast<size_t>(expert) * p.n * half_k;
+        const uint16_t* const scales = p.scales + static_cast<size_t>(expert) * p.n * p.groups;
+        const uint8_t* const zeros = kZeros ? p.zeros + static_cast<size_t>(expert) * p.n * p.groups : nullptr;
 
-        Slot ring[kAhead];
-        int load_group = 0, load_unit = first_unit;
-        auto load_next = [&](Slot& s) {
-            load(s, first_group + load_group * lanes_of_groups, load_unit);
-            if (++load_unit == last_unit) {
-                load_unit = first_unit;
-                load_group = min(load_group + 1, p.per - 1);
+        struct Slot {
+            u32x4 low[kTiles], high[kTiles];
+            uint32_t scale[kTiles][2], zero[kTiles][2];
+        };
+        auto load = [&](Slot& s, int g, int u) {
+            const uint32_t at = (u == p.units - 1 ? tail_chunk : loaded_chunk) * 16;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                const int row = tile_row(g, t);
+                const uint8_t* const base = packed + static_cast<size_t>(row) * half_k + u * (kUnit / 2);
+                s.low[t] = load16_nt(base + (row_low + at));
+                s.high[t] = load16_nt(base + (row_high + at));
+                const size_t first_scale = static_cast<size_t>(row) * p.groups;
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    const int part = u * 2 + f;
+                    int of = kDiag == 1 ? (part * p.group_inverse) >> 20 : part * kDiag + chunk / (4 / kDiag);
+                    of = min(of, p.groups - 1);
+                    const uint32_t index = scale_row + of;
+                    s.scale[t][f] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(scales + first_scale) + 2 * index);
+                    if constexpr (kZeros) s.zero[t][f] = (zeros + first_scale)[index];
+                }
             }
         };
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
 
-        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.
-        for (int i = tid; i < rows * p.units * 8; i += kThreads) {
-            const int m = i / (p.units * 8), c32 = i - m * (p.units * 8);
-            const int which = first_row + m;
-            const uint16_t* from;
-            if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
-            else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
-            else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
-            float sum = 0.0f;
-            const bool real = c32 < p.k / 32;
-            unsigned char* const to = x_lds + static_cast<size_t>((((c32 >> 2) * 4) * 4 + (c32 & 3)) * rows + m) * 16;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 v = {0u, 0u, 0u, 0u};
-                if (real) v = load16(from + c32 * 32 + j * 8);
-#pragma unroll
-                for (int d = 0; d < 4; ++d) sum += widen(v[d] & 0xffffu, kHalfRows) + widen(v[d] >> 16, kHalfRows);
-                const u32x4 pairs = {(v[0] & 0xffffu) | (v[2] << 16), (v[0] >> 16) | (v[2] & 0xffff0000u), (v[1] & 0xffffu) | (v[3] << 16),
-                                     (v[1] >> 16) | (v[3] & 0xffff0000u)};
-                *reinterpret_cast<u32x4*>(to + static_cast<size_t>(j * 4 * rows) * 16) = pairs;
-            }
-            if constexpr (kDiag < 4) sum += __shfl_xor(sum, 1);
-            if constexpr (kDiag < 2) sum += __shfl_xor(sum, 2);
-            if ((c32 & (4 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(c32 / (4 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
-        }
-        lds_barrier();
-
-        f32x4 acc[kTiles][kBlocks] = {};
-        const int x_lane = own ? (chunk * rows + min(token_of_lane, rows - 1)) * 16 : 0;
-        auto consume = [&](const Slot& s, int u) {
-            u32x4 w[2][kTiles];
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    w[0][t][d] = __builtin_amdgcn_update_dpp(s.low[t][d], s.high[t][d], 0x128, 0xf, 0xc, false);
-                    w[1][t][d] = __builtin_amdgcn_update_dpp(s.high[t][d], s.low[t][d], 0x128, 0xf, 0x3, false);
+        bool listed = kKind == kMatvec;
+        do {
+            Slot ring[kAhead];
+            int load_step = first_step, load_unit = first_unit;
+            asm volatile("" : "+s"(load_step), "+s"(load_unit));  // (or every pass's first addresses are kept in registers all along)
+            auto load_next = [&](Slot& s) {
+                load(s, load_step * lanes_of_groups + mine, load_unit);
+                if (++load_unit == last_unit) {
+                    load_unit = first_unit;
+                    load_step = min(load_step + 1, first_step + steps - 1);
                 }
+            };
 #pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                const int part = u * 2 + f;
-                f32x4 c[kTiles][kBlocks];
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
-                    const int sub = kDiag == 1 ? 0 : chunk / (4 / kDiag), token = (kDiag == 1 ? chunk * 4 : kDiag == 2 ? (chunk & 1) * 4 : 0) + b * kTokens;
-                    const f32x4 start = *reinterpret_cast<const f32x4*>(sums_lds + static_cast<size_t>(part * kDiag + sub) * padded + token);
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) {
-                        c[t][b] = start;
-                        if constexpr (kZeros) {
-                            const float zero = 16.0f + static_cast<float>(s.zero[t][f]);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) c[t][b][i] *= zero;
-                        }
+            for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
+
+            lds_barrier();  // nobody reads the rows and routes that were there
+            if (!listed) {
+                if (wave == 0) {
+                    int held = 0;
+                    for (int base = 0; base < p.routes; base += kWave) {
+                        const bool hit = base + lane < p.routes && expert_of[base + lane] == expert;
+                        const unsigned long long mask = __ballot(hit);
+                        if (hit) my_routes[held + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(base + lane);
+                        held += __popcll(mask);
                     }
+                    if (lane == 0) my_count = held * (kKind == kDown ? 2 : 1);
                 }
+                lds_barrier();
+                count = __builtin_amdgcn_readfirstlane(my_count);
+                listed = true;
+            }
+            const int rows = min(count - first_row, p.row_cap), padded = (rows + kRows - 1) / kRows * kRows;
+            unsigned char* const x_lds = lds;
+            float* const sums_lds = reinterpret_cast<float*>(lds + x_bytes(p.units, p.row_cap, kRows));
+
+            // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.
+            for (int i = tid; i < rows * p.units * 8; i += kThreads) {
+                const int m = i / (p.units * 8), c32 = i - m * (p.units * 8);
+                const int which = first_row + m;
+                const uint16_t* from;
+                if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
+                else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
+                else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
+                float sum = 0.0f;
+                const bool real = c32 < p.k / 32;
+                unsigned char* const to = x_lds + static_cast<size_t>((((c32 >> 2) * 4) * 4 + (c32 & 3)) * rows + m) * 16;
+                u32x4 octets[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) octets[j] = load16(from + (real ? c32 * 32 : 0) + j * 8);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const unsigned char* const from = own ? x_lds + (part * 4 + j) * 4 * rows * 16 + x_lane : reinterpret_cast<const unsigned char*>(zero16);
-                    u32x4 q[kTiles];
+                    const u32x4 v = real ? octets[j] : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-                    for (int t = 0; t < kTiles; ++t) q[t] = unpack<kHalfRows>(w[f][t][j]);
+                    for (int d = 0; d < 4; ++d) sum += widen(v[d] & 0xffffu, kHalfRows) + widen(v[d] >> 16, kHalfRows);
+                    const u32x4 pairs = {(v[0] & 0xffffu) | (v[2] << 16), (v[0] >> 16) | (v[2] & 0xffff0000u), (v[1] & 0xffffu) | (v[3] << 16),
+                                         (v[1] >> 16) | (v[3] & 0xffff0000u)};
+                    *reinterpret_cast<u32x4*>(to + static_cast<size_t>(j * 4 * rows) * 16) = pairs;
+                }
+                if constexpr (kDiag < 4) sum += __shfl_xor(sum, 1);
+                if constexpr (kDiag < 2) sum += __shfl_xor(sum, 2);
+                if ((c32 & (4 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(c32 / (4 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
+            }
+            lds_barrier();
+
+            f32x4 acc[kTiles][kBlocks] = {};
+            const int x_lane = own ? (chunk * rows + min(col % kTokens, rows - 1)) * 16 : 0;
+            auto consume = [&](const Slot& s, int u) {
+                u32x4 w[2][kTiles];
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        w[0][t][d] = __builtin_amdgcn_update_dpp(s.low[t][d], s.high[t][d], 0x128, 0xf, 0xc, false);
+                        w[1][t][d] = __builtin_amdgcn_update_dpp(s.high[t][d], s.low[t][d], 0x128, 0xf, 0x3, false);
+                    }
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    const int part = u * 2 + f;
+                    f32x4 c[kTiles][kBlocks];
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b) {
-                        const u32x4 a = *reinterpret_cast<const u32x4*>(from + (own ? b * kTokens * 16 : 0));
+                        const int sub = kDiag == 1 ? 0 : chunk / (4 / kDiag), token = (kDiag == 1 ? chunk * 4 : kDiag == 2 ? (chunk & 1) * 4 : 0) + b * kTokens;
+                        const f32x4 start = *reinterpret_cast<const f32x4*>(sums_lds + static_cast<size_t>(part * kDiag + sub) * padded + token);
 #pragma unroll
-                        for (int t = 0; t < kTiles; ++t) c[t][b] = multiply<kHalfRows>(a, q[t], c[t][b]);
+                        for (int t = 0; t < kTiles; ++t) {
+                            c[t][b] = start;
+                            if constexpr (kZeros) {
+                                const float zero = 16.0f + static_cast<float>(s.zero[t][f]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) c[t][b][i] *= zero;
+                            }
+                        }
                     }
-                }
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t) {
-                    const float scale = widen(s.scale[t][f], kHalf);
+                    for (int j = 0; j < 4; ++j) {
+                        const unsigned char* const from = own ? x_lds + (part * 4 + j) * 4 * rows * 16 + x_lane : reinterpret_cast<const unsigned char*>(zero16);
+                        u32x4 q[kTiles];
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) q[t] = codes.unpack(w[f][t][j]);
+#pragma unroll
+                        for (int b = 0; b < kBlocks; ++b) {
+                            const u32x4 a = *reinterpret_cast<const u32x4*>(from + (own ? b * kTokens * 16 : 0));
+#pragma unroll
+                            for (int t = 0; t < kTiles; ++t) c[t][b] = multiply<kHalfRows>(a, q[t], c[t][b]);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        const float scale = widen(s.scale[t][f], kHalf);
+#pragma unroll
+                        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[t][b][i] = fmaf(scale, c[t][b][i], acc[t][b][i]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // (the other half's operands would be fetched here, and cost registers)
+                }
+            };
+
+            // Sum of a result over the waves that share its tile and, for short groups, over the lanes that hold its groups.
+            auto result = [&](int group, int tile, int m, int n) {
+                const int b = m / kTokens, token = m % kTokens;
+                float sum = 0.0f;
+                for (int w = 0; w < split; ++w)
+#pragma unroll
+                    for (int d = 0; d < kDiag; ++d) {
+                        const int from = kDiag == 1 ? token / 4 : kDiag == 2 ? token / 4 + 2 * d : d;
+                        sum += results[group * split + w][tile][b][token % 4][from * 16 + n];
+                    }
+                return sum;
+            };
+            auto finish = [&](int at_step) {
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[t][b][i] = fmaf(scale, c[t][b][i], acc[t][b][i]);
-                }
-                __builtin_amdgcn_sched_barrier(0);  // (the other half's operands would be fetched here, and cost registers)
-            }
-        };
-
-        // Sum of a result over the waves that share its tile and, for short groups, over the lanes that hold its groups.
-        auto result = [&](int group, int tile, int m, int n) {
-            const int b = m / kTokens, token = m % kTokens;
-            float sum = 0.0f;
-            for (int w = 0; w < split; ++w)
-#pragma unroll
-                for (int d = 0; d < kDiag; ++d) {
-                    const int from = kDiag == 1 ? token / 4 : kDiag == 2 ? token / 4 + 2 * d : d;
-                    sum += results[group * split + w][tile][b][token % 4][from * 16 + n];
-                }
-            return sum;
-        };
-        auto finish = [&](int done) {  // tile groups number `done` of this workgroup's waves
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        results[wave][t][b][i][lane] = acc[t][b][i];
-                        acc[t][b][i] = 0.0f;
+                        for (int i = 0; i < 4; ++i) {
+                            results[wave][t][b][i][lane] = acc[t][b][i];
+                            acc[t][b][i] = 0.0f;
+                        }
+                lds_barrier();
+                constexpr int kOut = kKind == kGateUp ? 1 : kTiles;  // result tiles of a tile group
+                const int outputs = lanes_of_groups * kOut * 16 * (kKind == kDown ? rows / 2 : rows);
+                for (int o = tid; o < outputs; o += kThreads) {
+                    const int n = o & 15, tile = (o >> 4) % kOut, rest = (o >> 4) / kOut, group = rest % lanes_of_groups, m = rest / lanes_of_groups;
+                    const int g = at_step * lanes_of_groups + group;
+                    const int to = tile_row(g, tile) + n;
+                    if (g >= p.tile_groups || to >= matrix_rows) continue;
+                    if constexpr (kKind == kMatvec) {
+                        static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(result(group, tile, m, n), kHalf);
+                    } else if constexpr (kKind == kGateUp) {
+                        const float gate = result(group, 0, m, n), up = result(group, 1, m, n);
+                        const int route = my_routes[first_row + m];
+                        // The route's weight is folded in here.  Two BF16 numbers hold the product's high and low part, together 16 bits of mantissa.
+                        const float h = gate / (1.0f + expf(-gate)) * up * route_weights[route];
+                        const uint32_t high = f32_to_bf16(h);
+                        uint16_t* const row = static_cast<uint16_t*>(p.out) + static_cast<size_t>(route) * 2 * matrix_rows + to;
+                        row[0] = static_cast<uint16_t>(high);
+                        row[matrix_rows] = static_cast<uint16_t>(f32_to_bf16(h - bf16_to_f32(high)));
+                    } else {
+                        const int route = my_routes[(first_row >> 1) + m];
+                        static_cast<float*>(p.out)[static_cast<size_t>(route) * p.n + to] = result(group, tile, 2 * m, n) + result(group, tile, 2 * m + 1, n);
                     }
-            lds_barrier();
-            constexpr int kOut = kKind == kGateUp ? 1 : kTiles;  // result tiles of a tile group
-            const int outputs = lanes_of_groups * kOut * 16 * (kKind == kDown ? rows / 2 : rows);
-            for (int o = tid; o < outputs; o += kThreads) {
-                const int n = o & 15, tile = (o >> 4) % kOut, rest = (o >> 4) / kOut, group = rest % lanes_of_groups, m = rest / lanes_of_groups;
-                const int g = blockIdx.x * p.per * lanes_of_groups + done * lanes_of_groups + group;
-                const int to = tile_row(g, tile) + n;
-                if (g >= p.tile_groups || to >= matrix_rows) continue;
-                if constexpr (kKind == kMatvec) {
-                    static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(result(group, tile, m, n), kHalf);
-                } else if constexpr (kKind == kGateUp) {
-                    const float gate = result(group, 0, m, n), up = result(group, 1, m, n);
-                    const int route = my_routes[first_row + m];
-                    // The route's weight is folded in here.  Two BF16 numbers hold the product's high and low part, together 16 bits of mantissa.
-                    const float h = gate / (1.0f + expf(-gate)) * up * my_weights[first_row + m];
-                    const uint32_t high = f32_to_bf16(h);
-                    uint16_t* const row = static_cast<uint16_t*>(p.out) + static_cast<size_t>(route) * 2 * matrix_rows + to;
-                    row[0] = static_cast<uint16_t>(high);
-                    row[matrix_rows] = static_cast<uint16_t>(f32_to_bf16(h - bf16_to_f32(high)));
-                } else {
-                    const int route = my_routes[(first_row >> 1) + m];
-                    static_cast<float*>(p.out)[static_cast<size_t>(route) * p.n + to] = result(group, tile, 2 * m, n) + result(group, tile, 2 * m + 1, n);
                 }
-            }
-            lds_barrier();
-        };
+                lds_barrier();
+            };
 
-        int unit = first_unit, done = 0;
-        while (done < p.per) {
+            int unit = first_unit, at_step = first_step;
+            while (at_step < first_step + steps) {
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                if (done >= p.per) break;
-                consume(ring[i], unit);
-                load_next(ring[i]);
-                if (++unit == last_unit) {
-                    unit = first_unit;
-                    finish(done++);
+                for (int i = 0; i < kAhead; ++i) {
+                    if (at_step >= first_step + steps) break;
+                    consume(ring[i], unit);
+                    load_next(ring[i]);
+                    if (++unit == last_unit) {
+                        unit = first_unit;
+                        finish(at_step++);
+                    }
                 }
             }
-        }
+            first_row += rows;
+        } while (first_row < count);
     }
 }
 
@@ -383,29 +418,29 @@ __global__ __launch_bounds__(256) void sum_routes_kernel(const float* rows, cons
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------
-constexpr int kLdsBytes = 48 << 10;  // of a workgroup's rows and sums, so that two share a CU
-
 template <Kind kKind>
-int launch_product(Product p, int type, int slots, int rows_expected, int rows_most, hipStream_t stream)
+int launch_product(Product p, int type, int matrices_most, int rows_expected, int rows_most, hipStream_t stream)
 {
     p.units = (p.k + kUnit - 1) / kUnit;
     p.groups = p.k / p.group;
     const int diag = p.group >= 128 ? 1 : 128 / p.group;
     p.group_inverse = diag == 1 ? ((1 << 20) + p.group / 128 - 1) / (p.group / 128) : 0;
+    const int tiles = kKind == kMatvec ? 1 : 2, counted = kKind == kGateUp ? p.n / 2 : (p.n + tiles - 1) / tiles;
+    p.tile_groups = (counted + 15) / 16;
     p.split = 1;
     while (p.split < kWaves && p.split * 2 * 3 <= p.units) p.split *= 2;
-    const int counted = kKind == kGateUp ? p.n / 2 : (p.n + 1) / 2;
-    p.tile_groups = (counted + 15) / 16;
-    const int at_once = kWaves / p.split, steps = (p.tile_groups + at_once - 1) / at_once;
-    p.per = std::max(1, std::min(8, steps * slots / 1024));
-    const int tokens = 16 / diag, blocks = std::min(4, std::max(1, (rows_expected + tokens - 1) / tokens));
-    const int by_blocks = blocks <= 1 ? 1 : 4, most = tokens * by_blocks;
+    const int at_once = kWaves / p.split;
+    p.steps = (p.tile_groups + at_once - 1) / at_once;
+    const int tokens = 16 / diag, by_blocks = rows_expected <= tokens ? 1 : 4, most = tokens * by_blocks;
+    // Two workgroups share a CU's 160 KiB where one block of rows will do.
+    const int limit = by_blocks == 1 ? 46 << 10 : kKind == kMatvec ? 120 << 10 : 72 << 10;
     int rows = std::min(rows_most, most);
-    while (rows > (kKind == kDown ? 2 : 1) && x_bytes(p.units, rows, most) + sum_bytes(p.units, diag, most) > kLdsBytes) --rows;
+    while (rows > (kKind == kDown ? 2 : 1) && x_bytes(p.units, rows, most) + sum_bytes(p.units, diag, most) > limit) --rows;
     if (kKind == kDown) rows &= ~1;
     p.row_cap = rows;
     const int bytes = x_bytes(p.units, rows, most) + sum_bytes(p.units, diag, most);
-    const dim3 grid((steps + p.per - 1) / p.per, slots);
+    const int matrices = kKind == kMatvec ? (p.rows + rows - 1) / rows : matrices_most;
+    const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(matrices) * p.steps, by_blocks == 1 ? 512 : 256));
     int status = DPEP_OK;
     auto go = [&](auto half, auto zeros, auto d, auto b) {
         const auto kernel = product_kernel<kKind, half(), zeros(), d(), b()>;
