@@ -106,9 +106,23 @@ __device__ __forceinline__ void lds_barrier()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Sizes of a launch's LDS: the rows in the MFMA's order, their groups' sums, the waves' results.
-__host__ __device__ inline int x_bytes(int units, int rows, int padded) { return (units * 32 * rows + padded) * 16; }  // (a short block of rows reads on)
-__host__ __device__ inline int sum_bytes(int units, int diag, int padded) { return units * 2 * diag * padded * 4; }
+// A launch's LDS: the rows in the MFMA's order, their groups' sums, the waves' results, what is kept of the routes.  Rows come in fours (the rows of
+// one lane's results); what lies behind the last is read and not used.
+struct LdsPlan {
+    int sums, results, counts, routes, weights, bytes;
+    int lanes;  // of a wave that hold results of these rows
+    __host__ __device__ LdsPlan(int units, int diag, int blocks, int tiles, int rows, int experts, int num_routes, bool weighted)
+    {
+        const int fours = (rows + 3) / 4, tokens = 16 / diag;
+        lanes = diag == 1 && blocks == 1 ? fours * 16 : kWave;
+        sums = (units * 32 * rows + tokens * blocks) * 16;
+        results = sums + units * 2 * diag * fours * 16 + tokens * blocks * 4;
+        counts = results + kWaves * tiles * blocks * 4 * lanes * 4;
+        routes = counts + (experts + 63) / 64 * 256;
+        weights = routes + (num_routes + 3) / 4 * 16;  // (an expert each, and a list of those of one expert)
+        bytes = weights + (weighted ? (num_routes + 3) / 4 * 16 : 0);
+    }
+};
 
 // A workgroup takes an even share of all steps: of the matrices that have rows one after the other (matvec: of the passes over the rows), each
 // with the rows it multiplies in LDS.
@@ -118,47 +132,52 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
     constexpr bool kHalfRows = kHalf && kKind != kDown;  // the down product's rows are BF16 pairs whatever the type
     constexpr int kTiles = kKind == kMatvec ? 1 : 2;     // tiles of 16 rows of W to a tile group; gate_up: a gate tile and its up tile
     constexpr int kAhead = kKind == kMatvec ? 4 : 2;     // units in flight
-    constexpr int kTokens = 16 / kDiag, kRows = kTokens * kBlocks;
-    constexpr int kRouteSlots = kKind == kMatvec ? 1 : kMaxRoutes;
+    constexpr int kTokens = 16 / kDiag;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    __shared__ uint32_t experts_hit[DPEP_MAX_LOCAL_EXPERTS / 32];
-    __shared__ int16_t expert_of[kRouteSlots];
-    __shared__ uint16_t my_routes[kRouteSlots];
-    __shared__ float route_weights[kKind == kGateUp ? kMaxRoutes : 1];
-    __shared__ int my_count;
     __shared__ __attribute__((aligned(16))) uint32_t zero16[4];
-    __shared__ float results[kWaves][kTiles][kBlocks][4][kWave];
+    const int experts = kKind == kMatvec ? 0 : p.ids.local;
+    const LdsPlan plan(p.units, kDiag, kBlocks, kTiles, p.row_cap, experts, p.routes, kKind == kGateUp);
+    unsigned char* const x_lds = lds;
+    float* const sums_lds = reinterpret_cast<float*>(lds + plan.sums);
+    float* const results = reinterpret_cast<float*>(lds + plan.results);  // [wave][tile][block][four of a lane][lane]
+    int* const counts = reinterpret_cast<int*>(lds + plan.counts);
+    int16_t* const expert_of = reinterpret_cast<int16_t*>(lds + plan.routes);
+    uint16_t* const my_routes = reinterpret_cast<uint16_t*>(expert_of) + p.routes;
+    float* const route_weights = reinterpret_cast<float*>(lds + plan.weights);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, chunk = lane >> 4;
     if (tid < 4) zero16[tid] = 0;
-    uint32_t hit_word = 0;  // lane l: which of experts 32 l .. 32 l + 31 have a route
-    int hit_before = 0, matrices = 0;
+    // Passes of row_cap rows: matvec's, or each expert's; lane l counts those of experts l * per_lane and on.
+    const int per_lane = (experts + kWave - 1) / kWave;
+    int passes = 0, passes_before = 0, matrices = 0;
     if constexpr (kKind == kMatvec) {
         matrices = (p.rows + p.row_cap - 1) / p.row_cap;
     } else {
-        if (tid < DPEP_MAX_LOCAL_EXPERTS / 32) experts_hit[tid] = 0;
+        for (int e = tid; e < per_lane * kWave; e += kThreads) counts[e] = 0;
         __syncthreads();
         for (int i = tid; i < p.routes; i += kThreads) {
             const int e = p.ids[i];
             if constexpr (kKind == kGateUp) route_weights[i] = p.route_weights[i];
             expert_of[i] = static_cast<int16_t>(e);
-            if (e >= 0) atomicOr(&experts_hit[e >> 5], 1u << (e & 31));
+            if (e >= 0) atomicAdd(&counts[e], kKind == kDown ? 2 : 1);
         }
         __syncthreads();
-        hit_word = lane < DPEP_MAX_LOCAL_EXPERTS / 32 ? experts_hit[lane] : 0;
-        const int until = wave_scan(__popc(hit_word));
-        hit_before = until - __popc(hit_word);
+        for (int i = 0; i < per_lane; ++i) passes += (counts[lane * per_lane + i] + p.row_cap - 1) / p.row_cap;
+        const int until = wave_scan(passes);
+        passes_before = until - passes;
         matrices = __builtin_amdgcn_readlane(until, 63);
     }
     const int all_steps = matrices * p.steps;
-    int step = static_cast<int>(static_cast<long long>(all_steps) * blockIdx.x / gridDim.x);
-    const int end_step = static_cast<int>(static_cast<long long>(all_steps) * (blockIdx.x + 1) / gridDim.x);
+    const int even = all_steps / static_cast<int>(gridDim.x), over = all_steps - even * static_cast<int>(gridDim.x), block = blockIdx.x;
+    int step = block * even + min(block, over);
+    const int end_step = step + even + (block < over ? 1 : 0);
 
     // What this wave streams: units first_unit .. last_unit - 1 of its tile groups.
     const int split = p.split, lanes_of_groups = kWaves / split;
     const int share = wave & (split - 1), mine = wave / split;
     const int first_unit = p.units * share / split, last_unit = p.units * (share + 1) / split;
+    const int slots = ((p.units + split - 1) / split + kAhead - 1) / kAhead * kAhead;  // to a step, the same for all waves
     const int matrix_rows = kKind == kGateUp ? p.n / 2 : p.n;  // among which tiles are counted
     const int half_k = p.k / 2;
     // (a matrix of fewer than 16 rows: lanes past its end load its last row; the last tile of others is moved up to end with the matrix)
@@ -178,16 +197,19 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
     while (step < end_step) {
         const int matrix = step / p.steps, first_step = step - matrix * p.steps, steps = min(p.steps - first_step, end_step - step);
         step += steps;
-        int expert = 0, count = p.rows, first_row = 0;
-        if constexpr (kKind == kMatvec) {
-            first_row = matrix * p.row_cap;
-            count = min(p.rows, first_row + p.row_cap);
-        } else {
-            // The matrix-th of the experts that have a route, and its routes in order.
-            const int at = __ffsll(__ballot(matrix >= hit_before && matrix < hit_before + __popc(hit_word))) - 1;
-            uint32_t word = __builtin_amdgcn_readlane(hit_word, at);
-            for (int skip = matrix - __builtin_amdgcn_readlane(hit_before, at); skip > 0; --skip) word &= word - 1;
-            expert = __builtin_amdgcn_readfirstlane(at * 32 + __ffs(word) - 1);
+        int expert = 0, count = p.rows, first_row = matrix * p.row_cap;
+        if constexpr (kKind != kMatvec) {
+            // The expert of the matrix-th pass, and which of its passes that is.
+            const int at = __ffsll(__ballot(matrix >= passes_before && matrix < passes_before + passes)) - 1;
+            int skip = matrix - __builtin_amdgcn_readlane(passes_before, at);
+            expert = at * per_lane;
+            for (;; ++expert) {
+                count = __builtin_amdgcn_readfirstlane(counts[expert]);
+                const int here = (count + p.row_cap - 1) / p.row_cap;
+                if (skip < here) break;
+                skip -= here;
+            }
+            first_row = skip * p.row_cap;
         }
         const uint8_t* const packed = p.packed + static_cast<size_t>(expert) * p.n * half_k;
         const uint16_t* const scales = p.scales + static_cast<size_t>(expert) * p.n * p.groups;
@@ -197,14 +219,17 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
             u32x4 low[kTiles], high[kTiles];
             uint32_t scale[kTiles][2], zero[kTiles][2];
         };
-        auto load = [&](Slot& s, int g, int u) {
+        // (real = false: a slot that nobody consumes, filled all the same from one place, so that the loads in flight can be counted)
+        auto load = [&](Slot& s, int g, int u, bool real) {
+            asm volatile("" : "+s"(u));  // (as below)
             const uint32_t at = (u == p.units - 1 ? tail_chunk : loaded_chunk) * 16;
+            const uint32_t low = real ? row_low + at : 0, high = real ? row_high + at : 0;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) {
                 const int row = tile_row(g, t);
                 const uint8_t* const base = packed + static_cast<size_t>(row) * half_k + u * (kUnit / 2);
-                s.low[t] = load16_nt(base + (row_low + at));
-                s.high[t] = load16_nt(base + (row_high + at));
+                s.low[t] = load16_nt(base + low);
+                s.high[t] = load16_nt(base + high);
                 const size_t first_scale = static_cast<size_t>(row) * p.groups;
 #pragma unroll
                 for (int f = 0; f < 2; ++f) {
@@ -218,188 +243,177 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
             }
         };
 
-        bool listed = kKind == kMatvec;
-        do {
-            Slot ring[kAhead];
-            int load_step = first_step, load_unit = first_unit;
-            asm volatile("" : "+s"(load_step), "+s"(load_unit));  // (or every pass's first addresses are kept in registers all along)
-            auto load_next = [&](Slot& s) {
-                load(s, load_step * lanes_of_groups + mine, load_unit);
-                if (++load_unit == last_unit) {
-                    load_unit = first_unit;
-                    load_step = min(load_step + 1, first_step + steps - 1);
-                }
-            };
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
-
-            lds_barrier();  // nobody reads the rows and routes that were there
-            if (!listed) {
-                if (wave == 0) {
-                    int held = 0;
-                    for (int base = 0; base < p.routes; base += kWave) {
-                        const bool hit = base + lane < p.routes && expert_of[base + lane] == expert;
-                        const unsigned long long mask = __ballot(hit);
-                        if (hit) my_routes[held + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(base + lane);
-                        held += __popcll(mask);
-                    }
-                    if (lane == 0) my_count = held * (kKind == kDown ? 2 : 1);
-                }
-                lds_barrier();
-                count = __builtin_amdgcn_readfirstlane(my_count);
-                listed = true;
+        Slot ring[kAhead];
+        int load_step = first_step, load_slot = 0;
+        auto load_next = [&](Slot& s) {
+            const int u = first_unit + load_slot;
+            load(s, load_step * lanes_of_groups + mine, min(u, last_unit - 1), u < last_unit);
+            if (++load_slot == slots) {
+                load_slot = 0;
+                load_step = min(load_step + 1, first_step + steps - 1);
             }
-            const int rows = min(count - first_row, p.row_cap), padded = (rows + kRows - 1) / kRows * kRows;
-            unsigned char* const x_lds = lds;
-            float* const sums_lds = reinterpret_cast<float*>(lds + x_bytes(p.units, p.row_cap, kRows));
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
 
-            // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.
-            for (int i = tid; i < rows * p.units * 8; i += kThreads) {
-                const int m = i / (p.units * 8), c32 = i - m * (p.units * 8);
-                const int which = first_row + m;
-                const uint16_t* from;
-                if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
-                else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
-                else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
-                float sum = 0.0f;
-                const bool real = c32 < p.k / 32;
-                unsigned char* const to = x_lds + static_cast<size_t>((((c32 >> 2) * 4) * 4 + (c32 & 3)) * rows + m) * 16;
-                u32x4 octets[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) octets[j] = load16(from + (real ? c32 * 32 : 0) + j * 8);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const u32x4 v = real ? octets[j] : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) sum += widen(v[d] & 0xffffu, kHalfRows) + widen(v[d] >> 16, kHalfRows);
-                    const u32x4 pairs = {(v[0] & 0xffffu) | (v[2] << 16), (v[0] >> 16) | (v[2] & 0xffff0000u), (v[1] & 0xffffu) | (v[3] << 16),
-                                         (v[1] >> 16) | (v[3] & 0xffff0000u)};
-                    *reinterpret_cast<u32x4*>(to + static_cast<size_t>(j * 4 * rows) * 16) = pairs;
+        lds_barrier();  // nobody reads the rows and routes that were there
+        if constexpr (kKind != kMatvec) {
+            if (wave == 0) {
+                int held = 0;
+                for (int base = 0; base < p.routes; base += kWave) {
+                    const bool hit = base + lane < p.routes && expert_of[base + lane] == expert;
+                    const unsigned long long mask = __ballot(hit);
+                    if (hit) my_routes[held + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(base + lane);
+                    held += __popcll(mask);
                 }
-                if constexpr (kDiag < 4) sum += __shfl_xor(sum, 1);
-                if constexpr (kDiag < 2) sum += __shfl_xor(sum, 2);
-                if ((c32 & (4 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(c32 / (4 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
             }
             lds_barrier();
+        }
+        const int rows = min(count - first_row, p.row_cap), padded = (rows + 3) & ~3;
 
-            f32x4 acc[kTiles][kBlocks] = {};
-            const int x_lane = own ? (chunk * rows + min(col % kTokens, rows - 1)) * 16 : 0;
-            auto consume = [&](const Slot& s, int u) {
-                u32x4 w[2][kTiles];
+        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.
+        for (int i = tid; i < rows * p.units * 8; i += kThreads) {
+            const int m = i / (p.units * 8), c32 = i - m * (p.units * 8);
+            const int which = first_row + m;
+            const uint16_t* from;
+            if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
+            else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
+            else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
+            float sum = 0.0f;
+            const bool real = c32 < p.k / 32;
+            unsigned char* const to = x_lds + static_cast<size_t>((((c32 >> 2) * 4) * 4 + (c32 & 3)) * rows + m) * 16;
+            u32x4 octets[4];
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t)
+            for (int j = 0; j < 4; ++j) octets[j] = load16(from + (real ? c32 * 32 : 0) + j * 8);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        w[0][t][d] = __builtin_amdgcn_update_dpp(s.low[t][d], s.high[t][d], 0x128, 0xf, 0xc, false);
-                        w[1][t][d] = __builtin_amdgcn_update_dpp(s.high[t][d], s.low[t][d], 0x128, 0xf, 0x3, false);
-                    }
+            for (int j = 0; j < 4; ++j) {
+                const u32x4 v = real ? octets[j] : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    const int part = u * 2 + f;
-                    f32x4 c[kTiles][kBlocks];
+                for (int d = 0; d < 4; ++d) sum += widen(v[d] & 0xffffu, kHalfRows) + widen(v[d] >> 16, kHalfRows);
+                const u32x4 pairs = {(v[0] & 0xffffu) | (v[2] << 16), (v[0] >> 16) | (v[2] & 0xffff0000u), (v[1] & 0xffffu) | (v[3] << 16),
+                                     (v[1] >> 16) | (v[3] & 0xffff0000u)};
+                *reinterpret_cast<u32x4*>(to + static_cast<size_t>(j * 4 * rows) * 16) = pairs;
+            }
+            if constexpr (kDiag < 4) sum += __shfl_xor(sum, 1);
+            if constexpr (kDiag < 2) sum += __shfl_xor(sum, 2);
+            if ((c32 & (4 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(c32 / (4 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
+        }
+        lds_barrier();
+
+        f32x4 acc[kTiles][kBlocks] = {};
+        const int x_lane = own ? (chunk * rows + min(col % kTokens, rows - 1)) * 16 : 0;
+        auto consume = [&](const Slot& s, int u) {
+            asm volatile("" : "+s"(u));  // (or each of its LDS addresses becomes an induction variable in a register)
+            u32x4 w[2][kTiles];
 #pragma unroll
-                    for (int b = 0; b < kBlocks; ++b) {
-                        const int sub = kDiag == 1 ? 0 : chunk / (4 / kDiag), token = (kDiag == 1 ? chunk * 4 : kDiag == 2 ? (chunk & 1) * 4 : 0) + b * kTokens;
-                        const f32x4 start = *reinterpret_cast<const f32x4*>(sums_lds + static_cast<size_t>(part * kDiag + sub) * padded + token);
+            for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                        for (int t = 0; t < kTiles; ++t) {
-                            c[t][b] = start;
-                            if constexpr (kZeros) {
-                                const float zero = 16.0f + static_cast<float>(s.zero[t][f]);
+                for (int d = 0; d < 4; ++d) {
+                    w[0][t][d] = __builtin_amdgcn_update_dpp(s.low[t][d], s.high[t][d], 0x128, 0xf, 0xc, false);
+                    w[1][t][d] = __builtin_amdgcn_update_dpp(s.high[t][d], s.low[t][d], 0x128, 0xf, 0x3, false);
+                }
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) c[t][b][i] *= zero;
-                            }
-                        }
-                    }
+            for (int f = 0; f < 2; ++f) {
+                const int part = u * 2 + f;
+                f32x4 c[kTiles][kBlocks];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const unsigned char* const from = own ? x_lds + (part * 4 + j) * 4 * rows * 16 + x_lane : reinterpret_cast<const unsigned char*>(zero16);
-                        u32x4 q[kTiles];
-#pragma unroll
-                        for (int t = 0; t < kTiles; ++t) q[t] = codes.unpack(w[f][t][j]);
-#pragma unroll
-                        for (int b = 0; b < kBlocks; ++b) {
-                            const u32x4 a = *reinterpret_cast<const u32x4*>(from + (own ? b * kTokens * 16 : 0));
-#pragma unroll
-                            for (int t = 0; t < kTiles; ++t) c[t][b] = multiply<kHalfRows>(a, q[t], c[t][b]);
-                        }
-                    }
+                for (int b = 0; b < kBlocks; ++b) {
+                    const int sub = kDiag == 1 ? 0 : chunk / (4 / kDiag), token = (kDiag == 1 ? chunk * 4 : kDiag == 2 ? (chunk & 1) * 4 : 0) + b * kTokens;
+                    const f32x4 start = *reinterpret_cast<const f32x4*>(sums_lds + static_cast<size_t>(part * kDiag + sub) * padded + token);
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
-                        const float scale = widen(s.scale[t][f], kHalf);
+                        c[t][b] = start;
+                        if constexpr (kZeros) {
+                            const float zero = 16.0f + static_cast<float>(s.zero[t][f]);
 #pragma unroll
-                        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[t][b][i] = fmaf(scale, c[t][b][i], acc[t][b][i]);
+                            for (int i = 0; i < 4; ++i) c[t][b][i] *= zero;
+                        }
                     }
-                    __builtin_amdgcn_sched_barrier(0);  // (the other half's operands would be fetched here, and cost registers)
                 }
-            };
-
-            // Sum of a result over the waves that share its tile and, for short groups, over the lanes that hold its groups.
-            auto result = [&](int group, int tile, int m, int n) {
-                const int b = m / kTokens, token = m % kTokens;
-                float sum = 0.0f;
-                for (int w = 0; w < split; ++w)
 #pragma unroll
-                    for (int d = 0; d < kDiag; ++d) {
-                        const int from = kDiag == 1 ? token / 4 : kDiag == 2 ? token / 4 + 2 * d : d;
-                        sum += results[group * split + w][tile][b][token % 4][from * 16 + n];
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned char* const from = own ? x_lds + (part * 4 + j) * 4 * rows * 16 + x_lane : reinterpret_cast<const unsigned char*>(zero16);
+                    u32x4 q[kTiles];
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) q[t] = codes.unpack(w[f][t][j]);
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        const u32x4 a = *reinterpret_cast<const u32x4*>(from + (own ? b * kTokens * 16 : 0));
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) c[t][b] = multiply<kHalfRows>(a, q[t], c[t][b]);
                     }
-                return sum;
-            };
-            auto finish = [&](int at_step) {
+                }
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t)
+                for (int t = 0; t < kTiles; ++t) {
+                    const float scale = widen(s.scale[t][f], kHalf);
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            results[wave][t][b][i][lane] = acc[t][b][i];
-                            acc[t][b][i] = 0.0f;
-                        }
-                lds_barrier();
-                constexpr int kOut = kKind == kGateUp ? 1 : kTiles;  // result tiles of a tile group
-                const int outputs = lanes_of_groups * kOut * 16 * (kKind == kDown ? rows / 2 : rows);
-                for (int o = tid; o < outputs; o += kThreads) {
-                    const int n = o & 15, tile = (o >> 4) % kOut, rest = (o >> 4) / kOut, group = rest % lanes_of_groups, m = rest / lanes_of_groups;
-                    const int g = at_step * lanes_of_groups + group;
-                    const int to = tile_row(g, tile) + n;
-                    if (g >= p.tile_groups || to >= matrix_rows) continue;
-                    if constexpr (kKind == kMatvec) {
-                        static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(result(group, tile, m, n), kHalf);
-                    } else if constexpr (kKind == kGateUp) {
-                        const float gate = result(group, 0, m, n), up = result(group, 1, m, n);
-                        const int route = my_routes[first_row + m];
-                        // The route's weight is folded in here.  Two BF16 numbers hold the product's high and low part, together 16 bits of mantissa.
-                        const float h = gate / (1.0f + expf(-gate)) * up * route_weights[route];
-                        const uint32_t high = f32_to_bf16(h);
-                        uint16_t* const row = static_cast<uint16_t*>(p.out) + static_cast<size_t>(route) * 2 * matrix_rows + to;
-                        row[0] = static_cast<uint16_t>(high);
-                        row[matrix_rows] = static_cast<uint16_t>(f32_to_bf16(h - bf16_to_f32(high)));
-                    } else {
-                        const int route = my_routes[(first_row >> 1) + m];
-                        static_cast<float*>(p.out)[static_cast<size_t>(route) * p.n + to] = result(group, tile, 2 * m, n) + result(group, tile, 2 * m + 1, n);
-                    }
+                        for (int i = 0; i < 4; ++i) acc[t][b][i] = fmaf(scale, c[t][b][i], acc[t][b][i]);
                 }
-                lds_barrier();
-            };
+                __builtin_amdgcn_sched_barrier(0);  // (the other half's operands would be fetched here, and cost registers)
+            }
+        };
 
-            int unit = first_unit, at_step = first_step;
-            while (at_step < first_step + steps) {
+        // Sum of a result over the waves that share its tile and, for short groups, over the lanes that hold its groups.
+        auto result = [&](int group, int tile, int m, int n) {
+            const int b = m / kTokens, token = m % kTokens;
+            float sum = 0.0f;
+            for (int w = 0; w < split; ++w)
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    if (at_step >= first_step + steps) break;
-                    consume(ring[i], unit);
-                    load_next(ring[i]);
-                    if (++unit == last_unit) {
-                        unit = first_unit;
-                        finish(at_step++);
+                for (int d = 0; d < kDiag; ++d) {
+                    const int from = kDiag == 1 ? token / 4 : kDiag == 2 ? token / 4 + 2 * d : d;
+                    sum += results[((((group * split + w) * kTiles + tile) * kBlocks + b) * 4 + token % 4) * plan.lanes + from * 16 + n];
+                }
+            return sum;
+        };
+        auto finish = [&](int at_step) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (lane < plan.lanes) results[(((wave * kTiles + t) * kBlocks + b) * 4 + i) * plan.lanes + lane] = acc[t][b][i];
+                        acc[t][b][i] = 0.0f;
                     }
+            lds_barrier();
+            constexpr int kOut = kKind == kGateUp ? 1 : kTiles;  // result tiles of a tile group
+            const int outputs = lanes_of_groups * kOut * 16 * (kKind == kDown ? rows / 2 : rows);
+            for (int o = tid; o < outputs; o += kThreads) {
+                const int n = o & 15, tile = (o >> 4) % kOut, rest = (o >> 4) / kOut, group = rest % lanes_of_groups, m = rest / lanes_of_groups;
+                const int g = at_step * lanes_of_groups + group;
+                const int to = tile_row(g, tile) + n;
+                if (g >= p.tile_groups || to >= matrix_rows) continue;
+                if constexpr (kKind == kMatvec) {
+                    static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(result(group, tile, m, n), kHalf);
+                } else if constexpr (kKind == kGateUp) {
+                    const float gate = result(group, 0, m, n), up = result(group, 1, m, n);
+                    const int route = my_routes[first_row + m];
+                    // The route's weight is folded in here.  Two BF16 numbers hold the product's high and low part, together 16 bits of mantissa.
+                    const float h = gate / (1.0f + expf(-gate)) * up * route_weights[route];
+                    const uint32_t high = f32_to_bf16(h);
+                    uint16_t* const row = static_cast<uint16_t*>(p.out) + static_cast<size_t>(route) * 2 * matrix_rows + to;
+                    row[0] = static_cast<uint16_t>(high);
+                    row[matrix_rows] = static_cast<uint16_t>(f32_to_bf16(h - bf16_to_f32(high)));
+                } else {
+                    const int route = my_routes[(first_row >> 1) + m];
+                    static_cast<float*>(p.out)[static_cast<size_t>(route) * p.n + to] = result(group, tile, 2 * m, n) + result(group, tile, 2 * m + 1, n);
                 }
             }
-            first_row += rows;
-        } while (first_row < count);
+            lds_barrier();
+        };
+
+        for (int at_step = first_step; at_step < first_step + steps; ++at_step) {
+            for (int slot = 0; slot < slots; slot += kAhead) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (first_unit + slot + i < last_unit) consume(ring[i], first_unit + slot + i);
+                    load_next(ring[i]);
+                }
+            }
+            finish(at_step);
+        }
     }
 }
 
@@ -433,12 +447,14 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     p.steps = (p.tile_groups + at_once - 1) / at_once;
     const int tokens = 16 / diag, by_blocks = rows_expected <= tokens ? 1 : 4, most = tokens * by_blocks;
     // Two workgroups share a CU's 160 KiB where one block of rows will do.
-    const int limit = by_blocks == 1 ? 46 << 10 : kKind == kMatvec ? 120 << 10 : 72 << 10;
+    const int limit = by_blocks == 1 ? 80 << 10 : 160 << 10;
+    const int experts = kKind == kMatvec ? 0 : p.ids.local;
+    auto plan = [&](int rows) { return LdsPlan(p.units, diag, by_blocks, tiles, rows, experts, p.routes, kKind == kGateUp).bytes + 64; };
     int rows = std::min(rows_most, most);
-    while (rows > (kKind == kDown ? 2 : 1) && x_bytes(p.units, rows, most) + sum_bytes(p.units, diag, most) > limit) --rows;
+    while (rows > (kKind == kDown ? 2 : 1) && plan(rows) > limit) --rows;
     if (kKind == kDown) rows &= ~1;
     p.row_cap = rows;
-    const int bytes = x_bytes(p.units, rows, most) + sum_bytes(p.units, diag, most);
+    const int bytes = plan(rows) - 64;
     const int matrices = kKind == kMatvec ? (p.rows + rows - 1) / rows : matrices_most;
     const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(matrices) * p.steps, by_blocks == 1 ? 512 : 256));
     int status = DPEP_OK;
