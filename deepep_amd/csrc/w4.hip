@@ -49,7 +49,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / kWave;
+constexpr int kWaves = kThreads / kWave, kLogWaves = 3;
 constexpr int kUnit = 256;  // values of k
 
 enum Kind { kMatvec, kGateUp, kDown };
@@ -62,9 +62,12 @@ struct Product {
     int n, k, group;    // of one matrix
     int units, groups;  // of a row
     int group_inverse;  // ceil(2^20 / (group / 128)), for groups of 128 and more
-    int split;          // waves that share a tile's k, a power of two
+    bool ragged;        // units and groups do not end together: a unit's scales may reach past their row
+    size_t all_scales;  // of all matrices
+    int split, log_split;  // waves that share a tile's k
     int tile_groups;    // of a matrix, kTiles tiles each
     int steps;          // a matrix in steps of a workgroup: kWaves / split tile groups at a time
+    int batch;          // steps whose results wait in LDS for one another
     int row_cap;        // rows of x held in LDS
     // rows: matvec: x [rows, k]; gate_up: x [token, k]; down: the routes' (high, low) rows [route][2][k]
     const uint16_t* x;
@@ -111,13 +114,13 @@ __device__ __forceinline__ void lds_barrier()
 struct LdsPlan {
     int sums, results, counts, routes, weights, bytes;
     int lanes;  // of a wave that hold results of these rows
-    __host__ __device__ LdsPlan(int units, int diag, int blocks, int tiles, int rows, int experts, int num_routes, bool weighted)
+    __host__ __device__ LdsPlan(int units, int diag, int blocks, int tiles, int rows, int batch, int experts, int num_routes, bool weighted)
     {
         const int fours = (rows + 3) / 4, tokens = 16 / diag;
         lanes = diag == 1 && blocks == 1 ? fours * 16 : kWave;
         sums = (units * 32 * rows + tokens * blocks) * 16;
         results = sums + units * 2 * diag * fours * 16 + tokens * blocks * 4;
-        counts = results + kWaves * tiles * blocks * 4 * lanes * 4;
+        counts = results + batch * kWaves * tiles * blocks * 4 * lanes * 4;
         routes = counts + (experts + 63) / 64 * 256;
         weights = routes + (num_routes + 3) / 4 * 16;  // (an expert each, and a list of those of one expert)
         bytes = weights + (weighted ? (num_routes + 3) / 4 * 16 : 0);
@@ -136,7 +139,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ __attribute__((aligned(16))) uint32_t zero16[4];
     const int experts = kKind == kMatvec ? 0 : p.ids.local;
-    const LdsPlan plan(p.units, kDiag, kBlocks, kTiles, p.row_cap, experts, p.routes, kKind == kGateUp);
+    const LdsPlan plan(p.units, kDiag, kBlocks, kTiles, p.row_cap, p.batch, experts, p.routes, kKind == kGateUp);
     unsigned char* const x_lds = lds;
     float* const sums_lds = reinterpret_cast<float*>(lds + plan.sums);
     float* const results = reinterpret_cast<float*>(lds + plan.results);  // [wave][tile][block][four of a lane][lane]
@@ -175,9 +178,11 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
 
     // What this wave streams: units first_unit .. last_unit - 1 of its tile groups.
     const int split = p.split, lanes_of_groups = kWaves / split;
-    const int share = wave & (split - 1), mine = wave / split;
-    const int first_unit = p.units * share / split, last_unit = p.units * (share + 1) / split;
-    const int slots = ((p.units + split - 1) / split + kAhead - 1) / kAhead * kAhead;  // to a step, the same for all waves
+    const int mine = wave >> p.log_split;
+    // (shares of k differ by a unit where the split leaves a rest, so the waves take them in turn)
+    auto first_unit = [&](int step) { return p.units * ((wave + step) & (split - 1)) >> p.log_split; };
+    auto last_unit = [&](int step) { return p.units * (((wave + step) & (split - 1)) + 1) >> p.log_split; };
+    const int slots = ((p.units + split - 1) / split + 3) / 4 * 4;  // to a step, the same for all waves
     const int matrix_rows = kKind == kGateUp ? p.n / 2 : p.n;  // among which tiles are counted
     const int half_k = p.k / 2;
     // (a matrix of fewer than 16 rows: lanes past its end load its last row; the last tile of others is moved up to end with the matrix)
@@ -217,7 +222,6 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
 
         struct Slot {
             u32x4 low[kTiles], high[kTiles];
-            uint32_t scale[kTiles][2], zero[kTiles][2];
         };
         // (real = false: a slot that nobody consumes, filled all the same from one place, so that the loads in flight can be counted)
         auto load = [&](Slot& s, int g, int u, bool real) {
@@ -230,61 +234,166 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                 const uint8_t* const base = packed + static_cast<size_t>(row) * half_k + u * (kUnit / 2);
                 s.low[t] = load16_nt(base + low);
                 s.high[t] = load16_nt(base + high);
-                const size_t first_scale = static_cast<size_t>(row) * p.groups;
-#pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    const int part = u * 2 + f;
-                    int of = kDiag == 1 ? (part * p.group_inverse) >> 20 : part * kDiag + chunk / (4 / kDiag);
-                    of = min(of, p.groups - 1);
-                    const uint32_t index = scale_row + of;
-                    s.scale[t][f] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(scales + first_scale) + 2 * index);
-                    if constexpr (kZeros) s.zero[t][f] = (zeros + first_scale)[index];
-                }
             }
         };
 
+        // Scales: a lane takes those of row l % 16 and of the (l / 16)-th of four units, 2 kDiag of them next to one another, in one load.  (One load for a
+        // unit and a lane's own two would touch 16 lines for 64 bytes each time; these filled the queue of misses, 430 us against 330 for the
+        // largest call.)
+        struct Scales {
+            uint32_t scale[kTiles][kDiag], zero[kTiles][kDiag == 4 ? 2 : 1];
+        };
+        auto first_scale = [&](int unit) { return kDiag == 1 ? (2 * unit * p.group_inverse) >> 20 : unit * 2 * kDiag; };  // of a unit, in its row
+        auto scales_left = [&](int row) {  // from the beginning of a row to the end of the tensor
+            const size_t left = p.all_scales - (static_cast<size_t>(expert) * p.n + row) * p.groups;
+            return static_cast<int>(left < (1u << 30) ? left : 1u << 30);
+        };
+        auto block_unit = [&](int step, int block) { return min(first_unit(step) + block * 4 + chunk, last_unit(step) - 1); };
+        auto load_scales = [&](Scales& s, int step, int block) {
+            const uint32_t at = scale_row + first_scale(block_unit(step, block));
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                const int row = tile_row(step * lanes_of_groups + mine, t);
+                const size_t begin = static_cast<size_t>(row) * p.groups;
+                const uint8_t* const scale = reinterpret_cast<const uint8_t*>(scales + begin);
+                if (p.ragged && p.all_scales < 2 * kDiag) {  // fewer than one load takes: one by one
+                    for (int d = 0; d < kDiag; ++d) s.scale[t][d] = 0;
+                    if constexpr (kZeros) s.zero[t][0] = s.zero[t][kDiag == 4 ? 1 : 0] = 0;
+                    for (int i = 0; i < scales_left(row) - static_cast<int>(at); ++i) {
+                        const uint32_t half = (scales + begin)[at + i];
+                        if constexpr (kZeros) s.zero[t][i / 4] |= static_cast<uint32_t>((zeros + begin)[at + i]) << (8 * (i % 4));
+#pragma unroll
+                        for (int d = 0; d < kDiag; ++d)
+                            if (i / 2 == d) s.scale[t][d] |= half << (16 * (i % 2));
+                    }
+                    continue;
+                }
+                const uint32_t from = p.ragged ? min(at, static_cast<uint32_t>(scales_left(row) - 2 * kDiag)) : at;
+                __builtin_memcpy(s.scale[t], scale + 2 * from, 4 * kDiag);
+                if constexpr (kZeros) __builtin_memcpy(s.zero[t], zeros + begin + from, 2 * kDiag);
+            }
+        };
+        // What becomes of them: for each of the four units a register with a lane's two scales (zero points), those of operand X below those of Y.
+        auto spread = [&](uint32_t (&pairs)[kDiag], uint32_t (&of_unit)[4], int step, int block, int t) {
+            if (p.ragged) {
+                // a load that was moved back to end with the tensor is shifted, and what lies behind the row becomes zero
+                const int unit = block_unit(step, block), start = first_scale(unit), row = tile_row(step * lanes_of_groups + mine, t);
+                const int over = p.all_scales < 2 * kDiag ? 0 : max(0, static_cast<int>(scale_row) + start + 2 * kDiag - scales_left(row));
+                if constexpr (kDiag == 4) {
+                    const bool four = (over & 4) != 0;
+                    pairs[0] = four ? pairs[2] : pairs[0];
+                    pairs[1] = four ? pairs[3] : pairs[1];
+                }
+                if constexpr (kDiag >= 2)
+#pragma unroll
+                    for (int d = 0; d < kDiag; ++d) pairs[d] = (over & 2) == 0 ? pairs[d] : d + 1 < kDiag ? pairs[d + 1] : 0u;
+#pragma unroll
+                for (int d = 0; d < kDiag; ++d) pairs[d] = (over & 1) == 0 ? pairs[d] : (pairs[d] >> 16) | (d + 1 < kDiag ? pairs[d + 1] << 16 : 0u);
+                if constexpr (kDiag == 1) {  // long groups: both halves of a unit may be of one
+                    const int second = ((2 * unit + 1) * p.group_inverse) >> 20;
+                    if (second == start) pairs[0] = (pairs[0] & 0xffffu) | (pairs[0] << 16);
+                    else if (second >= p.groups) pairs[0] &= 0xffffu;
+                } else {
+                    const int valid = p.groups - start;
+#pragma unroll
+                    for (int d = 0; d < kDiag; ++d) pairs[d] = 2 * d + 1 < valid ? pairs[d] : 2 * d < valid ? pairs[d] & 0xffffu : 0u;
+                }
+            }
+            uint32_t both[kDiag];  // X and Y of the lane group
+            if constexpr (kDiag == 1) both[0] = pairs[0];
+            else
+#pragma unroll
+                for (int d = 0; d < kDiag / 2; ++d) {
+                    both[2 * d] = (pairs[d] & 0xffffu) | (pairs[kDiag / 2 + d] << 16);
+                    both[2 * d + 1] = (pairs[d] >> 16) | (pairs[kDiag / 2 + d] & 0xffff0000u);
+                }
+            // Rows of 16 lanes change places with registers, so that every lane has its own group's of all four units.
+            auto swap16 = [](uint32_t& a, uint32_t& b) {  // odd rows of a with even rows of b
+                const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+                a = r[0];
+                b = r[1];
+            };
+            auto swap32 = [](uint32_t& a, uint32_t& b) {  // the upper half of a with the lower half of b
+                const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+                a = r[0];
+                b = r[1];
+            };
+            if constexpr (kDiag == 1) {
+                of_unit[0] = of_unit[1] = both[0];
+                swap16(of_unit[0], of_unit[1]);  // rows 0 0 2 2 and 1 1 3 3
+                of_unit[2] = of_unit[0];
+                of_unit[3] = of_unit[1];
+                swap32(of_unit[0], of_unit[2]);
+                swap32(of_unit[1], of_unit[3]);
+            } else if constexpr (kDiag == 2) {
+                of_unit[0] = both[0];
+                of_unit[2] = both[1];
+                swap32(of_unit[0], of_unit[2]);
+                of_unit[1] = of_unit[0];
+                of_unit[3] = of_unit[2];
+                swap16(of_unit[0], of_unit[1]);
+                swap16(of_unit[2], of_unit[3]);
+            } else {
+                of_unit[0] = both[0];
+                of_unit[1] = both[1];
+                of_unit[2] = both[2];
+                of_unit[3] = both[3];
+                swap16(of_unit[0], of_unit[1]);
+                swap16(of_unit[2], of_unit[3]);
+                swap32(of_unit[0], of_unit[2]);
+                swap32(of_unit[1], of_unit[3]);
+            }
+        };
+
+        lds_barrier();  // nobody reads the rows and routes that were there
+        if constexpr (kKind != kMatvec) {  // (every wave makes the same list, and need not wait for another)
+            int held = 0;
+            for (int base = 0; base < p.routes; base += kWave) {
+                const bool hit = base + lane < p.routes && expert_of[base + lane] == expert;
+                const unsigned long long mask = __ballot(hit);
+                if (hit) my_routes[held + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(base + lane);
+                held += __popcll(mask);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        const int rows = min(count - first_row, p.row_cap), padded = (rows + 3) & ~3;
+
+        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.  The first of
+        // them are asked for in front of the weights, which arrive behind them.
+        const int pieces = rows * p.units * 8, per_row = p.units * 8;
+        u32x4 octets[4];
+        auto fetch = [&](int i) {
+            const int m = i / per_row, c32 = i - m * per_row, which = first_row + min(m, rows - 1);
+            const uint16_t* from;
+            if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
+            else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
+            else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) octets[j] = load16(from + (c32 < p.k / 32 ? c32 * 32 : 0) + j * 8);
+        };
+        fetch(tid);
+
         Slot ring[kAhead];
+        Scales next_scales;
         int load_step = first_step, load_slot = 0;
         auto load_next = [&](Slot& s) {
-            const int u = first_unit + load_slot;
-            load(s, load_step * lanes_of_groups + mine, min(u, last_unit - 1), u < last_unit);
+            const int u = first_unit(load_step) + load_slot, end = last_unit(load_step);
+            load(s, load_step * lanes_of_groups + mine, min(u, end - 1), u < end);
             if (++load_slot == slots) {
                 load_slot = 0;
                 load_step = min(load_step + 1, first_step + steps - 1);
             }
         };
+        load_scales(next_scales, first_step, 0);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
 
-        lds_barrier();  // nobody reads the rows and routes that were there
-        if constexpr (kKind != kMatvec) {
-            if (wave == 0) {
-                int held = 0;
-                for (int base = 0; base < p.routes; base += kWave) {
-                    const bool hit = base + lane < p.routes && expert_of[base + lane] == expert;
-                    const unsigned long long mask = __ballot(hit);
-                    if (hit) my_routes[held + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(base + lane);
-                    held += __popcll(mask);
-                }
-            }
-            lds_barrier();
-        }
-        const int rows = min(count - first_row, p.row_cap), padded = (rows + 3) & ~3;
-
-        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.
-        for (int i = tid; i < rows * p.units * 8; i += kThreads) {
-            const int m = i / (p.units * 8), c32 = i - m * (p.units * 8);
-            const int which = first_row + m;
-            const uint16_t* from;
-            if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
-            else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
-            else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
-            float sum = 0.0f;
+        for (int i = tid; i < pieces; i += kThreads) {
+            if (i != tid) fetch(i);
+            const int m = i / per_row, c32 = i - m * per_row;
             const bool real = c32 < p.k / 32;
+            float sum = 0.0f;
             unsigned char* const to = x_lds + static_cast<size_t>((((c32 >> 2) * 4) * 4 + (c32 & 3)) * rows + m) * 16;
-            u32x4 octets[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) octets[j] = load16(from + (real ? c32 * 32 : 0) + j * 8);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const u32x4 v = real ? octets[j] : u32x4{0u, 0u, 0u, 0u};
@@ -302,8 +411,20 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
 
         f32x4 acc[kTiles][kBlocks] = {};
         const int x_lane = own ? (chunk * rows + min(col % kTokens, rows - 1)) * 16 : 0;
-        auto consume = [&](const Slot& s, int u) {
+        auto consume = [&](const Slot& s, int u, const uint32_t (&scale_pair)[kTiles], const uint32_t (&zero_pair)[kTiles]) {
             asm volatile("" : "+s"(u));  // (or each of its LDS addresses becomes an induction variable in a register)
+            // What LDS holds is asked for before the weights are waited for.
+            auto x_at = [&](int part, int j) {
+                return own ? x_lds + (part * 4 + j) * 4 * rows * 16 + x_lane : reinterpret_cast<const unsigned char*>(zero16);
+            };
+            u32x4 x[2][4];
+            if constexpr (kBlocks == 1) {
+#pragma unroll
+                for (int f = 0; f < 2; ++f)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[f][j] = *reinterpret_cast<const u32x4*>(x_at(u * 2 + f, j));
+                __builtin_amdgcn_sched_barrier(0);
+            }
             u32x4 w[2][kTiles];
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
@@ -324,7 +445,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                     for (int t = 0; t < kTiles; ++t) {
                         c[t][b] = start;
                         if constexpr (kZeros) {
-                            const float zero = 16.0f + static_cast<float>(s.zero[t][f]);
+                            const float zero = 16.0f + static_cast<float>(f == 0 ? zero_pair[t] & 0xffu : (zero_pair[t] >> 16) & 0xffu);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) c[t][b][i] *= zero;
                         }
@@ -332,87 +453,124 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const unsigned char* const from = own ? x_lds + (part * 4 + j) * 4 * rows * 16 + x_lane : reinterpret_cast<const unsigned char*>(zero16);
                     u32x4 q[kTiles];
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) q[t] = codes.unpack(w[f][t][j]);
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b) {
-                        const u32x4 a = *reinterpret_cast<const u32x4*>(from + (own ? b * kTokens * 16 : 0));
+                        u32x4 a;
+                        if constexpr (kBlocks == 1) a = x[f][j];
+                        else a = *reinterpret_cast<const u32x4*>(x_at(part, j) + (own ? b * kTokens * 16 : 0));
 #pragma unroll
                         for (int t = 0; t < kTiles; ++t) c[t][b] = multiply<kHalfRows>(a, q[t], c[t][b]);
                     }
                 }
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
-                    const float scale = widen(s.scale[t][f], kHalf);
+                    const float scale = widen(f == 0 ? scale_pair[t] & 0xffffu : scale_pair[t] >> 16, kHalf);
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[t][b][i] = fmaf(scale, c[t][b][i], acc[t][b][i]);
                 }
-                __builtin_amdgcn_sched_barrier(0);  // (the other half's operands would be fetched here, and cost registers)
+                if constexpr (kBlocks > 1) __builtin_amdgcn_sched_barrier(0);  // (the other half's operands would be fetched here, and cost registers)
             }
         };
 
-        // Sum of a result over the waves that share its tile and, for short groups, over the lanes that hold its groups.
-        auto result = [&](int group, int tile, int m, int n) {
-            const int b = m / kTokens, token = m % kTokens;
-            float sum = 0.0f;
-            for (int w = 0; w < split; ++w)
-#pragma unroll
-                for (int d = 0; d < kDiag; ++d) {
-                    const int from = kDiag == 1 ? token / 4 : kDiag == 2 ? token / 4 + 2 * d : d;
-                    sum += results[((((group * split + w) * kTiles + tile) * kBlocks + b) * 4 + token % 4) * plan.lanes + from * 16 + n];
-                }
-            return sum;
-        };
-        auto finish = [&](int at_step) {
+        // Results: the waves that share a tile leave theirs in LDS, those of a batch of steps behind one another; then as many lanes next to one
+        // another add them up (for short groups also over the lanes that hold a tile's groups).
+        const int step_results = kWaves * kTiles * kBlocks * 4 * plan.lanes;
+        auto leave = [&](int place) {
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (lane < plan.lanes) results[(((wave * kTiles + t) * kBlocks + b) * 4 + i) * plan.lanes + lane] = acc[t][b][i];
+                        if (lane < plan.lanes) results[place * step_results + (((wave * kTiles + t) * kBlocks + b) * 4 + i) * plan.lanes + lane] = acc[t][b][i];
                         acc[t][b][i] = 0.0f;
                     }
+        };
+        auto finish = [&](int from_step, int number) {
             lds_barrier();
+            auto shared = [&](int place, int group, int tile, int m, int n, int w) {
+                const int b = m / kTokens, token = m % kTokens;
+                float sum = 0.0f;
+#pragma unroll
+                for (int d = 0; d < kDiag; ++d) {
+                    const int from = kDiag == 1 ? token / 4 : kDiag == 2 ? token / 4 + 2 * d : d;
+                    sum += results[place * step_results + ((((group * split + w) * kTiles + tile) * kBlocks + b) * 4 + token % 4) * plan.lanes + from * 16 + n];
+                }
+                if (split >= 2) sum += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(sum), 0xB1, 0xf, 0xf, false));   // lane ^ 1
+                if (split >= 4) sum += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(sum), 0x4E, 0xf, 0xf, false));   // lane ^ 2
+                if (split >= 8) sum += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(sum), 0x141, 0xf, 0xf, false));  // 7 - lane
+                return sum;
+            };
             constexpr int kOut = kKind == kGateUp ? 1 : kTiles;  // result tiles of a tile group
-            const int outputs = lanes_of_groups * kOut * 16 * (kKind == kDown ? rows / 2 : rows);
-            for (int o = tid; o < outputs; o += kThreads) {
-                const int n = o & 15, tile = (o >> 4) % kOut, rest = (o >> 4) / kOut, group = rest % lanes_of_groups, m = rest / lanes_of_groups;
-                const int g = at_step * lanes_of_groups + group;
+            const int per_step = lanes_of_groups * kOut * 16 * (kKind == kDown ? rows / 2 : rows) * split;
+            for (int i = tid; i < per_step * number; i += kThreads) {  // (per_step is a multiple of 16: lanes that add up stay together)
+                const int place = number == 1 ? 0 : i / per_step, at = i - place * per_step;
+                const int w = at & (split - 1), o = at >> p.log_split, n = o & 15, tile = (o >> 4) % kOut, rest = (o >> 4) / kOut;
+                const int group = rest & (lanes_of_groups - 1), m = rest >> (kLogWaves - p.log_split);
+                const int g = (from_step + place) * lanes_of_groups + group;
                 const int to = tile_row(g, tile) + n;
-                if (g >= p.tile_groups || to >= matrix_rows) continue;
+                const bool mine_to_store = w == 0 && g < p.tile_groups && to < matrix_rows;
                 if constexpr (kKind == kMatvec) {
-                    static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(result(group, tile, m, n), kHalf);
+                    const float y = shared(place, group, tile, m, n, w);
+                    if (mine_to_store) static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(y, kHalf);
                 } else if constexpr (kKind == kGateUp) {
-                    const float gate = result(group, 0, m, n), up = result(group, 1, m, n);
+                    const float gate = shared(place, group, 0, m, n, w), up = shared(place, group, 1, m, n, w);
                     const int route = my_routes[first_row + m];
                     // The route's weight is folded in here.  Two BF16 numbers hold the product's high and low part, together 16 bits of mantissa.
                     const float h = gate / (1.0f + expf(-gate)) * up * route_weights[route];
                     const uint32_t high = f32_to_bf16(h);
                     uint16_t* const row = static_cast<uint16_t*>(p.out) + static_cast<size_t>(route) * 2 * matrix_rows + to;
-                    row[0] = static_cast<uint16_t>(high);
-                    row[matrix_rows] = static_cast<uint16_t>(f32_to_bf16(h - bf16_to_f32(high)));
+                    if (mine_to_store) {
+                        row[0] = static_cast<uint16_t>(high);
+                        row[matrix_rows] = static_cast<uint16_t>(f32_to_bf16(h - bf16_to_f32(high)));
+                    }
                 } else {
                     const int route = my_routes[(first_row >> 1) + m];
-                    static_cast<float*>(p.out)[static_cast<size_t>(route) * p.n + to] = result(group, tile, 2 * m, n) + result(group, tile, 2 * m + 1, n);
+                    const float y = shared(place, group, tile, 2 * m, n, w) + shared(place, group, tile, 2 * m + 1, n, w);
+                    if (mine_to_store) static_cast<float*>(p.out)[static_cast<size_t>(route) * p.n + to] = y;
                 }
             }
-            lds_barrier();
         };
 
-        for (int at_step = first_step; at_step < first_step + steps; ++at_step) {
-            for (int slot = 0; slot < slots; slot += kAhead) {
+        for (int done = 0; done < steps; done += p.batch) {
+            const int number = min(p.batch, steps - done);
+            for (int i = 0; i < number; ++i) {
+                const int at_step = first_step + done + i, from = first_unit(at_step), to = last_unit(at_step);
+                for (int block = 0; block < slots / 4; ++block) {
+                    uint32_t scale_of[kTiles][4], zero_of[kTiles][4] = {};
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    if (first_unit + slot + i < last_unit) consume(ring[i], first_unit + slot + i);
-                    load_next(ring[i]);
+                    for (int t = 0; t < kTiles; ++t) {
+                        spread(next_scales.scale[t], scale_of[t], at_step, block, t);
+                        if constexpr (kZeros) {
+                            uint32_t pairs[kDiag];
+#pragma unroll
+                            for (int d = 0; d < kDiag; ++d) pairs[d] = (next_scales.zero[t][d / 2] >> (16 * (d % 2)) & 0xffu) | (next_scales.zero[t][d / 2] >> (16 * (d % 2)) & 0xff00u) << 8;
+                            spread(pairs, zero_of[t], at_step, block, t);
+                        }
+                    }
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        uint32_t scale_pair[kTiles], zero_pair[kTiles];
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) {
+                            scale_pair[t] = scale_of[t][a];
+                            zero_pair[t] = zero_of[t][a];
+                        }
+                        const int u = from + block * 4 + a;
+                        if (u < to) consume(ring[a % kAhead], u, scale_pair, zero_pair);
+                        if ((a + kAhead) % 4 == 0) load_scales(next_scales, load_step, load_slot / 4);
+                        load_next(ring[a % kAhead]);
+                    }
                 }
+                leave(i);
             }
-            finish(at_step);
+            finish(first_step + done, number);
+            if (done + p.batch < steps) lds_barrier();  // (the results' place is free)
         }
     }
 }
@@ -441,20 +599,23 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     p.group_inverse = diag == 1 ? ((1 << 20) + p.group / 128 - 1) / (p.group / 128) : 0;
     const int tiles = kKind == kMatvec ? 1 : 2, counted = kKind == kGateUp ? p.n / 2 : (p.n + tiles - 1) / tiles;
     p.tile_groups = (counted + 15) / 16;
+    p.ragged = p.k % kUnit != 0 || p.group > 128;
     p.split = 1;
-    while (p.split < kWaves && p.split * 2 * 3 <= p.units) p.split *= 2;
+    while (p.split < kWaves && p.split * 4 < p.units) p.split *= 2, ++p.log_split;  // (four units to a wave and step)
     const int at_once = kWaves / p.split;
     p.steps = (p.tile_groups + at_once - 1) / at_once;
     const int tokens = 16 / diag, by_blocks = rows_expected <= tokens ? 1 : 4, most = tokens * by_blocks;
     // Two workgroups share a CU's 160 KiB where one block of rows will do.
     const int limit = by_blocks == 1 ? 80 << 10 : 160 << 10;
     const int experts = kKind == kMatvec ? 0 : p.ids.local;
-    auto plan = [&](int rows) { return LdsPlan(p.units, diag, by_blocks, tiles, rows, experts, p.routes, kKind == kGateUp).bytes + 64; };
+    auto plan = [&](int rows, int batch) { return LdsPlan(p.units, diag, by_blocks, tiles, rows, batch, experts, p.routes, kKind == kGateUp).bytes + 64; };
     int rows = std::min(rows_most, most);
-    while (rows > (kKind == kDown ? 2 : 1) && plan(rows) > limit) --rows;
+    while (rows > (kKind == kDown ? 2 : 1) && plan(rows, 1) > limit) --rows;
     if (kKind == kDown) rows &= ~1;
     p.row_cap = rows;
-    const int bytes = plan(rows) - 64;
+    p.batch = 1;
+    while (p.batch < 8 && plan(rows, p.batch + 1) <= limit) ++p.batch;
+    const int bytes = plan(rows, p.batch) - 64;
     const int matrices = kKind == kMatvec ? (p.rows + rows - 1) / rows : matrices_most;
     const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(matrices) * p.steps, by_blocks == 1 ? 512 : 256));
     int status = DPEP_OK;
@@ -520,6 +681,7 @@ int dpep_w4_matvec(const dpep_w4* w, int type, const void* x, int num_rows, void
     p.n = w->n;
     p.k = w->k;
     p.group = w->group;
+    p.all_scales = static_cast<size_t>(p.n) * (p.k / p.group);
     p.x = static_cast<const uint16_t*>(x);
     p.rows = num_rows;
     p.out = y;
@@ -557,6 +719,7 @@ int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const
     p.n = gate_up->n;
     p.k = gate_up->k;
     p.group = gate_up->group;
+    p.all_scales = static_cast<size_t>(num_local) * p.n * (p.k / p.group);
     p.x = static_cast<const uint16_t*>(x);
     p.ids = {topk_idx, index_bytes == 8, expert_begin, num_local};
     p.routes = routes;
@@ -571,6 +734,7 @@ int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const
     p.n = down->n;
     p.k = down->k;
     p.group = down->group;
+    p.all_scales = static_cast<size_t>(num_local) * p.n * (p.k / p.group);
     p.x = static_cast<const uint16_t*>(scratch);
     p.out = rows;
     if (int rc = launch_product<kDown>(p, type, slots, 2 * expected, 2 * routes, s); rc != DPEP_OK) return rc;
