@@ -129,12 +129,14 @@ struct LdsPlan {
 
 // A workgroup takes an even share of all steps: of the matrices that have rows one after the other (matvec: of the passes over the rows), each
 // with the rows it multiplies in LDS.
-template <Kind kKind, bool kHalf, bool kZeros, int kDiag, int kBlocks>
+template <Kind kKind, bool kHalf, bool kZeros, int kDiag, int kBlocks, bool kStreamed>
 __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel(const Product p)
 {
     constexpr bool kHalfRows = kHalf && kKind != kDown;  // the down product's rows are BF16 pairs whatever the type
     constexpr int kTiles = kKind == kMatvec ? 1 : 2;     // tiles of 16 rows of W to a tile group; gate_up: a gate tile and its up tile
-    constexpr int kAhead = kKind == kMatvec ? 4 : 2;     // units in flight
+    // Units in flight.  The waves of a CU (sixteen, 4 KiB each) need not ask for more: with two units each, requests queued for 5 us, and so did
+    // everything that was cold, instructions among it (one token through 8 of 256 experts 64 us against 51, sixteen tokens 372 against 340).
+    constexpr int kAhead = kKind == kMatvec ? 2 : 1;
     constexpr int kTokens = 16 / kDiag;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ __attribute__((aligned(16))) uint32_t zero16[4];
@@ -232,8 +234,13 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
             for (int t = 0; t < kTiles; ++t) {
                 const int row = tile_row(g, t);
                 const uint8_t* const base = packed + static_cast<size_t>(row) * half_k + u * (kUnit / 2);
-                s.low[t] = load16_nt(base + low);
-                s.high[t] = load16_nt(base + high);
+                if constexpr (kStreamed) {
+                    s.low[t] = load16_nt(base + low);
+                    s.high[t] = load16_nt(base + high);
+                } else {
+                    s.low[t] = load16(base + low);
+                    s.high[t] = load16(base + high);
+                }
             }
         };
 
@@ -358,8 +365,8 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
         }
         const int rows = min(count - first_row, p.row_cap), padded = (rows + 3) & ~3;
 
-        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.  The first of
-        // them are asked for in front of the weights, which arrive behind them.
+        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.  The weights are
+        // asked for when the rows are there: behind weights in the CU's queue rows take 5 us to come, and the waves hold units that wait for them.
         const int pieces = rows * p.units * 8, per_row = p.units * 8;
         u32x4 octets[4];
         auto fetch = [&](int i) {
@@ -384,12 +391,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                 load_step = min(load_step + 1, first_step + steps - 1);
             }
         };
-        load_scales(next_scales, first_step, 0);
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
-
-        for (int i = tid; i < pieces; i += kThreads) {
-            if (i != tid) fetch(i);
+        auto put = [&](int i) {
             const int m = i / per_row, c32 = i - m * per_row;
             const bool real = c32 < p.k / 32;
             float sum = 0.0f;
@@ -406,8 +408,17 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
             if constexpr (kDiag < 4) sum += __shfl_xor(sum, 1);
             if constexpr (kDiag < 2) sum += __shfl_xor(sum, 2);
             if ((c32 & (4 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(c32 / (4 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
+        };
+        if (tid < pieces) put(tid);
+        for (int i = tid + kThreads; i < pieces; i += kThreads) {
+            fetch(i);
+            put(i);
         }
         lds_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        load_scales(next_scales, first_step, 0);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) load_next(ring[i]);
 
         f32x4 acc[kTiles][kBlocks] = {};
         const int x_lane = own ? (chunk * rows + min(col % kTokens, rows - 1)) * 16 : 0;
@@ -619,8 +630,8 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     const int matrices = kKind == kMatvec ? (p.rows + rows - 1) / rows : matrices_most;
     const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(matrices) * p.steps, by_blocks == 1 ? 512 : 256));
     int status = DPEP_OK;
-    auto go = [&](auto half, auto zeros, auto d, auto b) {
-        const auto kernel = product_kernel<kKind, half(), zeros(), d(), b()>;
+    auto go = [&](auto half, auto zeros, auto d, auto b, auto streamed) {
+        const auto kernel = product_kernel<kKind, half(), zeros(), d(), b(), streamed()>;
         if (bytes > 32 << 10) {
             const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
             if (err != hipSuccess) {
@@ -632,8 +643,11 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
         status = launch_status("w4 product");
     };
     auto by_block = [&](auto half, auto zeros, auto d) {
-        if (by_blocks == 1) go(half, zeros, d, std::integral_constant<int, 1>{});
-        else go(half, zeros, d, std::integral_constant<int, 4>{});
+        // Rows of whole lines are read once and go past the caches; of other rows every other line is read by two waves (through 8 of 256 experts
+        // 51 us, plain loads 53; through 4 of 32 with rows of 1440 and 704 bytes 63 and 55).  (A branch around the loads costs a tenth.)
+        if (by_blocks == 4) go(half, zeros, d, std::integral_constant<int, 4>{}, std::false_type{});
+        else if (p.k % kUnit == 0) go(half, zeros, d, std::integral_constant<int, 1>{}, std::true_type{});
+        else go(half, zeros, d, std::integral_constant<int, 1>{}, std::false_type{});
     };
     auto by_group = [&](auto half, auto zeros) {
         if (diag == 1) by_block(half, zeros, std::integral_constant<int, 1>{});
