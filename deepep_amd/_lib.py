@@ -60,6 +60,7 @@ SIGNATURES = {
     "dpep_route": (_I, (_P, _P, _P, _P, _I, _P, _P, _P)),
     "dpep_balance_scratch_bytes": (_Z, (_I, _I, _I)),
     "dpep_balance_loss": (_I, (_P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P)),
+    "dpep_route_balance": (_I, (_P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P)),
     "dpep_router_backward": (_I, (_P, _P, _I, _P)),
     "dpep_w4_matvec": (_I, (_P, _I, _P, _I, _P, _P)),
     "dpep_w4_experts_scratch_bytes": (_Z, (_I, _I, _I, _I)),

@@ -20,43 +20,48 @@ namespace {
 
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kTiny = 1e-20f;  // keeps the sum of chosen sigmoids off zero (all of them underflow below a logit of -88)
-constexpr int kRouterThreads = 256;
+constexpr int kRouterThreads = 512;
 constexpr int kRouterWaves = kRouterThreads / kWave;
 constexpr int kMaxRouterExperts = 1024;
+constexpr int kNone = INT32_MIN;  // below every key
 
-template <int kType>
-__device__ __forceinline__ float load_logit(const void* p, size_t i)
+// ---- a row in a wave's registers ---------------------------------------------------------------------------------------------------
+template <int kControl, int kRows>
+__device__ __forceinline__ int dpp_or(int other, int v)
 {
-    if constexpr (kType == DPEP_TYPE_F32) return static_cast<const float*>(p)[i];
-    if constexpr (kType == DPEP_TYPE_BF16) return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
-    return f16_to_f32(static_cast<const uint16_t*>(p)[i]);
+    return __builtin_amdgcn_update_dpp(other, v, kControl, kRows, 0xf, false);
 }
-template <int kType>
-__device__ __forceinline__ void store_logit(void* p, size_t i, float v)
+// Largest / sum over the wave, the same in every lane, by row shifts and row broadcasts (an LDS permute a step costs 50 ns and more).
+__device__ __forceinline__ int wave_max(int v)
 {
-    if constexpr (kType == DPEP_TYPE_F32) static_cast<float*>(p)[i] = v;
-    if constexpr (kType == DPEP_TYPE_BF16) static_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(f32_to_bf16(v));
-    if constexpr (kType == DPEP_TYPE_F16) static_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(pack_f16x2(v, 0.0f) & 0xffffu);
-}
-__device__ __forceinline__ int load_index(const void* p, bool wide, size_t i, int experts)
-{
-    const long long e = wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
-    return e >= 0 && e < experts ? static_cast<int>(e) : -1;
-}
-
-// (The choice compares keys, so a key has to be the same 32 bits whoever computes it: IEEE divide and the library's exp.)
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
-
-__device__ __forceinline__ float wave_max(float v)
-{
-    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    v = max(v, dpp_or<0x111, 0xf>(kNone, v));  // row_shr:1
+    v = max(v, dpp_or<0x112, 0xf>(kNone, v));
+    v = max(v, dpp_or<0x114, 0xf>(kNone, v));
+    v = max(v, dpp_or<0x118, 0xf>(kNone, v));
+    v = max(v, dpp_or<0x142, 0xa>(kNone, v));  // row_bcast:15
+    v = max(v, dpp_or<0x143, 0xc>(kNone, v));  // row_bcast:31
+    return __builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ float wave_sum(float v)
 {
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    auto add = [&](int shifted) { v += __int_as_float(shifted); };
+    add(dpp_or<0x111, 0xf>(0, __float_as_int(v)));
+    add(dpp_or<0x112, 0xf>(0, __float_as_int(v)));
+    add(dpp_or<0x114, 0xf>(0, __float_as_int(v)));
+    add(dpp_or<0x118, 0xf>(0, __float_as_int(v)));
+    add(dpp_or<0x142, 0xa>(0, __float_as_int(v)));
+    add(dpp_or<0x143, 0xc>(0, __float_as_int(v)));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+// Integers in the order of the floats (-0 and +0 made one, NaN above everything).
+__device__ __forceinline__ int ordered(float v)
+{
+    const int bits = __float_as_int(fminf(v, kInf) + 0.0f);
+    return bits ^ ((bits >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int key) { return __int_as_float(key ^ ((key >> 31) & 0x7fffffff)); }
 
 // What the wave's lanes stored to LDS is there for all of them.
 __device__ __forceinline__ void wave_sync()
@@ -66,139 +71,127 @@ __device__ __forceinline__ void wave_sync()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-struct Route {
-    const void* logits;
-    const float* bias;
-    const uint8_t* token_mask;
-    void* topk_idx;
-    float* topk_weights;
-    int tokens, experts, topk, groups, topk_groups;
-    bool normalize, wide;
-    float scale;
-};
-
-// Keeps the experts of the best groups: every other key becomes -inf.  keys_lds: the row's keys; groups_lds: a group's score each.
-template <int V, bool kSigmoid>
-__device__ void limit_groups(float (&key)[V], const Route& r, float* keys_lds, float* groups_lds, int lane)
+template <int kType>
+using Logit = std::conditional_t<kType == DPEP_TYPE_F32, uint32_t, uint16_t>;
+template <int kType>
+__device__ __forceinline__ float widen(uint32_t bits)
 {
-    const int width = r.experts / r.groups;
+    if constexpr (kType == DPEP_TYPE_F32) return __uint_as_float(bits);
+    if constexpr (kType == DPEP_TYPE_BF16) return bf16_to_f32(bits);
+    return f16_to_f32(bits);
+}
+template <int kType>
+__device__ __forceinline__ float load_logit(const void* p, size_t i)
+{
+    return widen<kType>(static_cast<const Logit<kType>*>(p)[i]);
+}
+// V values next to one another as the memory holds them: in one piece where rows allow it (whole: the number of experts is a multiple of V and rows
+// are aligned to pieces), else one by one.
+template <int V, int kType>
+struct Piece {
+    using Word = Logit<kType>;
+    Word at[V];
+    __device__ __forceinline__ void load(const void* rows, size_t row, int experts, int lane, bool whole)
+    {
+        const Word* const from = static_cast<const Word*>(rows) + row;
+        const int first = lane * V;
+        if (whole) {
+            const int clamped = first < experts ? first : 0;
+            __builtin_memcpy(at, __builtin_assume_aligned(from + clamped, V * sizeof(Word) < 16 ? V * sizeof(Word) : 16), sizeof(at));
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) at[v] = from[min(first + v, experts - 1)];
+        }
+    }
+    __device__ __forceinline__ void store(void* rows, size_t row, int experts, int lane, bool whole) const
+    {
+        Word* const to = static_cast<Word*>(rows) + row;
+        const int first = lane * V;
+        if (whole) {
+            if (first < experts) __builtin_memcpy(__builtin_assume_aligned(to + first, V * sizeof(Word) < 16 ? V * sizeof(Word) : 16), at, sizeof(at));
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (first + v < experts) to[first + v] = at[v];
+        }
+    }
+    __device__ __forceinline__ float value(int v, int experts, int lane) const { return lane * V + v < experts ? widen<kType>(at[v]) : -kInf; }
+    __device__ __forceinline__ void set(int v, float value)
+    {
+        if constexpr (kType == DPEP_TYPE_F32) at[v] = __float_as_uint(value);
+        if constexpr (kType == DPEP_TYPE_BF16) at[v] = static_cast<uint16_t>(f32_to_bf16(value));
+        if constexpr (kType == DPEP_TYPE_F16) at[v] = static_cast<uint16_t>(pack_f16x2(value, 0.0f) & 0xffffu);
+    }
+};
+__device__ __forceinline__ int load_index(const void* p, bool wide, size_t i, int experts)
+{
+    const long long e = wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+    return e >= 0 && e < experts ? static_cast<int>(e) : -1;
+}
+
+// 1 / (1 + exp(-z)) as IEEE divide and the library's exp give it, bit for bit (the choice compares such values, so everybody has to get the
+// same): one step from the hardware's reciprocal is correctly rounded for every mantissa and exponent below 2^126 (checked for all of
+// them), and beyond that, below a logit of -87, the divide itself is taken.  grown: exp(-z).
+__device__ __forceinline__ float sigmoid_of(float grown)
+{
+    const float d = 1.0f + grown, r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.0f), r, r);
+}
+template <int V>
+__device__ __forceinline__ void sigmoids(const float (&z)[V], float (&s)[V], float (&grown)[V])
+{
+    float largest = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        grown[v] = expf(-z[v]);
+        s[v] = sigmoid_of(grown[v]);
+        largest = z[v] == -kInf ? largest : fmaxf(largest, grown[v]);
+    }
+    if (__ballot(largest > 0x1p125f) != 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) s[v] = 1.0f / (1.0f + grown[v]);
 #pragma unroll
     for (int v = 0; v < V; ++v)
-        if (lane * V + v < r.experts) keys_lds[lane * V + v] = key[v];
-    wave_sync();
-    for (int g = lane; g < r.groups; g += kWave) {
-        float first = -kInf, second = -kInf;
-        for (int j = 0; j < width; ++j) {
-            const float k = keys_lds[g * width + j];
-            second = fmaxf(second, fminf(first, k));
-            first = fmaxf(first, k);
-        }
-        groups_lds[g] = !kSigmoid || second == -kInf ? first : first + second;
-    }
-    wave_sync();
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int e = lane * V + v;
-        if (e >= r.experts) continue;
-        const int g = e / width;
-        const float mine = groups_lds[g];
-        int ahead = 0;
-        for (int o = 0; o < r.groups; ++o) {
-            const float other = groups_lds[o];
-            ahead += other > mine || (other == mine && o < g);
-        }
-        if (ahead >= r.topk_groups) key[v] = -kInf;
-    }
+        if (z[v] == -kInf) s[v] = 0.0f;
 }
-
-template <int V, int kType, bool kSigmoid>
-__global__ __launch_bounds__(kRouterThreads) void route_kernel(const Route r)
+__device__ __forceinline__ float sigmoid(float z)
 {
-    __shared__ float keys_lds[kRouterWaves][kWave * V];
-    __shared__ float groups_lds[kRouterWaves][kWave * V];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int token = blockIdx.x * kRouterWaves + wave;
-    if (token >= r.tokens) return;
-    const size_t row = static_cast<size_t>(token) * r.experts;
-    const bool real = r.token_mask == nullptr || r.token_mask[token] != 0;
-    float key[V], z[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int e = lane * V + v;
-        z[v] = e < r.experts ? load_logit<kType>(r.logits, row + e) : -kInf;
-        float k = z[v];
-        if constexpr (kSigmoid) {
-            k = sigmoid(z[v]);
-            if (r.bias != nullptr && e < r.experts) k += r.bias[e];
-        }
-        // a NaN ranks with +inf, so that it is chosen and shows in the weights; what is out of service ranks nowhere
-        key[v] = z[v] == -kInf || !real ? -kInf : fminf(k, kInf);
-    }
-    float top = -kInf, total = 0.0f;
-    if (!kSigmoid && !r.normalize) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) top = fmaxf(top, z[v]);
-        top = wave_max(top);
-#pragma unroll
-        for (int v = 0; v < V; ++v) total += z[v] == -kInf ? 0.0f : expf(z[v] - top);
-        total = wave_sum(total);
-    }
-    if (r.groups > 1) limit_groups<V, kSigmoid>(key, r, keys_lds[wave], groups_lds[wave], lane);
-
-    int mine = -1;  // lane k: the expert of slot k
-    for (int k = 0; k < r.topk; ++k) {
-        float best = key[0];
-#pragma unroll
-        for (int v = 1; v < V; ++v) best = fmaxf(best, key[v]);
-        best = wave_max(best);
-        if (best == -kInf) break;
-        int at = 0x7fffffff;
-#pragma unroll
-        for (int v = V - 1; v >= 0; --v)
-            if (key[v] == best) at = lane * V + v;
-        for (int d = 32; d > 0; d >>= 1) at = min(at, __shfl_xor(at, d));
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (lane * V + v == at) key[v] = -kInf;
-        if (lane == k) mine = at;
-    }
-
-    float weight = 0.0f;
-    const float chosen = mine >= 0 ? load_logit<kType>(r.logits, row + mine) : -kInf;
-    if constexpr (kSigmoid) {
-        weight = mine >= 0 ? sigmoid(chosen) : 0.0f;
-        if (r.normalize) weight = weight / (wave_sum(weight) + kTiny);
-    } else {
-        if (r.normalize) top = wave_max(chosen);
-        weight = mine >= 0 ? expf(chosen - top) : 0.0f;
-        if (r.normalize) total = wave_sum(weight);
-        weight = mine >= 0 ? weight / total : 0.0f;
-    }
-    if (lane < r.topk) {
-        const size_t to = static_cast<size_t>(token) * r.topk + lane;
-        if (r.wide) static_cast<int64_t*>(r.topk_idx)[to] = mine;
-        else static_cast<int32_t*>(r.topk_idx)[to] = mine;
-        r.topk_weights[to] = weight * r.scale;
-    }
+    const float z1[1] = {z};
+    float s[1], grown[1];
+    sigmoids<1>(z1, s, grown);
+    return s[0];
+}
+__device__ __forceinline__ float reciprocal(float d)  // of 1e-20 .. 1e30
+{
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.0f), r, r);
 }
 
-// ---- balance loss ------------------------------------------------------------------------------------------------------------------
-// Sequence b of N tokens with a route and R routes, c_e of them to expert e; p a token's softmax, or its sigmoids over their sum:
-//   f_e = E c_e / R,  loss_b = sum_e f_e (sum_t p_te) / N
-// Chunks of tokens leave one row of sums for every sequence they touch; (chunk + sequence) numbers these rows without a gap to spare.
-struct Balance {
-    const void* logits;
-    const void* topk_idx;
-    const int32_t* offsets;  // [sequences + 1], or null: one sequence
-    int tokens, experts, topk, sequences, chunk, chunks;
-    bool wide;
-    float* sums;             // [chunks + sequences][experts]
-    int32_t* counts;         // the same
-    int32_t* members;        // [chunks + sequences]
-};
+// A row's scores: exp(z - max) or the sigmoids, and 1 / their sum (the balance loss's probabilities are their products).  rest: exp(-z) (sigmoid).
+template <int V, bool kSigmoid>
+__device__ __forceinline__ float row_scores(const float (&z)[V], float (&s)[V], float (&grown)[V])
+{
+    float total = 0.0f;
+    if constexpr (kSigmoid) {
+        sigmoids<V>(z, s, grown);
+    } else {
+        int top = kNone;
+#pragma unroll
+        for (int v = 0; v < V; ++v) top = max(top, ordered(z[v] == z[v] ? z[v] : -kInf));
+        const float largest = unordered(wave_max(top));
+#pragma unroll
+        for (int v = 0; v < V; ++v) s[v] = z[v] == -kInf ? 0.0f : expf(z[v] - largest);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) total += s[v];
+    total = wave_sum(total);
+    return kSigmoid ? reciprocal(total + kTiny) : total == 0.0f ? 0.0f : 1.0f / total;
+}
 
+// ---- sequences -------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int sequence_begin(const int32_t* offsets, int b, int sequences, int tokens)
 {
+    if (b >= sequences) return tokens;
     if (offsets == nullptr) return b == 0 ? 0 : tokens;
     return min(max(offsets[b], 0), tokens);
 }
@@ -215,119 +208,302 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences
     return low;
 }
 
-// A row's probabilities; false for padding.  (1 / the sum of sigmoids for the gradient.)
-template <int V, int kType, bool kSigmoid>
-__device__ __forceinline__ void row_probabilities(const void* logits, size_t row, int experts, int lane, float (&p)[V], float (&s)[V], float& inverse)
+// ---- choice and balance sums --------------------------------------------------------------------------------------------------------
+struct Forward {
+    const void* logits;
+    // choice
+    const float* bias;
+    const uint8_t* token_mask;
+    void* topk_idx;
+    float* topk_weights;
+    int groups, topk_groups;
+    int group_lanes;  // a group's lanes where groups are 1, 2, 4 .. 16 lanes of whole registers, else 0
+    bool normalize;
+    float scale;
+    // sums of the balance loss.  Chunks of tokens (a workgroup each) leave one row of sums for every sequence that they touch; (chunk + sequence)
+    // numbers these rows.
+    const int32_t* offsets;
+    int sequences;
+    float* sums;       // [chunks + sequences][experts]: of the probabilities
+    int32_t* counts;   // the same: routes
+    int32_t* members;  // [chunks + sequences]: tokens with a route
+    uint32_t* tickets; // [sequences]
+    int tokens, experts, topk, chunk;
+    bool wide, whole;
+};
+
+// Keys of experts outside the best groups become -inf.  Groups of whole lanes: a lane's two largest, then the group's by exchanges among its lanes;
+// other groups by way of LDS.
+template <int V, bool kSigmoid>
+__device__ __forceinline__ void limit_groups(float (&key)[V], const Forward& c, float* keys_lds, float* scores_lds, int lane)
 {
-    float z[V], top = -kInf, total = 0.0f;
+    const int width = c.experts / c.groups;
+    if (c.group_lanes > 0) {
+        float first = key[0], second = -kInf;
+#pragma unroll
+        for (int v = 1; v < V; ++v) {
+            second = fmaxf(second, fminf(first, key[v]));
+            first = fmaxf(first, key[v]);
+        }
+        auto merge = [&](float other, float other_second) {
+            second = fmaxf(fmaxf(second, other_second), fminf(first, other));
+            first = fmaxf(first, other);
+        };
+        auto step = [&](auto control) {
+            merge(__int_as_float(dpp_or<control(), 0xf>(0, __float_as_int(first))), __int_as_float(dpp_or<control(), 0xf>(0, __float_as_int(second))));
+        };
+        if (c.group_lanes >= 2) step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+        if (c.group_lanes >= 4) step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+        if (c.group_lanes >= 8) step(std::integral_constant<int, 0x141>{});  // the other four of eight
+        if (c.group_lanes >= 16) step(std::integral_constant<int, 0x140>{}); // the other eight of sixteen
+        const float mine = !kSigmoid || second == -kInf ? first : first + second;
+        int ahead = 0;
+        for (int o = 0; o < c.groups; ++o) {
+            const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), o * c.group_lanes));
+            ahead += other > mine || (other == mine && lane >= (o + 1) * c.group_lanes);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = ahead >= c.topk_groups ? -kInf : key[v];
+        return;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        if (lane * V + v < c.experts) keys_lds[lane * V + v] = key[v];
+    wave_sync();
+    for (int g = lane; g < c.groups; g += kWave) {
+        float first = -kInf, second = -kInf;
+        for (int j = 0; j < width; ++j) {
+            const float k = keys_lds[g * width + j];
+            second = fmaxf(second, fminf(first, k));
+            first = fmaxf(first, k);
+        }
+        scores_lds[g] = !kSigmoid || second == -kInf ? first : first + second;
+    }
+    wave_sync();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int e = lane * V + v;
-        z[v] = e < experts ? load_logit<kType>(logits, row + e) : -kInf;
-        top = fmaxf(top, z[v]);
+        if (e >= c.experts) continue;
+        const int g = e / width;
+        const float mine = scores_lds[g];
+        int ahead = 0;
+        for (int o = 0; o < c.groups; ++o) {
+            const float other = scores_lds[o];
+            ahead += other > mine || (other == mine && o < g);
+        }
+        if (ahead >= c.topk_groups) key[v] = -kInf;
     }
-    if constexpr (!kSigmoid) top = wave_max(top);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        s[v] = z[v] == -kInf ? 0.0f : kSigmoid ? sigmoid(z[v]) : expf(z[v] - top);
-        total += s[v];
-    }
-    total = wave_sum(total);
-    inverse = kSigmoid ? 1.0f / (total + kTiny) : total > 0.0f || total != total ? 1.0f / total : 0.0f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        p[v] = s[v] * inverse;
-        if constexpr (kSigmoid) s[v] = z[v] == -kInf ? 0.0f : s[v] * sigmoid(-z[v]);  // ds/dz (1 - s would cancel)
-    }
+    wave_sync();
 }
 
-template <int V, int kType, bool kSigmoid>
-__global__ __launch_bounds__(kRouterThreads) void balance_sums_kernel(const Balance c)
+// Lane k gets the expert of slot k, -1 where none is left: each time the largest key of the wave, in its lowest lane and there in the lowest
+// register (experts are counted along lanes, so that is the lowest index).
+template <int V>
+__device__ __forceinline__ int choose(const float (&key)[V], int topk)
 {
-    __shared__ int counts[kWave * V];
-    __shared__ float sums[kRouterWaves][kWave * V];
+    int left[V], mine = -1;
+#pragma unroll
+    for (int v = 0; v < V; ++v) left[v] = key[v] == -kInf ? kNone : ordered(key[v]);
+    for (int k = 0; k < topk; ++k) {
+        int best = left[0];
+#pragma unroll
+        for (int v = 1; v < V; ++v) best = max(best, left[v]);
+        const int largest = wave_max(best);
+        if (largest == kNone) break;
+        const int lane = __ffsll(__ballot(best == largest)) - 1;
+        int at = V - 1;
+        bool open = true;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const bool here = open && ((__ballot(left[v] == largest) >> lane) & 1) != 0;
+            at = here ? v : at;
+            open = open && !here;
+            left[v] = __builtin_amdgcn_inverse_ballot_w64(here ? 1ull << lane : 0ull) ? kNone : left[v];
+        }
+        mine = (threadIdx.x & 63) == static_cast<unsigned>(k) ? lane * V + at : mine;
+    }
+    return mine;
+}
+
+template <int V, int kType, bool kSigmoid, bool kRoute, bool kBalance>
+__global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Forward c)
+{
+    __shared__ float rows_lds[kRouterWaves][kWave * V];  // keys of irregular groups, then the waves' sums
+    __shared__ float scores_lds[kRoute ? kRouterWaves : 1][kWave * V];
+    __shared__ int counts[kBalance ? kWave * V : 1];
     __shared__ int members[kRouterWaves];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int first = blockIdx.x * c.chunk, last = min(first + c.chunk, c.tokens);
+    if (kBalance && blockIdx.x == 0)
+        for (int b = threadIdx.x; b < c.sequences; b += kRouterThreads) c.tickets[b] = 0;
+    float bias[V];
+    if constexpr (kRoute && kSigmoid)
+#pragma unroll
+        for (int v = 0; v < V; ++v) bias[v] = c.bias != nullptr && lane * V + v < c.experts ? c.bias[lane * V + v] : 0.0f;
+
     int begin = first;
-    for (int b = sequence_of(c.offsets, c.sequences, first); b < c.sequences && begin < last; ++b) {
-        const int end = b + 1 == c.sequences ? last : min(last, sequence_begin(c.offsets, b + 1, c.sequences, c.tokens));
+    for (int b = kBalance ? sequence_of(c.offsets, c.sequences, first) : 0; begin < last && b < c.sequences; ++b) {
+        const int end = !kBalance || b + 1 == c.sequences ? last : min(last, sequence_begin(c.offsets, b + 1, c.sequences, c.tokens));
         if (end <= begin) continue;
-        for (int e = threadIdx.x; e < c.experts; e += kRouterThreads) counts[e] = 0;
-        __syncthreads();
-        float acc[V] = {};
+        float sum[V] = {};
         int held = 0;
+        if constexpr (kBalance) {
+            for (int e = threadIdx.x; e < c.experts; e += kRouterThreads) counts[e] = 0;
+            __syncthreads();
+        }
+        Piece<V, kType> next;
+        if (begin + wave < end) next.load(c.logits, static_cast<size_t>(begin + wave) * c.experts, c.experts, lane, c.whole);
         for (int t = begin + wave; t < end; t += kRouterWaves) {
-            const int e = lane < c.topk ? load_index(c.topk_idx, c.wide, static_cast<size_t>(t) * c.topk + lane, c.experts) : -1;
-            if (__ballot(e >= 0) == 0) continue;
-            if (e >= 0) atomicAdd(&counts[e], 1);
-            ++held;
-            float p[V], s[V], inverse;
-            row_probabilities<V, kType, kSigmoid>(c.logits, static_cast<size_t>(t) * c.experts, c.experts, lane, p, s, inverse);
+            const size_t row = static_cast<size_t>(t) * c.experts, to = static_cast<size_t>(t) * c.topk + lane;
+            const Piece<V, kType> piece = next;
+            if (t + kRouterWaves < end) next.load(c.logits, static_cast<size_t>(t + kRouterWaves) * c.experts, c.experts, lane, c.whole);
+            int mine = -1;
+            if constexpr (!kRoute) mine = lane < c.topk ? load_index(c.topk_idx, c.wide, to, c.experts) : -1;
+            float z[V], s[V], grown[V], inverse = 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] += p[v];
-        }
+            for (int v = 0; v < V; ++v) z[v] = piece.value(v, c.experts, lane);
+            if (kBalance || (!kSigmoid && !c.normalize)) inverse = row_scores<V, kSigmoid>(z, s, grown);
+            else if constexpr (kSigmoid) sigmoids<V>(z, s, grown);
+            if constexpr (kRoute) {
+                const bool real = c.token_mask == nullptr || c.token_mask[t] != 0;
+                if (real) {
+                    float key[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) sums[wave][lane * V + v] = acc[v];
-        if (lane == 0) members[wave] = held;
-        __syncthreads();
-        const size_t slot = blockIdx.x + b;
-        for (int e = threadIdx.x; e < c.experts; e += kRouterThreads) {
-            float sum = 0.0f;
+                    for (int v = 0; v < V; ++v) {
+                        // a NaN ranks with +inf, so that it is chosen and shows in the weights; what is out of service ranks nowhere
+                        if constexpr (kSigmoid) key[v] = c.bias != nullptr ? s[v] + bias[v] : s[v];
+                        else key[v] = z[v];
+                        key[v] = z[v] == -kInf ? -kInf : fminf(key[v], kInf);
+                    }
+                    if (c.groups > 1) limit_groups<V, kSigmoid>(key, c, rows_lds[wave], scores_lds[wave], lane);
+                    mine = choose<V>(key, c.topk);
+                }
+                float weight = 0.0f;
+                const float chosen = mine >= 0 ? load_logit<kType>(c.logits, row + mine) : -kInf;
+                if constexpr (kSigmoid) {
+                    weight = mine >= 0 ? sigmoid(chosen) : 0.0f;
+                    if (c.normalize) weight = weight / (wave_sum(weight) + kTiny);
+                } else if (c.normalize) {
+                    const float top = unordered(wave_max(chosen == chosen ? ordered(chosen) : kNone));
+                    weight = mine >= 0 ? expf(chosen - top) : 0.0f;
+                    const float total = wave_sum(weight);
+                    weight = mine >= 0 ? weight / total : 0.0f;
+                } else {
+                    const int owner = mine >= 0 ? mine / V : 0;
+                    float score = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kRouterWaves; ++w) sum += sums[w][e];
-            c.sums[slot * c.experts + e] = sum;
-            c.counts[slot * c.experts + e] = counts[e];
+                    for (int v = 0; v < V; ++v) {
+                        const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(owner * 4, __float_as_int(s[v])));
+                        score = mine - owner * V == v ? other : score;
+                    }
+                    weight = mine >= 0 ? score * inverse : 0.0f;
+                }
+                if (lane < c.topk) {
+                    if (c.wide) static_cast<int64_t*>(c.topk_idx)[to] = mine;
+                    else static_cast<int32_t*>(c.topk_idx)[to] = mine;
+                    c.topk_weights[to] = weight * c.scale;
+                }
+            }
+            if constexpr (kBalance) {
+                if (__ballot(mine >= 0) == 0) continue;
+                if (mine >= 0) atomicAdd(&counts[mine], 1);
+                ++held;
+#pragma unroll
+                for (int v = 0; v < V; ++v) sum[v] += s[v] * inverse;
+            }
         }
-        if (threadIdx.x == 0) {
-            int total = 0;
-            for (int w = 0; w < kRouterWaves; ++w) total += members[w];
-            c.members[slot] = total;
+        if constexpr (kBalance) {
+            wave_sync();
+#pragma unroll
+            for (int v = 0; v < V; ++v) rows_lds[wave][lane * V + v] = sum[v];
+            if (lane == 0) members[wave] = held;
+            __syncthreads();
+            const size_t slot = blockIdx.x + b;
+            for (int e = threadIdx.x; e < c.experts; e += kRouterThreads) {
+                float total = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kRouterWaves; ++w) total += rows_lds[w][e];
+                c.sums[slot * c.experts + e] = total;
+                c.counts[slot * c.experts + e] = counts[e];
+            }
+            if (threadIdx.x == 0) {
+                int total = 0;
+                for (int w = 0; w < kRouterWaves; ++w) total += members[w];
+                c.members[slot] = total;
+            }
+            __syncthreads();
         }
-        __syncthreads();
         begin = end;
     }
 }
 
-constexpr int kFinishThreads = 1024;
-__global__ __launch_bounds__(kFinishThreads) void balance_finish_kernel(const Balance c, float* losses, int32_t* counts, int32_t* members)
+// Sequence b of N tokens with a route and R routes, c_e of them to expert e; p a token's softmax, or its sigmoids over their sum:
+//   f_e = E c_e / R,  loss_b = sum_e f_e (sum_t p_te) / N = E / (R N) sum_e c_e sum_t p_te
+// A workgroup adds up 64 experts' rows of sums, sixteen at a time; the last of a sequence's workgroups has the loss.
+constexpr int kFinishWaves = 16;
+struct Finish {
+    const float* sums;
+    const int32_t* counts;
+    const int32_t* members;
+    const int32_t* offsets;
+    uint32_t* tickets;
+    float* products;  // [sequences][pieces of 64 experts]
+    int32_t* routes;  // the same
+    float* losses;
+    int32_t* all_counts;
+    int32_t* all_members;
+    int tokens, experts, sequences, chunk;
+};
+__global__ __launch_bounds__(kFinishWaves * kWave) void balance_finish_kernel(const Finish c)
 {
-    __shared__ float part[kFinishThreads / kWave];
-    __shared__ int routes[kFinishThreads / kWave];
-    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int begin = sequence_begin(c.offsets, b, c.sequences, c.tokens);
-    const int end = b + 1 == c.sequences ? c.tokens : sequence_begin(c.offsets, b + 1, c.sequences, c.tokens);
-    const int first = begin / max(c.chunk, 1), last = end > begin ? (end - 1) / c.chunk : first - 1;
-    const int e = threadIdx.x;
+    __shared__ float part[kFinishWaves][kWave];
+    __shared__ int part_count[kFinishWaves][kWave];
+    __shared__ int part_members[kFinishWaves];
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, e = blockIdx.y * kWave + lane;
+    const int begin = sequence_begin(c.offsets, b, c.sequences, c.tokens), end = sequence_begin(c.offsets, b + 1, c.sequences, c.tokens);
+    const int first = begin / c.chunk, last = end > begin ? (end - 1) / c.chunk : first - 1;
     float sum = 0.0f;
-    int count = 0;
-    if (e < c.experts) {
-        for (int i = first; i <= last; ++i) {
-            sum += c.sums[static_cast<size_t>(i + b) * c.experts + e];
-            count += c.counts[static_cast<size_t>(i + b) * c.experts + e];
-        }
-        counts[static_cast<size_t>(b) * c.experts + e] = count;
+    int count = 0, held = 0;
+    const int at = min(e, c.experts - 1);
+#pragma unroll 4
+    for (int i = first + wave; i <= last; i += kFinishWaves) {
+        const size_t row = static_cast<size_t>(i + b);
+        sum += c.sums[row * c.experts + at];
+        count += c.counts[row * c.experts + at];
+        held += c.members[row];
     }
-    float product = wave_sum(sum * static_cast<float>(count));
-    int total = count;
-    for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
-    if (lane == 0) {
-        part[wave] = product;
-        routes[wave] = total;
-    }
+    part[wave][lane] = sum;
+    part_count[wave][lane] = count;
+    if (lane == 0) part_members[wave] = held;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int held = 0;
-        for (int i = first; i <= last; ++i) held += c.members[i + b];
-        product = 0.0f;
-        total = 0;
-        for (int w = 0; w < kFinishThreads / kWave; ++w) {
-            product += part[w];
-            total += routes[w];
-        }
-        losses[b] = held > 0 ? product / static_cast<float>(held) * (static_cast<float>(c.experts) / static_cast<float>(total)) : 0.0f;
-        members[b] = held;
+    if (wave != 0) return;
+    sum = 0.0f;
+    count = held = 0;
+#pragma unroll
+    for (int w = 0; w < kFinishWaves; ++w) {
+        sum += part[w][lane];
+        count += part_count[w][lane];
+        held += part_members[w];
     }
+    if (e < c.experts) c.all_counts[static_cast<size_t>(b) * c.experts + e] = count;
+    else count = 0;
+    const float product = wave_sum(sum * static_cast<float>(count));
+    const int routes = wave_total(count);
+    if (lane != 0) return;
+    // (relaxed stores that go past this die's cache, then the ticket; the last one reads them the same way)
+    const int pieces = gridDim.y;
+    __hip_atomic_store(c.products + b * pieces + blockIdx.y, product, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(c.routes + b * pieces + blockIdx.y, routes, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t ticket = __hip_atomic_fetch_add(c.tickets + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    if (ticket != static_cast<uint32_t>(pieces) - 1) return;
+    float all = 0.0f;
+    int total = 0;
+    for (int i = 0; i < pieces; ++i) {
+        all += __hip_atomic_load(c.products + b * pieces + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        total += __hip_atomic_load(c.routes + b * pieces + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    c.losses[b] = held > 0 ? all / static_cast<float>(held) * (static_cast<float>(c.experts) / static_cast<float>(total)) : 0.0f;
+    c.all_members[b] = held;
 }
 
 // ---- gradient of the logits --------------------------------------------------------------------------------------------------------
@@ -341,91 +517,109 @@ struct Backward {
     const int32_t* members;
     const float* grad_losses;
     void* grad_logits;
-    int tokens, experts, topk, sequences;
-    bool normalize, wide;
+    int tokens, experts, topk, sequences, chunk;
+    bool normalize, wide, whole;
     float scale;
 };
 
 template <int V, int kType, bool kSigmoid>
 __global__ __launch_bounds__(kRouterThreads) void router_backward_kernel(const Backward c)
 {
-    __shared__ float rows[kRouterWaves][kWave * V];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int token = blockIdx.x * kRouterWaves + wave;
-    if (token >= c.tokens) return;
-    const size_t row = static_cast<size_t>(token) * c.experts, slot = static_cast<size_t>(token) * c.topk + lane;
-    const int e = lane < c.topk ? load_index(c.topk_idx, c.wide, slot, c.experts) : -1;
-    const bool padding = __ballot(e >= 0) == 0;
-    float grad[V] = {};
-    const bool dense = c.grad_weights != nullptr && !kSigmoid && !c.normalize;
-    float p[V], s[V], inverse = 0.0f;
-    if (!padding && (dense || c.counts != nullptr))
-        row_probabilities<V, kType, kSigmoid>(c.logits, row, c.experts, lane, p, s, inverse);
-    if (!padding && c.counts != nullptr) {
-        // softmax: a p (f - sum f p); sigmoid: a s (1 - s) / sum s (f - sum f p);  a = grad / N
-        const int b = sequence_of(c.offsets, c.sequences, token);
-        float f[V], mean = 0.0f;
-        int routes = 0;
+    __shared__ __attribute__((aligned(16))) float rows[kRouterWaves][kWave * V];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int first = blockIdx.x * c.chunk, last = min(first + c.chunk, c.tokens);
+    const bool dense = c.grad_weights != nullptr && !kSigmoid && !c.normalize, balance = c.counts != nullptr;
+    float* const mine = rows[wave];
+    // the sequence of the token at hand: its loads f, where it ends, and grad / N
+    float f[V] = {}, of_loss = 0.0f;
+    int sequence = -1, sequence_end = 0;
+    Piece<V, kType> next = {};
+    if ((dense || balance) && first + wave < last) next.load(c.logits, static_cast<size_t>(first + wave) * c.experts, c.experts, lane, c.whole);
+    for (int t = first + wave; t < last; t += kRouterWaves) {
+        const size_t row = static_cast<size_t>(t) * c.experts, slot = static_cast<size_t>(t) * c.topk + lane;
+        const Piece<V, kType> piece = next;
+        if ((dense || balance) && t + kRouterWaves < last)
+            next.load(c.logits, static_cast<size_t>(t + kRouterWaves) * c.experts, c.experts, lane, c.whole);
+        const int e = lane < c.topk ? load_index(c.topk_idx, c.wide, slot, c.experts) : -1;
+        const bool padding = __ballot(e >= 0) == 0;
+        float grad[V] = {}, s[V] = {}, inverse = 0.0f;
+        if (!padding && (dense || balance)) {
+            float z[V], grown[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int at = lane * V + v;
-            const int count = at < c.experts ? c.counts[static_cast<size_t>(b) * c.experts + at] : 0;
-            routes += count;
-            f[v] = static_cast<float>(count);
-        }
-        for (int d = 32; d > 0; d >>= 1) routes += __shfl_xor(routes, d);
-        const float unit = routes > 0 ? static_cast<float>(c.experts) / static_cast<float>(routes) : 0.0f;
+            for (int v = 0; v < V; ++v) z[v] = piece.value(v, c.experts, lane);
+            inverse = row_scores<V, kSigmoid>(z, s, grown);
+            if (balance) {
+                // softmax: a p (f - sum f p); sigmoid: a s (1 - s) / sum s (f - sum f p);  a = grad / N
+                if (t >= sequence_end) {
+                    sequence = sequence < 0 ? sequence_of(c.offsets, c.sequences, t) : sequence;
+                    while (sequence + 1 < c.sequences && sequence_begin(c.offsets, sequence + 1, c.sequences, c.tokens) <= t) ++sequence;
+                    sequence_end = sequence_begin(c.offsets, sequence + 1, c.sequences, c.tokens);
+                    int routes = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            f[v] *= unit;
-            mean += f[v] * p[v];
-        }
-        mean = wave_sum(mean);
-        const float a = c.grad_losses[b] / static_cast<float>(max(c.members[b], 1));
+                    for (int v = 0; v < V; ++v) {
+                        const int at = lane * V + v, count = at < c.experts ? c.counts[static_cast<size_t>(sequence) * c.experts + at] : 0;
+                        routes += count;
+                        f[v] = static_cast<float>(count);
+                    }
+                    routes = wave_total(routes);
+                    const float unit = routes > 0 ? static_cast<float>(c.experts) / static_cast<float>(routes) : 0.0f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) grad[v] = a * (f[v] - mean) * (kSigmoid ? s[v] * inverse : p[v]);
-    }
-    if (c.grad_weights != nullptr) {
+                    for (int v = 0; v < V; ++v) f[v] *= unit;
+                    of_loss = c.grad_losses[sequence] / static_cast<float>(max(c.members[sequence], 1));
+                }
+                float mean = 0.0f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) rows[wave][lane * V + v] = 0.0f;
-        wave_sync();
-        float g = e >= 0 ? c.grad_weights[slot] * c.scale : 0.0f, through = 0.0f;
-        if (c.normalize) {
-            const float w = e >= 0 ? c.topk_weights[slot] / c.scale : 0.0f;
-            const float inner = wave_sum(g * w);
-            g = e >= 0 ? g - inner : 0.0f;
-            through = w * g;
-        }
-        if constexpr (kSigmoid) {
-            const float z = e >= 0 ? load_logit<kType>(c.logits, row + e) : 0.0f;
-            const float score = e >= 0 ? sigmoid(z) : 0.0f;
-            through = g * score * sigmoid(-z);
-            if (c.normalize) through = through / (wave_sum(score) + kTiny);
-        }
-        if (dense) {
-            // p_e ([e chosen] g_e - sum_j g_j p_j)
-            if (e >= 0) atomicAdd(&rows[wave][e], g);
-            wave_sync();
-            float inner = 0.0f, own[V];
+                for (int v = 0; v < V; ++v) mean += f[v] * (s[v] * inverse);
+                mean = wave_sum(mean);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                own[v] = rows[wave][lane * V + v];
-                inner += padding ? 0.0f : own[v] * p[v];
+                for (int v = 0; v < V; ++v) {
+                    // 1 - s = exp(-z) s (the difference would cancel); where exp(-z) is past the range, s is 0
+                    const float slope = kSigmoid ? s[v] * (fminf(grown[v], 3e38f) * s[v]) : s[v];
+                    grad[v] = of_loss * (f[v] - mean) * (z[v] == -kInf ? 0.0f : slope * inverse);
+                }
             }
-            inner = wave_sum(inner);
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (!padding) grad[v] += p[v] * (own[v] - inner);
-        } else {
-            if (e >= 0) atomicAdd(&rows[wave][e], through);
-            wave_sync();
-#pragma unroll
-            for (int v = 0; v < V; ++v) grad[v] += rows[wave][lane * V + v];
         }
-    }
+        if (c.grad_weights != nullptr && !padding) {
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-        if (lane * V + v < c.experts) store_logit<kType>(c.grad_logits, row + lane * V + v, grad[v]);
+            for (int v = 0; v < V; ++v) mine[lane * V + v] = 0.0f;
+            wave_sync();
+            float g = e >= 0 ? c.grad_weights[slot] * c.scale : 0.0f, through = 0.0f;
+            if (c.normalize) {
+                const float w = e >= 0 ? c.topk_weights[slot] / c.scale : 0.0f;
+                const float inner = wave_sum(g * w);
+                g = e >= 0 ? g - inner : 0.0f;
+                through = w * g;
+            }
+            if constexpr (kSigmoid) {
+                const float z = e >= 0 ? load_logit<kType>(c.logits, row + e) : 0.0f;
+                const float grown = expf(-z), score = e >= 0 ? sigmoid(z) : 0.0f;
+                through = g * score * (fminf(grown, 3e38f) * score);
+                if (c.normalize) through = through / (wave_sum(score) + kTiny);
+            }
+            if (e >= 0) atomicAdd(&mine[e], dense ? g : through);
+            wave_sync();
+            float own[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) own[v] = mine[lane * V + v];
+            if (dense) {
+                // p_e ([e chosen] g_e - sum_j g_j p_j)
+                float inner = 0.0f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) inner += own[v] * (s[v] * inverse);
+                inner = wave_sum(inner);
+#pragma unroll
+                for (int v = 0; v < V; ++v) grad[v] += s[v] * inverse * (own[v] - inner);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) grad[v] += own[v];
+            }
+            wave_sync();
+        }
+        Piece<V, kType> out;
+#pragma unroll
+        for (int v = 0; v < V; ++v) out.set(v, grad[v]);
+        out.store(c.grad_logits, row, c.experts, lane, c.whole);
+    }
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------
@@ -450,7 +644,36 @@ void with_variant(const dpep_router* r, F&& f)
     else by_type(std::integral_constant<int, 16>{});
 }
 
-int balance_chunk(int tokens) { return std::max(64, (tokens + 511) / 512); }
+// Registers of a lane for a number of experts, as with_variant chooses them.
+int row_registers(int experts)
+{
+    int v = 1;
+    while (v * kWave < experts) v *= 2;
+    return v;
+}
+// Whether rows of `experts` logits can be read in pieces of a lane's registers.
+bool whole_pieces(const dpep_router* r, const void* a, const void* b)
+{
+    const size_t piece = std::min<size_t>(16, row_registers(r->num_experts) * (r->logits_type == DPEP_TYPE_F32 ? 4 : 2));
+    return r->num_experts % row_registers(r->num_experts) == 0 && (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % piece == 0;
+}
+// Tokens to a workgroup: about two workgroups of eight waves to a CU; rows of sums stay few.
+int router_chunk(int tokens) { return std::max(kRouterWaves, (tokens + 511) / 512); }
+
+// Scratch of a balance loss.
+struct BalanceScratch {
+    size_t counts, members, tickets, products, routes, bytes;
+    BalanceScratch(int experts, int tokens, int sequences)
+    {
+        const size_t chunk = router_chunk(tokens), rows = (tokens + chunk - 1) / chunk + sequences, pieces = (experts + kWave - 1) / kWave;
+        counts = rows * experts * 4;
+        members = counts + rows * experts * 4;
+        tickets = members + rows * 4;
+        products = tickets + static_cast<size_t>(sequences) * 4;
+        routes = products + sequences * pieces * 4;
+        bytes = routes + sequences * pieces * 4;
+    }
+};
 
 int check_router(const dpep_router* r, int num_tokens, const char* what)
 {
@@ -474,6 +697,57 @@ int check_router(const dpep_router* r, int num_tokens, const char* what)
 
 using namespace dpep;
 
+namespace {
+
+// Choice (out: topk_idx, topk_weights), balance sums, or both in one pass.
+int run_forward(const dpep_router* r, Forward call, int num_tokens, bool route, bool balance, float* losses, int32_t* counts, int32_t* tokens, void* scratch,
+                void* stream, const char* what)
+{
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int experts = r->num_experts, v = row_registers(experts), width = experts / r->num_groups;
+    call.groups = r->num_groups;
+    call.topk_groups = r->num_topk_groups;
+    call.group_lanes = width % v == 0 && width / v <= 16 && (width / v & (width / v - 1)) == 0 ? width / v : 0;
+    call.normalize = r->normalize != 0;
+    call.scale = r->scale;
+    call.tokens = num_tokens;
+    call.experts = experts;
+    call.topk = r->num_topk;
+    call.chunk = router_chunk(num_tokens);
+    call.wide = r->index_bytes == 8;
+    call.whole = whole_pieces(r, call.logits, nullptr);
+    const BalanceScratch at(experts, num_tokens, call.sequences);
+    unsigned char* const base = static_cast<unsigned char*>(scratch);
+    if (balance) {
+        call.sums = reinterpret_cast<float*>(base);
+        call.counts = reinterpret_cast<int32_t*>(base + at.counts);
+        call.members = reinterpret_cast<int32_t*>(base + at.members);
+        call.tickets = reinterpret_cast<uint32_t*>(base + at.tickets);
+    }
+    const int chunks = std::max(1, (num_tokens + call.chunk - 1) / call.chunk);  // (without tokens: the one that clears the tickets)
+    with_variant(r, [&](auto registers, auto type, auto sigmoid) {
+        if (route && balance) router_forward_kernel<registers(), type(), sigmoid(), true, true><<<chunks, kRouterThreads, 0, s>>>(call);
+        else if (route) router_forward_kernel<registers(), type(), sigmoid(), true, false><<<chunks, kRouterThreads, 0, s>>>(call);
+        else router_forward_kernel<registers(), type(), sigmoid(), false, true><<<chunks, kRouterThreads, 0, s>>>(call);
+    });
+    if (balance) {
+        const Finish finish = {call.sums, call.counts, call.members, call.offsets, call.tickets, reinterpret_cast<float*>(base + at.products),
+                               reinterpret_cast<int32_t*>(base + at.routes), losses, counts, tokens, num_tokens, experts, call.sequences, call.chunk};
+        balance_finish_kernel<<<dim3(call.sequences, (experts + kWave - 1) / kWave), kFinishWaves * kWave, 0, s>>>(finish);
+    }
+    return launch_status(what);
+}
+
+int check_balance(const dpep_router* r, const int32_t* sequence_offsets, int num_sequences, const float* losses, const int32_t* counts, const int32_t* tokens,
+                  const void* scratch, const char* what)
+{
+    DPEP_REQUIRE(num_sequences >= 1 && (sequence_offsets != nullptr || num_sequences == 1), "%s: num_sequences=%d", what, num_sequences);
+    DPEP_REQUIRE(losses != nullptr && counts != nullptr && tokens != nullptr && scratch != nullptr, "%s: a NULL buffer", what);
+    return DPEP_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 int dpep_route(const dpep_router* r, const void* logits, const float* bias, const uint8_t* token_mask, int num_tokens, void* topk_idx,
@@ -483,39 +757,52 @@ int dpep_route(const dpep_router* r, const void* logits, const float* bias, cons
     DPEP_REQUIRE(bias == nullptr || r->score == DPEP_SCORE_SIGMOID, "route: a bias needs sigmoid scores");
     if (num_tokens == 0) return DPEP_OK;
     DPEP_REQUIRE(logits != nullptr && topk_idx != nullptr && topk_weights != nullptr, "route: a NULL buffer");
-    const Route call = {logits, bias, token_mask, topk_idx, topk_weights, num_tokens, r->num_experts, r->num_topk, r->num_groups, r->num_topk_groups,
-                        r->normalize != 0, r->index_bytes == 8, r->scale};
-    with_variant(r, [&](auto v, auto type, auto sigmoid) {
-        route_kernel<v(), type(), sigmoid()><<<(num_tokens + kRouterWaves - 1) / kRouterWaves, kRouterThreads, 0, static_cast<hipStream_t>(stream)>>>(call);
-    });
-    return launch_status("route");
+    Forward call = {};
+    call.logits = logits;
+    call.bias = bias;
+    call.token_mask = token_mask;
+    call.topk_idx = topk_idx;
+    call.topk_weights = topk_weights;
+    call.sequences = 1;
+    return run_forward(r, call, num_tokens, true, false, nullptr, nullptr, nullptr, nullptr, stream, "route");
 }
 
 size_t dpep_balance_scratch_bytes(int num_experts, int num_tokens, int num_sequences)
 {
     if (num_experts < 1 || num_tokens < 0 || num_sequences < 1) return 0;
-    const size_t chunk = balance_chunk(num_tokens), rows = (num_tokens + chunk - 1) / chunk + num_sequences;
-    return rows * (static_cast<size_t>(num_experts) * 8 + 4);
+    return BalanceScratch(num_experts, num_tokens, num_sequences).bytes;
 }
 
 int dpep_balance_loss(const dpep_router* r, const void* logits, const void* topk_idx, int num_tokens, const int32_t* sequence_offsets, int num_sequences,
                       float* losses, int32_t* counts, int32_t* tokens, void* scratch, void* stream)
 {
     if (int rc = check_router(r, num_tokens, "balance_loss"); rc != DPEP_OK) return rc;
-    DPEP_REQUIRE(num_sequences >= 1 && (sequence_offsets != nullptr || num_sequences == 1), "balance_loss: num_sequences=%d", num_sequences);
-    DPEP_REQUIRE(losses != nullptr && counts != nullptr && tokens != nullptr && scratch != nullptr, "balance_loss: a NULL buffer");
+    if (int rc = check_balance(r, sequence_offsets, num_sequences, losses, counts, tokens, scratch, "balance_loss"); rc != DPEP_OK) return rc;
     DPEP_REQUIRE(num_tokens == 0 || (logits != nullptr && topk_idx != nullptr), "balance_loss: a NULL buffer");
-    const int chunk = balance_chunk(num_tokens), chunks = (num_tokens + chunk - 1) / chunk;
-    const size_t rows = static_cast<size_t>(chunks) + num_sequences;
-    float* sums = static_cast<float*>(scratch);
-    int32_t* partial_counts = reinterpret_cast<int32_t*>(sums + rows * r->num_experts);
-    const Balance call = {logits, topk_idx, sequence_offsets, num_tokens, r->num_experts, r->num_topk, num_sequences, chunk, chunks, r->index_bytes == 8,
-                          sums, partial_counts, partial_counts + rows * r->num_experts};
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (chunks > 0)
-        with_variant(r, [&](auto v, auto type, auto sigmoid) { balance_sums_kernel<v(), type(), sigmoid()><<<chunks, kRouterThreads, 0, s>>>(call); });
-    balance_finish_kernel<<<num_sequences, kFinishThreads, 0, s>>>(call, losses, counts, tokens);
-    return launch_status("balance_loss");
+    Forward call = {};
+    call.logits = logits;
+    call.topk_idx = const_cast<void*>(topk_idx);
+    call.offsets = sequence_offsets;
+    call.sequences = num_sequences;
+    return run_forward(r, call, num_tokens, false, true, losses, counts, tokens, scratch, stream, "balance_loss");
+}
+
+int dpep_route_balance(const dpep_router* r, const void* logits, const float* bias, const uint8_t* token_mask, int num_tokens, const int32_t* sequence_offsets,
+                       int num_sequences, void* topk_idx, float* topk_weights, float* losses, int32_t* counts, int32_t* tokens, void* scratch, void* stream)
+{
+    if (int rc = check_router(r, num_tokens, "route_balance"); rc != DPEP_OK) return rc;
+    DPEP_REQUIRE(bias == nullptr || r->score == DPEP_SCORE_SIGMOID, "route_balance: a bias needs sigmoid scores");
+    if (int rc = check_balance(r, sequence_offsets, num_sequences, losses, counts, tokens, scratch, "route_balance"); rc != DPEP_OK) return rc;
+    DPEP_REQUIRE(num_tokens == 0 || (logits != nullptr && topk_idx != nullptr && topk_weights != nullptr), "route_balance: a NULL buffer");
+    Forward call = {};
+    call.logits = logits;
+    call.bias = bias;
+    call.token_mask = token_mask;
+    call.topk_idx = topk_idx;
+    call.topk_weights = topk_weights;
+    call.offsets = sequence_offsets;
+    call.sequences = num_sequences;
+    return run_forward(r, call, num_tokens, true, true, losses, counts, tokens, scratch, stream, "route_balance");
 }
 
 int dpep_router_backward(const dpep_router* r, const dpep_router_gradients* g, int num_tokens, void* stream)
@@ -531,9 +818,11 @@ int dpep_router_backward(const dpep_router* r, const dpep_router_gradients* g, i
     DPEP_REQUIRE(g->logits != nullptr && g->topk_idx != nullptr && g->grad_logits != nullptr, "router_backward: a NULL buffer");
     const bool balance = g->grad_losses != nullptr;
     const Backward call = {g->logits, g->topk_idx, g->topk_weights, g->grad_weights, g->sequence_offsets, balance ? g->counts : nullptr, g->tokens, g->grad_losses,
-                           g->grad_logits, num_tokens, r->num_experts, r->num_topk, balance ? g->num_sequences : 1, r->normalize != 0, r->index_bytes == 8, r->scale};
+                           g->grad_logits, num_tokens, r->num_experts, r->num_topk, balance ? g->num_sequences : 1, router_chunk(num_tokens), r->normalize != 0,
+                           r->index_bytes == 8, whole_pieces(r, g->logits, g->grad_logits), r->scale};
+    const int chunks = (num_tokens + call.chunk - 1) / call.chunk;
     with_variant(r, [&](auto v, auto type, auto sigmoid) {
-        router_backward_kernel<v(), type(), sigmoid()><<<(num_tokens + kRouterWaves - 1) / kRouterWaves, kRouterThreads, 0, static_cast<hipStream_t>(stream)>>>(call);
+        router_backward_kernel<v(), type(), sigmoid()><<<chunks, kRouterThreads, 0, static_cast<hipStream_t>(stream)>>>(call);
     });
     return launch_status("router_backward");
 }

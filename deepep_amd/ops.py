@@ -632,6 +632,31 @@ def balance_loss(spec: RouterSpec, logits, topk_idx, sequence_offsets=None):
     return losses, counts, members
 
 
+def route_balance(spec: RouterSpec, logits, bias=None, token_mask=None, sequence_offsets=None, index_dtype=torch.int64):
+    """``route`` and the ``balance_loss`` of its routes in one pass: ``(topk_idx, topk_weights, losses, counts, tokens)``."""
+    tokens, dev = _require_logits(spec, logits)
+    if index_dtype not in (torch.int64, torch.int32):
+        raise ValueError("index_dtype must be torch.int64 or torch.int32")
+    if bias is not None:
+        _require("bias", bias, torch.float32, (spec.num_experts,), dev)
+    if token_mask is not None:
+        _require("token_mask", token_mask, torch.bool, (tokens,), dev)
+    sequences = _require_sequences(sequence_offsets, dev)
+    spec.index_bytes = 8 if index_dtype == torch.int64 else 4
+    lib = _lib.load()
+    topk_idx = torch.empty((tokens, spec.num_topk), dtype=index_dtype, device=dev)
+    topk_weights = torch.empty((tokens, spec.num_topk), dtype=torch.float32, device=dev)
+    losses = torch.empty((sequences,), dtype=torch.float32, device=dev)
+    counts = torch.empty((sequences, spec.num_experts), dtype=torch.int32, device=dev)
+    members = torch.empty((sequences,), dtype=torch.int32, device=dev)
+    scratch = torch.empty((lib.dpep_balance_scratch_bytes(spec.num_experts, tokens, sequences),), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        status = lib.dpep_route_balance(ctypes.byref(spec), _ptr(logits), _ptr(bias), _ptr(token_mask), tokens, _ptr(sequence_offsets), sequences,
+                                        _ptr(topk_idx), _ptr(topk_weights), _ptr(losses), _ptr(counts), _ptr(members), _ptr(scratch), _stream(dev))
+    _lib.check(status, "route_balance")
+    return topk_idx, topk_weights, losses, counts, members
+
+
 def router_backward(spec: RouterSpec, logits, topk_idx, topk_weights=None, grad_weights=None, sequence_offsets=None, counts=None,
                     tokens=None, grad_losses=None):
     """Gradient of ``logits`` in their type, from ``grad_weights`` FP32 [T,K], from ``grad_losses`` FP32 [B] with what

@@ -90,9 +90,10 @@ class Router:
 
     def route_with_balance(self, logits: torch.Tensor, bias: Optional[torch.Tensor] = None, token_mask: Optional[torch.Tensor] = None, *,
                            sequence_offsets: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, BalanceLoss]:
-        """``route`` and the ``balance_loss`` of its routes."""
-        topk_idx, topk_weights = self.route(logits, bias, token_mask)
-        return topk_idx, topk_weights, self.balance_loss(logits, topk_idx, sequence_offsets)
+        """``route`` and the ``balance_loss`` of its routes, in one pass over the logits."""
+        self._check_bias(bias)
+        topk_idx, topk_weights, *sums = ops.route_balance(self._spec(), logits, bias, token_mask, sequence_offsets, self.index_dtype)
+        return topk_idx, topk_weights, BalanceLoss(*sums, sequence_offsets)
 
     def backward(self, logits: torch.Tensor, topk_idx: torch.Tensor, *, topk_weights: Optional[torch.Tensor] = None,
                  grad_weights: Optional[torch.Tensor] = None, balance: Optional[BalanceLoss] = None,

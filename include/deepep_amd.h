@@ -391,6 +391,9 @@ int dpep_route(const dpep_router* r, const void* logits, const float* bias, cons
 size_t dpep_balance_scratch_bytes(int num_experts, int num_tokens, int num_sequences);
 int dpep_balance_loss(const dpep_router* r, const void* logits, const void* topk_idx, int num_tokens, const int32_t* sequence_offsets, int num_sequences,
                       float* losses, int32_t* counts, int32_t* tokens, void* scratch, void* stream);
+/* dpep_route and the dpep_balance_loss of its routes, in one pass over the logits. */
+int dpep_route_balance(const dpep_router* r, const void* logits, const float* bias, const uint8_t* token_mask, int num_tokens, const int32_t* sequence_offsets,
+                       int num_sequences, void* topk_idx, float* topk_weights, float* losses, int32_t* counts, int32_t* tokens, void* scratch, void* stream);
 
 /* Gradient of the logits, in their type, from the gradient of the route weights (grad_weights, as dpep_combine's return channel gives
  * it; entries without a route are not read into it), of the balance losses (grad_losses, with what dpep_balance_loss was given and
