@@ -260,7 +260,7 @@ __device__ __forceinline__ void limit_groups(float (&key)[V], const Forward& c, 
         int ahead = 0;
         for (int o = 0; o < c.groups; ++o) {
             const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), o * c.group_lanes));
-            ahead += other > mine || (other == mine && lane >= (o + 1) * c.group_lanes);
+            ahead += static_cast<int>(other > mine) | (static_cast<int>(other == mine) & static_cast<int>(lane >= (o + 1) * c.group_lanes));
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) key[v] = ahead >= c.topk_groups ? -kInf : key[v];
@@ -296,33 +296,81 @@ __device__ __forceinline__ void limit_groups(float (&key)[V], const Forward& c, 
     wave_sync();
 }
 
-// Lane k gets the expert of slot k, -1 where none is left: each time the largest key of the wave, in its lowest lane and there in the lowest
-// register (experts are counted along lanes, so that is the lowest index).
+// Sorts a lane's keys, largest first and equal ones in their order, and packs where they were, a byte each (V == 16: half a byte).
 template <int V>
-__device__ __forceinline__ int choose(const float (&key)[V], int topk)
+struct Places {
+    static constexpr int kBits = V == 16 ? 4 : 8;
+    using Word = std::conditional_t<V <= 4, uint32_t, uint64_t>;
+    Word word;
+    __device__ __forceinline__ int first() const { return static_cast<int>(word) & ((1 << kBits) - 1); }
+};
+template <int V>
+__device__ __forceinline__ Places<V> sort_keys(int (&key)[V])
+{
+    int at[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) at[v] = v;
+    // a merge of odd and even places; equal keys are told apart by their place
+#pragma unroll
+    for (int p = 1; p < V; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j <= V - 1 - k; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i) {
+                    const int a = i + j, b = i + j + k;
+                    if (b >= V || a / (2 * p) != b / (2 * p)) continue;
+                    const bool swap = (key[b] > key[a]) | ((key[b] == key[a]) & (at[b] < at[a]));
+                    const int high = swap ? key[b] : key[a], low = swap ? key[a] : key[b], first = swap ? at[b] : at[a], second = swap ? at[a] : at[b];
+                    key[a] = high;
+                    key[b] = low;
+                    at[a] = first;
+                    at[b] = second;
+                }
+    Places<V> places = {0};
+#pragma unroll
+    for (int v = 0; v < V; ++v) places.word |= static_cast<typename Places<V>::Word>(at[v]) << (Places<V>::kBits * v);
+    return places;
+}
+
+// Lane k gets the expert of slot k, -1 where none is left: each time the largest key of the wave, in its lowest lane (experts are counted along lanes,
+// and a lane's equal keys stand in their order, so that is the lowest index).  Every lane's keys are sorted first: a step then compares and
+// removes heads alone.  (Finding the register of the largest key in each step took 45 scalar instructions, which issue no faster than the
+// 17 of the vector unit beside them: 65 536 tokens of 256 experts 101 us against 63.)
+template <int V>
+__device__ __forceinline__ int choose(const float (&key)[V], int topk, int self)
 {
     int left[V], mine = -1;
 #pragma unroll
     for (int v = 0; v < V; ++v) left[v] = key[v] == -kInf ? kNone : ordered(key[v]);
+    Places<V> places = sort_keys(left);
     for (int k = 0; k < topk; ++k) {
-        int best = left[0];
-#pragma unroll
-        for (int v = 1; v < V; ++v) best = max(best, left[v]);
-        const int largest = wave_max(best);
+        const int largest = wave_max(left[0]);
         if (largest == kNone) break;
-        const int lane = __ffsll(__ballot(best == largest)) - 1;
-        int at = V - 1;
-        bool open = true;
+        const int lane = __ffsll(__ballot(left[0] == largest)) - 1;
+        const int expert = lane * V + (__builtin_amdgcn_readlane(static_cast<int>(places.word), lane) & ((1 << Places<V>::kBits) - 1));
+        mine = self == k ? expert : mine;
+        const bool taken = __builtin_amdgcn_inverse_ballot_w64(1ull << lane);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const bool here = open && ((__ballot(left[v] == largest) >> lane) & 1) != 0;
-            at = here ? v : at;
-            open = open && !here;
-            left[v] = __builtin_amdgcn_inverse_ballot_w64(here ? 1ull << lane : 0ull) ? kNone : left[v];
-        }
-        mine = (threadIdx.x & 63) == static_cast<unsigned>(k) ? lane * V + at : mine;
+        for (int v = 0; v < V; ++v) left[v] = !taken ? left[v] : v + 1 < V ? left[v + 1] : kNone;
+        places.word = taken ? places.word >> Places<V>::kBits : places.word;
     }
     return mine;
+}
+
+// In lane k: the value that belongs to expert `mine` (0 where there is none) of a row in the wave's registers.
+template <int V>
+__device__ __forceinline__ float pick(const float (&x)[V], int mine)
+{
+    const int owner = max(mine, 0) / V;
+    float found = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(owner * 4, __float_as_int(x[v])));
+        found = mine == owner * V + v ? other : found;
+    }
+    return found;
 }
 
 template <int V, int kType, bool kSigmoid, bool kRoute, bool kBalance>
@@ -351,21 +399,29 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
             for (int e = threadIdx.x; e < c.experts; e += kRouterThreads) counts[e] = 0;
             __syncthreads();
         }
+        // (what the next token needs is asked for while this one is worked on)
         Piece<V, kType> next;
-        if (begin + wave < end) next.load(c.logits, static_cast<size_t>(begin + wave) * c.experts, c.experts, lane, c.whole);
+        int next_route = -1;
+        uint8_t next_real = 1;
+        auto fetch = [&](int t) {
+            if (t >= end) return;
+            next.load(c.logits, static_cast<size_t>(t) * c.experts, c.experts, lane, c.whole);
+            if constexpr (kRoute) next_real = c.token_mask == nullptr ? 1 : c.token_mask[t];
+            else next_route = lane < c.topk ? load_index(c.topk_idx, c.wide, static_cast<size_t>(t) * c.topk + lane, c.experts) : -1;
+        };
+        fetch(begin + wave);
         for (int t = begin + wave; t < end; t += kRouterWaves) {
-            const size_t row = static_cast<size_t>(t) * c.experts, to = static_cast<size_t>(t) * c.topk + lane;
+            const size_t to = static_cast<size_t>(t) * c.topk + lane;
             const Piece<V, kType> piece = next;
-            if (t + kRouterWaves < end) next.load(c.logits, static_cast<size_t>(t + kRouterWaves) * c.experts, c.experts, lane, c.whole);
-            int mine = -1;
-            if constexpr (!kRoute) mine = lane < c.topk ? load_index(c.topk_idx, c.wide, to, c.experts) : -1;
+            const bool real = __builtin_amdgcn_readfirstlane(next_real) != 0;
+            int mine = kRoute ? -1 : next_route;
+            fetch(t + kRouterWaves);
             float z[V], s[V], grown[V], inverse = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) z[v] = piece.value(v, c.experts, lane);
             if (kBalance || (!kSigmoid && !c.normalize)) inverse = row_scores<V, kSigmoid>(z, s, grown);
             else if constexpr (kSigmoid) sigmoids<V>(z, s, grown);
             if constexpr (kRoute) {
-                const bool real = c.token_mask == nullptr || c.token_mask[t] != 0;
                 if (real) {
                     float key[V];
 #pragma unroll
@@ -376,27 +432,20 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
                         key[v] = z[v] == -kInf ? -kInf : fminf(key[v], kInf);
                     }
                     if (c.groups > 1) limit_groups<V, kSigmoid>(key, c, rows_lds[wave], scores_lds[wave], lane);
-                    mine = choose<V>(key, c.topk);
+                    mine = choose<V>(key, c.topk, lane);
                 }
-                float weight = 0.0f;
-                const float chosen = mine >= 0 ? load_logit<kType>(c.logits, row + mine) : -kInf;
+                float weight;
                 if constexpr (kSigmoid) {
-                    weight = mine >= 0 ? sigmoid(chosen) : 0.0f;
+                    weight = pick<V>(s, mine);
                     if (c.normalize) weight = weight / (wave_sum(weight) + kTiny);
                 } else if (c.normalize) {
+                    const float picked = pick<V>(z, mine), chosen = mine >= 0 ? picked : -kInf;
                     const float top = unordered(wave_max(chosen == chosen ? ordered(chosen) : kNone));
                     weight = mine >= 0 ? expf(chosen - top) : 0.0f;
                     const float total = wave_sum(weight);
                     weight = mine >= 0 ? weight / total : 0.0f;
                 } else {
-                    const int owner = mine >= 0 ? mine / V : 0;
-                    float score = 0.0f;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const float other = __int_as_float(__builtin_amdgcn_ds_bpermute(owner * 4, __float_as_int(s[v])));
-                        score = mine - owner * V == v ? other : score;
-                    }
-                    weight = mine >= 0 ? score * inverse : 0.0f;
+                    weight = pick<V>(s, mine) * inverse;
                 }
                 if (lane < c.topk) {
                     if (c.wide) static_cast<int64_t*>(c.topk_idx)[to] = mine;
@@ -534,17 +583,30 @@ __global__ __launch_bounds__(kRouterThreads) void router_backward_kernel(const B
     float f[V] = {}, of_loss = 0.0f;
     int sequence = -1, sequence_end = 0;
     Piece<V, kType> next = {};
-    if ((dense || balance) && first + wave < last) next.load(c.logits, static_cast<size_t>(first + wave) * c.experts, c.experts, lane, c.whole);
+    int next_route = -1;
+    float next_grad = 0.0f, next_weight = 0.0f;
+    auto fetch = [&](int t) {
+        if (t >= last) return;
+        const size_t slot = static_cast<size_t>(t) * c.topk + lane;
+        if (dense || balance) next.load(c.logits, static_cast<size_t>(t) * c.experts, c.experts, lane, c.whole);
+        if (lane >= c.topk) return;
+        next_route = load_index(c.topk_idx, c.wide, slot, c.experts);
+        if (c.grad_weights != nullptr) {
+            next_grad = c.grad_weights[slot];
+            if (c.normalize) next_weight = c.topk_weights[slot];
+        }
+    };
+    fetch(first + wave);
     for (int t = first + wave; t < last; t += kRouterWaves) {
-        const size_t row = static_cast<size_t>(t) * c.experts, slot = static_cast<size_t>(t) * c.topk + lane;
+        const size_t row = static_cast<size_t>(t) * c.experts;
         const Piece<V, kType> piece = next;
-        if ((dense || balance) && t + kRouterWaves < last)
-            next.load(c.logits, static_cast<size_t>(t + kRouterWaves) * c.experts, c.experts, lane, c.whole);
-        const int e = lane < c.topk ? load_index(c.topk_idx, c.wide, slot, c.experts) : -1;
+        const int e = next_route;
+        const float through_weight = next_grad, weight_of_route = next_weight;
+        fetch(t + kRouterWaves);
         const bool padding = __ballot(e >= 0) == 0;
-        float grad[V] = {}, s[V] = {}, inverse = 0.0f;
+        float grad[V] = {}, s[V] = {}, grown[V] = {}, inverse = 0.0f;
         if (!padding && (dense || balance)) {
-            float z[V], grown[V];
+            float z[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) z[v] = piece.value(v, c.experts, lane);
             inverse = row_scores<V, kSigmoid>(z, s, grown);
@@ -583,17 +645,24 @@ __global__ __launch_bounds__(kRouterThreads) void router_backward_kernel(const B
 #pragma unroll
             for (int v = 0; v < V; ++v) mine[lane * V + v] = 0.0f;
             wave_sync();
-            float g = e >= 0 ? c.grad_weights[slot] * c.scale : 0.0f, through = 0.0f;
+            float g = e >= 0 ? through_weight * c.scale : 0.0f, through = 0.0f;
             if (c.normalize) {
-                const float w = e >= 0 ? c.topk_weights[slot] / c.scale : 0.0f;
+                const float w = e >= 0 ? weight_of_route / c.scale : 0.0f;
                 const float inner = wave_sum(g * w);
                 g = e >= 0 ? g - inner : 0.0f;
                 through = w * g;
             }
             if constexpr (kSigmoid) {
-                const float z = e >= 0 ? load_logit<kType>(c.logits, row + e) : 0.0f;
-                const float grown = expf(-z), score = e >= 0 ? sigmoid(z) : 0.0f;
-                through = g * score * (fminf(grown, 3e38f) * score);
+                float score, of_exp;
+                if (balance) {
+                    score = pick<V>(s, e);
+                    of_exp = pick<V>(grown, e);
+                } else {
+                    const float z = e >= 0 ? load_logit<kType>(c.logits, row + e) : 0.0f;
+                    of_exp = expf(-z);
+                    score = e >= 0 ? sigmoid(z) : 0.0f;
+                }
+                through = g * score * (fminf(of_exp, 3e38f) * score);
                 if (c.normalize) through = through / (wave_sum(score) + kTiny);
             }
             if (e >= 0) atomicAdd(&mine[e], dense ? g : through);
@@ -657,8 +726,8 @@ bool whole_pieces(const dpep_router* r, const void* a, const void* b)
     const size_t piece = std::min<size_t>(16, row_registers(r->num_experts) * (r->logits_type == DPEP_TYPE_F32 ? 4 : 2));
     return r->num_experts % row_registers(r->num_experts) == 0 && (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % piece == 0;
 }
-// Tokens to a workgroup: about two workgroups of eight waves to a CU; rows of sums stay few.
-int router_chunk(int tokens) { return std::max(kRouterWaves, (tokens + 511) / 512); }
+// Tokens to a workgroup: about four workgroups of eight waves to a CU; rows of sums stay few.
+int router_chunk(int tokens) { return std::max(kRouterWaves, (tokens + 1023) / 1024); }
 
 // Scratch of a balance loss.
 struct BalanceScratch {
