@@ -1363,6 +1363,247 @@ PyObject* cast_back(PyObject*, PyObject* const* a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+// ---- router and 4-bit products ---------------------------------------------------------------------------------------------------
+// The kernels of a decode step's router or matrix take 4 to 8 us; the same calls through the Python layer take 11.
+// A tensor argument that may be None: true if it is, or is a plain one of this type and shape.
+inline bool optional_plain(PyObject* o, int device, at::ScalarType type, std::initializer_list<int64_t> shape, const at::Tensor** out)
+{
+    *out = nullptr;
+    if (o == Py_None) return true;
+    const at::Tensor* t = plain(o, device);
+    if (t == nullptr || t->scalar_type() != type || t->dim() != static_cast<int64_t>(shape.size())) return false;
+    int64_t d = 0;
+    for (const int64_t n : shape)
+        if (t->size(d++) != n) return false;
+    *out = t;
+    return true;
+}
+inline int type_code(at::ScalarType t) { return t == at::kFloat ? DPEP_TYPE_F32 : t == at::kBFloat16 ? DPEP_TYPE_BF16 : t == at::kHalf ? DPEP_TYPE_F16 : -1; }
+template <class T>
+T* data(const at::Tensor* t)
+{
+    return t != nullptr ? static_cast<T*>(t->data_ptr()) : nullptr;
+}
+// A tuple of new tensors' Python objects.
+PyObject* tuple_of(std::initializer_list<at::Tensor> tensors)
+{
+    Ref tuple(PyTuple_New(static_cast<Py_ssize_t>(tensors.size())));
+    if (!tuple) return nullptr;
+    Py_ssize_t i = 0;
+    for (const at::Tensor& t : tensors) {
+        PyObject* o = wrap(t);
+        if (o == nullptr) return nullptr;
+        PyTuple_SET_ITEM(tuple.p, i++, o);
+    }
+    return tuple.release();
+}
+
+struct Router {
+    PyObject_HEAD
+    dpep_router spec;
+};
+extern PyTypeObject RouterType;
+// Router(experts, top-k, groups, top-k groups, score, normalize, scale, bytes of an id)
+PyObject* Router_new(PyTypeObject* type, PyObject* args, PyObject*)
+{
+    dpep_router r = {};
+    double scale;
+    if (!PyArg_ParseTuple(args, "iiiiiidi", &r.num_experts, &r.num_topk, &r.num_groups, &r.num_topk_groups, &r.score, &r.normalize, &scale, &r.index_bytes))
+        return nullptr;
+    r.scale = static_cast<float>(scale);
+    Router* self = reinterpret_cast<Router*>(type->tp_alloc(type, 0));
+    if (self != nullptr) self->spec = r;
+    return reinterpret_cast<PyObject*>(self);
+}
+// The logits of a call this path takes, [T,E] on the current GPU; nullptr otherwise.
+const at::Tensor* router_logits(PyObject* o, dpep_router* r, int* device)
+{
+    if (!on_gpu(o) || c10::InferenceMode::is_enabled()) return nullptr;
+    *device = c10::hip::current_device();
+    const at::Tensor* t = plain(o, *device);
+    if (t == nullptr || t->dim() != 2 || t->size(1) != r->num_experts || t->size(0) > 0x7fffffff || (r->logits_type = type_code(t->scalar_type())) < 0) return nullptr;
+    return t;
+}
+// Number of sequences, 0 for offsets this path does not take.
+int64_t router_sequences(PyObject* o, int device, const at::Tensor** offsets)
+{
+    *offsets = nullptr;
+    if (o == Py_None) return 1;
+    const at::Tensor* t = plain(o, device);
+    if (t == nullptr || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) < 2 || t->size(0) > 0x7fffffff) return 0;
+    *offsets = t;
+    return t->size(0) - 1;
+}
+// route(logits, bias, token_mask) -> (ids, weights); route(logits, bias, token_mask, offsets) -> (ids, weights, losses, counts, tokens)
+PyObject* Router_route(PyObject* o, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    dpep_router r = reinterpret_cast<Router*>(o)->spec;
+    int device;
+    const at::Tensor* logits = n == 3 || n == 4 ? router_logits(a[0], &r, &device) : nullptr;
+    if (logits == nullptr) Py_RETURN_NONE;
+    const int64_t tokens = logits->size(0);
+    const at::Tensor *bias, *mask, *offsets = nullptr;
+    if (!optional_plain(a[1], device, at::kFloat, {r.num_experts}, &bias) || !optional_plain(a[2], device, at::kBool, {tokens}, &mask)) Py_RETURN_NONE;
+    const int64_t sequences = n == 4 ? router_sequences(a[3], device, &offsets) : 1;
+    if (sequences == 0) Py_RETURN_NONE;
+    at::Tensor idx = allocate({tokens, r.num_topk}, r.index_bytes == 8 ? at::kLong : at::kInt, device);
+    at::Tensor weights = allocate({tokens, r.num_topk}, at::kFloat, device);
+    const hipStream_t stream = current_stream(device).raw;
+    if (n == 3) {
+        if (const int status = dpep_route(&r, logits->data_ptr(), data<float>(bias), data<uint8_t>(mask), static_cast<int>(tokens), idx.data_ptr(),
+                                          static_cast<float*>(weights.data_ptr()), stream))
+            return raise_native(status);
+        return tuple_of({std::move(idx), std::move(weights)});
+    }
+    at::Tensor losses = allocate({sequences}, at::kFloat, device), counts = allocate({sequences, r.num_experts}, at::kInt, device);
+    at::Tensor members = allocate({sequences}, at::kInt, device);
+    at::Tensor scratch = allocate({static_cast<int64_t>(dpep_balance_scratch_bytes(r.num_experts, static_cast<int>(tokens), static_cast<int>(sequences)))}, at::kByte, device);
+    if (const int status = dpep_route_balance(&r, logits->data_ptr(), data<float>(bias), data<uint8_t>(mask), static_cast<int>(tokens), data<int32_t>(offsets),
+                                              static_cast<int>(sequences), idx.data_ptr(), static_cast<float*>(weights.data_ptr()), static_cast<float*>(losses.data_ptr()),
+                                              static_cast<int32_t*>(counts.data_ptr()), static_cast<int32_t*>(members.data_ptr()), scratch.data_ptr(), stream))
+        return raise_native(status);
+    return tuple_of({std::move(idx), std::move(weights), std::move(losses), std::move(counts), std::move(members)});
+    END_HANDLE_TH_ERRORS
+}
+// Ids [T,K] of either width.
+const at::Tensor* router_ids(PyObject* o, dpep_router* r, int64_t tokens, int device)
+{
+    const at::Tensor* t = plain(o, device);
+    if (t == nullptr || !has_shape(*t, tokens, r->num_topk) || (t->scalar_type() != at::kLong && t->scalar_type() != at::kInt)) return nullptr;
+    r->index_bytes = t->scalar_type() == at::kLong ? 8 : 4;
+    return t;
+}
+// balance_loss(logits, ids, offsets) -> (losses, counts, tokens)
+PyObject* Router_balance_loss(PyObject* o, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    dpep_router r = reinterpret_cast<Router*>(o)->spec;
+    int device;
+    const at::Tensor *logits = n == 3 ? router_logits(a[0], &r, &device) : nullptr, *offsets;
+    if (logits == nullptr) Py_RETURN_NONE;
+    const int64_t tokens = logits->size(0);
+    const at::Tensor* idx = router_ids(a[1], &r, tokens, device);
+    if (idx == nullptr) Py_RETURN_NONE;
+    const int64_t sequences = router_sequences(a[2], device, &offsets);
+    if (sequences == 0) Py_RETURN_NONE;
+    at::Tensor losses = allocate({sequences}, at::kFloat, device), counts = allocate({sequences, r.num_experts}, at::kInt, device);
+    at::Tensor members = allocate({sequences}, at::kInt, device);
+    at::Tensor scratch = allocate({static_cast<int64_t>(dpep_balance_scratch_bytes(r.num_experts, static_cast<int>(tokens), static_cast<int>(sequences)))}, at::kByte, device);
+    if (const int status = dpep_balance_loss(&r, logits->data_ptr(), idx->data_ptr(), static_cast<int>(tokens), data<int32_t>(offsets), static_cast<int>(sequences),
+                                             static_cast<float*>(losses.data_ptr()), static_cast<int32_t*>(counts.data_ptr()),
+                                             static_cast<int32_t*>(members.data_ptr()), scratch.data_ptr(), current_stream(device).raw))
+        return raise_native(status);
+    return tuple_of({std::move(losses), std::move(counts), std::move(members)});
+    END_HANDLE_TH_ERRORS
+}
+// backward(logits, ids, weights, grad_weights, offsets, counts, tokens, grad_losses) -> grad_logits
+PyObject* Router_backward(PyObject* o, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    dpep_router r = reinterpret_cast<Router*>(o)->spec;
+    int device;
+    const at::Tensor* logits = n == 8 ? router_logits(a[0], &r, &device) : nullptr;
+    if (logits == nullptr) Py_RETURN_NONE;
+    const int64_t tokens = logits->size(0);
+    const at::Tensor *idx = router_ids(a[1], &r, tokens, device), *weights, *grad_weights, *offsets, *counts, *members, *grad_losses;
+    const int64_t sequences = router_sequences(a[4], device, &offsets);
+    if (idx == nullptr || sequences == 0 || !optional_plain(a[2], device, at::kFloat, {tokens, r.num_topk}, &weights) ||
+        !optional_plain(a[3], device, at::kFloat, {tokens, r.num_topk}, &grad_weights) ||
+        !optional_plain(a[5], device, at::kInt, {sequences, r.num_experts}, &counts) || !optional_plain(a[6], device, at::kInt, {sequences}, &members) ||
+        !optional_plain(a[7], device, at::kFloat, {sequences}, &grad_losses))
+        Py_RETURN_NONE;
+    if ((grad_weights == nullptr && grad_losses == nullptr) || (grad_weights != nullptr && r.normalize && weights == nullptr) ||
+        (grad_losses != nullptr && (counts == nullptr || members == nullptr)))
+        Py_RETURN_NONE;
+    at::Tensor grad = allocate({tokens, r.num_experts}, logits->scalar_type(), device);
+    const dpep_router_gradients g = {logits->data_ptr(), idx->data_ptr(), data<float>(weights), data<float>(grad_weights), data<int32_t>(offsets), data<int32_t>(counts),
+                                     data<int32_t>(members), data<float>(grad_losses), grad.data_ptr(), static_cast<int32_t>(sequences)};
+    if (const int status = dpep_router_backward(&r, &g, static_cast<int>(tokens), current_stream(device).raw)) return raise_native(status);
+    return wrap(std::move(grad));
+    END_HANDLE_TH_ERRORS
+}
+PyMethodDef router_methods[] = {
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(Router_route)), METH_FASTCALL, nullptr},
+    {"balance_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(Router_balance_loss)), METH_FASTCALL, nullptr},
+    {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(Router_backward)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+void Router_dealloc(PyObject* o) { Py_TYPE(o)->tp_free(o); }
+PyTypeObject RouterType = {PyVarObject_HEAD_INIT(nullptr, 0) "deepep_amd._host.Router", sizeof(Router)};
+
+// A matrix (or experts' matrices) from (packed, scales, zeros) Python objects.
+bool w4_weights(PyObject* packed_object, PyObject* scales_object, PyObject* zeros_object, int64_t dims, at::ScalarType type, int device, dpep_w4* w, int64_t* leading)
+{
+    const at::Tensor *packed = plain(packed_object, device), *scales = plain(scales_object, device), *zeros = zeros_object == Py_None ? nullptr : plain(zeros_object, device);
+    if (packed == nullptr || scales == nullptr || (zeros == nullptr && zeros_object != Py_None)) return false;
+    if (packed->scalar_type() != at::kByte || packed->dim() != dims || scales->scalar_type() != type || scales->dim() != dims) return false;
+    for (int64_t d = 0; d + 1 < dims; ++d)
+        if (scales->size(d) != packed->size(d)) return false;
+    const int64_t n = packed->size(dims - 2), k = 2 * packed->size(dims - 1), groups = scales->size(dims - 1);
+    if (n < 1 || k < 1 || groups < 1 || n > 0x7fffffff || k > 0x7fffffff || k % groups != 0) return false;
+    if (zeros != nullptr && (zeros->scalar_type() != at::kByte || zeros->sizes() != scales->sizes())) return false;
+    *w = {static_cast<const uint8_t*>(packed->data_ptr()), scales->data_ptr(), data<uint8_t>(zeros), static_cast<int32_t>(n), static_cast<int32_t>(k),
+          static_cast<int32_t>(k / groups)};
+    *leading = dims == 3 ? packed->size(0) : 1;
+    return true;
+}
+// The rows of a product this path takes: BF16 or FP16 [M,K], 16-byte aligned, on the current GPU.
+const at::Tensor* w4_rows(PyObject* o, int* device)
+{
+    if (!on_gpu(o) || c10::InferenceMode::is_enabled()) return nullptr;
+    *device = c10::hip::current_device();
+    const at::Tensor* x = plain(o, *device);
+    if (x == nullptr || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) || x->dim() != 2 || x->size(0) > 0x7fffffff || !aligned16(*x)) return nullptr;
+    return x;
+}
+// w4_matvec(x, packed, scales, zeros, out) -> y
+PyObject* w4_matvec(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int device;
+    const at::Tensor *x = n == 5 ? w4_rows(a[0], &device) : nullptr, *out;
+    dpep_w4 w;
+    int64_t one;
+    if (x == nullptr || !w4_weights(a[1], a[2], a[3], 2, x->scalar_type(), device, &w, &one) || x->size(1) != w.k ||
+        !optional_plain(a[4], device, x->scalar_type(), {x->size(0), w.n}, &out))
+        Py_RETURN_NONE;
+    at::Tensor y = out != nullptr ? *out : allocate({x->size(0), w.n}, x->scalar_type(), device);
+    if (const int status = dpep_w4_matvec(&w, type_code(x->scalar_type()), x->data_ptr(), static_cast<int>(x->size(0)), y.data_ptr(), current_stream(device).raw))
+        return raise_native(status);
+    return out != nullptr ? new_ref(a[4]) : wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+// w4_experts(x, ids, weights, gate_up packed, scales, zeros, down packed, scales, zeros, first expert, out) -> y
+PyObject* w4_experts(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int device;
+    const at::Tensor *x = n == 11 ? w4_rows(a[0], &device) : nullptr, *weights, *out;
+    dpep_w4 gate_up, down;
+    int64_t local, local_down;
+    if (x == nullptr || !w4_weights(a[3], a[4], a[5], 3, x->scalar_type(), device, &gate_up, &local) ||
+        !w4_weights(a[6], a[7], a[8], 3, x->scalar_type(), device, &down, &local_down) || local != local_down || local > 0x7fffffff || gate_up.n != 2 * down.k ||
+        gate_up.k != down.n || x->size(1) != gate_up.k)
+        Py_RETURN_NONE;
+    const int64_t tokens = x->size(0);
+    const at::Tensor* idx = plain(a[1], device);
+    if (idx == nullptr || idx->dim() != 2 || idx->size(0) != tokens || idx->size(1) < 1 || idx->size(1) > 0x7fffffff ||
+        (idx->scalar_type() != at::kLong && idx->scalar_type() != at::kInt) || !optional_plain(a[2], device, at::kFloat, {tokens, idx->size(1)}, &weights) ||
+        weights == nullptr || !optional_plain(a[10], device, x->scalar_type(), {tokens, gate_up.k}, &out))
+        Py_RETURN_NONE;
+    const long long begin = exact_int(a[9], 0, 0x7fffffff);
+    if (begin < 0) Py_RETURN_NONE;
+    const int topk = static_cast<int>(idx->size(1));
+    at::Tensor y = out != nullptr ? *out : allocate({tokens, gate_up.k}, x->scalar_type(), device);
+    at::Tensor scratch = allocate({static_cast<int64_t>(dpep_w4_experts_scratch_bytes(static_cast<int>(tokens), topk, gate_up.k, down.k))}, at::kByte, device);
+    if (const int status = dpep_w4_experts(&gate_up, &down, type_code(x->scalar_type()), x->data_ptr(), idx->data_ptr(), idx->scalar_type() == at::kLong ? 8 : 4,
+                                           static_cast<const float*>(weights->data_ptr()), static_cast<int>(tokens), topk, static_cast<int>(begin),
+                                           static_cast<int>(local), y.data_ptr(), scratch.data_ptr(), current_stream(device).raw))
+        return raise_native(status);
+    return out != nullptr ? new_ref(a[10]) : wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // configure_mega(_PreparedPair, NativeError)
 PyObject* configure_mega(PyObject*, PyObject* args)
 {
@@ -1394,6 +1635,8 @@ PyMethodDef module_methods[] = {{"configure", configure, METH_VARARGS, nullptr},
                                 {"configure_mega", configure_mega, METH_VARARGS, nullptr},
                                 {"cast_to_fp8", cast_to_fp8, METH_O, nullptr},
                                 {"cast_back", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(cast_back)), METH_FASTCALL, nullptr},
+                                {"w4_matvec", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w4_matvec)), METH_FASTCALL, nullptr},
+                                {"w4_experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w4_experts)), METH_FASTCALL, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of deepep_amd (see csrc/host.cpp).", -1, module_methods};
 
@@ -1420,14 +1663,18 @@ PyMODINIT_FUNC PyInit__host()
     MegaType.tp_methods = mega_methods;
     MegaType.tp_getset = mega_getset;
     MegaType.tp_new = Mega_new;
+    RouterType.tp_dealloc = Router_dealloc;
+    RouterType.tp_methods = router_methods;
+    RouterType.tp_new = Router_new;
     if ((g_native_error = new_ref(PyExc_RuntimeError)) == nullptr) return nullptr;  // (until the Python layer names its own)
-    for (PyTypeObject* t : {&LeaseType, &MarkerType, &PlanType, &ExchangeType, &MegaType}) {
+    for (PyTypeObject* t : {&LeaseType, &MarkerType, &PlanType, &ExchangeType, &MegaType, &RouterType}) {
         t->tp_flags = Py_TPFLAGS_DEFAULT;
         if (PyType_Ready(t) < 0) return nullptr;
     }
     PyObject* m = PyModule_Create(&module_def);
     if (m == nullptr) return nullptr;
     if (PyModule_AddObject(m, "Exchange", new_ref(reinterpret_cast<PyObject*>(&ExchangeType))) < 0) return nullptr;
+    if (PyModule_AddObject(m, "Router", new_ref(reinterpret_cast<PyObject*>(&RouterType))) < 0) return nullptr;
     if (PyModule_AddObject(m, "Mega", new_ref(reinterpret_cast<PyObject*>(&MegaType))) < 0) return nullptr;
     return m;
 }

@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 class BalanceLoss(NamedTuple):
@@ -65,6 +65,9 @@ class Router:
         self.num_experts, self.num_topk = num_experts, num_topk
         self.num_groups, self.num_topk_groups = num_groups, num_topk_groups
         self.score, self.normalize, self.scale, self.index_dtype = score, bool(normalize), float(scale), index_dtype
+        # Ordinary calls are made natively (csrc/host.cpp); the ones that come back as None, faulty or unusual, go through ops.
+        self._native = _lib.host().Router(num_experts, num_topk, num_groups, num_topk_groups, ops.SCORES.index(score), int(self.normalize),
+                                          self.scale, 8 if index_dtype == torch.int64 else 4)
 
     def _spec(self) -> ops.RouterSpec:
         return ops.RouterSpec(self.num_experts, self.num_topk, self.num_groups, self.num_topk_groups, ops.SCORES.index(self.score),
@@ -80,20 +83,28 @@ class Router:
         K experts are left, and throughout for tokens that ``token_mask`` (bool [T]) has as False.  ``bias`` FP32 [E] takes part in the
         choice only."""
         self._check_bias(bias)
+        done = self._native.route(logits, bias, token_mask)
+        if done is not None:
+            return done
         return ops.route(self._spec(), logits, bias, token_mask, self.index_dtype)
 
     def balance_loss(self, logits: torch.Tensor, topk_idx: torch.Tensor, sequence_offsets: Optional[torch.Tensor] = None) -> BalanceLoss:
         """Loss and counts of every sequence; ``sequence_offsets`` int32 [B+1] ascends from 0 to T (None: one sequence).  With c_e of a
         sequence's R routes on expert e and p the softmax of its N tokens' logits (sigmoid: the sigmoids over their sum), the loss is
         sum_e (E c_e / R) (sum_t p_te / N).  Tokens without a route are padding."""
-        return BalanceLoss(*ops.balance_loss(self._spec(), logits, topk_idx, sequence_offsets), sequence_offsets)
+        sums = self._native.balance_loss(logits, topk_idx, sequence_offsets)
+        if sums is None:
+            sums = ops.balance_loss(self._spec(), logits, topk_idx, sequence_offsets)
+        return BalanceLoss(*sums, sequence_offsets)
 
     def route_with_balance(self, logits: torch.Tensor, bias: Optional[torch.Tensor] = None, token_mask: Optional[torch.Tensor] = None, *,
                            sequence_offsets: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, BalanceLoss]:
         """``route`` and the ``balance_loss`` of its routes, in one pass over the logits."""
         self._check_bias(bias)
-        topk_idx, topk_weights, *sums = ops.route_balance(self._spec(), logits, bias, token_mask, sequence_offsets, self.index_dtype)
-        return topk_idx, topk_weights, BalanceLoss(*sums, sequence_offsets)
+        done = self._native.route(logits, bias, token_mask, sequence_offsets)
+        if done is None:
+            done = ops.route_balance(self._spec(), logits, bias, token_mask, sequence_offsets, self.index_dtype)
+        return done[0], done[1], BalanceLoss(done[2], done[3], done[4], sequence_offsets)
 
     def backward(self, logits: torch.Tensor, topk_idx: torch.Tensor, *, topk_weights: Optional[torch.Tensor] = None,
                  grad_weights: Optional[torch.Tensor] = None, balance: Optional[BalanceLoss] = None,
@@ -104,4 +115,7 @@ class Router:
         if (balance is None) != (grad_losses is None):
             raise ValueError("balance and grad_losses belong together")
         offsets, counts, tokens = (None, None, None) if balance is None else (balance.sequence_offsets, balance.counts, balance.tokens)
+        grad = self._native.backward(logits, topk_idx, topk_weights, grad_weights, offsets, counts, tokens, grad_losses)
+        if grad is not None:
+            return grad
         return ops.router_backward(self._spec(), logits, topk_idx, topk_weights, grad_weights, offsets, counts, tokens, grad_losses)

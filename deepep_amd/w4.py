@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 class W4Weights(NamedTuple):
@@ -50,7 +50,9 @@ def dequantize(weights: W4Weights) -> torch.Tensor:
 
 def matvec(x: torch.Tensor, weights: W4Weights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [M,K] times the matrix [N,K]: [M,N] in x's type (BF16 or FP16)."""
-    return ops.w4_matvec(x, *weights, out=out)
+    packed, scales, zeros = weights
+    done = _lib.host().w4_matvec(x, packed, scales, zeros, out)  # the ordinary call, made natively
+    return ops.w4_matvec(x, packed, scales, zeros, out=out) if done is None else done
 
 
 def expert_ffn(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: torch.Tensor, gate_up: W4Weights, down: W4Weights, *,
@@ -60,4 +62,7 @@ def expert_ffn(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: torch.Tens
 
     x [T,H] BF16 or FP16, topk_idx int64 or int32 [T,K] (T * K at most 2048; -1 and experts that are not local do not count),
     topk_weights FP32 [T,K], gate_up [L,2I,H] (gate rows, then up rows), down [L,H,I].  Returns [T,H] in x's type."""
+    done = _lib.host().w4_experts(x, topk_idx, topk_weights, *gate_up, *down, expert_begin, out)  # the ordinary call, made natively
+    if done is not None:
+        return done
     return ops.w4_experts(x, topk_idx, topk_weights, gate_up, down, expert_begin, out)

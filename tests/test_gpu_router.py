@@ -310,3 +310,31 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+def test_native_and_python_layers_agree():
+    """Logits that carry a gradient go through the Python layer; the bits are the same."""
+    from deepep_amd import Router
+
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    for score, index in (("sigmoid", torch.int64), ("softmax", torch.int32)):
+        router = Router(48, 5, score=score, normalize=score == "sigmoid", num_groups=6, num_topk_groups=3, index_dtype=index)
+        logits = torch.randn((300, 48), generator=gen, device="cuda")
+        bias = torch.randn((48,), generator=gen, device="cuda") if score == "sigmoid" else None
+        mask = torch.rand((300,), generator=gen, device="cuda") < 0.8
+        offsets = torch.tensor([0, 77, 300], dtype=torch.int32).cuda()
+        g, g_losses = torch.randn((300, 5), generator=gen, device="cuda"), torch.randn((2,), generator=gen, device="cuda")
+
+        def step(logits):
+            idx, weights = router.route(logits, bias, mask)
+            idx2, weights2, balance = router.route_with_balance(logits, bias, mask, sequence_offsets=offsets)
+            again = router.balance_loss(logits, idx, offsets)
+            grad = router.backward(logits, idx, topk_weights=weights, grad_weights=g, balance=balance, grad_losses=g_losses)
+            return [idx, weights, idx2, weights2, *balance[:3], *again[:3], grad]
+
+        native = step(logits)
+        assert router._native.route(logits, bias, mask) is not None
+        leaf = logits.clone().requires_grad_()
+        assert router._native.route(leaf, bias, mask) is None
+        for a, b in zip(native, step(leaf)):
+            assert torch.equal(a, b.detach())

@@ -228,3 +228,19 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+def test_native_and_python_layers_agree():
+    """Rows that carry a gradient go through the Python layer; the bits are the same."""
+    from deepep_amd import _lib, w4
+
+    rng = np.random.default_rng(14)
+    gate_up, down = w4.W4Weights(*_weights(rng, (6, 192, 256), 64, True, "bf16")[0]), w4.W4Weights(*_weights(rng, (6, 256, 96), 32, False, "bf16")[0])
+    x = torch.randn((4, 256), device="cuda").bfloat16()
+    ids, route_weights = torch.randint(0, 6, (4, 3), device="cuda"), torch.rand((4, 3), device="cuda")
+    matrix = w4.W4Weights(gate_up.packed[1], gate_up.scales[1], gate_up.zeros[1])
+    assert _lib.host().w4_matvec(x, *matrix, None) is not None
+    leaf = x.clone().requires_grad_()
+    assert _lib.host().w4_matvec(leaf, *matrix, None) is None
+    assert torch.equal(w4.matvec(leaf, matrix), w4.matvec(x, matrix))
+    assert torch.equal(w4.expert_ffn(leaf, ids, route_weights, gate_up, down), w4.expert_ffn(x, ids, route_weights, gate_up, down))
