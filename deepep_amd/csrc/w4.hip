@@ -365,18 +365,44 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
         }
         const int rows = min(count - first_row, p.row_cap), padded = (rows + 3) & ~3;
 
-        // Rows into LDS: 32 values to a thread, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.  The weights are
-        // asked for when the rows are there: behind weights in the CU's queue rows take 5 us to come, and the waves hold units that wait for them.
-        const int pieces = rows * p.units * 8, per_row = p.units * 8;
-        u32x4 octets[4];
-        auto fetch = [&](int i) {
-            const int m = i / per_row, c32 = i - m * per_row, which = first_row + min(m, rows - 1);
-            const uint16_t* from;
-            if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
-            else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
-            else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
+        // Rows into LDS, an octet of values to a thread and turn, as the MFMA wants them: [unit][half][octet][chunk][row], an octet's pairs four apart.
+        // Sixteen lanes next to one another have 128 values, so their groups' sums are a few exchanges away.  The weights are asked for when the
+        // rows are there: behind weights in the CU's queue rows take 5 us to come, and the waves hold units that wait for them.
+        const int pieces = rows * p.units * 32, per_row = p.units * 32;  // (units are whole: a multiple of 16)
+        constexpr int kTurns = 2;
+        u32x4 octets[kTurns];
+        auto fetch = [&](int first) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) octets[j] = load16(from + (c32 < p.k / 32 ? c32 * 32 : 0) + j * 8);
+            for (int turn = 0; turn < kTurns; ++turn) {
+                const int i = first + turn * kThreads, m = i / per_row, at = i - m * per_row, which = first_row + min(m, rows - 1);
+                const uint16_t* from;
+                if constexpr (kKind == kMatvec) from = p.x + static_cast<size_t>(which) * p.k;
+                else if constexpr (kKind == kGateUp) from = p.x + static_cast<size_t>(my_routes[which] / p.topk) * p.k;
+                else from = p.x + (static_cast<size_t>(my_routes[which >> 1]) * 2 + (which & 1)) * p.k;
+                octets[turn] = load16(from + (at * 8 < p.k ? at * 8 : 0));
+            }
+        };
+        auto put = [&](int first) {
+#pragma unroll
+            for (int turn = 0; turn < kTurns; ++turn) {
+                const int i = first + turn * kThreads, m = i / per_row, at = i - m * per_row, c32 = at >> 2;
+                if (i >= pieces) break;  // (sixteen lanes at a time)
+                const u32x4 v = at * 8 < p.k ? octets[turn] : u32x4{0u, 0u, 0u, 0u};
+                float sum = 0.0f;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) sum += widen(v[d] & 0xffffu, kHalfRows) + widen(v[d] >> 16, kHalfRows);
+                const u32x4 pairs = {(v[0] & 0xffffu) | (v[2] << 16), (v[0] >> 16) | (v[2] & 0xffff0000u), (v[1] & 0xffffu) | (v[3] << 16),
+                                     (v[1] >> 16) | (v[3] & 0xffff0000u)};
+                *reinterpret_cast<u32x4*>(x_lds + static_cast<size_t>((((c32 >> 2) * 4 + (at & 3)) * 4 + (c32 & 3)) * rows + m) * 16) = pairs;
+                auto exchange = [&](auto control) {
+                    sum += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(sum), control(), 0xf, 0xf, false));
+                };
+                exchange(std::integral_constant<int, 0xB1>{});                                // lane ^ 1
+                exchange(std::integral_constant<int, 0x4E>{});                                // lane ^ 2: a chunk
+                if constexpr (kDiag < 4) exchange(std::integral_constant<int, 0x141>{});  // the other chunk of two
+                if constexpr (kDiag < 2) exchange(std::integral_constant<int, 0x140>{});  // the other two of four
+                if ((at & (16 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(at / (16 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
+            }
         };
         fetch(tid);
 
@@ -391,26 +417,8 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                 load_step = min(load_step + 1, first_step + steps - 1);
             }
         };
-        auto put = [&](int i) {
-            const int m = i / per_row, c32 = i - m * per_row;
-            const bool real = c32 < p.k / 32;
-            float sum = 0.0f;
-            unsigned char* const to = x_lds + static_cast<size_t>((((c32 >> 2) * 4) * 4 + (c32 & 3)) * rows + m) * 16;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const u32x4 v = real ? octets[j] : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-                for (int d = 0; d < 4; ++d) sum += widen(v[d] & 0xffffu, kHalfRows) + widen(v[d] >> 16, kHalfRows);
-                const u32x4 pairs = {(v[0] & 0xffffu) | (v[2] << 16), (v[0] >> 16) | (v[2] & 0xffff0000u), (v[1] & 0xffffu) | (v[3] << 16),
-                                     (v[1] >> 16) | (v[3] & 0xffff0000u)};
-                *reinterpret_cast<u32x4*>(to + static_cast<size_t>(j * 4 * rows) * 16) = pairs;
-            }
-            if constexpr (kDiag < 4) sum += __shfl_xor(sum, 1);
-            if constexpr (kDiag < 2) sum += __shfl_xor(sum, 2);
-            if ((c32 & (4 / kDiag - 1)) == 0) sums_lds[static_cast<size_t>(c32 / (4 / kDiag)) * padded + m] = kZeros ? -sum : -24.0f * sum;
-        };
-        if (tid < pieces) put(tid);
-        for (int i = tid + kThreads; i < pieces; i += kThreads) {
+        put(tid);
+        for (int i = tid + kTurns * kThreads; i < pieces; i += kTurns * kThreads) {
             fetch(i);
             put(i);
         }
@@ -593,8 +601,19 @@ __global__ __launch_bounds__(256) void sum_routes_kernel(const float* rows, cons
     if (i >= tokens * per_row) return;
     const int token = i / per_row, at = (i - token * per_row) * 4;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < topk; ++s)
-        if (const int route = token * topk + s; ids[route] >= 0) sum += *reinterpret_cast<const f32x4*>(rows + static_cast<size_t>(route) * hidden + at);
+    for (int first = 0; first < topk; first += 8) {  // (ids and rows of eight slots are asked for together; rows nobody wrote are not added)
+        int expert[8];
+        f32x4 row[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int route = token * topk + min(first + i, topk - 1);
+            expert[i] = ids[route];
+            row[i] = *reinterpret_cast<const f32x4*>(rows + static_cast<size_t>(route) * hidden + at);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (first + i < topk && expert[i] >= 0) sum += row[i];
+    }
     uint16_t* const to = y + static_cast<size_t>(token) * hidden + at;
 #pragma unroll
     for (int d = 0; d < 4; ++d) to[d] = narrow(sum[d], half);
