@@ -55,11 +55,11 @@ __device__ __forceinline__ float wave_sum(float v)
 }
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
-// Integers in the order of the floats (-0 and +0 made one, NaN above everything).
+// Integers in the order of the floats (-0 and +0 made one; no NaN).
 __device__ __forceinline__ int ordered(float v)
 {
-    const int bits = __float_as_int(fminf(v, kInf) + 0.0f);
-    return bits ^ ((bits >> 31) & 0x7fffffff);
+    const int bits = __float_as_int(v + 0.0f);
+    return bits ^ static_cast<int>(static_cast<uint32_t>(bits >> 31) >> 1);
 }
 __device__ __forceinline__ float unordered(int key) { return __int_as_float(key ^ ((key >> 31) & 0x7fffffff)); }
 
@@ -232,77 +232,75 @@ struct Forward {
     bool wide, whole;
 };
 
-// Keys of experts outside the best groups become -inf.  Groups of whole lanes: a lane's two largest, then the group's by exchanges among its lanes;
-// other groups by way of LDS.
+// Keys of experts outside the best groups become kNone.  Groups of whole lanes: a lane's two largest, then the group's by exchanges among its lanes;
+// other groups one after the other, each over the whole wave.  A group's rank is how many are ahead of it.
 template <int V, bool kSigmoid>
-__device__ __forceinline__ void limit_groups(float (&key)[V], const Forward& c, float* keys_lds, float* scores_lds, int lane)
+__device__ __forceinline__ void limit_groups(int (&key)[V], const Forward& c, int lane)
 {
-    const int width = c.experts / c.groups;
-    if (c.group_lanes > 0) {
-        float first = key[0], second = -kInf;
+    auto score = [](int first, int second) {
+        return !kSigmoid || second == kNone ? first : ordered(fminf(unordered(first) + unordered(second), kInf));
+    };
+    auto two_largest = [&](const int (&of)[V], int& first, int& second) {
+        first = of[0];
+        second = kNone;
 #pragma unroll
         for (int v = 1; v < V; ++v) {
-            second = fmaxf(second, fminf(first, key[v]));
-            first = fmaxf(first, key[v]);
+            second = max(second, min(first, of[v]));
+            first = max(first, of[v]);
         }
-        auto merge = [&](float other, float other_second) {
-            second = fmaxf(fmaxf(second, other_second), fminf(first, other));
-            first = fmaxf(first, other);
-        };
-        auto step = [&](auto control) {
-            merge(__int_as_float(dpp_or<control(), 0xf>(0, __float_as_int(first))), __int_as_float(dpp_or<control(), 0xf>(0, __float_as_int(second))));
-        };
-        if (c.group_lanes >= 2) step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
-        if (c.group_lanes >= 4) step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
-        if (c.group_lanes >= 8) step(std::integral_constant<int, 0x141>{});  // the other four of eight
-        if (c.group_lanes >= 16) step(std::integral_constant<int, 0x140>{}); // the other eight of sixteen
-        const float mine = !kSigmoid || second == -kInf ? first : first + second;
+    };
+    // lane g * stride (a group's first lane, or lane g) has group g's score
+    auto ahead_of = [&](int mine, int stride) {
         int ahead = 0;
         for (int o = 0; o < c.groups; ++o) {
-            const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), o * c.group_lanes));
-            ahead += static_cast<int>(other > mine) | (static_cast<int>(other == mine) & static_cast<int>(lane >= (o + 1) * c.group_lanes));
+            const int other = __builtin_amdgcn_readlane(mine, o * stride), behind = (o + 1) * stride;  // (lanes of later groups lose a tie)
+            const unsigned long long later = behind < kWave ? ~0ull << behind : 0ull;
+            ahead += __builtin_amdgcn_inverse_ballot_w64(__ballot(other > mine) | (__ballot(other == mine) & later));
         }
+        return ahead;
+    };
+    if (c.group_lanes > 0) {
+        int first, second;
+        two_largest(key, first, second);
+        auto merge = [&](auto control) {
+            const int other = dpp_or<control(), 0xf>(kNone, first), other_second = dpp_or<control(), 0xf>(kNone, second);
+            second = max(max(second, other_second), min(first, other));
+            first = max(first, other);
+        };
+        if (c.group_lanes >= 2) merge(std::integral_constant<int, 0xB1>{});    // lane ^ 1
+        if (c.group_lanes >= 4) merge(std::integral_constant<int, 0x4E>{});    // lane ^ 2
+        if (c.group_lanes >= 8) merge(std::integral_constant<int, 0x141>{});   // the other four of eight
+        if (c.group_lanes >= 16) merge(std::integral_constant<int, 0x140>{});  // the other eight of sixteen
+        const bool out = ahead_of(score(first, second), c.group_lanes) >= c.topk_groups;
 #pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = ahead >= c.topk_groups ? -kInf : key[v];
+        for (int v = 0; v < V; ++v) key[v] = out ? kNone : key[v];
         return;
     }
+    const int width = c.experts / c.groups;
+    int mine = kNone;
+    for (int g = 0; g < c.groups; ++g) {
+        int in[V], first, second;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-        if (lane * V + v < c.experts) keys_lds[lane * V + v] = key[v];
-    wave_sync();
-    for (int g = lane; g < c.groups; g += kWave) {
-        float first = -kInf, second = -kInf;
-        for (int j = 0; j < width; ++j) {
-            const float k = keys_lds[g * width + j];
-            second = fmaxf(second, fminf(first, k));
-            first = fmaxf(first, k);
-        }
-        scores_lds[g] = !kSigmoid || second == -kInf ? first : first + second;
+        for (int v = 0; v < V; ++v) in[v] = static_cast<unsigned>(lane * V + v - g * width) < static_cast<unsigned>(width) ? key[v] : kNone;
+        two_largest(in, first, second);
+        const int largest = wave_max(first), owner = __ffsll(__ballot(first == largest)) - 1;
+        const int of_group = score(largest, wave_max(lane == owner ? second : first));
+        mine = lane == g ? of_group : mine;
     }
-    wave_sync();
+    const unsigned long long out = __ballot(ahead_of(mine, 1) >= c.topk_groups);
+    for (int g = 0; g < c.groups; ++g)
+        if ((out >> g) & 1)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int e = lane * V + v;
-        if (e >= c.experts) continue;
-        const int g = e / width;
-        const float mine = scores_lds[g];
-        int ahead = 0;
-        for (int o = 0; o < c.groups; ++o) {
-            const float other = scores_lds[o];
-            ahead += other > mine || (other == mine && o < g);
-        }
-        if (ahead >= c.topk_groups) key[v] = -kInf;
-    }
-    wave_sync();
+            for (int v = 0; v < V; ++v) key[v] = static_cast<unsigned>(lane * V + v - g * width) < static_cast<unsigned>(width) ? kNone : key[v];
 }
 
-// Sorts a lane's keys, largest first and equal ones in their order, and packs where they were, a byte each (V == 16: half a byte).
+// Sorts a lane's keys, largest first and equal ones in their order (neighbours change places only where the second is larger), and packs where they
+// were, a byte each (V == 16: half a byte).
 template <int V>
 struct Places {
     static constexpr int kBits = V == 16 ? 4 : 8;
     using Word = std::conditional_t<V <= 4, uint32_t, uint64_t>;
     Word word;
-    __device__ __forceinline__ int first() const { return static_cast<int>(word) & ((1 << kBits) - 1); }
 };
 template <int V>
 __device__ __forceinline__ Places<V> sort_keys(int (&key)[V])
@@ -310,24 +308,17 @@ __device__ __forceinline__ Places<V> sort_keys(int (&key)[V])
     int at[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) at[v] = v;
-    // a merge of odd and even places; equal keys are told apart by their place
 #pragma unroll
-    for (int p = 1; p < V; p *= 2)
+    for (int turn = 0; turn < V; ++turn)
 #pragma unroll
-        for (int k = p; k >= 1; k /= 2)
-#pragma unroll
-            for (int j = k % p; j <= V - 1 - k; j += 2 * k)
-#pragma unroll
-                for (int i = 0; i < k; ++i) {
-                    const int a = i + j, b = i + j + k;
-                    if (b >= V || a / (2 * p) != b / (2 * p)) continue;
-                    const bool swap = (key[b] > key[a]) | ((key[b] == key[a]) & (at[b] < at[a]));
-                    const int high = swap ? key[b] : key[a], low = swap ? key[a] : key[b], first = swap ? at[b] : at[a], second = swap ? at[a] : at[b];
-                    key[a] = high;
-                    key[b] = low;
-                    at[a] = first;
-                    at[b] = second;
-                }
+        for (int a = turn & 1; a + 1 < V; a += 2) {
+            const bool swap = key[a + 1] > key[a];
+            const int high = max(key[a], key[a + 1]), low = min(key[a], key[a + 1]), first = swap ? at[a + 1] : at[a], second = swap ? at[a] : at[a + 1];
+            key[a] = high;
+            key[a + 1] = low;
+            at[a] = first;
+            at[a + 1] = second;
+        }
     Places<V> places = {0};
 #pragma unroll
     for (int v = 0; v < V; ++v) places.word |= static_cast<typename Places<V>::Word>(at[v]) << (Places<V>::kBits * v);
@@ -336,14 +327,12 @@ __device__ __forceinline__ Places<V> sort_keys(int (&key)[V])
 
 // Lane k gets the expert of slot k, -1 where none is left: each time the largest key of the wave, in its lowest lane (experts are counted along lanes,
 // and a lane's equal keys stand in their order, so that is the lowest index).  Every lane's keys are sorted first: a step then compares and
-// removes heads alone.  (Finding the register of the largest key in each step took 45 scalar instructions, which issue no faster than the
-// 17 of the vector unit beside them: 65 536 tokens of 256 experts 101 us against 63.)
+// removes heads alone.  (Finding the register of the largest key in each step takes 45 scalar instructions, which issue no faster than the
+// 17 of the vector unit beside them.  Sorting 64-bit items of key and place instead took 6 % more vector instructions in all.)
 template <int V>
-__device__ __forceinline__ int choose(const float (&key)[V], int topk, int self)
+__device__ __forceinline__ int choose(int (&left)[V], int topk, int self)
 {
-    int left[V], mine = -1;
-#pragma unroll
-    for (int v = 0; v < V; ++v) left[v] = key[v] == -kInf ? kNone : ordered(key[v]);
+    int mine = -1;
     Places<V> places = sort_keys(left);
     for (int k = 0; k < topk; ++k) {
         const int largest = wave_max(left[0]);
@@ -376,8 +365,7 @@ __device__ __forceinline__ float pick(const float (&x)[V], int mine)
 template <int V, int kType, bool kSigmoid, bool kRoute, bool kBalance>
 __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Forward c)
 {
-    __shared__ float rows_lds[kRouterWaves][kWave * V];  // keys of irregular groups, then the waves' sums
-    __shared__ float scores_lds[kRoute ? kRouterWaves : 1][kWave * V];
+    __shared__ float rows_lds[kBalance ? kRouterWaves : 1][kWave * V];  // the waves' sums
     __shared__ int counts[kBalance ? kWave * V : 1];
     __shared__ int members[kRouterWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -423,15 +411,14 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
             else if constexpr (kSigmoid) sigmoids<V>(z, s, grown);
             if constexpr (kRoute) {
                 if (real) {
-                    float key[V];
+                    int key[V];
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
                         // a NaN ranks with +inf, so that it is chosen and shows in the weights; what is out of service ranks nowhere
-                        if constexpr (kSigmoid) key[v] = c.bias != nullptr ? s[v] + bias[v] : s[v];
-                        else key[v] = z[v];
-                        key[v] = z[v] == -kInf ? -kInf : fminf(key[v], kInf);
+                        const float k = kSigmoid ? s[v] + bias[v] : z[v];
+                        key[v] = z[v] == -kInf || k == -kInf ? kNone : ordered(fminf(k, kInf));
                     }
-                    if (c.groups > 1) limit_groups<V, kSigmoid>(key, c, rows_lds[wave], scores_lds[wave], lane);
+                    if (c.groups > 1) limit_groups<V, kSigmoid>(key, c, lane);
                     mine = choose<V>(key, c.topk, lane);
                 }
                 float weight;
@@ -728,13 +715,15 @@ bool whole_pieces(const dpep_router* r, const void* a, const void* b)
 }
 // Tokens to a workgroup: about four workgroups of eight waves to a CU; rows of sums stay few.
 int router_chunk(int tokens) { return std::max(kRouterWaves, (tokens + 1023) / 1024); }
+// With balance sums at least four tokens to a wave: a workgroup leaves a row of sums, which costs about as much as a token and is read again.
+int balance_chunk(int tokens) { return std::max(4 * kRouterWaves, (tokens + 1023) / 1024); }
 
 // Scratch of a balance loss.
 struct BalanceScratch {
     size_t counts, members, tickets, products, routes, bytes;
     BalanceScratch(int experts, int tokens, int sequences)
     {
-        const size_t chunk = router_chunk(tokens), rows = (tokens + chunk - 1) / chunk + sequences, pieces = (experts + kWave - 1) / kWave;
+        const size_t chunk = balance_chunk(tokens), rows = (tokens + chunk - 1) / chunk + sequences, pieces = (experts + kWave - 1) / kWave;
         counts = rows * experts * 4;
         members = counts + rows * experts * 4;
         tickets = members + rows * 4;
@@ -747,11 +736,12 @@ struct BalanceScratch {
 int check_router(const dpep_router* r, int num_tokens, const char* what)
 {
     DPEP_REQUIRE(r != nullptr, "%s: router is NULL", what);
-    DPEP_REQUIRE(num_tokens >= 0, "%s: num_tokens=%d", what, num_tokens);
+    DPEP_REQUIRE(num_tokens >= 0 && num_tokens <= 1 << 30, "%s: num_tokens=%d is not in [0, 2^30]", what, num_tokens);
     DPEP_REQUIRE(r->num_experts >= 1 && r->num_experts <= kMaxRouterExperts, "%s: num_experts=%d is not in [1, %d]", what, r->num_experts, kMaxRouterExperts);
     DPEP_REQUIRE(r->num_topk >= 1 && r->num_topk <= DPEP_MAX_TOPK && r->num_topk <= r->num_experts, "%s: num_topk=%d is not in [1, min(%d, num_experts)]", what,
                  r->num_topk, DPEP_MAX_TOPK);
     DPEP_REQUIRE(r->num_groups >= 1 && r->num_experts % r->num_groups == 0, "%s: num_groups=%d does not divide num_experts=%d", what, r->num_groups, r->num_experts);
+    DPEP_REQUIRE(r->num_groups <= kWave, "%s: num_groups=%d is more than %d", what, r->num_groups, kWave);
     DPEP_REQUIRE(r->num_topk_groups >= 1 && r->num_topk_groups <= r->num_groups, "%s: num_topk_groups=%d is not in [1, num_groups]", what, r->num_topk_groups);
     DPEP_REQUIRE(r->num_topk <= r->num_topk_groups * (r->num_experts / r->num_groups), "%s: the chosen groups hold fewer than num_topk=%d experts", what, r->num_topk);
     DPEP_REQUIRE(r->score == DPEP_SCORE_SOFTMAX || r->score == DPEP_SCORE_SIGMOID, "%s: score=%d", what, r->score);
@@ -782,7 +772,7 @@ int run_forward(const dpep_router* r, Forward call, int num_tokens, bool route, 
     call.tokens = num_tokens;
     call.experts = experts;
     call.topk = r->num_topk;
-    call.chunk = router_chunk(num_tokens);
+    call.chunk = balance ? balance_chunk(num_tokens) : router_chunk(num_tokens);
     call.wide = r->index_bytes == 8;
     call.whole = whole_pieces(r, call.logits, nullptr);
     const BalanceScratch at(experts, num_tokens, call.sequences);

@@ -50,7 +50,7 @@ class Router:
                  num_groups: int = 1, num_topk_groups: int = 1, index_dtype: torch.dtype = torch.int64):
         _integer("num_experts", num_experts, 1, 1024)
         _integer("num_topk", num_topk, 1, min(32, num_experts))
-        _integer("num_groups", num_groups, 1, num_experts)
+        _integer("num_groups", num_groups, 1, min(64, num_experts))
         _integer("num_topk_groups", num_topk_groups, 1, num_groups)
         if num_experts % num_groups:
             raise ValueError("num_groups must divide num_experts")

@@ -367,7 +367,7 @@ int dpep_megamoe_run(void* ws, const dpep_megamoe_call* call, void* stream);
  * sigmoid plus the expert's bias, rounded to fp32; an expert whose logit is -inf is never chosen, a NaN ranks with +inf.  With
  * num_groups > 1 the num_experts / num_groups experts of a group stand together: the num_topk_groups groups of the largest key
  * (softmax), or of the largest sum of two keys (sigmoid), stay in the choice.  Ties go to the lowest index.
- *   num_experts  1..1024;  num_topk  1..DPEP_MAX_TOPK, at most the experts of num_topk_groups groups
+ *   num_experts  1..1024;  num_topk  1..DPEP_MAX_TOPK, at most the experts of num_topk_groups groups;  num_groups  1..64, a divisor of num_experts
  *   normalize    != 0: the chosen experts' scores are divided by their sum (sigmoid: plus 1e-20)
  *   scale        factor of the weights, finite and not 0
  *   logits_type  DPEP_TYPE_*;  index_bytes  of an expert id: 8, or 4 */
