@@ -3,6 +3,7 @@
 //   W[n,k] = (q[n,k] - zero[n,k/G]) * scale[n,k/G],  y[m,n] = sum_k x[m,k] W[n,k]
 //   experts: h = silu(W1g[e] x_t) * (W1u[e] x_t),  y_t = sum_s w_ts W2[e] h
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -620,6 +621,24 @@ __global__ __launch_bounds__(256) void sum_routes_kernel(const float* rows, cons
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------
+constexpr int kMaxLds = 160 << 10, kStaticLds = 64;
+
+// Lets a kernel have all of a CU's LDS, once for each device: the call takes about 7 us of the host.
+template <auto kKernel>
+int allow_lds()
+{
+    constexpr int kMaxDevices = 64;
+    static std::atomic<bool> configured[kMaxDevices];
+    int device = 0;
+    DPEP_HIP(hipGetDevice(&device));
+    const bool tracked = device >= 0 && device < kMaxDevices;
+    if (!tracked || !configured[device].load(std::memory_order_acquire)) {
+        DPEP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds - kStaticLds));
+        if (tracked) configured[device].store(true, std::memory_order_release);
+    }
+    return DPEP_OK;
+}
+
 template <Kind kKind>
 int launch_product(Product p, int type, int matrices_most, int rows_expected, int rows_most, hipStream_t stream)
 {
@@ -636,28 +655,32 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     p.steps = (p.tile_groups + at_once - 1) / at_once;
     const int tokens = 16 / diag, by_blocks = rows_expected <= tokens ? 1 : 4, most = tokens * by_blocks;
     // Two workgroups share a CU's 160 KiB where one block of rows will do.
-    const int limit = by_blocks == 1 ? 80 << 10 : 160 << 10;
+    const int limit = by_blocks == 1 ? kMaxLds / 2 : kMaxLds;
     const int experts = kKind == kMatvec ? 0 : p.ids.local;
-    auto plan = [&](int rows, int batch) { return LdsPlan(p.units, diag, by_blocks, tiles, rows, batch, experts, p.routes, kKind == kGateUp).bytes + 64; };
+    auto plan = [&](int rows, int batch) { return LdsPlan(p.units, diag, by_blocks, tiles, rows, batch, experts, p.routes, kKind == kGateUp).bytes + kStaticLds; };
     int rows = std::min(rows_most, most);
     while (rows > (kKind == kDown ? 2 : 1) && plan(rows, 1) > limit) --rows;
     if (kKind == kDown) rows &= ~1;
+    if constexpr (kKind == kMatvec) {
+        // A pass waits for its rows, so there are as many passes, even ones of four rows and more, as CUs without work can take (33 rows through
+        // 1407 x 2880: 11.5 us, 14.1 in passes of 16, 16 and 1; 16 through 2048 x 2048: 7.2 and 10.0; 64 through 512 x 2048: 9.0 and 14.4; where
+        // LDS asks for more passes than CUs anyhow it makes no odds: 64 through 4096 x 7168 50.9 and 50.7).
+        const int passes = std::max((p.rows + rows - 1) / rows, std::min(256 / p.steps, (p.rows + 3) / 4));
+        rows = (p.rows + passes - 1) / passes;
+    }
     p.row_cap = rows;
     p.batch = 1;
     while (p.batch < 8 && plan(rows, p.batch + 1) <= limit) ++p.batch;
-    const int bytes = plan(rows, p.batch) - 64;
+    const int bytes = plan(rows, p.batch) - kStaticLds;
     const int matrices = kKind == kMatvec ? (p.rows + rows - 1) / rows : matrices_most;
-    const int grid = static_cast<int>(std::min<long long>(static_cast<long long>(matrices) * p.steps, by_blocks == 1 ? 512 : 256));
+    const long long all_steps = static_cast<long long>(matrices) * p.steps;
+    DPEP_REQUIRE(all_steps <= INT32_MAX, "w4: N=%d is too much for %d rows of K=%d", p.n, p.rows, p.k);
+    const int grid = static_cast<int>(std::min<long long>(all_steps, by_blocks == 1 ? 512 : 256));
     int status = DPEP_OK;
     auto go = [&](auto half, auto zeros, auto d, auto b, auto streamed) {
-        const auto kernel = product_kernel<kKind, half(), zeros(), d(), b(), streamed()>;
-        if (bytes > 32 << 10) {
-            const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-            if (err != hipSuccess) {
-                status = fail(DPEP_ERUNTIME, "w4: %s", hipGetErrorString(err));
-                return;
-            }
-        }
+        constexpr auto kernel = product_kernel<kKind, half(), zeros(), d(), b(), streamed()>;
+        if (bytes > 32 << 10) status = allow_lds<kernel>();
+        if (status != DPEP_OK) return;
         kernel<<<grid, kThreads, bytes, stream>>>(p);
         status = launch_status("w4 product");
     };
@@ -686,7 +709,7 @@ int check_w4(const dpep_w4* w, int type, const char* what)
 {
     DPEP_REQUIRE(w != nullptr, "%s: weights is NULL", what);
     DPEP_REQUIRE(type == DPEP_TYPE_BF16 || type == DPEP_TYPE_F16, "%s: type=%d is neither BF16 nor FP16", what, type);
-    DPEP_REQUIRE(w->n >= 1 && w->k >= 32 && w->k <= kMaxK, "%s: N=%d K=%d: K is at most %d", what, w->n, w->k, kMaxK);
+    DPEP_REQUIRE(w->n >= 1 && w->n <= 1 << 30 && w->k >= 32 && w->k <= kMaxK, "%s: N=%d K=%d: N is at most 2^30, K %d", what, w->n, w->k, kMaxK);
     DPEP_REQUIRE((w->group == 32 || w->group == 64 || (w->group >= 128 && w->group % 128 == 0)) && w->k % w->group == 0,
                  "%s: group=%d is not 32, 64 or a multiple of 128 that divides K=%d", what, w->group, w->k);
     DPEP_REQUIRE(w->packed != nullptr && w->scales != nullptr, "%s: a NULL buffer", what);
