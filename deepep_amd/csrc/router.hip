@@ -23,42 +23,43 @@ constexpr float kTiny = 1e-20f;  // keeps the sum of chosen sigmoids off zero (a
 constexpr int kRouterThreads = 512;
 constexpr int kRouterWaves = kRouterThreads / kWave;
 constexpr int kMaxRouterExperts = 1024;
-constexpr int kNone = INT32_MIN;  // below every key
+constexpr int kNone = INT32_MIN + 0x7fffff;  // the key of -inf: what is out of service ranks nowhere
 
 // ---- a row in a wave's registers ---------------------------------------------------------------------------------------------------
-template <int kControl, int kRows>
+template <int kControl>
 __device__ __forceinline__ int dpp_or(int other, int v)
 {
-    return __builtin_amdgcn_update_dpp(other, v, kControl, kRows, 0xf, false);
+    return __builtin_amdgcn_update_dpp(other, v, kControl, 0xf, 0xf, false);
 }
-// Largest / sum over the wave, the same in every lane, by row shifts and row broadcasts (an LDS permute a step costs 50 ns and more).
+// Largest / sum over the wave, the same in every lane, by row shifts and row broadcasts (an LDS permute a step costs 50 ns and more).  Only lane 63 is
+// looked at, so broadcasts go to all rows, which makes each step one instruction.
 __device__ __forceinline__ int wave_max(int v)
 {
-    v = max(v, dpp_or<0x111, 0xf>(kNone, v));  // row_shr:1
-    v = max(v, dpp_or<0x112, 0xf>(kNone, v));
-    v = max(v, dpp_or<0x114, 0xf>(kNone, v));
-    v = max(v, dpp_or<0x118, 0xf>(kNone, v));
-    v = max(v, dpp_or<0x142, 0xa>(kNone, v));  // row_bcast:15
-    v = max(v, dpp_or<0x143, 0xc>(kNone, v));  // row_bcast:31
+    v = max(v, dpp_or<0x111>(INT32_MIN, v));  // row_shr:1
+    v = max(v, dpp_or<0x112>(INT32_MIN, v));
+    v = max(v, dpp_or<0x114>(INT32_MIN, v));
+    v = max(v, dpp_or<0x118>(INT32_MIN, v));
+    v = max(v, dpp_or<0x142>(INT32_MIN, v));  // row_bcast:15
+    v = max(v, dpp_or<0x143>(INT32_MIN, v));  // row_bcast:31
     return __builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ float wave_sum(float v)
 {
     auto add = [&](int shifted) { v += __int_as_float(shifted); };
-    add(dpp_or<0x111, 0xf>(0, __float_as_int(v)));
-    add(dpp_or<0x112, 0xf>(0, __float_as_int(v)));
-    add(dpp_or<0x114, 0xf>(0, __float_as_int(v)));
-    add(dpp_or<0x118, 0xf>(0, __float_as_int(v)));
-    add(dpp_or<0x142, 0xa>(0, __float_as_int(v)));
-    add(dpp_or<0x143, 0xc>(0, __float_as_int(v)));
+    add(dpp_or<0x111>(0, __float_as_int(v)));
+    add(dpp_or<0x112>(0, __float_as_int(v)));
+    add(dpp_or<0x114>(0, __float_as_int(v)));
+    add(dpp_or<0x118>(0, __float_as_int(v)));
+    add(dpp_or<0x142>(0, __float_as_int(v)));
+    add(dpp_or<0x143>(0, __float_as_int(v)));
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
-// Integers in the order of the floats (-0 and +0 made one; no NaN).
+// Integers in the order of the floats (no NaN and no -0: adding +0, or a sum of a score and anything, leaves none).
 __device__ __forceinline__ int ordered(float v)
 {
-    const int bits = __float_as_int(v + 0.0f);
+    const int bits = __float_as_int(v);
     return bits ^ static_cast<int>(static_cast<uint32_t>(bits >> 31) >> 1);
 }
 __device__ __forceinline__ float unordered(int key) { return __int_as_float(key ^ ((key >> 31) & 0x7fffffff)); }
@@ -90,6 +91,9 @@ __device__ __forceinline__ float load_logit(const void* p, size_t i)
 template <int V, int kType>
 struct Piece {
     using Word = Logit<kType>;
+    static constexpr int kBytes = V * sizeof(Word);
+    using Part = std::conditional_t<kBytes >= 16, u32x4, std::conditional_t<kBytes == 8, u32x2, std::conditional_t<kBytes == 4, uint32_t, Word>>>;
+    static constexpr int kParts = kBytes / sizeof(Part);
     Word at[V];
     __device__ __forceinline__ void load(const void* rows, size_t row, int experts, int lane, bool whole)
     {
@@ -97,7 +101,12 @@ struct Piece {
         const int first = lane * V;
         if (whole) {
             const int clamped = first < experts ? first : 0;
-            __builtin_memcpy(at, __builtin_assume_aligned(from + clamped, V * sizeof(Word) < 16 ? V * sizeof(Word) : 16), sizeof(at));
+            const Part* const parts = reinterpret_cast<const Part*>(from + clamped);
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                const Part part = parts[i];
+                __builtin_memcpy(at + i * (V / kParts), &part, sizeof(Part));
+            }
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v) at[v] = from[min(first + v, experts - 1)];
@@ -108,7 +117,13 @@ struct Piece {
         Word* const to = static_cast<Word*>(rows) + row;
         const int first = lane * V;
         if (whole) {
-            if (first < experts) __builtin_memcpy(__builtin_assume_aligned(to + first, V * sizeof(Word) < 16 ? V * sizeof(Word) : 16), at, sizeof(at));
+            if (first < experts)
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) {
+                    Part part;
+                    __builtin_memcpy(&part, at + i * (V / kParts), sizeof(Part));
+                    reinterpret_cast<Part*>(to + first)[i] = part;
+                }
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v)
@@ -131,7 +146,7 @@ __device__ __forceinline__ int load_index(const void* p, bool wide, size_t i, in
 
 // 1 / (1 + exp(-z)) as IEEE divide and the library's exp give it, bit for bit (the choice compares such values, so everybody has to get the
 // same): one step from the hardware's reciprocal is correctly rounded for every mantissa and exponent below 2^126 (checked for all of
-// them), and beyond that, below a logit of -87, the divide itself is taken.  grown: exp(-z).
+// them), and beyond that, below a logit of -86, the divide itself is taken.  grown: exp(-z).
 __device__ __forceinline__ float sigmoid_of(float grown)
 {
     const float d = 1.0f + grown, r = __builtin_amdgcn_rcpf(d);
@@ -140,14 +155,14 @@ __device__ __forceinline__ float sigmoid_of(float grown)
 template <int V>
 __device__ __forceinline__ void sigmoids(const float (&z)[V], float (&s)[V], float (&grown)[V])
 {
-    float largest = 0.0f;
+    unsigned long long far = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         grown[v] = expf(-z[v]);
         s[v] = sigmoid_of(grown[v]);
-        largest = z[v] == -kInf ? largest : fmaxf(largest, grown[v]);
+        far |= __ballot(z[v] < -86.0f && z[v] != -kInf);
     }
-    if (__ballot(largest > 0x1p125f) != 0)
+    if (far != 0)
 #pragma unroll
         for (int v = 0; v < V; ++v) s[v] = 1.0f / (1.0f + grown[v]);
 #pragma unroll
@@ -263,7 +278,7 @@ __device__ __forceinline__ void limit_groups(int (&key)[V], const Forward& c, in
         int first, second;
         two_largest(key, first, second);
         auto merge = [&](auto control) {
-            const int other = dpp_or<control(), 0xf>(kNone, first), other_second = dpp_or<control(), 0xf>(kNone, second);
+            const int other = dpp_or<control()>(kNone, first), other_second = dpp_or<control()>(kNone, second);
             second = max(max(second, other_second), min(first, other));
             first = max(first, other);
         };
@@ -271,7 +286,18 @@ __device__ __forceinline__ void limit_groups(int (&key)[V], const Forward& c, in
         if (c.group_lanes >= 4) merge(std::integral_constant<int, 0x4E>{});    // lane ^ 2
         if (c.group_lanes >= 8) merge(std::integral_constant<int, 0x141>{});   // the other four of eight
         if (c.group_lanes >= 16) merge(std::integral_constant<int, 0x140>{});  // the other eight of sixteen
-        const bool out = ahead_of(score(first, second), c.group_lanes) >= c.topk_groups;
+        const int mine = score(first, second);
+        int ahead;
+        if (c.groups <= c.group_lanes) {
+            // a group's lane j compares it with group j: its share of the ballot is who is ahead
+            const int other = __builtin_amdgcn_ds_bpermute((lane & (c.group_lanes - 1)) * c.group_lanes * 4, mine);
+            const int group_first = lane & -c.group_lanes, j = lane - group_first;
+            const bool is_ahead = j < c.groups && (other > mine || (other == mine && j * c.group_lanes < group_first));
+            ahead = __popc(static_cast<uint32_t>(__ballot(is_ahead) >> group_first) & ((1u << c.group_lanes) - 1));
+        } else {
+            ahead = ahead_of(mine, c.group_lanes);
+        }
+        const bool out = ahead >= c.topk_groups;
 #pragma unroll
         for (int v = 0; v < V; ++v) key[v] = out ? kNone : key[v];
         return;
@@ -312,12 +338,12 @@ __device__ __forceinline__ Places<V> sort_keys(int (&key)[V])
     for (int turn = 0; turn < V; ++turn)
 #pragma unroll
         for (int a = turn & 1; a + 1 < V; a += 2) {
-            const bool swap = key[a + 1] > key[a];
-            const int high = max(key[a], key[a + 1]), low = min(key[a], key[a + 1]), first = swap ? at[a + 1] : at[a], second = swap ? at[a] : at[a + 1];
-            key[a] = high;
-            key[a + 1] = low;
-            at[a] = first;
-            at[a + 1] = second;
+            // (by value: a choice between elements would become one between their addresses)
+            const int x = key[a], y = key[a + 1], at_x = at[a], at_y = at[a + 1];
+            key[a] = max(x, y);
+            key[a + 1] = min(x, y);
+            at[a] = y > x ? at_y : at_x;
+            at[a + 1] = y > x ? at_x : at_y;
         }
     Places<V> places = {0};
 #pragma unroll
@@ -328,18 +354,18 @@ __device__ __forceinline__ Places<V> sort_keys(int (&key)[V])
 // Lane k gets the expert of slot k, -1 where none is left: each time the largest key of the wave, in its lowest lane (experts are counted along lanes,
 // and a lane's equal keys stand in their order, so that is the lowest index).  Every lane's keys are sorted first: a step then compares and
 // removes heads alone.  (Finding the register of the largest key in each step takes 45 scalar instructions, which issue no faster than the
-// 17 of the vector unit beside them.  Sorting 64-bit items of key and place instead took 6 % more vector instructions in all.)
+// 17 of the vector unit beside them.)
 template <int V>
-__device__ __forceinline__ int choose(int (&left)[V], int topk, int self)
+__device__ __forceinline__ int choose(int (&left)[V], int topk)
 {
     int mine = -1;
     Places<V> places = sort_keys(left);
     for (int k = 0; k < topk; ++k) {
         const int largest = wave_max(left[0]);
         if (largest == kNone) break;
-        const int lane = __ffsll(__ballot(left[0] == largest)) - 1;
+        const int lane = __builtin_ctzll(__ballot(left[0] == largest));
         const int expert = lane * V + (__builtin_amdgcn_readlane(static_cast<int>(places.word), lane) & ((1 << Places<V>::kBits) - 1));
-        mine = self == k ? expert : mine;
+        mine = __builtin_amdgcn_inverse_ballot_w64(1ull << k) ? expert : mine;
         const bool taken = __builtin_amdgcn_inverse_ballot_w64(1ull << lane);
 #pragma unroll
         for (int v = 0; v < V; ++v) left[v] = !taken ? left[v] : v + 1 < V ? left[v + 1] : kNone;
@@ -399,7 +425,7 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
         };
         fetch(begin + wave);
         for (int t = begin + wave; t < end; t += kRouterWaves) {
-            const size_t to = static_cast<size_t>(t) * c.topk + lane;
+            const size_t to = static_cast<size_t>(t) * c.topk;
             const Piece<V, kType> piece = next;
             const bool real = __builtin_amdgcn_readfirstlane(next_real) != 0;
             int mine = kRoute ? -1 : next_route;
@@ -414,12 +440,12 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
                     int key[V];
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        // a NaN ranks with +inf, so that it is chosen and shows in the weights; what is out of service ranks nowhere
-                        const float k = kSigmoid ? s[v] + bias[v] : z[v];
-                        key[v] = z[v] == -kInf || k == -kInf ? kNone : ordered(fminf(k, kInf));
+                        // a NaN ranks with +inf, so that it is chosen and shows in the weights
+                        const float k = !kSigmoid ? z[v] + 0.0f : z[v] == -kInf ? -kInf : s[v] + bias[v];
+                        key[v] = ordered(fminf(k, kInf));
                     }
                     if (c.groups > 1) limit_groups<V, kSigmoid>(key, c, lane);
-                    mine = choose<V>(key, c.topk, lane);
+                    mine = choose<V>(key, c.topk);
                 }
                 float weight;
                 if constexpr (kSigmoid) {
@@ -435,9 +461,9 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
                     weight = pick<V>(s, mine) * inverse;
                 }
                 if (lane < c.topk) {
-                    if (c.wide) static_cast<int64_t*>(c.topk_idx)[to] = mine;
-                    else static_cast<int32_t*>(c.topk_idx)[to] = mine;
-                    c.topk_weights[to] = weight * c.scale;
+                    if (c.wide) (static_cast<int64_t*>(c.topk_idx) + to)[lane] = mine;
+                    else (static_cast<int32_t*>(c.topk_idx) + to)[lane] = mine;
+                    (c.topk_weights + to)[lane] = weight * c.scale;
                 }
             }
             if constexpr (kBalance) {
@@ -445,7 +471,7 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
                 if (mine >= 0) atomicAdd(&counts[mine], 1);
                 ++held;
 #pragma unroll
-                for (int v = 0; v < V; ++v) sum[v] += s[v] * inverse;
+                for (int v = 0; v < V; ++v) sum[v] = fmaf(s[v], inverse, sum[v]);
             }
         }
         if constexpr (kBalance) {
