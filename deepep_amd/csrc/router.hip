@@ -138,9 +138,10 @@ struct Piece {
         if constexpr (kType == DPEP_TYPE_F16) at[v] = static_cast<uint16_t>(pack_f16x2(value, 0.0f) & 0xffffu);
     }
 };
-__device__ __forceinline__ int load_index(const void* p, bool wide, size_t i, int experts)
+// Id of a slot of the row that begins at id `row` (the same in all lanes).
+__device__ __forceinline__ int load_index(const void* p, bool wide, size_t row, int slot, int experts)
 {
-    const long long e = wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+    const long long e = wide ? (static_cast<const int64_t*>(p) + row)[slot] : (static_cast<const int32_t*>(p) + row)[slot];
     return e >= 0 && e < experts ? static_cast<int>(e) : -1;
 }
 
@@ -160,7 +161,7 @@ __device__ __forceinline__ void sigmoids(const float (&z)[V], float (&s)[V], flo
     for (int v = 0; v < V; ++v) {
         grown[v] = expf(-z[v]);
         s[v] = sigmoid_of(grown[v]);
-        far |= __ballot(z[v] < -86.0f && z[v] != -kInf);
+        far |= __ballot(z[v] < -86.0f) & ~__ballot(z[v] == -kInf);
     }
     if (far != 0)
 #pragma unroll
@@ -210,15 +211,16 @@ __device__ __forceinline__ int sequence_begin(const int32_t* offsets, int b, int
     if (offsets == nullptr) return b == 0 ? 0 : tokens;
     return min(max(offsets[b], 0), tokens);
 }
-// The last sequence that begins at `token` or in front of it.
-__device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences, int token)
+// The last sequence that begins at `token` (the same in all lanes) or in front of it: 64 are looked at in a step.
+__device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences, int token, int lane)
 {
     if (offsets == nullptr) return 0;
     int low = 0, high = sequences;
     while (high - low > 1) {
-        const int mid = (low + high) / 2;
-        if (offsets[mid] <= token) low = mid;
-        else high = mid;
+        const int step = (high - low + kWave - 1) / kWave, at = low + lane * step;
+        const int begun = __popcll(__ballot(at < high && offsets[min(at, high - 1)] <= token));
+        low += max(begun - 1, 0) * step;
+        high = min(low + step, high);
     }
     return low;
 }
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
         for (int v = 0; v < V; ++v) bias[v] = c.bias != nullptr && lane * V + v < c.experts ? c.bias[lane * V + v] : 0.0f;
 
     int begin = first;
-    for (int b = kBalance ? sequence_of(c.offsets, c.sequences, first) : 0; begin < last && b < c.sequences; ++b) {
+    for (int b = kBalance ? sequence_of(c.offsets, c.sequences, first, lane) : 0; begin < last && b < c.sequences; ++b) {
         const int end = !kBalance || b + 1 == c.sequences ? last : min(last, sequence_begin(c.offsets, b + 1, c.sequences, c.tokens));
         if (end <= begin) continue;
         float sum[V] = {};
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
             if (t >= end) return;
             next.load(c.logits, static_cast<size_t>(t) * c.experts, c.experts, lane, c.whole);
             if constexpr (kRoute) next_real = c.token_mask == nullptr ? 1 : c.token_mask[t];
-            else next_route = lane < c.topk ? load_index(c.topk_idx, c.wide, static_cast<size_t>(t) * c.topk + lane, c.experts) : -1;
+            else next_route = lane < c.topk ? load_index(c.topk_idx, c.wide, static_cast<size_t>(t) * c.topk, lane, c.experts) : -1;
         };
         fetch(begin + wave);
         for (int t = begin + wave; t < end; t += kRouterWaves) {
@@ -581,7 +583,7 @@ struct Backward {
     void* grad_logits;
     int tokens, experts, topk, sequences, chunk;
     bool normalize, wide, whole;
-    float scale;
+    float scale, inverse_scale;
 };
 
 template <int V, int kType, bool kSigmoid>
@@ -600,13 +602,13 @@ __global__ __launch_bounds__(kRouterThreads) void router_backward_kernel(const B
     float next_grad = 0.0f, next_weight = 0.0f;
     auto fetch = [&](int t) {
         if (t >= last) return;
-        const size_t slot = static_cast<size_t>(t) * c.topk + lane;
+        const size_t slots = static_cast<size_t>(t) * c.topk;
         if (dense || balance) next.load(c.logits, static_cast<size_t>(t) * c.experts, c.experts, lane, c.whole);
         if (lane >= c.topk) return;
-        next_route = load_index(c.topk_idx, c.wide, slot, c.experts);
+        next_route = load_index(c.topk_idx, c.wide, slots, lane, c.experts);
         if (c.grad_weights != nullptr) {
-            next_grad = c.grad_weights[slot];
-            if (c.normalize) next_weight = c.topk_weights[slot];
+            next_grad = (c.grad_weights + slots)[lane];
+            if (c.normalize) next_weight = (c.topk_weights + slots)[lane];
         }
     };
     fetch(first + wave);
@@ -626,7 +628,7 @@ __global__ __launch_bounds__(kRouterThreads) void router_backward_kernel(const B
             if (balance) {
                 // softmax: a p (f - sum f p); sigmoid: a s (1 - s) / sum s (f - sum f p);  a = grad / N
                 if (t >= sequence_end) {
-                    sequence = sequence < 0 ? sequence_of(c.offsets, c.sequences, t) : sequence;
+                    sequence = sequence < 0 ? sequence_of(c.offsets, c.sequences, t, lane) : sequence;
                     while (sequence + 1 < c.sequences && sequence_begin(c.offsets, sequence + 1, c.sequences, c.tokens) <= t) ++sequence;
                     sequence_end = sequence_begin(c.offsets, sequence + 1, c.sequences, c.tokens);
                     int routes = 0;
@@ -660,7 +662,7 @@ __global__ __launch_bounds__(kRouterThreads) void router_backward_kernel(const B
             wave_sync();
             float g = e >= 0 ? through_weight * c.scale : 0.0f, through = 0.0f;
             if (c.normalize) {
-                const float w = e >= 0 ? weight_of_route / c.scale : 0.0f;
+                const float w = e >= 0 ? weight_of_route * c.inverse_scale : 0.0f;
                 const float inner = wave_sum(g * w);
                 g = e >= 0 ? g - inner : 0.0f;
                 through = w * g;
@@ -676,7 +678,7 @@ __global__ __launch_bounds__(kRouterThreads) void router_backward_kernel(const B
                     score = e >= 0 ? sigmoid(z) : 0.0f;
                 }
                 through = g * score * (fminf(of_exp, 3e38f) * score);
-                if (c.normalize) through = through / (wave_sum(score) + kTiny);
+                if (c.normalize) through = through * reciprocal(wave_sum(score) + kTiny);
             }
             if (e >= 0) atomicAdd(&mine[e], dense ? g : through);
             wave_sync();
@@ -773,7 +775,7 @@ int check_router(const dpep_router* r, int num_tokens, const char* what)
     DPEP_REQUIRE(r->score == DPEP_SCORE_SOFTMAX || r->score == DPEP_SCORE_SIGMOID, "%s: score=%d", what, r->score);
     DPEP_REQUIRE(r->logits_type >= DPEP_TYPE_F32 && r->logits_type <= DPEP_TYPE_F16, "%s: logits_type=%d", what, r->logits_type);
     DPEP_REQUIRE(r->index_bytes == 4 || r->index_bytes == 8, "%s: index_bytes=%d", what, r->index_bytes);
-    DPEP_REQUIRE(r->scale == r->scale && r->scale != 0.0f && r->scale - r->scale == 0.0f, "%s: scale must be finite and not zero", what);
+    DPEP_REQUIRE(r->scale >= 1e-30f && r->scale <= 1e30f || r->scale <= -1e-30f && r->scale >= -1e30f, "%s: scale must be of 1e-30 to 1e30 in magnitude", what);
     return DPEP_OK;
 }
 
@@ -904,7 +906,7 @@ int dpep_router_backward(const dpep_router* r, const dpep_router_gradients* g, i
     const bool balance = g->grad_losses != nullptr;
     const Backward call = {g->logits, g->topk_idx, g->topk_weights, g->grad_weights, g->sequence_offsets, balance ? g->counts : nullptr, g->tokens, g->grad_losses,
                            g->grad_logits, num_tokens, r->num_experts, r->num_topk, balance ? g->num_sequences : 1, router_chunk(num_tokens), r->normalize != 0,
-                           r->index_bytes == 8, whole_pieces(r, g->logits, g->grad_logits), r->scale};
+                           r->index_bytes == 8, whole_pieces(r, g->logits, g->grad_logits), r->scale, 1.0f / r->scale};
     const int chunks = (num_tokens + call.chunk - 1) / call.chunk;
     with_variant(r, [&](auto v, auto type, auto sigmoid) {
         router_backward_kernel<v(), type(), sigmoid()><<<chunks, kRouterThreads, 0, static_cast<hipStream_t>(stream)>>>(call);

@@ -13,7 +13,6 @@ Calls are queued on torch's current stream.  Nothing is recorded for autograd: t
 
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -58,8 +57,8 @@ class Router:
             raise ValueError("num_topk exceeds the experts of num_topk_groups groups")
         if score not in ops.SCORES:
             raise ValueError(f"score must be one of {ops.SCORES}")
-        if not isinstance(scale, (int, float)) or not math.isfinite(scale) or scale == 0:
-            raise ValueError("scale must be finite and not zero")
+        if not isinstance(scale, (int, float)) or not 1e-30 <= abs(scale) <= 1e30:
+            raise ValueError("scale must be a number of 1e-30 to 1e30 in magnitude")
         if index_dtype not in (torch.int64, torch.int32):
             raise ValueError("index_dtype must be torch.int64 or torch.int32")
         self.num_experts, self.num_topk = num_experts, num_topk

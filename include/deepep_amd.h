@@ -369,7 +369,7 @@ int dpep_megamoe_run(void* ws, const dpep_megamoe_call* call, void* stream);
  * (softmax), or of the largest sum of two keys (sigmoid), stay in the choice.  Ties go to the lowest index.
  *   num_experts  1..1024;  num_topk  1..DPEP_MAX_TOPK, at most the experts of num_topk_groups groups;  num_groups  1..64, a divisor of num_experts
  *   normalize    != 0: the chosen experts' scores are divided by their sum (sigmoid: plus 1e-20)
- *   scale        factor of the weights, finite and not 0
+ *   scale        factor of the weights, 1e-30 to 1e30 in magnitude
  *   logits_type  DPEP_TYPE_*;  index_bytes  of an expert id: 8, or 4 */
 typedef struct dpep_router {
     int32_t num_experts, num_topk, num_groups, num_topk_groups;
