@@ -416,14 +416,17 @@ int dpep_router_backward(const dpep_router* r, const dpep_router_gradients* g, i
 /* Matrices [L,N,K] in 4 bits: value (q - zero) * scale, q two to a byte along K (low nibble: even k), one scale and zero point for each
  * `group` values of a row.
  *   packed [L,N,K/2], 16-byte aligned;  scales [L,N,K/group] in the type of the rows multiplied;  zeros bytes [L,N,K/group] (0..15), or
- *   NULL: 8;  group 32, 64 or a multiple of 128, a divisor of K */
+ *   NULL: 8;  group 32, 64 or a multiple of 128, a divisor of K;  K at most 16384
+ * x is multiplied by 16 + q and (16 + zero) times its group's sum taken off again, in fp32: a row of x that holds an infinity or a NaN, or
+ * values whose sums pass the range of fp32, gets results that are not finite. */
 typedef struct dpep_w4 {
     const uint8_t* packed;
     const void* scales;
     const uint8_t* zeros;
     int32_t n, k, group;
 } dpep_w4;
-/* y[m] = W x[m]: x, y of `type` (BF16 or FP16), x [M,K] 16-byte aligned, y [M,N], sums in fp32, rounded once. */
+/* y[m] = W x[m]: x, y of `type` (BF16 or FP16), x [M,K] 16-byte aligned, y [M,N], sums in fp32, rounded once.  M at most 65535; meant for a
+ * few rows: beyond about 16 the time grows with M. */
 int dpep_w4_matvec(const dpep_w4* w, int type, const void* x, int num_rows, void* y, void* stream);
 /* An expert layer for few tokens (T*K <= 2048 routes): y[t] = sum over the slots s of topk_weights[t,s] * W2[e] (silu(g) * u) with
  * (g, u) = W1[e] x[t], e = topk_idx[t,s] - expert_begin; slots whose expert is not one of the num_local do not count, a token without
