@@ -271,13 +271,13 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                 if (p.ragged && p.all_scales < 2 * kDiag) {  // fewer than one load takes: one by one
                     for (int d = 0; d < kDiag; ++d) s.scale[t][d] = 0;
                     if constexpr (kZeros) s.zero[t][0] = s.zero[t][kDiag == 4 ? 1 : 0] = 0;
-                    for (int i = 0; i < scales_left(row) - static_cast<int>(at); ++i) {
-                        const uint32_t half = (scales + begin)[at + i];
-                        if constexpr (kZeros) s.zero[t][i / 4] |= static_cast<uint32_t>((zeros + begin)[at + i]) << (8 * (i % 4));
+                    const int left = scales_left(row) - static_cast<int>(at);
 #pragma unroll
-                        for (int d = 0; d < kDiag; ++d)
-                            if (i / 2 == d) s.scale[t][d] |= half << (16 * (i % 2));
-                    }
+                    for (int i = 0; i < 2 * kDiag; ++i)  // (indices that are constants keep these arrays in registers)
+                        if (i < left) {
+                            s.scale[t][i / 2] |= static_cast<uint32_t>((scales + begin)[at + i]) << (16 * (i % 2));
+                            if constexpr (kZeros) s.zero[t][i / 4] |= static_cast<uint32_t>((zeros + begin)[at + i]) << (8 * (i % 4));
+                        }
                     continue;
                 }
                 const uint32_t from = p.ragged ? min(at, static_cast<uint32_t>(scales_left(row) - 2 * kDiag)) : at;
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
 
         f32x4 acc[kTiles][kBlocks] = {};
         const int x_lane = own ? (chunk * rows + min(col % kTokens, rows - 1)) * 16 : 0;
-        auto consume = [&](const Slot& s, int u, const uint32_t (&scale_pair)[kTiles], const uint32_t (&zero_pair)[kTiles]) {
+        auto consume = [&](const Slot& s, int u, const uint32_t (&scale_pair)[kTiles], const uint32_t (&zero_pair)[kTiles], int zero_byte) {
             asm volatile("" : "+s"(u));  // (or each of its LDS addresses becomes an induction variable in a register)
             // What LDS holds is asked for before the weights are waited for.
             auto x_at = [&](int part, int j) {
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                     for (int t = 0; t < kTiles; ++t) {
                         c[t][b] = start;
                         if constexpr (kZeros) {
-                            const float zero = 16.0f + static_cast<float>(f == 0 ? zero_pair[t] & 0xffu : (zero_pair[t] >> 16) & 0xffu);
+                            const float zero = 16.0f + static_cast<float>((zero_pair[t] >> (16 * f + 8 * zero_byte)) & 0xffu);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) c[t][b][i] *= zero;
                         }
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
             for (int i = 0; i < number; ++i) {
                 const int at_step = first_step + done + i, from = first_unit(at_step), to = last_unit(at_step);
                 for (int block = 0; block < slots / 4; ++block) {
-                    uint32_t scale_of[kTiles][4], zero_of[kTiles][4] = {};
+                    uint32_t scale_of[kTiles][4], zero_of[kTiles][2] = {};  // (zero points: bytes, those of units 0 and 1, of 2 and 3 in one register)
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
                         spread(next_scales.scale[t], scale_of[t], at_step, block, t);
@@ -574,7 +574,10 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                             uint32_t pairs[kDiag];
 #pragma unroll
                             for (int d = 0; d < kDiag; ++d) pairs[d] = (next_scales.zero[t][d / 2] >> (16 * (d % 2)) & 0xffu) | (next_scales.zero[t][d / 2] >> (16 * (d % 2)) & 0xff00u) << 8;
-                            spread(pairs, zero_of[t], at_step, block, t);
+                            uint32_t of_unit[4];
+                            spread(pairs, of_unit, at_step, block, t);
+                            zero_of[t][0] = of_unit[0] | of_unit[1] << 8;
+                            zero_of[t][1] = of_unit[2] | of_unit[3] << 8;
                         }
                     }
 #pragma unroll
@@ -583,10 +586,10 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
 #pragma unroll
                         for (int t = 0; t < kTiles; ++t) {
                             scale_pair[t] = scale_of[t][a];
-                            zero_pair[t] = zero_of[t][a];
+                            zero_pair[t] = zero_of[t][a / 2];
                         }
                         const int u = from + block * 4 + a;
-                        if (u < to) consume(ring[a % kAhead], u, scale_pair, zero_pair);
+                        if (u < to) consume(ring[a % kAhead], u, scale_pair, zero_pair, a % 2);
                         if ((a + kAhead) % 4 == 0) load_scales(next_scales, load_step, load_slot / 4);
                         load_next(ring[a % kAhead]);
                     }
