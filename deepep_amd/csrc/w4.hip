@@ -670,7 +670,7 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     if (kKind == kDown) rows &= ~1;
     if constexpr (kKind == kMatvec) {
         // A pass waits for its rows, so there are as many passes, even ones of four rows and more, as CUs without work can take (33 rows through
-        // 1407 x 2880: 11.5 us, 14.1 in passes of 16, 16 and 1; 16 through 2048 x 2048: 7.2 and 10.0; 64 through 512 x 2048: 9.0 and 14.4; where
+        // 1407 x 2880: 11.5 us, 14.1 in passes of 16, 16 and 1 (10.1 since scales stay in registers); 16 through 2048 x 2048: 7.2 and 10.0; 64 through 512 x 2048: 9.0 and 14.4; where
         // LDS asks for more passes than CUs anyhow it makes no odds: 64 through 4096 x 7168 50.9 and 50.7).
         const int passes = std::max((p.rows + rows - 1) / rows, std::min(256 / p.steps, (p.rows + 3) / 4));
         rows = (p.rows + passes - 1) / passes;
@@ -693,7 +693,7 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     };
     auto by_block = [&](auto half, auto zeros, auto d) {
         // Rows of whole lines are read once and go past the caches; of other rows every other line is read by two waves (through 8 of 256 experts
-        // 51 us, plain loads 53; through 4 of 32 with rows of 1440 and 704 bytes 63 and 55).  (A branch around the loads costs a tenth.)
+        // 48 us, plain loads 53; through 4 of 32 with rows of 1440 and 704 bytes 53 and 44).  (A branch around the loads costs a tenth.)
         if (by_blocks == 4) go(half, zeros, d, std::integral_constant<int, 4>{}, std::false_type{});
         else if (p.k % kUnit == 0) go(half, zeros, d, std::integral_constant<int, 1>{}, std::true_type{});
         else go(half, zeros, d, std::integral_constant<int, 1>{}, std::false_type{});
