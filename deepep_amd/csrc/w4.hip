@@ -133,7 +133,7 @@ struct LdsPlan {
 //
 // Few rows: reading the codes bounds it.  Sixteen tokens through 8 of 256 experts, 1.9 GB of weights: 350 us in all, 5.6 TB/s.  One token, 121 MB and
 // 60 MB: 27 and 18 us, 4.4 and 3.3 TB/s, of which 5 to 6 pass before the first weights are asked for (ids, then rows, then the barrier) and 2
-// behind the last.  Many rows: the rows' way into LDS, once for every 16 columns and pass (64 rows through 4096 x 7168: 51 us).
+// behind the last.  Many rows: the rows' way into LDS, once for every 16 columns and pass (64 rows through 4096 x 7168: 42 us).
 template <Kind kKind, bool kHalf, bool kZeros, int kDiag, int kBlocks, bool kStreamed>
 __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel(const Product p)
 {
@@ -660,18 +660,25 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     while (p.split < kWaves && p.split * 4 < p.units) p.split *= 2, ++p.log_split;  // (four units to a wave and step)
     const int at_once = kWaves / p.split;
     p.steps = (p.tile_groups + at_once - 1) / at_once;
-    const int tokens = 16 / diag, by_blocks = rows_expected <= tokens ? 1 : 4, most = tokens * by_blocks;
-    // Two workgroups share a CU's 160 KiB where one block of rows will do.
-    const int limit = by_blocks == 1 ? kMaxLds / 2 : kMaxLds;
-    const int experts = kKind == kMatvec ? 0 : p.ids.local;
+    const int tokens = 16 / diag, experts = kKind == kMatvec ? 0 : p.ids.local;
+    int by_blocks = rows_expected <= tokens ? 1 : 4;
     auto plan = [&](int rows, int batch) { return LdsPlan(p.units, diag, by_blocks, tiles, rows, batch, experts, p.routes, kKind == kGateUp).bytes + kStaticLds; };
-    int rows = std::min(rows_most, most);
-    while (rows > (kKind == kDown ? 2 : 1) && plan(rows, 1) > limit) --rows;
+    auto rows_in = [&](int limit) {
+        int rows = std::min(rows_most, tokens * by_blocks);
+        while (rows > (kKind == kDown ? 2 : 1) && plan(rows, 1) > limit) --rows;
+        return rows;
+    };
+    // Four blocks of rows where LDS holds them, with one workgroup to a CU; else one block: with two workgroups, which share the LDS, if the rows that are
+    // expected fit half of it, with one if they do not.  (64 rows through 8192 x 8192 and 4096 x 7168 take 61 and 42 us, in four blocks that are never
+    // full 112 and 50, with two workgroups 84 and 51; 16 through 4096 x 7168 14.4, with two workgroups 18; 6 through 8192 x 8192 14.5 and 21.)
+    if (by_blocks == 4 && rows_in(kMaxLds) <= tokens) by_blocks = 1;
+    const bool two = by_blocks == 1 && rows_in(kMaxLds / 2) >= std::min(rows_expected, tokens);
+    const int limit = two ? kMaxLds / 2 : kMaxLds;
+    int rows = rows_in(limit);
     if (kKind == kDown) rows &= ~1;
     if constexpr (kKind == kMatvec) {
         // A pass waits for its rows, so there are as many passes, even ones of four rows and more, as CUs without work can take (33 rows through
-        // 1407 x 2880: 11.5 us, 14.1 in passes of 16, 16 and 1 (10.1 since scales stay in registers); 16 through 2048 x 2048: 7.2 and 10.0; 64 through 512 x 2048: 9.0 and 14.4; where
-        // LDS asks for more passes than CUs anyhow it makes no odds: 64 through 4096 x 7168 50.9 and 50.7).
+        // 1407 x 2880: 11.5 us, 14.1 in passes of 16, 16 and 1 (10.1 since scales stay in registers); 16 through 2048 x 2048: 7.2 and 10.0; 64 through 512 x 2048: 9.0 and 14.4).
         const int passes = std::max((p.rows + rows - 1) / rows, std::min(256 / p.steps, (p.rows + 3) / 4));
         rows = (p.rows + passes - 1) / passes;
     }
@@ -682,7 +689,7 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     const int matrices = kKind == kMatvec ? (p.rows + rows - 1) / rows : matrices_most;
     const long long all_steps = static_cast<long long>(matrices) * p.steps;
     DPEP_REQUIRE(all_steps <= INT32_MAX, "w4: N=%d is too much for %d rows of K=%d", p.n, p.rows, p.k);
-    const int grid = static_cast<int>(std::min<long long>(all_steps, by_blocks == 1 ? 512 : 256));
+    const int grid = static_cast<int>(std::min<long long>(all_steps, two ? 512 : 256));
     int status = DPEP_OK;
     auto go = [&](auto half, auto zeros, auto d, auto b, auto streamed) {
         constexpr auto kernel = product_kernel<kKind, half(), zeros(), d(), b(), streamed()>;
