@@ -96,6 +96,23 @@ def test_experts(tokens, hidden, inter, topk, experts, group, zeros, dtype, mask
     assert torch.equal(y, again)
 
 
+# Long rows, of which LDS holds fewer than a pass could take: in halves and all of it, one block of rows and several passes.
+@pytest.mark.parametrize("rows,n,k,group,zeros,dtype", [
+    (20, 48, 8192, 128, False, "bf16"), (64, 40, 7168, 128, True, "fp16"), (12, 33, 8192, 256, False, "bf16"), (6, 65, 8192, 64, True, "bf16"),
+    (9, 64, 16384, 64, True, "bf16"), (70, 20, 16384, 32, False, "fp16"), (5, 2, 16384, 16384, False, "bf16"), (17, 16, 4096, 128, False, "fp16"),
+])
+def test_matvec_of_long_rows(rows, n, k, group, zeros, dtype):
+    test_matvec(rows, n, k, group, zeros, dtype)
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,topk,experts,group,zeros,dtype", [
+    (24, 7168, 64, 2, 2, 64, False, "bf16"), (12, 8192, 128, 1, 1, 128, True, "bf16"), (6, 8192, 64, 1, 2, 32, True, "fp16"),
+    (10, 128, 8192, 1, 2, 128, False, "fp16"), (30, 128, 4096, 2, 3, 64, True, "bf16"),
+])
+def test_experts_of_long_rows(tokens, hidden, inter, topk, experts, group, zeros, dtype):
+    test_experts(tokens, hidden, inter, topk, experts, group, zeros, dtype, 0.1, 0, torch.int64)
+
+
 def test_one_expert_twice_in_a_token():
     from deepep_amd import w4
 
