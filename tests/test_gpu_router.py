@@ -200,6 +200,29 @@ def test_infinities_and_nans(score):
     assert torch.isfinite(grad).all() and grad[0].tolist() == [0] * 4
 
 
+@pytest.mark.parametrize("experts,groups,topk_groups", [
+    (64, 4, 2), (64, 16, 5), (64, 64, 9), (63, 7, 3), (128, 8, 4), (128, 32, 8), (256, 8, 4), (256, 4, 3), (256, 64, 31), (240, 6, 2), (512, 4, 1),
+    (512, 8, 7), (1024, 64, 20), (1024, 2, 1),
+])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_with_ties(experts, groups, topk_groups, score):
+    """Groups of one lane to all of them, whole registers or not, with equal scores everywhere: the lower group and expert come first.  Softmax: small
+    whole logits; sigmoid: logits of zero, whose score is 1/2 exactly, and biases of eighths, so that sums are exact."""
+    from deepep_amd import Router
+
+    rng = np.random.default_rng(experts + groups)
+    tokens, bias = 40, None
+    z = rng.integers(-2, 3, size=(tokens, experts)).astype(np.float64)
+    if score == "sigmoid":
+        z, bias = np.zeros((tokens, experts)), rng.integers(-2, 3, size=experts) / 8.0
+    z[rng.random(z.shape) < 0.4] = -np.inf
+    z[5, : experts - experts // groups] = -np.inf  # only the last group has any
+    topk = min(8, experts // groups * topk_groups)
+    router = Router(experts, topk, score=score, num_groups=groups, num_topk_groups=topk_groups)
+    idx, _ = router.route(torch.from_numpy(z).float().cuda(), None if bias is None else torch.from_numpy(bias).float().cuda())
+    np.testing.assert_array_equal(idx.cpu().numpy(), _oracle_ids(router, z, bias, None))
+
+
 def test_underflowing_scores():
     """Sigmoids that are all zero in fp32: the weights and gradients stay finite, ties go to the lowest index."""
     from deepep_amd import Router

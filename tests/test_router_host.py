@@ -20,6 +20,29 @@ def test_router_arguments(arguments):
         Router(**arguments)
 
 
+@pytest.mark.parametrize("arguments", [
+    dict(num_experts=256, num_topk=2, num_groups=128), dict(num_experts=8, num_topk=2, scale=1e-31), dict(num_experts=8, num_topk=2, scale=-1e31),
+    dict(num_experts=8, num_topk=2, scale="1"),
+])
+def test_router_limits(arguments):
+    with pytest.raises(ValueError):
+        Router(**arguments)
+
+
+def test_c_abi_limits():
+    lib = _lib.load()
+
+    def refused(spec, tokens, word):
+        assert lib.dpep_route(ctypes.byref(spec), None, None, None, tokens, None, None, None) == -1
+        assert word in lib.dpep_last_error().decode()
+
+    refused(ops.RouterSpec(256, 4, 128, 1, 0, 1, 1.0, 0, 8), 1, "num_groups")
+    refused(ops.RouterSpec(16, 4, 1, 1, 0, 1, 1e-31, 0, 8), 1, "scale")
+    refused(ops.RouterSpec(16, 4, 1, 1, 0, 1, 1.0, 0, 8), (1 << 30) + 1, "num_tokens")
+    big = ops._W4(256, 256, None, (1 << 30) + 1, 128, 32)
+    assert lib.dpep_w4_matvec(ctypes.byref(big), 1, 256, 1, 256, None) == -1 and "N=" in lib.dpep_last_error().decode()
+
+
 def test_c_abi_refuses_before_it_launches():
     lib = _lib.load()
     spec = ops.RouterSpec(16, 4, 1, 1, 0, 1, 1.0, 0, 8)
