@@ -469,7 +469,8 @@ __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Fo
                 if (lane < c.topk) {
                     if (c.wide) (static_cast<int64_t*>(c.topk_idx) + to)[lane] = mine;
                     else (static_cast<int32_t*>(c.topk_idx) + to)[lane] = mine;
-                    (c.topk_weights + to)[lane] = weight * c.scale;
+                    // (not a product: a slot without an expert weighs 0 whatever the row holds, and padding rows may hold anything)
+                    (c.topk_weights + to)[lane] = mine >= 0 ? weight * c.scale : 0.0f;
                 }
             }
             if constexpr (kBalance) {

@@ -361,3 +361,37 @@ def test_native_and_python_layers_agree():
         assert router._native.route(leaf, bias, mask) is None
         for a, b in zip(native, step(leaf)):
             assert torch.equal(a, b.detach())
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("experts,groups", [(4, 1), (300, 1), (256, 4)])
+def test_slots_without_a_route_weigh_nothing(score, normalize, experts, groups):
+    """Padding rows may hold anything, and a row that runs out of experts may hold a NaN or +inf among those it has: the slots that are left
+    get -1 and 0, and padding takes no part in loss or gradient."""
+    from deepep_amd import Router
+
+    inf, nan = float("inf"), float("nan")
+    gen = torch.Generator().manual_seed(experts)
+    z = torch.randn(10, experts, generator=gen)
+    real = torch.tensor([True, False, False, False, True, True, True, False, True, True])
+    z[1], z[2, 1], z[3, 2], z[7] = nan, nan, inf, -inf
+    z[1, 0] = 0.0
+    for row, first in ((4, nan), (5, inf), (6, 1.0)):
+        z[row] = -inf
+        z[row, 3] = first
+    router = Router(experts, 3, score=score, normalize=normalize, scale=-1.5, num_groups=groups, num_topk_groups=min(groups, 2))
+    z, real_gpu = z.cuda(), real.cuda()
+    idx, weights = router.route(z, token_mask=real_gpu)
+    idx2, weights2, balance = router.route_with_balance(z, token_mask=real_gpu)
+    assert torch.equal(idx, idx2) and torch.equal(weights.view(torch.int32), weights2.view(torch.int32))
+    assert (idx[~real_gpu] == -1).all() and (idx[4:7] == torch.tensor([3, -1, -1]).cuda()).all() and (idx[[0, 8, 9]] >= 0).all()
+    assert (weights[idx < 0] == 0).all(), weights.tolist()
+    assert torch.isnan(weights[4, 0]) and torch.isfinite(weights[[0, 6, 8, 9]]).all()
+    kept = torch.tensor([0, 1, 2, 3, 6, 7, 8, 9]).cuda()
+    z, idx, weights, real = z[kept].contiguous(), idx[kept].contiguous(), weights[kept].contiguous(), real[kept.cpu()]
+    again = router.balance_loss(z, idx)
+    assert again.tokens.tolist() == [int(real.sum())] and torch.isfinite(again.losses).all()
+    grad = router.backward(z, idx, topk_weights=weights, grad_weights=torch.full_like(weights, nan).masked_fill(idx >= 0, 1.0), balance=again,
+                           grad_losses=torch.ones(1).cuda())
+    assert torch.isfinite(grad).all() and not grad[~real.cuda()].any()
