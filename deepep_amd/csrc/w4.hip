@@ -540,8 +540,10 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
                 const int to = tile_row(g, tile) + n;
                 const bool mine_to_store = w == 0 && g < p.tile_groups && to < matrix_rows;
                 if constexpr (kKind == kMatvec) {
+                    // A last tile that was moved up stores its own columns alone: it adds the shares of k in another order than the tile in front (they
+                    // go round with the step), so the columns that both hold may differ in their last bits.  (Experts' matrices have whole tiles.)
                     const float y = shared(place, group, tile, m, n, w);
-                    if (mine_to_store) static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(y, kHalf);
+                    if (mine_to_store && to >= g * 16) static_cast<uint16_t*>(p.out)[static_cast<size_t>(first_row + m) * p.n + to] = narrow(y, kHalf);
                 } else if constexpr (kKind == kGateUp) {
                     const float gate = shared(place, group, 0, m, n, w), up = shared(place, group, 1, m, n, w);
                     const int route = my_routes[first_row + m];

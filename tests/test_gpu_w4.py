@@ -261,3 +261,22 @@ def test_native_and_python_layers_agree():
     assert _lib.host().w4_matvec(leaf, *matrix, None) is None
     assert torch.equal(w4.matvec(leaf, matrix), w4.matvec(x, matrix))
     assert torch.equal(w4.expert_ffn(leaf, ids, route_weights, gate_up, down), w4.expert_ffn(x, ids, route_weights, gate_up, down))
+
+
+@pytest.mark.parametrize("rows,n,k", [(16, 17, 8192), (16, 129, 4096), (33, 65, 8192), (1, 4097, 7168), (64, 31, 2048), (4, 1407, 2816), (3, 250, 16384)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_columns_of_a_matrix_that_ends_inside_a_tile(rows, n, k, dtype):
+    """The bits are those of the same columns of a matrix of whole tiles.  Eight parts of k cancel (the same weights, whole numbers that add up to
+    zero), so a result is what its sums in 32 bits left over, and any other order of them shows."""
+    from deepep_amd import w4
+
+    rng = np.random.default_rng(n + k)
+    whole = -(-n // 16) * 16
+    parts = [rng.integers(-15, 16, size=(rows, k // 8)) for _ in range(7)]
+    x = torch.from_numpy(np.concatenate([*parts, -sum(parts)], axis=1).astype(np.float64)).to(DTYPES[dtype]).cuda()
+    packed = torch.from_numpy(np.tile(rng.integers(0, 256, size=(whole, k // 16)).astype(np.uint8), (1, 8))).cuda()
+    scales = torch.from_numpy(np.tile(2 ** rng.uniform(-6, 8, size=(whole, k // 8 // 32)), (1, 8))).to(DTYPES[dtype]).cuda()
+    want = w4.matvec(x, w4.W4Weights(packed, scales))
+    assert (want != 0).float().mean() > 0.2  # (there are rounding errors to compare)
+    for _ in range(3):
+        assert torch.equal(w4.matvec(x, w4.W4Weights(packed[:n].contiguous(), scales[:n].contiguous())), want[:, :n])
