@@ -35,6 +35,10 @@ def _integer(name, value, lower, upper):
         raise ValueError(f"{name} must be an integer in [{lower}, {upper}]")
 
 
+def _parameter(name):
+    return property(lambda router: router._parameters[name])
+
+
 class Router:
     """How a layer routes.
 
@@ -42,8 +46,12 @@ class Router:
     sigmoid(logit) + bias, weights are the sigmoids.  An expert whose logit is -inf is never chosen.  ``normalize``: the chosen
     weights are divided by their sum; ``scale`` multiplies them.  ``num_groups`` > 1: the experts of the ``num_topk_groups`` best
     groups stay (a group's score: its largest key for softmax, the sum of its two largest for sigmoid).  Ties go to the lowest index.
-    ``index_dtype``: int64 as ``ElasticBuffer.dispatch`` takes ids, or int32 as ``mega_moe`` does.
+    ``index_dtype``: int64 as ``ElasticBuffer.dispatch`` takes ids, or int32 as ``mega_moe`` does.  The parameters can be read and not set;
+    a router can be copied and pickled.
     """
+
+    num_experts, num_topk, num_groups, num_topk_groups, score, normalize, scale, index_dtype = map(_parameter, (
+        "num_experts", "num_topk", "num_groups", "num_topk_groups", "score", "normalize", "scale", "index_dtype"))
 
     def __init__(self, num_experts: int, num_topk: int, *, score: str = "softmax", normalize: bool = True, scale: float = 1.0,
                  num_groups: int = 1, num_topk_groups: int = 1, index_dtype: torch.dtype = torch.int64):
@@ -61,12 +69,21 @@ class Router:
             raise ValueError("scale must be a number of 1e-30 to 1e30 in magnitude")
         if index_dtype not in (torch.int64, torch.int32):
             raise ValueError("index_dtype must be torch.int64 or torch.int32")
-        self.num_experts, self.num_topk = num_experts, num_topk
-        self.num_groups, self.num_topk_groups = num_groups, num_topk_groups
-        self.score, self.normalize, self.scale, self.index_dtype = score, bool(normalize), float(scale), index_dtype
+        self._parameters = dict(num_experts=num_experts, num_topk=num_topk, num_groups=num_groups, num_topk_groups=num_topk_groups, score=score,
+                                normalize=bool(normalize), scale=float(scale), index_dtype=index_dtype)
+        self._make_native()
+
+    def _make_native(self):
         # Ordinary calls are made natively (csrc/host.cpp); the ones that come back as None, faulty or unusual, go through ops.
-        self._native = _lib.host().Router(num_experts, num_topk, num_groups, num_topk_groups, ops.SCORES.index(score), int(self.normalize),
-                                          self.scale, 8 if index_dtype == torch.int64 else 4)
+        self._native = _lib.host().Router(self.num_experts, self.num_topk, self.num_groups, self.num_topk_groups, ops.SCORES.index(self.score),
+                                          int(self.normalize), self.scale, 8 if self.index_dtype == torch.int64 else 4)
+
+    def __getstate__(self):
+        return {name: value for name, value in self.__dict__.items() if name != "_native"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._make_native()
 
     def _spec(self) -> ops.RouterSpec:
         return ops.RouterSpec(self.num_experts, self.num_topk, self.num_groups, self.num_topk_groups, ops.SCORES.index(self.score),

@@ -29,6 +29,27 @@ def test_router_limits(arguments):
         Router(**arguments)
 
 
+def test_parameters_are_fixed_and_survive_copies():
+    """One set of parameters serves the native and the Python path: it cannot change under either of them."""
+    import copy
+    import pickle
+
+    class Named(Router):
+        pass
+
+    parameters = dict(num_experts=64, num_topk=6, score="sigmoid", normalize=False, scale=2.5, num_groups=8, num_topk_groups=3, index_dtype=torch.int32)
+    router = Named(**parameters)
+    router.layer = 7
+    for name, value in parameters.items():
+        assert getattr(router, name) == value
+        with pytest.raises(AttributeError):
+            setattr(router, name, value)
+    for other in (copy.copy(router), copy.deepcopy(router), pickle.loads(pickle.dumps(Router(**parameters)))):
+        assert {name: getattr(other, name) for name in parameters} == parameters and isinstance(other, Router)
+        assert type(other._native) is type(router._native) and bytes(other._spec()) == bytes(router._spec())
+    assert copy.deepcopy(router).layer == 7 and type(copy.copy(router)) is Named
+
+
 def test_c_abi_limits():
     lib = _lib.load()
 
