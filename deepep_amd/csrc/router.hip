@@ -838,9 +838,17 @@ int run_forward(const dpep_router* r, Forward call, int num_tokens, bool route, 
     return launch_status(what);
 }
 
-int check_balance(const dpep_router* r, const int32_t* sequence_offsets, int num_sequences, const float* losses, const int32_t* counts, const int32_t* tokens,
-                  const void* scratch, const char* what)
+// A sequence's routes are counted in 32 bits.
+int check_routes(const dpep_router* r, int num_tokens, const char* what)
 {
+    DPEP_REQUIRE(static_cast<long long>(num_tokens) * r->num_topk < (1ll << 31), "%s: T*K must fit int32", what);
+    return DPEP_OK;
+}
+
+int check_balance(const dpep_router* r, int num_tokens, const int32_t* sequence_offsets, int num_sequences, const float* losses, const int32_t* counts,
+                  const int32_t* tokens, const void* scratch, const char* what)
+{
+    if (int rc = check_routes(r, num_tokens, what); rc != DPEP_OK) return rc;
     DPEP_REQUIRE(num_sequences >= 1 && (sequence_offsets != nullptr || num_sequences == 1), "%s: num_sequences=%d", what, num_sequences);
     DPEP_REQUIRE(losses != nullptr && counts != nullptr && tokens != nullptr && scratch != nullptr, "%s: a NULL buffer", what);
     return DPEP_OK;
@@ -877,7 +885,7 @@ int dpep_balance_loss(const dpep_router* r, const void* logits, const void* topk
                       float* losses, int32_t* counts, int32_t* tokens, void* scratch, void* stream)
 {
     if (int rc = check_router(r, num_tokens, "balance_loss"); rc != DPEP_OK) return rc;
-    if (int rc = check_balance(r, sequence_offsets, num_sequences, losses, counts, tokens, scratch, "balance_loss"); rc != DPEP_OK) return rc;
+    if (int rc = check_balance(r, num_tokens, sequence_offsets, num_sequences, losses, counts, tokens, scratch, "balance_loss"); rc != DPEP_OK) return rc;
     DPEP_REQUIRE(num_tokens == 0 || (logits != nullptr && topk_idx != nullptr), "balance_loss: a NULL buffer");
     Forward call = {};
     call.logits = logits;
@@ -892,7 +900,7 @@ int dpep_route_balance(const dpep_router* r, const void* logits, const float* bi
 {
     if (int rc = check_router(r, num_tokens, "route_balance"); rc != DPEP_OK) return rc;
     DPEP_REQUIRE(bias == nullptr || r->score == DPEP_SCORE_SIGMOID, "route_balance: a bias needs sigmoid scores");
-    if (int rc = check_balance(r, sequence_offsets, num_sequences, losses, counts, tokens, scratch, "route_balance"); rc != DPEP_OK) return rc;
+    if (int rc = check_balance(r, num_tokens, sequence_offsets, num_sequences, losses, counts, tokens, scratch, "route_balance"); rc != DPEP_OK) return rc;
     DPEP_REQUIRE(num_tokens == 0 || (logits != nullptr && topk_idx != nullptr && topk_weights != nullptr), "route_balance: a NULL buffer");
     Forward call = {};
     call.logits = logits;
@@ -913,6 +921,8 @@ int dpep_router_backward(const dpep_router* r, const dpep_router_gradients* g, i
     DPEP_REQUIRE(g->grad_losses == nullptr || (g->counts != nullptr && g->tokens != nullptr && g->num_sequences >= 1 &&
                                                (g->sequence_offsets != nullptr || g->num_sequences == 1)),
                  "router_backward: grad_losses needs the counts and tokens of its sequences");
+    if (g->grad_losses != nullptr)
+        if (int rc = check_routes(r, num_tokens, "router_backward"); rc != DPEP_OK) return rc;
     DPEP_REQUIRE(g->grad_weights == nullptr || !r->normalize || g->topk_weights != nullptr || num_tokens == 0, "router_backward: normalised weights are needed");
     if (num_tokens == 0) return DPEP_OK;
     DPEP_REQUIRE(g->logits != nullptr && g->topk_idx != nullptr && g->grad_logits != nullptr, "router_backward: a NULL buffer");

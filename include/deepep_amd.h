@@ -385,7 +385,8 @@ int dpep_route(const dpep_router* r, const void* logits, const float* bias, cons
 
 /* Balance loss of every sequence, and its counts.  A token without a route (ids outside 0..E-1) is padding.  In a sequence of N other
  * tokens with R routes, c_e of them to expert e: loss = sum_e (E c_e / R) (sum_t p_te / N), p a token's softmax, or its sigmoids over
- * (their sum + 1e-20); 0 for a sequence without tokens.  Sums are taken in an order that depends on the sizes alone.
+ * (their sum + 1e-20); 0 for a sequence without tokens.  Sums are taken in an order that depends on the sizes alone.  T*K < 2^31, here and in
+ * the loss's gradient.
  *   sequence_offsets  int32 [B+1] ascending from 0 to T, or NULL: one sequence
  *   losses fp32 [B];  counts int32 [B,E];  tokens int32 [B] (N);  scratch  dpep_balance_scratch_bytes, 4-byte aligned */
 size_t dpep_balance_scratch_bytes(int num_experts, int num_tokens, int num_sequences);

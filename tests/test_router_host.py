@@ -64,6 +64,22 @@ def test_c_abi_limits():
     assert lib.dpep_w4_matvec(ctypes.byref(big), 1, 256, 1, 256, None) == -1 and "N=" in lib.dpep_last_error().decode()
 
 
+def test_routes_of_a_balance_loss_fit_32_bits():
+    """A sequence's routes are added up in 32 bits: a batch of 2^31 and more has no loss and no gradient of one.  (Without buffers, so
+    that nothing is launched.)"""
+    lib = _lib.load()
+    spec = ops.RouterSpec(16, 16, 1, 1, 0, 1, 1.0, 0, 8)
+    from_weights = ops._RouterGradients(None, None, 256, 256, None, None, None, None, None, 1)
+    from_losses = ops._RouterGradients(None, None, 256, 256, None, 256, 256, 256, None, 1)
+    calls = (lambda tokens: lib.dpep_balance_loss(ctypes.byref(spec), None, None, tokens, None, 1, 256, 256, 256, 256, None),
+             lambda tokens: lib.dpep_route_balance(ctypes.byref(spec), None, None, None, tokens, None, 1, None, None, 256, 256, 256, 256, None),
+             lambda tokens: lib.dpep_router_backward(ctypes.byref(spec), ctypes.byref(from_losses), tokens, None))
+    for call in calls:
+        assert call(1 << 27) == -1 and "T*K" in lib.dpep_last_error().decode()
+        assert call((1 << 27) - 1) == -1 and "NULL" in lib.dpep_last_error().decode()
+    assert lib.dpep_router_backward(ctypes.byref(spec), ctypes.byref(from_weights), 1 << 27, None) == -1 and "NULL" in lib.dpep_last_error().decode()
+
+
 def test_c_abi_refuses_before_it_launches():
     lib = _lib.load()
     spec = ops.RouterSpec(16, 4, 1, 1, 0, 1, 1.0, 0, 8)
