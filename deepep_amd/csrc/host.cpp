@@ -1365,6 +1365,7 @@ PyObject* cast_back(PyObject*, PyObject* const* a, Py_ssize_t n)
 
 // ---- router and 4-bit products ---------------------------------------------------------------------------------------------------
 // The kernels of a decode step's router or matrix take 4 to 8 us; the same calls through the Python layer take 11.
+// Sizes beyond the operators' limits are left to the Python layer too, which names them before anything is allocated.
 // A tensor argument that may be None: true if it is, or is a plain one of this type and shape.
 inline bool optional_plain(PyObject* o, int device, at::ScalarType type, std::initializer_list<int64_t> shape, const at::Tensor** out)
 {
@@ -1421,9 +1422,11 @@ const at::Tensor* router_logits(PyObject* o, dpep_router* r, int* device)
     if (!on_gpu(o) || c10::InferenceMode::is_enabled()) return nullptr;
     *device = c10::hip::current_device();
     const at::Tensor* t = plain(o, *device);
-    if (t == nullptr || t->dim() != 2 || t->size(1) != r->num_experts || t->size(0) > 0x7fffffff || (r->logits_type = type_code(t->scalar_type())) < 0) return nullptr;
+    if (t == nullptr || t->dim() != 2 || t->size(1) != r->num_experts || t->size(0) > DPEP_MAX_ROUTER_TOKENS || (r->logits_type = type_code(t->scalar_type())) < 0) return nullptr;
     return t;
 }
+// Whether a batch's routes can be added up (a balance loss and its gradient).
+inline bool routes_fit(const dpep_router& r, int64_t tokens) { return tokens * r.num_topk <= 0x7fffffff; }
 // Number of sequences, 0 for offsets this path does not take.
 int64_t router_sequences(PyObject* o, int device, const at::Tensor** offsets)
 {
@@ -1446,7 +1449,7 @@ PyObject* Router_route(PyObject* o, PyObject* const* a, Py_ssize_t n)
     const at::Tensor *bias, *mask, *offsets = nullptr;
     if (!optional_plain(a[1], device, at::kFloat, {r.num_experts}, &bias) || !optional_plain(a[2], device, at::kBool, {tokens}, &mask)) Py_RETURN_NONE;
     const int64_t sequences = n == 4 ? router_sequences(a[3], device, &offsets) : 1;
-    if (sequences == 0) Py_RETURN_NONE;
+    if (sequences == 0 || (n == 4 && !routes_fit(r, tokens))) Py_RETURN_NONE;
     at::Tensor idx = allocate({tokens, r.num_topk}, r.index_bytes == 8 ? at::kLong : at::kInt, device);
     at::Tensor weights = allocate({tokens, r.num_topk}, at::kFloat, device);
     const hipStream_t stream = current_stream(device).raw;
@@ -1486,7 +1489,7 @@ PyObject* Router_balance_loss(PyObject* o, PyObject* const* a, Py_ssize_t n)
     const at::Tensor* idx = router_ids(a[1], &r, tokens, device);
     if (idx == nullptr) Py_RETURN_NONE;
     const int64_t sequences = router_sequences(a[2], device, &offsets);
-    if (sequences == 0) Py_RETURN_NONE;
+    if (sequences == 0 || !routes_fit(r, tokens)) Py_RETURN_NONE;
     at::Tensor losses = allocate({sequences}, at::kFloat, device), counts = allocate({sequences, r.num_experts}, at::kInt, device);
     at::Tensor members = allocate({sequences}, at::kInt, device);
     at::Tensor scratch = allocate({static_cast<int64_t>(dpep_balance_scratch_bytes(r.num_experts, static_cast<int>(tokens), static_cast<int>(sequences)))}, at::kByte, device);
@@ -1514,7 +1517,7 @@ PyObject* Router_backward(PyObject* o, PyObject* const* a, Py_ssize_t n)
         !optional_plain(a[7], device, at::kFloat, {sequences}, &grad_losses))
         Py_RETURN_NONE;
     if ((grad_weights == nullptr && grad_losses == nullptr) || (grad_weights != nullptr && r.normalize && weights == nullptr) ||
-        (grad_losses != nullptr && (counts == nullptr || members == nullptr)))
+        (grad_losses != nullptr && (counts == nullptr || members == nullptr || !routes_fit(r, tokens))))
         Py_RETURN_NONE;
     at::Tensor grad = allocate({tokens, r.num_experts}, logits->scalar_type(), device);
     const dpep_router_gradients g = {logits->data_ptr(), idx->data_ptr(), data<float>(weights), data<float>(grad_weights), data<int32_t>(offsets), data<int32_t>(counts),
@@ -1540,7 +1543,7 @@ bool w4_weights(PyObject* packed_object, PyObject* scales_object, PyObject* zero
     for (int64_t d = 0; d + 1 < dims; ++d)
         if (scales->size(d) != packed->size(d)) return false;
     const int64_t n = packed->size(dims - 2), k = 2 * packed->size(dims - 1), groups = scales->size(dims - 1);
-    if (n < 1 || k < 1 || groups < 1 || n > 0x7fffffff || k > 0x7fffffff || k % groups != 0) return false;
+    if (n < 1 || k < 1 || groups < 1 || n > DPEP_W4_MAX_N || k > DPEP_W4_MAX_K || k % groups != 0) return false;
     if (zeros != nullptr && (zeros->scalar_type() != at::kByte || zeros->sizes() != scales->sizes())) return false;
     *w = {static_cast<const uint8_t*>(packed->data_ptr()), scales->data_ptr(), data<uint8_t>(zeros), static_cast<int32_t>(n), static_cast<int32_t>(k),
           static_cast<int32_t>(k / groups)};
@@ -1553,7 +1556,7 @@ const at::Tensor* w4_rows(PyObject* o, int* device)
     if (!on_gpu(o) || c10::InferenceMode::is_enabled()) return nullptr;
     *device = c10::hip::current_device();
     const at::Tensor* x = plain(o, *device);
-    if (x == nullptr || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) || x->dim() != 2 || x->size(0) > 0x7fffffff || !aligned16(*x)) return nullptr;
+    if (x == nullptr || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) || x->dim() != 2 || x->size(0) > DPEP_W4_MAX_ROWS || !aligned16(*x)) return nullptr;
     return x;
 }
 // w4_matvec(x, packed, scales, zeros, out) -> y
@@ -1582,12 +1585,12 @@ PyObject* w4_experts(PyObject*, PyObject* const* a, Py_ssize_t n)
     dpep_w4 gate_up, down;
     int64_t local, local_down;
     if (x == nullptr || !w4_weights(a[3], a[4], a[5], 3, x->scalar_type(), device, &gate_up, &local) ||
-        !w4_weights(a[6], a[7], a[8], 3, x->scalar_type(), device, &down, &local_down) || local != local_down || local > 0x7fffffff || gate_up.n != 2 * down.k ||
+        !w4_weights(a[6], a[7], a[8], 3, x->scalar_type(), device, &down, &local_down) || local != local_down || local > DPEP_MAX_LOCAL_EXPERTS || gate_up.n != 2 * down.k ||
         gate_up.k != down.n || x->size(1) != gate_up.k)
         Py_RETURN_NONE;
     const int64_t tokens = x->size(0);
     const at::Tensor* idx = plain(a[1], device);
-    if (idx == nullptr || idx->dim() != 2 || idx->size(0) != tokens || idx->size(1) < 1 || idx->size(1) > 0x7fffffff ||
+    if (idx == nullptr || idx->dim() != 2 || idx->size(0) != tokens || idx->size(1) < 1 || idx->size(1) > DPEP_MAX_TOPK || tokens * idx->size(1) > DPEP_W4_MAX_ROUTES ||
         (idx->scalar_type() != at::kLong && idx->scalar_type() != at::kInt) || !optional_plain(a[2], device, at::kFloat, {tokens, idx->size(1)}, &weights) ||
         weights == nullptr || !optional_plain(a[10], device, x->scalar_type(), {tokens, gate_up.k}, &out))
         Py_RETURN_NONE;

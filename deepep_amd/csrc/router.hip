@@ -777,7 +777,7 @@ struct BalanceScratch {
 int check_router(const dpep_router* r, int num_tokens, const char* what)
 {
     DPEP_REQUIRE(r != nullptr, "%s: router is NULL", what);
-    DPEP_REQUIRE(num_tokens >= 0 && num_tokens <= 1 << 30, "%s: num_tokens=%d is not in [0, 2^30]", what, num_tokens);
+    DPEP_REQUIRE(num_tokens >= 0 && num_tokens <= DPEP_MAX_ROUTER_TOKENS, "%s: num_tokens=%d is not in [0, 2^30]", what, num_tokens);
     DPEP_REQUIRE(r->num_experts >= 1 && r->num_experts <= kMaxRouterExperts, "%s: num_experts=%d is not in [1, %d]", what, r->num_experts, kMaxRouterExperts);
     DPEP_REQUIRE(r->num_topk >= 1 && r->num_topk <= DPEP_MAX_TOPK && r->num_topk <= r->num_experts, "%s: num_topk=%d is not in [1, min(%d, num_experts)]", what,
                  r->num_topk, DPEP_MAX_TOPK);
@@ -877,7 +877,7 @@ int dpep_route(const dpep_router* r, const void* logits, const float* bias, cons
 
 size_t dpep_balance_scratch_bytes(int num_experts, int num_tokens, int num_sequences)
 {
-    if (num_experts < 1 || num_tokens < 0 || num_sequences < 1) return 0;
+    if (num_experts < 1 || num_experts > kMaxRouterExperts || num_tokens < 0 || num_tokens > DPEP_MAX_ROUTER_TOKENS || num_sequences < 1) return 0;
     return BalanceScratch(num_experts, num_tokens, num_sequences).bytes;
 }
 

@@ -13,8 +13,8 @@
 namespace dpep {
 namespace {
 
-constexpr int kMaxRoutes = 2048;
-constexpr int kMaxK = 16384;
+constexpr int kMaxRoutes = DPEP_W4_MAX_ROUTES;
+constexpr int kMaxK = DPEP_W4_MAX_K;
 
 // Expert ids of 8 or 4 bytes.
 struct Ids {
@@ -725,7 +725,7 @@ int check_w4(const dpep_w4* w, int type, const char* what)
 {
     DPEP_REQUIRE(w != nullptr, "%s: weights is NULL", what);
     DPEP_REQUIRE(type == DPEP_TYPE_BF16 || type == DPEP_TYPE_F16, "%s: type=%d is neither BF16 nor FP16", what, type);
-    DPEP_REQUIRE(w->n >= 1 && w->n <= 1 << 30 && w->k >= 32 && w->k <= kMaxK, "%s: N=%d K=%d: N is at most 2^30, K %d", what, w->n, w->k, kMaxK);
+    DPEP_REQUIRE(w->n >= 1 && w->n <= DPEP_W4_MAX_N && w->k >= 32 && w->k <= kMaxK, "%s: N=%d K=%d: N is at most 2^30, K %d", what, w->n, w->k, kMaxK);
     DPEP_REQUIRE((w->group == 32 || w->group == 64 || (w->group >= 128 && w->group % 128 == 0)) && w->k % w->group == 0,
                  "%s: group=%d is not 32, 64 or a multiple of 128 that divides K=%d", what, w->group, w->k);
     DPEP_REQUIRE(w->packed != nullptr && w->scales != nullptr, "%s: a NULL buffer", what);
@@ -743,7 +743,7 @@ extern "C" {
 int dpep_w4_matvec(const dpep_w4* w, int type, const void* x, int num_rows, void* y, void* stream)
 {
     if (int rc = check_w4(w, type, "w4_matvec"); rc != DPEP_OK) return rc;
-    DPEP_REQUIRE(num_rows >= 0 && num_rows <= 65535, "w4_matvec: num_rows=%d is not in [0, 65535]", num_rows);
+    DPEP_REQUIRE(num_rows >= 0 && num_rows <= DPEP_W4_MAX_ROWS, "w4_matvec: num_rows=%d is not in [0, %d]", num_rows, DPEP_W4_MAX_ROWS);
     if (num_rows == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && y != nullptr && aligned16(x), "w4_matvec: a NULL or misaligned buffer");
     Product p = {};

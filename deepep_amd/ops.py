@@ -549,6 +549,8 @@ def megamoe_forward(ws, x_codes, x_scales, topk_idx, topk_weights, w1, s1, w2, s
 # ---------------------------------------------------------------------------------------------
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DPEP_TYPE_*
 SCORES = ("softmax", "sigmoid")  # DPEP_SCORE_*
+_MAX_ROUTER_TOKENS, _MAX_ROUTES = 1 << 30, (1 << 31) - 1  # DPEP_MAX_ROUTER_TOKENS; of a balance loss
+_W4_MAX_N, _W4_MAX_K, _W4_MAX_ROWS, _W4_MAX_ROUTES, _MAX_LOCAL_EXPERTS, _MAX_TOPK = 1 << 30, 16384, 65535, 2048, 1024, 32  # DPEP_*
 
 
 class RouterSpec(ctypes.Structure):
@@ -569,12 +571,21 @@ class _W4(ctypes.Structure):
                 ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("group", ctypes.c_int32)]
 
 
+def _at_most(limit, **sizes):
+    """Sizes are compared as Python holds them: the C struct or call that they go into would keep 32 bits of them, and the outputs and
+    scratch of a call that is refused need not be allocated."""
+    for name, size in sizes.items():
+        if size > limit:
+            raise ValueError(f"{name}={size} is more than {limit}")
+
+
 def _require_logits(spec: RouterSpec, logits):
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _TYPES:
         raise ValueError("logits must be an FP32, BF16 or FP16 tensor")
     _require("logits", logits, logits.dtype)
     if logits.ndim != 2 or logits.shape[1] != spec.num_experts:
         raise ValueError(f"logits must be [T, {spec.num_experts}] (got {tuple(logits.shape)})")
+    _at_most(_MAX_ROUTER_TOKENS, tokens=logits.shape[0])
     spec.logits_type = _TYPES[logits.dtype]
     return logits.shape[0], logits.device
 
@@ -586,12 +597,14 @@ def _require_routes(spec: RouterSpec, topk_idx, tokens, device):
     spec.index_bytes = topk_idx.element_size()
 
 
-def _require_sequences(sequence_offsets, device):
+def _require_sequences(spec: RouterSpec, tokens, sequence_offsets, device):
+    _at_most(_MAX_ROUTES, routes=tokens * spec.num_topk)
     if sequence_offsets is None:
         return 1
     _require("sequence_offsets", sequence_offsets, torch.int32, device=device)
     if sequence_offsets.ndim != 1 or sequence_offsets.shape[0] < 2:
         raise ValueError("sequence_offsets must be [B + 1] with B >= 1")
+    _at_most((1 << 31) - 1, sequences=sequence_offsets.shape[0] - 1)
     return sequence_offsets.shape[0] - 1
 
 
@@ -619,7 +632,7 @@ def balance_loss(spec: RouterSpec, logits, topk_idx, sequence_offsets=None):
     batch into (None: one)."""
     tokens, dev = _require_logits(spec, logits)
     _require_routes(spec, topk_idx, tokens, dev)
-    sequences = _require_sequences(sequence_offsets, dev)
+    sequences = _require_sequences(spec, tokens, sequence_offsets, dev)
     lib = _lib.load()
     losses = torch.empty((sequences,), dtype=torch.float32, device=dev)
     counts = torch.empty((sequences, spec.num_experts), dtype=torch.int32, device=dev)
@@ -641,7 +654,7 @@ def route_balance(spec: RouterSpec, logits, bias=None, token_mask=None, sequence
         _require("bias", bias, torch.float32, (spec.num_experts,), dev)
     if token_mask is not None:
         _require("token_mask", token_mask, torch.bool, (tokens,), dev)
-    sequences = _require_sequences(sequence_offsets, dev)
+    sequences = _require_sequences(spec, tokens, sequence_offsets, dev)
     spec.index_bytes = 8 if index_dtype == torch.int64 else 4
     lib = _lib.load()
     topk_idx = torch.empty((tokens, spec.num_topk), dtype=index_dtype, device=dev)
@@ -671,7 +684,7 @@ def router_backward(spec: RouterSpec, logits, topk_idx, topk_weights=None, grad_
         if spec.normalize:
             _require("topk_weights", topk_weights, torch.float32, (num_tokens, spec.num_topk), dev)
     if grad_losses is not None:
-        sequences = _require_sequences(sequence_offsets, dev)
+        sequences = _require_sequences(spec, num_tokens, sequence_offsets, dev)
         _require("grad_losses", grad_losses, torch.float32, (sequences,), dev)
         _require("counts", counts, torch.int32, (sequences, spec.num_experts), dev)
         _require("tokens", tokens, torch.int32, (sequences,), dev)
@@ -696,6 +709,8 @@ def _w4(name, packed, scales, zeros, dtype, device, ndim):
         raise ValueError(f"{name} scales must be {tuple(packed.shape[:-1])} + (K / group,) (got {tuple(scales.shape)})")
     if zeros is not None:
         _require(f"{name} zeros", zeros, torch.uint8, tuple(scales.shape), device)
+    _at_most(_W4_MAX_N, N=packed.shape[-2])
+    _at_most(_W4_MAX_K, K=k)
     return _W4(packed.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), packed.shape[-2], k, k // groups)
 
 
@@ -714,6 +729,7 @@ def w4_matvec(x, packed, scales, zeros=None, out=None):
     if x.ndim != 2 or x.shape[1] != weights.k:
         raise ValueError(f"x must be [M, {weights.k}] (got {tuple(x.shape)})")
     rows = x.shape[0]
+    _at_most(_W4_MAX_ROWS, rows=rows)
     if out is None:
         out = torch.empty((rows, weights.n), dtype=x.dtype, device=dev)
     else:
@@ -747,6 +763,9 @@ def w4_experts(x, topk_idx, topk_weights, gate_up, down, expert_begin: int = 0, 
         raise ValueError("topk_idx must be [T, K]")
     topk = topk_idx.shape[1]
     _require("topk_weights", topk_weights, torch.float32, (tokens, topk), dev)
+    _at_most(_MAX_TOPK, topk=topk)
+    _at_most(_W4_MAX_ROUTES, routes=tokens * topk)
+    _at_most(_MAX_LOCAL_EXPERTS, experts=local)
     if out is None:
         out = torch.empty((tokens, first.k), dtype=x.dtype, device=dev)
     else:

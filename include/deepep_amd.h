@@ -362,6 +362,11 @@ int dpep_megamoe_run(void* ws, const dpep_megamoe_call* call, void* stream);
 #define DPEP_TYPE_F16 2
 #define DPEP_SCORE_SOFTMAX 0
 #define DPEP_SCORE_SIGMOID 1
+#define DPEP_MAX_ROUTER_TOKENS (1 << 30)
+#define DPEP_W4_MAX_N (1 << 30)
+#define DPEP_W4_MAX_K 16384
+#define DPEP_W4_MAX_ROWS 65535
+#define DPEP_W4_MAX_ROUTES 2048
 
 /* A layer's router.  Scores: softmax over the row, or each logit's sigmoid.  Experts are chosen by key: the logit (softmax), or the
  * sigmoid plus the expert's bias, rounded to fp32; an expert whose logit is -inf is never chosen, a NaN ranks with +inf.  With

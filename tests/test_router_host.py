@@ -149,3 +149,53 @@ def test_quantize_rounds_to_half_a_step(symmetric, group):
         w4.quantize(weight, 48)
     with pytest.raises(ValueError):
         w4.quantize(weight[..., :250], 128)
+
+
+def test_sizes_are_refused_in_full_and_before_anything_is_allocated(monkeypatch):
+    """Sizes that 32 bits do not hold must not come through as what is left of them (2^32 + 5 tokens as 5), and a call beyond a limit
+    is refused for its size, not for the memory that its scratch would take.  Tensors without memory stand for those on a GPU."""
+    monkeypatch.setattr(ops, "_require", lambda name, t, *rest, **device: t)
+
+    def allocates(*_, **__):
+        raise AssertionError("allocated")
+
+    single = {dtype: torch.zeros((), dtype=dtype, device="meta") for dtype in (torch.int64, torch.int32, torch.float32, torch.bfloat16, torch.uint8)}
+
+    def shaped(shape, dtype):
+        return single[dtype].expand(shape)
+
+    many = (1 << 32) + 5
+    routes, weights = shaped((1 << 27, 16), torch.int64), shaped((1 << 27, 16), torch.float32)
+    logits, losses, ids = shaped((1 << 27, 16), torch.bfloat16), shaped((1,), torch.float32), shaped((many, 1), torch.int64)
+    router = Router(16, 16)
+    balance = (losses, shaped((1, 16), torch.int32), shaped((1,), torch.int32), None)
+    from deepep_amd import BalanceLoss
+
+    def matrix(n, k, experts=None):
+        lead = () if experts is None else (experts,)
+        return w4.W4Weights(shaped((*lead, n, k // 2), torch.uint8), shaped((*lead, n, k // 32), torch.bfloat16))
+
+    def experts(tokens, topk, inter, hidden, local):
+        return lambda: w4.expert_ffn(shaped((tokens, hidden), torch.bfloat16), shaped((tokens, topk), torch.int32), shaped((tokens, topk), torch.float32),
+                                     matrix(2 * inter, hidden, local), matrix(hidden, inter, local))
+
+    calls = {
+        "tokens": [lambda: Router(1, 1).route(shaped((many, 1), torch.bfloat16)), lambda: Router(1, 1).balance_loss(shaped((many, 1), torch.bfloat16), ids),
+                   lambda: Router(1, 1).backward(shaped((many, 1), torch.bfloat16), ids, topk_weights=ids, grad_weights=ids)],
+        "routes": [lambda: router.route_with_balance(logits), lambda: router.balance_loss(logits, routes),
+                   lambda: router.backward(logits, routes, balance=BalanceLoss(*balance), grad_losses=losses),
+                   experts(1 << 20, 32, 16384, 32, 1), experts(many, 1, 32, 32, 1)],
+        "sequences": [lambda: Router(1, 1).balance_loss(shaped((4, 1), torch.bfloat16), shaped((4, 1), torch.int64), shaped((many,), torch.int32))],
+        "N": [lambda: w4.matvec(shaped((1, 32), torch.bfloat16), matrix(many, 32))],
+        "K": [lambda: w4.matvec(shaped((1, 1 << 15), torch.bfloat16), matrix(1, 1 << 15))],
+        "rows": [lambda: w4.matvec(shaped((many, 32), torch.bfloat16), matrix(1, 32))],
+        "topk": [experts(1, many, 32, 32, 1)], "experts": [experts(1, 1, 32, 32, many)],
+    }
+    monkeypatch.setattr(torch, "empty", allocates)
+    monkeypatch.setattr(torch, "empty_like", allocates)
+    for what, refused in calls.items():
+        for call in refused:
+            with pytest.raises(ValueError, match=f"^{what}="):
+                call()
+    lib = _lib.load()
+    assert lib.dpep_balance_scratch_bytes(16, (1 << 30) + 1, 1) == 0 and lib.dpep_balance_scratch_bytes(1025, 4, 1) == 0
