@@ -10,6 +10,7 @@ torch's current stream and return without synchronising.
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional
 
 import torch
@@ -766,6 +767,12 @@ def w4_experts(x, topk_idx, topk_weights, gate_up, down, expert_begin: int = 0, 
     _at_most(_MAX_TOPK, topk=topk)
     _at_most(_W4_MAX_ROUTES, routes=tokens * topk)
     _at_most(_MAX_LOCAL_EXPERTS, experts=local)
+    try:
+        begin = operator.index(expert_begin)
+    except TypeError:
+        begin = -1
+    if not 0 <= begin < 1 << 31:
+        raise ValueError("expert_begin must be an integer in [0, 2^31)")
     if out is None:
         out = torch.empty((tokens, first.k), dtype=x.dtype, device=dev)
     else:
@@ -775,6 +782,6 @@ def w4_experts(x, topk_idx, topk_weights, gate_up, down, expert_begin: int = 0, 
     scratch = torch.empty((lib.dpep_w4_experts_scratch_bytes(tokens, topk, first.k, second.k),), dtype=torch.uint8, device=dev)
     with _on_device(dev):
         status = lib.dpep_w4_experts(ctypes.byref(first), ctypes.byref(second), _TYPES[x.dtype], _ptr(x), _ptr(topk_idx), topk_idx.element_size(),
-                                     _ptr(topk_weights), tokens, topk, int(expert_begin), local, _ptr(out), _ptr(scratch), _stream(dev))
+                                     _ptr(topk_weights), tokens, topk, begin, local, _ptr(out), _ptr(scratch), _stream(dev))
     _lib.check(status, "w4_experts")
     return out

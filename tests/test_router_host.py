@@ -199,3 +199,17 @@ def test_sizes_are_refused_in_full_and_before_anything_is_allocated(monkeypatch)
                 call()
     lib = _lib.load()
     assert lib.dpep_balance_scratch_bytes(16, (1 << 30) + 1, 1) == 0 and lib.dpep_balance_scratch_bytes(1025, 4, 1) == 0
+
+
+@pytest.mark.parametrize("begin", [1.5, "1", None, -1, 1 << 31, (1 << 32) + 1, torch.tensor(0.5)])
+def test_first_expert_is_an_integer_of_31_bits(monkeypatch, begin):
+    """1.5 must not come through as 1, nor 2^32 + 1."""
+    monkeypatch.setattr(ops, "_require", lambda name, t, *rest, **device: t)
+
+    def shaped(*shape, dtype=torch.bfloat16):
+        return torch.zeros(shape, dtype=dtype)
+
+    matrix = w4.W4Weights(shaped(2, 64, 16, dtype=torch.uint8), shaped(2, 64, 1))
+    down = w4.W4Weights(shaped(2, 32, 16, dtype=torch.uint8), shaped(2, 32, 1))
+    with pytest.raises(ValueError, match="expert_begin"):
+        w4.expert_ffn(shaped(1, 32), shaped(1, 1, dtype=torch.int32), shaped(1, 1, dtype=torch.float32), matrix, down, expert_begin=begin)
