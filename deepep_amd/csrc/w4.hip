@@ -721,6 +721,12 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     return status;
 }
 
+bool overlap(const void* a, size_t bytes_a, const void* b, size_t bytes_b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return b != nullptr && x < y + bytes_b && y < x + bytes_a;
+}
+
 int check_w4(const dpep_w4* w, int type, const char* what)
 {
     DPEP_REQUIRE(w != nullptr, "%s: weights is NULL", what);
@@ -746,6 +752,11 @@ int dpep_w4_matvec(const dpep_w4* w, int type, const void* x, int num_rows, void
     DPEP_REQUIRE(num_rows >= 0 && num_rows <= DPEP_W4_MAX_ROWS, "w4_matvec: num_rows=%d is not in [0, %d]", num_rows, DPEP_W4_MAX_ROWS);
     if (num_rows == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && y != nullptr && aligned16(x), "w4_matvec: a NULL or misaligned buffer");
+    // Workgroups store their columns while others still read rows and weights.
+    const size_t of_rows = static_cast<size_t>(num_rows) * 2, groups = static_cast<size_t>(w->n) * (w->k / w->group), y_bytes = of_rows * w->n;
+    DPEP_REQUIRE(!overlap(y, y_bytes, x, of_rows * w->k) && !overlap(y, y_bytes, w->packed, static_cast<size_t>(w->n) * (w->k / 2)) &&
+                     !overlap(y, y_bytes, w->scales, groups * 2) && !overlap(y, y_bytes, w->zeros, groups),
+                 "w4_matvec: y must not overlap x or the weights");
     Product p = {};
     p.packed = w->packed;
     p.scales = static_cast<const uint16_t*>(w->scales);
@@ -780,6 +791,9 @@ int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const
     if (num_tokens == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && topk_idx != nullptr && topk_weights != nullptr && y != nullptr && scratch != nullptr && aligned16(x) && aligned16(scratch),
                  "w4_experts: a NULL or misaligned buffer");
+    // (the sum of the routes reads ids while it stores y; rows and weights have been read by then)
+    DPEP_REQUIRE(!overlap(y, static_cast<size_t>(num_tokens) * down->n * 2, topk_idx, static_cast<size_t>(num_tokens) * num_topk * index_bytes),
+                 "w4_experts: y must not overlap topk_idx");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int routes = num_tokens * num_topk, slots = std::min(routes, num_local);
     // rows of an expert: about routes / experts, at most all of them (a token may name an expert twice)

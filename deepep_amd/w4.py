@@ -49,7 +49,7 @@ def dequantize(weights: W4Weights) -> torch.Tensor:
 
 
 def matvec(x: torch.Tensor, weights: W4Weights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x [M,K] times the matrix [N,K]: [M,N] in x's type (BF16 or FP16)."""
+    """x [M,K] times the matrix [N,K]: [M,N] in x's type (BF16 or FP16).  ``out`` must overlap neither x nor the weights."""
     packed, scales, zeros = weights
     done = _lib.host().w4_matvec(x, packed, scales, zeros, out)  # the ordinary call, made natively
     return ops.w4_matvec(x, packed, scales, zeros, out=out) if done is None else done
@@ -61,7 +61,7 @@ def expert_ffn(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: torch.Tens
     the halves of gate_up[e] x[t], e = topk_idx[t,s] - expert_begin.
 
     x [T,H] BF16 or FP16, topk_idx int64 or int32 [T,K] (T * K at most 2048; -1 and experts that are not local do not count),
-    topk_weights FP32 [T,K], gate_up [L,2I,H] (gate rows, then up rows), down [L,H,I].  Returns [T,H] in x's type."""
+    topk_weights FP32 [T,K], gate_up [L,2I,H] (gate rows, then up rows), down [L,H,I].  Returns [T,H] in x's type; ``out`` may be x."""
     done = _lib.host().w4_experts(x, topk_idx, topk_weights, *gate_up, *down, expert_begin, out)  # the ordinary call, made natively
     if done is not None:
         return done

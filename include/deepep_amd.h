@@ -431,13 +431,14 @@ typedef struct dpep_w4 {
     const uint8_t* zeros;
     int32_t n, k, group;
 } dpep_w4;
-/* y[m] = W x[m]: x, y of `type` (BF16 or FP16), x [M,K] 16-byte aligned, y [M,N], sums in fp32, rounded once.  M at most 65535; meant for a
- * few rows: beyond about 16 the time grows with M. */
+/* y[m] = W x[m]: x, y of `type` (BF16 or FP16), x [M,K] 16-byte aligned, y [M,N], which overlaps neither x nor the weights, sums
+ * in fp32, rounded once.  M at most 65535; meant for a few rows: beyond about 16 the time grows with M. */
 int dpep_w4_matvec(const dpep_w4* w, int type, const void* x, int num_rows, void* y, void* stream);
 /* An expert layer for few tokens (T*K <= 2048 routes): y[t] = sum over the slots s of topk_weights[t,s] * W2[e] (silu(g) * u) with
  * (g, u) = W1[e] x[t], e = topk_idx[t,s] - expert_begin; slots whose expert is not one of the num_local do not count, a token without
  * a slot that does gets zeros.  The rows between the products keep 16 bits of mantissa.
- *   gate_up [L,2I,H]: gate rows, then up rows;  down [L,H,I];  x [T,H] 16-byte aligned;  topk_idx [T,K] of index_bytes 8 or 4;  y [T,H]
+ *   gate_up [L,2I,H]: gate rows, then up rows;  down [L,H,I];  x [T,H] 16-byte aligned;  topk_idx [T,K] of index_bytes 8 or 4;  y [T,H],
+ *   which may be x, but overlaps topk_idx nowhere
  *   scratch  dpep_w4_experts_scratch_bytes, 16-byte aligned */
 size_t dpep_w4_experts_scratch_bytes(int num_tokens, int num_topk, int hidden, int intermediate);
 int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const void* x, const void* topk_idx, int index_bytes, const float* topk_weights,

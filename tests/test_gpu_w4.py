@@ -280,3 +280,22 @@ def test_columns_of_a_matrix_that_ends_inside_a_tile(rows, n, k, dtype):
     assert (want != 0).float().mean() > 0.2  # (there are rounding errors to compare)
     for _ in range(3):
         assert torch.equal(w4.matvec(x, w4.W4Weights(packed[:n].contiguous(), scales[:n].contiguous())), want[:, :n])
+
+
+def test_results_over_inputs():
+    """A product's rows are read until its end; the experts' are not, so a layer's output may take their place."""
+    from deepep_amd import w4
+
+    rng = np.random.default_rng(15)
+    square = w4.W4Weights(*_weights(rng, (256, 256), 64, True, "bf16")[0])
+    held = torch.randn((6, 256), device="cuda").bfloat16()
+    x, before = held[:4], held.clone()
+    for out in (x, held[1:5], held[2:]):
+        with pytest.raises(ValueError):
+            w4.matvec(x, square, out=out)
+    assert torch.equal(held, before)
+    assert torch.equal(w4.matvec(held[:3], square, out=held[3:]), w4.matvec(before[:3].clone(), square))
+    gate_up, down = w4.W4Weights(*_weights(rng, (4, 128, 256), 64, False, "bf16")[0]), w4.W4Weights(*_weights(rng, (4, 256, 64), 64, False, "bf16")[0])
+    x, ids, route_weights = torch.randn((5, 256), device="cuda").bfloat16(), torch.randint(-1, 4, (5, 2), device="cuda"), torch.rand((5, 2), device="cuda")
+    want = w4.expert_ffn(x, ids, route_weights, gate_up, down)
+    assert torch.equal(w4.expert_ffn(x, ids, route_weights, gate_up, down, out=x), want) and torch.equal(x, want)

@@ -213,3 +213,16 @@ def test_first_expert_is_an_integer_of_31_bits(monkeypatch, begin):
     down = w4.W4Weights(shaped(2, 32, 16, dtype=torch.uint8), shaped(2, 32, 1))
     with pytest.raises(ValueError, match="expert_begin"):
         w4.expert_ffn(shaped(1, 32), shaped(1, 1, dtype=torch.int32), shaped(1, 1, dtype=torch.float32), matrix, down, expert_begin=begin)
+
+
+def test_results_do_not_overlap_what_is_still_read():
+    lib = _lib.load()
+    matrix = ops._W4(1 << 20, 2 << 20, 3 << 20, 64, 64, 32)
+    x, row = 4 << 20, 128
+    for y in (x, x + 2, x + 3 * row - 2, x - 3 * row + 2, 1 << 20, (1 << 20) + 64 * 32 - 2, 2 << 20, (2 << 20) + 64 * 4 - 2, (3 << 20) + 64 * 2 - 2):
+        assert lib.dpep_w4_matvec(ctypes.byref(matrix), 1, x, 3, y, None) == -1 and "overlap" in lib.dpep_last_error().decode()
+    gate_up, down = ops._W4(1 << 20, 2 << 20, None, 64, 32, 32), ops._W4(1 << 20, 2 << 20, None, 32, 32, 32)
+    ids = 5 << 20
+    for y in (ids, ids + 3 * 2 * 8 - 2, ids - 3 * 64 + 2):
+        assert lib.dpep_w4_experts(ctypes.byref(gate_up), ctypes.byref(down), 1, x, ids, 8, 256, 3, 2, 0, 2, y, 6 << 20, None) == -1
+        assert "overlap" in lib.dpep_last_error().decode()
