@@ -24,7 +24,7 @@ class W4Weights(NamedTuple):
 
 def quantize(weight: torch.Tensor, group: int = 128, *, symmetric: bool = True, dtype: torch.dtype = torch.bfloat16) -> W4Weights:
     """Round a matrix [..., N, K] to 4 bits, each group of K by its own range, with scales in ``dtype``.  Torch operations; done once."""
-    if weight.shape[-1] % group or not (group in (32, 64) or group % 128 == 0 and group > 0):
+    if not (group in (32, 64) or group > 0 and group % 128 == 0) or weight.shape[-1] % group:
         raise ValueError("group must be 32, 64 or a multiple of 128, and divide K")
     w = weight.float().unflatten(-1, (-1, group))
     zeros = None

@@ -226,3 +226,9 @@ def test_results_do_not_overlap_what_is_still_read():
     for y in (ids, ids + 3 * 2 * 8 - 2, ids - 3 * 64 + 2):
         assert lib.dpep_w4_experts(ctypes.byref(gate_up), ctypes.byref(down), 1, x, ids, 8, 256, 3, 2, 0, 2, y, 6 << 20, None) == -1
         assert "overlap" in lib.dpep_last_error().decode()
+
+
+@pytest.mark.parametrize("group", [0, -32, -128, 16, 192, 512])
+def test_quantize_refuses_groups(group):
+    with pytest.raises(ValueError):
+        w4.quantize(torch.ones(4, 256), group)
