@@ -299,3 +299,35 @@ def test_results_over_inputs():
     x, ids, route_weights = torch.randn((5, 256), device="cuda").bfloat16(), torch.randint(-1, 4, (5, 2), device="cuda"), torch.rand((5, 2), device="cuda")
     want = w4.expert_ffn(x, ids, route_weights, gate_up, down)
     assert torch.equal(w4.expert_ffn(x, ids, route_weights, gate_up, down, out=x), want) and torch.equal(x, want)
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,topk,experts,group,zeros", [
+    (1, 512, 128, 1, 2, 128, False), (4, 128, 128, 2, 4, 32, True), (3, 512, 320, 3, 8, 64, True), (8, 384, 256, 2, 4, 128, False),
+    (2, 2048, 512, 2, 4, 128, True), (40, 256, 192, 2, 3, 64, False), (5, 768, 384, 2, 4, 384, True), (2, 7168, 256, 2, 4, 128, False),
+])
+def test_rows_between_the_products_keep_16_bits(tokens, hidden, inter, topk, experts, group, zeros):
+    """FP16 results within six deviations of what the sums and 16 bits of mantissa may be off by, and half a last place.  (The oracle's test
+    shows that rows of 8 bits leave this bound in many places.)"""
+    from deepep_amd import w4
+
+    rng = np.random.default_rng(hidden + inter)
+    gate_up, gate_up_host = _weights(rng, (experts, 2 * inter, hidden), group, zeros, "fp16")
+    down, down_host = _weights(rng, (experts, hidden, inter), group, zeros, "fp16")
+    x, wide = _rows(rng, (tokens, hidden), "fp16")
+    x = x * 0.25
+    wide = x.double().cpu().numpy()
+    ids, route_weights = np.argsort(rng.random((tokens, experts)), axis=1)[:, :topk], rng.random((tokens, topk)).astype(np.float32)
+    y = w4.expert_ffn(x, torch.from_numpy(ids).cuda(), torch.from_numpy(route_weights).cuda(), w4.W4Weights(*gate_up), w4.W4Weights(*down))
+    want, deviation = ow4.experts_and_deviation(wide, ids, route_weights.astype(np.float64), gate_up_host, down_host)
+    off = np.abs(y.double().cpu().numpy() - want)
+    bound = 6 * deviation + 2.0**-11 * np.abs(want) + 2.0**-25
+    assert (off <= bound).all(), float((off / bound).max())
+
+
+@pytest.mark.parametrize("rows,n,k,group,zeros,dtype", [
+    (1, 64, 384, 384, False, "bf16"), (3, 40, 1152, 384, True, "fp16"), (2, 33, 1920, 640, False, "bf16"), (17, 48, 2688, 896, True, "bf16"),
+    (5, 130, 16128, 384, False, "fp16"), (2, 20, 16128, 5376, True, "bf16"), (1, 16, 16000, 640, True, "bf16"),
+])
+def test_groups_that_are_no_power_of_two(rows, n, k, group, zeros, dtype):
+    """Which of its row's groups a half unit belongs to is found with a rounded reciprocal."""
+    test_matvec(rows, n, k, group, zeros, dtype)
