@@ -146,8 +146,8 @@ __device__ __forceinline__ int load_index(const void* p, bool wide, size_t row, 
 }
 
 // 1 / (1 + exp(-z)) as IEEE divide and the library's exp give it, bit for bit (the choice compares such values, so everybody has to get the
-// same): one step from the hardware's reciprocal is correctly rounded for every mantissa and exponent below 2^126 (checked for all of
-// them), and beyond that, below a logit of -86, the divide itself is taken.  grown: exp(-z).
+// same): one step from the hardware's reciprocal is correctly rounded for every mantissa and exponent below 2^126 (the tests compare
+// every float's), and beyond that, below a logit of -86, the divide itself is taken.  grown: exp(-z).
 __device__ __forceinline__ float sigmoid_of(float grown)
 {
     const float d = 1.0f + grown, r = __builtin_amdgcn_rcpf(d);
@@ -183,7 +183,7 @@ __device__ __forceinline__ float reciprocal(float d)  // of 1e-20 .. 1e30
     return fmaf(fmaf(-d, r, 1.0f), r, r);
 }
 
-// A row's scores: exp(z - max) or the sigmoids, and 1 / their sum (the balance loss's probabilities are their products).  rest: exp(-z) (sigmoid).
+// A row's scores: exp(z - max) or the sigmoids, and 1 / their sum (the balance loss's probabilities are their products).  grown: exp(-z) (sigmoid).
 template <int V, bool kSigmoid>
 __device__ __forceinline__ float row_scores(const float (&z)[V], float (&s)[V], float (&grown)[V])
 {
@@ -392,8 +392,9 @@ __device__ __forceinline__ float pick(const float (&x)[V], int mine)
 
 // A wave takes every eighth token of a workgroup's chunk, the whole row in its registers, so logits are read once and the choice, the weights and the
 // balance sums come out of one pass.  Vector instructions bound it, not HBM: 65536 x 256 in eight groups, sigmoid, K = 8, with the sums takes
-// 57 us (406 vector instructions a token, 43 us of issue; its 72 MB take 14), 128 x 384 4.8, one token 3.4.  Half of the instructions are the
-// exponentials and the eight steps of the choice.
+// 57 us (409 vector instructions a token, 43 us of issue; its 72 MB take 14), 128 x 384 4.8, one token 3.4.  Half of the instructions are the
+// exponentials and the eight steps of the choice.  Rows of more than 512 experts take sixteen registers a lane for each of their arrays: of those, 15 go to
+// the stack in a sigmoid route of FP32 logits, 28 to 36 where balance sums are taken with the choice.
 template <int V, int kType, bool kSigmoid, bool kRoute, bool kBalance>
 __global__ __launch_bounds__(kRouterThreads) void router_forward_kernel(const Forward c)
 {
@@ -754,7 +755,8 @@ bool whole_pieces(const dpep_router* r, const void* a, const void* b)
     const size_t piece = std::min<size_t>(16, row_registers(r->num_experts) * (r->logits_type == DPEP_TYPE_F32 ? 4 : 2));
     return r->num_experts % row_registers(r->num_experts) == 0 && (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % piece == 0;
 }
-// Tokens to a workgroup: about four workgroups of eight waves to a CU; rows of sums stay few.
+// Tokens to a workgroup: at most 1024 workgroups of eight waves, four to a CU where registers allow it (up to 128 experts; choice and sums
+// together over 256 take up to 68 registers, three at once, and wider rows more); rows of sums stay few.
 int router_chunk(int tokens) { return std::max(kRouterWaves, (tokens + 1023) / 1024); }
 // With balance sums at least four tokens to a wave: a workgroup leaves a row of sums, which costs about as much as a token and is read again.
 int balance_chunk(int tokens) { return std::max(4 * kRouterWaves, (tokens + 1023) / 1024); }

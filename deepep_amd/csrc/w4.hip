@@ -131,16 +131,18 @@ struct LdsPlan {
 // A workgroup takes an even share of all steps: of the matrices that have rows one after the other (matvec: of the passes over the rows), each
 // with the rows it multiplies in LDS.
 //
-// Few rows: reading the codes bounds it.  Sixteen tokens through 8 of 256 experts, 1.9 GB of weights: 350 us in all, 5.6 TB/s.  One token, 121 MB and
+// Few rows: reading the codes bounds it.  Sixteen tokens through 8 of 256 experts, 2.0 GB of weights: 352 to 367 us in all, 5.5 to 5.7 TB/s.  One token, 121 MB and
 // 60 MB: 27 and 18 us, 4.4 and 3.3 TB/s, of which 5 to 6 pass before the first weights are asked for (ids, then rows, then the barrier) and 2
 // behind the last.  Many rows: the rows' way into LDS, once for every 16 columns and pass (64 rows through 4096 x 7168: 42 us).
+// The experts' products with zero points and one block keep two to seven registers a lane on the stack (two workgroups to a CU leave 128);
+// with four blocks they have a CU to themselves, and 161 to 168 registers.
 template <Kind kKind, bool kHalf, bool kZeros, int kDiag, int kBlocks, bool kStreamed>
 __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel(const Product p)
 {
     constexpr bool kHalfRows = kHalf && kKind != kDown;  // the down product's rows are BF16 pairs whatever the type
     constexpr int kTiles = kKind == kMatvec ? 1 : 2;     // tiles of 16 rows of W to a tile group; gate_up: a gate tile and its up tile
     // Units in flight.  The waves of a CU (sixteen, 4 KiB each) need not ask for more: with two units each, requests queued for 5 us, and so did
-    // everything that was cold, instructions among it (one token through 8 of 256 experts 64 us against 51, sixteen tokens 372 against 340).
+    // everything that was cold, instructions among it (one token through 8 of 256 experts 65 us against 51, sixteen tokens 370 against 350).
     constexpr int kAhead = kKind == kMatvec ? 2 : 1;
     constexpr int kTokens = 16 / kDiag;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -250,8 +252,8 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void product_kernel
         };
 
         // Scales: a lane takes those of row l % 16 and of the (l / 16)-th of four units, 2 kDiag of them next to one another, in one load.  (One load for a
-        // unit and a lane's own two would touch 16 lines for 64 bytes each time; these filled the queue of misses, 430 us against 330 for the
-        // largest call.)
+        // unit and a lane's own two would touch 16 lines for 64 bytes each time; these filled the queue of misses: 443 us for the
+        // largest call, 388 with this and results of several steps behind one barrier.)
         struct Scales {
             uint32_t scale[kTiles][kDiag], zero[kTiles][kDiag == 4 ? 2 : 1];
         };

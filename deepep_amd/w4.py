@@ -4,7 +4,7 @@ A matrix [N,K] is (packed uint8 [N,K/2], scales [N,K/group], zeros uint8 [N,K/gr
 (q - zero) * scale, q two to a byte along K with the even k in the low nibble, zero 8 where none are given.  Experts' matrices carry
 one more leading dimension.  Scales have the type of the rows that are multiplied, BF16 or FP16; a group is 32, 64 or a multiple
 of 128 values.  Sums are taken in FP32 and rounded once.  The reference has no counterpart of this module: its experts are W4A8
-(``deepep_amd.megamoe``), which is the path for many tokens.
+(``deepep_amd.megamoe``, also for many tokens, from MXFP4 weights: it cannot read these).
 """
 
 from __future__ import annotations

@@ -398,7 +398,7 @@ def test_slots_without_a_route_weigh_nothing(score, normalize, experts, groups):
 
 
 def test_sigmoid_keys_have_the_bits_of_a_divide():
-    """Every float from 1/16 to 128 in magnitude as a logit: the scores are 1 / (1 + torch.exp(-z)) bit for bit, on both sides of where the sum leaves
+    """Every float from 2^-25 to 128 in magnitude as a logit (below, the sum is 2): the scores are 1 / (1 + torch.exp(-z)) bit for bit, on both sides of where the sum leaves
     the reciprocal's range (-86) and where the sigmoid becomes subnormal and zero, and ids and biased ids are in the order of such keys."""
     from deepep_amd import Router
 
@@ -406,7 +406,7 @@ def test_sigmoid_keys_have_the_bits_of_a_divide():
     bias = torch.linspace(-0.5, 0.5, experts, device="cuda")[torch.randperm(experts, generator=torch.Generator().manual_seed(1)).cuda()]
     router = Router(experts, experts, score="sigmoid", normalize=False)
     for sign in (0, 1 << 31):
-        for exponent in range(123, 134):  # of 2^-4 to 2^6
+        for exponent in range(102, 134):  # of 2^-25 to 2^6
             bits = torch.arange(1 << 23, dtype=torch.int64, device="cuda") + (exponent << 23) + sign
             z = torch.where(bits >= 1 << 31, bits - (1 << 32), bits).to(torch.int32).view(torch.float32)
             z = z.view(experts, -1).t().contiguous()  # (a row's logits are spread over the binade)

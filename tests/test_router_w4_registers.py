@@ -1,8 +1,8 @@
 """What the router's and the 4-bit products' kernels keep on the stack, on the code the build actually generates (no GPU needed).
 
 Values that do not fit a kernel's registers go to the stack without a word from the compiler.  The numbers are what was measured with:
-none for rows of up to 512 experts; route and balance sums in one pass over rows of 513 to 1024 keep some 36 registers there, and products with
-zero points up to seven, which 128 registers a lane (two workgroups to a CU) leave no room for."""
+none for rows of up to 512 experts; route and balance sums in one pass over rows of 513 to 1024 keep some 36 registers there, and the experts' products
+with zero points up to seven, which 128 registers a lane (two workgroups to a CU) leave no room for."""
 
 import os
 import re
@@ -51,6 +51,6 @@ def test_product_kernels(kernels):
     products = {name: re.search(r"product_kernelIL\w*E(\d)ELb(\d)ELb(\d)ELi(\d)ELi(\d)ELb(\d)E", name) for name in kernels["w4"]}
     products = {name: match.groups() for name, match in products.items() if match is not None}
     assert len(products) == 3 * 2 * 2 * 3 * 3  # kinds, types, zero points or none, groups; one block (streamed or not) or four
-    for name, (_, _, zeros, _, blocks, _) in products.items():
+    for name, (kind, _, zeros, _, blocks, _) in products.items():
         registers, stack = kernels["w4"][name]
-        assert stack <= (32 if zeros == "1" and blocks == "1" else 0), f"{name}: {registers} registers, {stack} bytes of stack"
+        assert stack <= (32 if kind != "0" and zeros == "1" and blocks == "1" else 0), f"{name}: {registers} registers, {stack} bytes of stack"
