@@ -1433,7 +1433,7 @@ int64_t router_sequences(PyObject* o, int device, const at::Tensor** offsets)
     *offsets = nullptr;
     if (o == Py_None) return 1;
     const at::Tensor* t = plain(o, device);
-    if (t == nullptr || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) < 2 || t->size(0) > 0x7fffffff) return 0;
+    if (t == nullptr || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) < 2 || t->size(0) - 1 > DPEP_MAX_SEQUENCES) return 0;
     *offsets = t;
     return t->size(0) - 1;
 }

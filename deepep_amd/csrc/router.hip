@@ -851,6 +851,8 @@ int check_balance(const dpep_router* r, int num_tokens, const int32_t* sequence_
                   const int32_t* tokens, const void* scratch, const char* what)
 {
     if (int rc = check_routes(r, num_tokens, what); rc != DPEP_OK) return rc;
+    // (a workgroup of 1024 lanes to a sequence, and a launch's lanes in a direction are counted in 32 bits)
+    DPEP_REQUIRE(num_sequences <= DPEP_MAX_SEQUENCES, "%s: num_sequences=%d is more than %d", what, num_sequences, DPEP_MAX_SEQUENCES);
     DPEP_REQUIRE(num_sequences >= 1 && (sequence_offsets != nullptr || num_sequences == 1), "%s: num_sequences=%d", what, num_sequences);
     DPEP_REQUIRE(losses != nullptr && counts != nullptr && tokens != nullptr && scratch != nullptr, "%s: a NULL buffer", what);
     return DPEP_OK;

@@ -550,7 +550,7 @@ def megamoe_forward(ws, x_codes, x_scales, topk_idx, topk_weights, w1, s1, w2, s
 # ---------------------------------------------------------------------------------------------
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DPEP_TYPE_*
 SCORES = ("softmax", "sigmoid")  # DPEP_SCORE_*
-_MAX_ROUTER_TOKENS, _MAX_ROUTES = 1 << 30, (1 << 31) - 1  # DPEP_MAX_ROUTER_TOKENS; of a balance loss
+_MAX_ROUTER_TOKENS, _MAX_SEQUENCES, _MAX_ROUTES = 1 << 30, (1 << 22) - 1, (1 << 31) - 1  # DPEP_MAX_*; routes of a balance loss
 _W4_MAX_N, _W4_MAX_K, _W4_MAX_ROWS, _W4_MAX_ROUTES, _MAX_LOCAL_EXPERTS, _MAX_TOPK = 1 << 30, 16384, 65535, 2048, 1024, 32  # DPEP_*
 
 
@@ -605,7 +605,7 @@ def _require_sequences(spec: RouterSpec, tokens, sequence_offsets, device):
     _require("sequence_offsets", sequence_offsets, torch.int32, device=device)
     if sequence_offsets.ndim != 1 or sequence_offsets.shape[0] < 2:
         raise ValueError("sequence_offsets must be [B + 1] with B >= 1")
-    _at_most((1 << 31) - 1, sequences=sequence_offsets.shape[0] - 1)
+    _at_most(_MAX_SEQUENCES, sequences=sequence_offsets.shape[0] - 1)
     return sequence_offsets.shape[0] - 1
 
 

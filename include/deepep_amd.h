@@ -363,6 +363,7 @@ int dpep_megamoe_run(void* ws, const dpep_megamoe_call* call, void* stream);
 #define DPEP_SCORE_SOFTMAX 0
 #define DPEP_SCORE_SIGMOID 1
 #define DPEP_MAX_ROUTER_TOKENS (1 << 30)
+#define DPEP_MAX_SEQUENCES ((1 << 22) - 1)
 #define DPEP_W4_MAX_N (1 << 30)
 #define DPEP_W4_MAX_K 16384
 #define DPEP_W4_MAX_ROWS 65535
@@ -391,7 +392,7 @@ int dpep_route(const dpep_router* r, const void* logits, const float* bias, cons
 /* Balance loss of every sequence, and its counts.  A token without a route (ids outside 0..E-1) is padding.  In a sequence of N other
  * tokens with R routes, c_e of them to expert e: loss = sum_e (E c_e / R) (sum_t p_te / N), p a token's softmax, or its sigmoids over
  * (their sum + 1e-20); 0 for a sequence without tokens.  Sums are taken in an order that depends on the sizes alone.  T*K < 2^31, here and in
- * the loss's gradient.
+ * the loss's gradient; B at most DPEP_MAX_SEQUENCES.
  *   sequence_offsets  int32 [B+1] ascending from 0 to T, or NULL: one sequence
  *   losses fp32 [B];  counts int32 [B,E];  tokens int32 [B] (N);  scratch  dpep_balance_scratch_bytes, 4-byte aligned */
 size_t dpep_balance_scratch_bytes(int num_experts, int num_tokens, int num_sequences);

@@ -232,3 +232,15 @@ def test_results_do_not_overlap_what_is_still_read():
 def test_quantize_refuses_groups(group):
     with pytest.raises(ValueError):
         w4.quantize(torch.ones(4, 256), group)
+
+
+def test_sequences_of_a_launch():
+    """A workgroup of 1024 lanes takes a sequence, and a launch holds fewer than 2^32 lanes: more are refused, and not by the launch of
+    the second kernel when the first has run.  (Without logits, so that nothing is launched.)"""
+    lib = _lib.load()
+    spec = ops.RouterSpec(16, 4, 1, 1, 0, 1, 1.0, 0, 8)
+    calls = (lambda sequences: lib.dpep_balance_loss(ctypes.byref(spec), None, None, 8, 256, sequences, 256, 256, 256, 256, None),
+             lambda sequences: lib.dpep_route_balance(ctypes.byref(spec), None, None, None, 8, 256, sequences, None, None, 256, 256, 256, 256, None))
+    for call in calls:
+        assert call(1 << 22) == -1 and "num_sequences" in lib.dpep_last_error().decode()
+        assert call((1 << 22) - 1) == -1 and "NULL" in lib.dpep_last_error().decode()
