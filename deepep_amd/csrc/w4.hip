@@ -131,7 +131,7 @@ struct LdsPlan {
 // A workgroup takes an even share of all steps: of the matrices that have rows one after the other (matvec: of the passes over the rows), each
 // with the rows it multiplies in LDS.
 //
-// Few rows: reading the codes bounds it.  Sixteen tokens through 8 of 256 experts, 2.0 GB of weights: 352 to 367 us in all, 5.5 to 5.7 TB/s.  One token, 121 MB and
+// Few rows: reading the codes bounds it.  Sixteen tokens through 8 of 256 experts, 2.0 GB of weights: 351 to 367 us in all, 5.5 to 5.7 TB/s.  One token, 121 MB and
 // 60 MB: 27 and 18 us, 4.4 and 3.3 TB/s, of which 5 to 6 pass before the first weights are asked for (ids, then rows, then the barrier) and 2
 // behind the last.  Many rows: the rows' way into LDS, once for every 16 columns and pass (64 rows through 4096 x 7168: 42 us).
 // The experts' products with zero points and one block keep two to seven registers a lane on the stack (two workgroups to a CU leave 128);
