@@ -3,8 +3,9 @@
 ``ElasticBuffer``, ``EPHandle``, ``EventHandle`` and ``EventOverlap`` keep the reference's names and
 signatures (deep_ep/__init__.py:11-16).  The V1 ``Buffer`` and ``Config`` classes are outside this
 build.  ``Router`` chooses the experts that ``ElasticBuffer`` dispatches to, with the balance loss and both gradients; ``w4`` holds
-the products of few tokens with 4-bit weights; the reference has neither.  ``install_as_deep_ep()`` registers this package under the name ``deep_ep`` for callers that
-import the reference's module path.
+the products of few tokens with 4-bit weights, ``dense`` the norm and the gated feed-forward block that every token passes through, ``w8``
+products in 8-bit integers; the reference has none of these.  ``install_as_deep_ep()`` registers this package under the name ``deep_ep`` for
+callers that import the reference's module path.
 """
 
 from __future__ import annotations
@@ -25,8 +26,8 @@ _LAZY = {
 
 
 def __getattr__(name):
-    if name == "w4":
-        return importlib.import_module("deepep_amd.w4")
+    if name in ("dense", "w4", "w8"):
+        return importlib.import_module(f"deepep_amd.{name}")
     target = _LAZY.get(name)
     if target is None:
         raise AttributeError(name)

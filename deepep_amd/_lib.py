@@ -65,6 +65,16 @@ SIGNATURES = {
     "dpep_w4_matvec": (_I, (_P, _I, _P, _I, _P, _P)),
     "dpep_w4_experts_scratch_bytes": (_Z, (_I, _I, _I, _I)),
     "dpep_w4_experts": (_I, (_P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P)),
+    "dpep_rms_norm": (_I, (_P, _P)),
+    "dpep_rms_norm_backward_scratch_bytes": (_Z, (_I, _I)),
+    "dpep_rms_norm_backward": (_I, (_P, _P, _P)),
+    "dpep_gated_ffn_scratch_bytes": (_Z, (_I, _I, _I)),
+    "dpep_gated_ffn": (_I, (_P, _P, _I, _P, _P, _P, _P)),
+    "dpep_gated_ffn_backward_scratch_bytes": (_Z, (_I, _I, _I)),
+    "dpep_gated_ffn_backward": (_I, (_P, _P, _P, _P, _I, _P, _P, _P, _P, _P)),
+    "dpep_quantize_tokens": (_I, (_P, _I, _I, _I, _P, _P, _P)),
+    "dpep_w8_matmul_scratch_bytes": (_Z, (_I, _I, _I)),
+    "dpep_w8_matmul": (_I, (_P, _P, _P, _I, _I, _P, _P, _P)),
 }
 
 _lock = threading.Lock()

@@ -14,7 +14,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libdeepep_amd.so")
-SOURCES = ("runtime.hip", "layout.hip", "dispatch.hip", "combine.hip", "megamoe.hip", "router.hip", "w4.hip")
+SOURCES = ("runtime.hip", "layout.hip", "dispatch.hip", "combine.hip", "megamoe.hip", "router.hip", "w4.hip", "norm.hip", "dense.hip")
 FLAGS = (
     "--offload-arch=gfx950",
     "-O3",

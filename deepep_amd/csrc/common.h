@@ -30,6 +30,12 @@ inline int launch_status(const char* what)
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Whether two pieces of memory share a byte; NULL shares none.
+inline bool overlap(const void* a, size_t bytes_a, const void* b, size_t bytes_b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a != nullptr && b != nullptr && x < y + bytes_b && y < x + bytes_a;
+}
 
 struct Workspace {
     uint32_t magic;

@@ -1607,6 +1607,220 @@ PyObject* w4_experts(PyObject*, PyObject* const* a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+// ---- norm, dense gated block, products in 8-bit integers ----------------------------------------------------------------------------
+// Rows [T,H] of one of the types, 16-byte aligned, on the current GPU; the calls below take no others.
+const at::Tensor* dense_rows(PyObject* o, bool wide, int64_t unit, int64_t most, int64_t most_rows, int* device)
+{
+    if (!on_gpu(o) || c10::InferenceMode::is_enabled()) return nullptr;
+    *device = c10::hip::current_device();
+    const at::Tensor* x = plain(o, *device);
+    if (x == nullptr || type_code(x->scalar_type()) < 0 || (!wide && x->scalar_type() == at::kFloat) || x->dim() != 2 || x->size(1) < unit || x->size(1) % unit != 0 ||
+        x->size(1) > most || x->size(0) > most_rows || !aligned16(*x))
+        return nullptr;
+    return x;
+}
+// The norm's weight: of the rows' type or FP32.
+const at::Tensor* norm_weight(PyObject* o, const at::Tensor& x, int device)
+{
+    const at::Tensor* w = plain(o, device);
+    if (w == nullptr || (w->scalar_type() != x.scalar_type() && w->scalar_type() != at::kFloat) || w->dim() != 1 || w->size(0) != x.size(1) || !aligned16(*w)) return nullptr;
+    return w;
+}
+// A tensor of the rows' type and shape, or None.
+bool rows_like(PyObject* o, const at::Tensor& x, int device, const at::Tensor** out)
+{
+    return optional_plain(o, device, x.scalar_type(), {x.size(0), x.size(1)}, out) && (*out == nullptr || aligned16(**out));
+}
+inline PyObject* wrap_or_none(at::Tensor t)
+{
+    return t.defined() ? wrap(std::move(t)) : new_ref(Py_None);
+}
+// rms_norm(x, weight, residual, eps, quantize, output) -> (y, stream, rstd, codes, scales)
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int device;
+    if (n != 6 || !PyFloat_CheckExact(a[3]) || !PyBool_Check(a[5])) Py_RETURN_NONE;
+    int quantize = DPEP_QUANT_NONE;
+    if (a[4] != Py_None) {
+        if (!PyUnicode_CheckExact(a[4])) Py_RETURN_NONE;
+        quantize = PyUnicode_CompareWithASCIIString(a[4], "fp8") == 0     ? DPEP_QUANT_FP8
+                   : PyUnicode_CompareWithASCIIString(a[4], "mxfp8") == 0 ? DPEP_QUANT_MXFP8
+                   : PyUnicode_CompareWithASCIIString(a[4], "int8") == 0  ? DPEP_QUANT_INT8
+                                                                          : -1;
+        if (quantize < 0) Py_RETURN_NONE;
+    }
+    const double eps = PyFloat_AS_DOUBLE(a[3]);
+    const bool output = a[5] == Py_True;
+    if (!(eps >= 0.0 && eps <= 1.0) || (!output && quantize == DPEP_QUANT_NONE)) Py_RETURN_NONE;
+    const at::Tensor* x = dense_rows(a[0], true, quantize == DPEP_QUANT_NONE ? 8 : quantize == DPEP_QUANT_MXFP8 ? 32 : 16, DPEP_NORM_MAX_HIDDEN, DPEP_NORM_MAX_TOKENS, &device);
+    if (x == nullptr) Py_RETURN_NONE;
+    const at::Tensor *weight = norm_weight(a[1], *x, device), *residual;
+    if (weight == nullptr || !rows_like(a[2], *x, device, &residual)) Py_RETURN_NONE;
+    const int64_t tokens = x->size(0), hidden = x->size(1);
+    at::Tensor y, stream, rstd = allocate({tokens}, at::kFloat, device), codes, scales;
+    if (output) y = allocate({tokens, hidden}, x->scalar_type(), device);
+    if (residual != nullptr) stream = allocate({tokens, hidden}, x->scalar_type(), device);
+    if (quantize != DPEP_QUANT_NONE) codes = allocate({tokens, hidden}, quantize == DPEP_QUANT_INT8 ? at::kChar : at::kFloat8_e4m3fn, device);
+    if (quantize == DPEP_QUANT_FP8) scales = allocate({tokens, (hidden + 127) / 128}, at::kFloat, device);
+    else if (quantize == DPEP_QUANT_MXFP8) scales = allocate({tokens, hidden / 32}, at::kByte, device);
+    else if (quantize == DPEP_QUANT_INT8) scales = allocate({tokens}, at::kFloat, device);
+    const auto of = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const dpep_norm call = {x->data_ptr(), data<void>(residual), weight->data_ptr(), of(stream), of(y), static_cast<float*>(rstd.data_ptr()), of(codes), of(scales),
+                            static_cast<float>(eps), type_code(x->scalar_type()), type_code(weight->scalar_type()), quantize, static_cast<int32_t>(tokens),
+                            static_cast<int32_t>(hidden)};
+    if (const int status = dpep_rms_norm(&call, current_stream(device).raw)) return raise_native(status);
+    Ref tuple(PyTuple_New(5));
+    if (!tuple) return nullptr;
+    at::Tensor* const results[] = {&y, &stream, &rstd, &codes, &scales};
+    for (Py_ssize_t i = 0; i < 5; ++i) {
+        PyObject* o = wrap_or_none(std::move(*results[i]));
+        if (o == nullptr) return nullptr;
+        PyTuple_SET_ITEM(tuple.p, i, o);
+    }
+    return tuple.release();
+    END_HANDLE_TH_ERRORS
+}
+// rms_norm_backward(grad_y, stream, weight, rstd, grad_stream) -> (grad_x, grad_weight)
+PyObject* rms_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int device;
+    const at::Tensor *x = n == 5 ? dense_rows(a[1], true, 8, DPEP_NORM_MAX_HIDDEN, DPEP_NORM_MAX_TOKENS, &device) : nullptr, *grad_y, *rstd, *grad_stream;
+    if (x == nullptr) Py_RETURN_NONE;
+    const at::Tensor* weight = norm_weight(a[2], *x, device);
+    const int64_t tokens = x->size(0), hidden = x->size(1);
+    if (weight == nullptr || !rows_like(a[0], *x, device, &grad_y) || grad_y == nullptr || !optional_plain(a[3], device, at::kFloat, {tokens}, &rstd) || rstd == nullptr ||
+        !rows_like(a[4], *x, device, &grad_stream))
+        Py_RETURN_NONE;
+    at::Tensor grad_x = allocate({tokens, hidden}, x->scalar_type(), device), grad_weight = allocate({hidden}, at::kFloat, device);
+    at::Tensor scratch = allocate({static_cast<int64_t>(dpep_rms_norm_backward_scratch_bytes(static_cast<int>(tokens), static_cast<int>(hidden)))}, at::kByte, device);
+    const dpep_norm_gradients call = {grad_y->data_ptr(), x->data_ptr(), weight->data_ptr(), static_cast<const float*>(rstd->data_ptr()), data<void>(grad_stream),
+                                      grad_x.data_ptr(), static_cast<float*>(grad_weight.data_ptr()), type_code(x->scalar_type()), type_code(weight->scalar_type()),
+                                      static_cast<int32_t>(tokens), static_cast<int32_t>(hidden)};
+    if (const int status = dpep_rms_norm_backward(&call, scratch.data_ptr(), current_stream(device).raw)) return raise_native(status);
+    return tuple_of({std::move(grad_x), std::move(grad_weight)});
+    END_HANDLE_TH_ERRORS
+}
+// A gated block's rows and matrices.
+const at::Tensor* gated_block(PyObject* rows, PyObject* gate_up_object, PyObject* down_object, int* device, dpep_ffn* f)
+{
+    const at::Tensor* x = dense_rows(rows, false, 8, DPEP_FFN_MAX_DIM, DPEP_FFN_MAX_TOKENS, device);
+    if (x == nullptr) return nullptr;
+    const at::Tensor *gate_up = plain(gate_up_object, *device), *down = plain(down_object, *device);
+    if (gate_up == nullptr || down == nullptr || gate_up->scalar_type() != x->scalar_type() || down->scalar_type() != x->scalar_type() || down->dim() != 2 ||
+        down->size(0) != x->size(1) || down->size(1) < 8 || down->size(1) % 8 != 0 || down->size(1) > DPEP_FFN_MAX_DIM || gate_up->dim() != 2 ||
+        gate_up->size(0) != 2 * down->size(1) || gate_up->size(1) != x->size(1) || !aligned16(*gate_up) || !aligned16(*down))
+        return nullptr;
+    *f = {gate_up->data_ptr(), down->data_ptr(), type_code(x->scalar_type()), static_cast<int32_t>(x->size(1)), static_cast<int32_t>(down->size(1))};
+    return x;
+}
+// gated_ffn(x, gate_up, down, keep) -> y or (y, kept)
+PyObject* gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int device;
+    dpep_ffn f;
+    const at::Tensor* x = n == 4 && PyBool_Check(a[3]) ? gated_block(a[0], a[1], a[2], &device, &f) : nullptr;
+    if (x == nullptr) Py_RETURN_NONE;
+    const int64_t tokens = x->size(0);
+    at::Tensor y = allocate({tokens, f.hidden}, x->scalar_type(), device), kept;
+    if (a[3] == Py_True) kept = allocate({tokens, 2 * static_cast<int64_t>(f.inter)}, at::kFloat, device);
+    at::Tensor scratch = allocate({static_cast<int64_t>(dpep_gated_ffn_scratch_bytes(static_cast<int>(tokens), f.hidden, f.inter))}, at::kByte, device);
+    if (const int status = dpep_gated_ffn(&f, x->data_ptr(), static_cast<int>(tokens), y.data_ptr(), kept.defined() ? static_cast<float*>(kept.data_ptr()) : nullptr,
+                                          scratch.data_ptr(), current_stream(device).raw))
+        return raise_native(status);
+    if (!kept.defined()) return wrap(std::move(y));
+    return tuple_of({std::move(y), std::move(kept)});
+    END_HANDLE_TH_ERRORS
+}
+// gated_ffn_backward(grad_y, x, gate_up, down, kept) -> (grad_x, grad_gate_up, grad_down)
+PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    int device;
+    dpep_ffn f;
+    const at::Tensor *x = n == 5 ? gated_block(a[1], a[2], a[3], &device, &f) : nullptr, *grad_y, *kept;
+    if (x == nullptr) Py_RETURN_NONE;
+    const int64_t tokens = x->size(0), inter = f.inter;
+    if (!rows_like(a[0], *x, device, &grad_y) || grad_y == nullptr || !optional_plain(a[4], device, at::kFloat, {tokens, 2 * inter}, &kept) || kept == nullptr ||
+        !aligned16(*kept))
+        Py_RETURN_NONE;
+    at::Tensor grad_x = allocate({tokens, f.hidden}, x->scalar_type(), device), grad_gate_up = allocate({2 * inter, f.hidden}, x->scalar_type(), device);
+    at::Tensor grad_down = allocate({f.hidden, inter}, x->scalar_type(), device);
+    at::Tensor scratch = allocate({static_cast<int64_t>(dpep_gated_ffn_backward_scratch_bytes(static_cast<int>(tokens), f.hidden, f.inter))}, at::kByte, device);
+    if (const int status = dpep_gated_ffn_backward(&f, grad_y->data_ptr(), x->data_ptr(), static_cast<const float*>(kept->data_ptr()), static_cast<int>(tokens),
+                                                   grad_x.data_ptr(), grad_gate_up.data_ptr(), grad_down.data_ptr(), scratch.data_ptr(), current_stream(device).raw))
+        return raise_native(status);
+    return tuple_of({std::move(grad_x), std::move(grad_gate_up), std::move(grad_down)});
+    END_HANDLE_TH_ERRORS
+}
+// quantize_tokens(x) -> (codes, scales)
+PyObject* quantize_tokens(PyObject*, PyObject* o)
+{
+    HANDLE_TH_ERRORS
+    int device;
+    const at::Tensor* x = dense_rows(o, true, 16, DPEP_W8_MAX_K, DPEP_W8_MAX_ROWS, &device);
+    if (x == nullptr) Py_RETURN_NONE;
+    at::Tensor codes = allocate({x->size(0), x->size(1)}, at::kChar, device), scales = allocate({x->size(0)}, at::kFloat, device);
+    if (const int status = dpep_quantize_tokens(x->data_ptr(), type_code(x->scalar_type()), static_cast<int>(x->size(0)), static_cast<int>(x->size(1)),
+                                                static_cast<int8_t*>(codes.data_ptr()), static_cast<float*>(scales.data_ptr()), current_stream(device).raw))
+        return raise_native(status);
+    return tuple_of({std::move(codes), std::move(scales)});
+    END_HANDLE_TH_ERRORS
+}
+// w8_matmul(x or (codes, scales), codes, scales, dtype) -> y
+PyObject* w8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    if (n != 4 || !on_gpu(a[1]) || c10::InferenceMode::is_enabled()) Py_RETURN_NONE;
+    int device = c10::hip::current_device();
+    const at::Tensor *codes = plain(a[1], device), *scales;
+    if (codes == nullptr || codes->scalar_type() != at::kChar || codes->dim() != 2 || codes->size(0) < 1 || codes->size(0) > DPEP_W8_MAX_N || codes->size(1) < 16 ||
+        codes->size(1) % 16 != 0 || codes->size(1) > DPEP_W8_MAX_K || !aligned16(*codes) || !optional_plain(a[2], device, at::kFloat, {codes->size(0)}, &scales) ||
+        scales == nullptr)
+        Py_RETURN_NONE;
+    const int64_t k = codes->size(1);
+    at::Tensor made_codes, made_scales;
+    const at::Tensor *x_codes, *x_scales;
+    at::ScalarType type = at::kBFloat16;
+    if (PyTuple_CheckExact(a[0])) {
+        if (PyTuple_GET_SIZE(a[0]) != 2) Py_RETURN_NONE;
+        x_codes = plain(PyTuple_GET_ITEM(a[0], 0), device);
+        if (x_codes == nullptr || x_codes->scalar_type() != at::kChar || x_codes->dim() != 2 || x_codes->size(1) != k || x_codes->size(0) > DPEP_W8_MAX_ROWS ||
+            !aligned16(*x_codes) || !optional_plain(PyTuple_GET_ITEM(a[0], 1), device, at::kFloat, {x_codes->size(0)}, &x_scales) || x_scales == nullptr)
+            Py_RETURN_NONE;
+    } else {
+        x_codes = dense_rows(a[0], true, 16, DPEP_W8_MAX_K, DPEP_W8_MAX_ROWS, &device);
+        if (x_codes == nullptr || x_codes->size(1) != k) Py_RETURN_NONE;
+        x_scales = nullptr;
+        type = x_codes->scalar_type();
+    }
+    if (a[3] != Py_None) {
+        if (!THPDtype_Check(a[3])) Py_RETURN_NONE;
+        type = reinterpret_cast<THPDtype*>(a[3])->scalar_type;
+        if (type_code(type) < 0) Py_RETURN_NONE;
+    }
+    const int64_t rows = x_codes->size(0);
+    const hipStream_t stream = current_stream(device).raw;
+    if (x_scales == nullptr) {
+        made_codes = allocate({rows, k}, at::kChar, device), made_scales = allocate({rows}, at::kFloat, device);
+        if (const int status = dpep_quantize_tokens(x_codes->data_ptr(), type_code(x_codes->scalar_type()), static_cast<int>(rows), static_cast<int>(k),
+                                                    static_cast<int8_t*>(made_codes.data_ptr()), static_cast<float*>(made_scales.data_ptr()), stream))
+            return raise_native(status);
+        x_codes = &made_codes, x_scales = &made_scales;
+    }
+    const dpep_w8 w = {static_cast<const int8_t*>(codes->data_ptr()), static_cast<const float*>(scales->data_ptr()), static_cast<int32_t>(codes->size(0)), static_cast<int32_t>(k)};
+    at::Tensor y = allocate({rows, codes->size(0)}, type, device), scratch;
+    const size_t bytes = dpep_w8_matmul_scratch_bytes(static_cast<int>(rows), w.n, w.k);
+    if (bytes > 0) scratch = allocate({static_cast<int64_t>(bytes)}, at::kByte, device);
+    if (const int status = dpep_w8_matmul(&w, static_cast<const int8_t*>(x_codes->data_ptr()), static_cast<const float*>(x_scales->data_ptr()), static_cast<int>(rows),
+                                          type_code(type), y.data_ptr(), bytes > 0 ? scratch.data_ptr() : nullptr, stream))
+        return raise_native(status);
+    return wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // configure_mega(_PreparedPair, NativeError)
 PyObject* configure_mega(PyObject*, PyObject* args)
 {
@@ -1640,6 +1854,12 @@ PyMethodDef module_methods[] = {{"configure", configure, METH_VARARGS, nullptr},
                                 {"cast_back", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(cast_back)), METH_FASTCALL, nullptr},
                                 {"w4_matvec", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w4_matvec)), METH_FASTCALL, nullptr},
                                 {"w4_experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w4_experts)), METH_FASTCALL, nullptr},
+                                {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rms_norm)), METH_FASTCALL, nullptr},
+                                {"rms_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rms_norm_backward)), METH_FASTCALL, nullptr},
+                                {"gated_ffn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gated_ffn)), METH_FASTCALL, nullptr},
+                                {"gated_ffn_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gated_ffn_backward)), METH_FASTCALL, nullptr},
+                                {"quantize_tokens", quantize_tokens, METH_O, nullptr},
+                                {"w8_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w8_matmul)), METH_FASTCALL, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of deepep_amd (see csrc/host.cpp).", -1, module_methods};
 

@@ -723,12 +723,6 @@ int launch_product(Product p, int type, int matrices_most, int rows_expected, in
     return status;
 }
 
-bool overlap(const void* a, size_t bytes_a, const void* b, size_t bytes_b)
-{
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return b != nullptr && x < y + bytes_b && y < x + bytes_a;
-}
-
 int check_w4(const dpep_w4* w, int type, const char* what)
 {
     DPEP_REQUIRE(w != nullptr, "%s: weights is NULL", what);

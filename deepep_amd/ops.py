@@ -785,3 +785,198 @@ def w4_experts(x, topk_idx, topk_weights, gate_up, down, expert_begin: int = 0, 
                                      _ptr(topk_weights), tokens, topk, begin, local, _ptr(out), _ptr(scratch), _stream(dev))
     _lib.check(status, "w4_experts")
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Norm, dense gated block, products in 8-bit integers
+# ---------------------------------------------------------------------------------------------
+_NORM_MAX_HIDDEN, _NORM_MAX_TOKENS = 16384, 0x7FFFFF
+_FFN_MAX_DIM, _FFN_MAX_TOKENS = 65536, 0x1FFFFF
+_W8_MAX_K, _W8_MAX_N, _W8_MAX_ROWS = 65536, 0x1FFFFF, 0x1FFFFF
+QUANTIZE = {None: (0, 8), "fp8": (1, 16), "mxfp8": (2, 32), "int8": (3, 16)}  # DPEP_QUANT_*, what H is a multiple of
+
+
+class _Norm(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "residual", "weight", "stream_out", "y", "rstd", "codes", "scales")] + [
+        ("eps", ctypes.c_float)] + [(name, ctypes.c_int32) for name in ("type", "weight_type", "quantize", "num_tokens", "hidden")]
+
+
+class _NormGradients(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("grad_y", "stream", "weight", "rstd", "grad_stream", "grad_x", "grad_weight")] + [
+        (name, ctypes.c_int32) for name in ("type", "weight_type", "num_tokens", "hidden")]
+
+
+class _Ffn(ctypes.Structure):
+    _fields_ = [("gate_up", ctypes.c_void_p), ("down", ctypes.c_void_p), ("type", ctypes.c_int32), ("hidden", ctypes.c_int32), ("inter", ctypes.c_int32)]
+
+
+class _W8(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("n", ctypes.c_int32), ("k", ctypes.c_int32)]
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _require_rows(name, x, types, unit, most, most_rows):
+    """x as rows [T,H] of one of `types`, H a multiple of `unit` up to `most`."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in types:
+        raise ValueError(f"{name} must be a tensor of " + ", ".join(str(t) for t in types))
+    _require(name, x, x.dtype)
+    if x.ndim != 2 or x.shape[1] == 0 or x.shape[1] % unit or x.shape[1] > most:
+        raise ValueError(f"{name} must be [rows, width], its width a multiple of {unit} up to {most} (got {tuple(x.shape)})")
+    _at_most(most_rows, rows=x.shape[0])
+    return x.shape
+
+
+def _require_norm_weight(weight, x):
+    if not isinstance(weight, torch.Tensor) or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError("weight must be a tensor of x's type or FP32")
+    _require("weight", weight, weight.dtype, (x.shape[1],), x.device)
+
+
+def rms_norm(x, weight, residual=None, eps: float = 1e-6, quantize=None, output: bool = True):
+    """(y or None, stream or None without a residual, rstd, codes or None, scales or None)."""
+    if quantize not in QUANTIZE:
+        raise ValueError(f"quantize must be one of {sorted(name for name in QUANTIZE if name)} or None")
+    code, unit = QUANTIZE[quantize]
+    tokens, hidden = _require_rows("x", x, tuple(_TYPES), unit, _NORM_MAX_HIDDEN, _NORM_MAX_TOKENS)
+    _require_norm_weight(weight, x)
+    if residual is not None:
+        _require("residual", residual, x.dtype, tuple(x.shape), x.device)
+    if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not 0 <= eps <= 1:
+        raise ValueError("eps must be a number in [0, 1]")
+    if not output and quantize is None:
+        raise ValueError("output=False leaves nothing without quantize")
+    dev = x.device
+    y = torch.empty_like(x) if output else None
+    stream = None if residual is None else torch.empty_like(x)
+    rstd = torch.empty((tokens,), dtype=torch.float32, device=dev)
+    codes = scales = None
+    if quantize == "fp8":
+        codes = torch.empty((tokens, hidden), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty((tokens, (hidden + 127) // 128), dtype=torch.float32, device=dev)
+    elif quantize == "mxfp8":
+        codes = torch.empty((tokens, hidden), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty((tokens, hidden // 32), dtype=torch.uint8, device=dev)
+    elif quantize == "int8":
+        codes = torch.empty((tokens, hidden), dtype=torch.int8, device=dev)
+        scales = torch.empty((tokens,), dtype=torch.float32, device=dev)
+    x, weight, residual = _aligned(x), _aligned(weight), None if residual is None else _aligned(residual)
+    call = _Norm(_address(x), _address(residual), _address(weight), _address(stream), _address(y), _address(rstd), _address(codes), _address(scales),
+                 float(eps), _TYPES[x.dtype], _TYPES[weight.dtype], code, tokens, hidden)
+    with _on_device(dev):
+        status = _lib.load().dpep_rms_norm(ctypes.byref(call), _stream(dev))
+    _lib.check(status, "rms_norm")
+    return y, stream, rstd, codes, scales
+
+
+def rms_norm_backward(grad_y, stream, weight, rstd, grad_stream=None):
+    """(grad_x in the rows' type, grad_weight FP32 [H])."""
+    tokens, hidden = _require_rows("stream", stream, tuple(_TYPES), 8, _NORM_MAX_HIDDEN, _NORM_MAX_TOKENS)
+    dev = stream.device
+    _require("grad_y", grad_y, stream.dtype, (tokens, hidden), dev)
+    _require_norm_weight(weight, stream)
+    _require("rstd", rstd, torch.float32, (tokens,), dev)
+    if grad_stream is not None:
+        _require("grad_stream", grad_stream, stream.dtype, (tokens, hidden), dev)
+    lib = _lib.load()
+    grad_x = torch.empty_like(stream)
+    grad_weight = torch.empty((hidden,), dtype=torch.float32, device=dev)
+    scratch = torch.empty((lib.dpep_rms_norm_backward_scratch_bytes(tokens, hidden),), dtype=torch.uint8, device=dev)
+    grad_y, stream, weight, grad_stream = _aligned(grad_y), _aligned(stream), _aligned(weight), None if grad_stream is None else _aligned(grad_stream)
+    call = _NormGradients(_address(grad_y), _address(stream), _address(weight), _address(rstd), _address(grad_stream), _address(grad_x), _address(grad_weight),
+                          _TYPES[stream.dtype], _TYPES[weight.dtype], tokens, hidden)
+    with _on_device(dev):
+        status = lib.dpep_rms_norm_backward(ctypes.byref(call), _ptr(scratch), _stream(dev))
+    _lib.check(status, "rms_norm_backward")
+    return grad_x, grad_weight
+
+
+def _ffn(x, gate_up, down):
+    """Sizes of a gated block after its checks: (tokens, hidden, inter)."""
+    tokens, hidden = _require_rows("x", x, (torch.bfloat16, torch.float16), 8, _FFN_MAX_DIM, _FFN_MAX_TOKENS)
+    if not isinstance(down, torch.Tensor) or down.ndim != 2 or down.shape[0] != hidden or down.shape[1] == 0 or down.shape[1] % 8 or down.shape[1] > _FFN_MAX_DIM:
+        raise ValueError(f"down must be [{hidden}, I], I a multiple of 8 up to {_FFN_MAX_DIM}")
+    inter = down.shape[1]
+    _require("gate_up", gate_up, x.dtype, (2 * inter, hidden), x.device)
+    _require("down", down, x.dtype, None, x.device)
+    return tokens, hidden, inter
+
+
+def gated_ffn(x, gate_up, down, keep: bool = False):
+    """y [T,H], or (y, kept FP32 [T,2I])."""
+    tokens, hidden, inter = _ffn(x, gate_up, down)
+    dev, lib = x.device, _lib.load()
+    y = torch.empty_like(x)
+    kept = torch.empty((tokens, 2 * inter), dtype=torch.float32, device=dev) if keep else None
+    scratch = torch.empty((lib.dpep_gated_ffn_scratch_bytes(tokens, hidden, inter),), dtype=torch.uint8, device=dev)
+    x, gate_up, down = _aligned(x), _aligned(gate_up), _aligned(down)
+    call = _Ffn(_address(gate_up), _address(down), _TYPES[x.dtype], hidden, inter)
+    with _on_device(dev):
+        status = lib.dpep_gated_ffn(ctypes.byref(call), _ptr(x), tokens, _ptr(y), _ptr(kept), _ptr(scratch), _stream(dev))
+    _lib.check(status, "gated_ffn")
+    return (y, kept) if keep else y
+
+
+def gated_ffn_backward(grad_y, x, gate_up, down, kept):
+    """(grad_x, grad_gate_up, grad_down) in x's type."""
+    tokens, hidden, inter = _ffn(x, gate_up, down)
+    dev, lib = x.device, _lib.load()
+    _require("grad_y", grad_y, x.dtype, (tokens, hidden), dev)
+    _require("kept", kept, torch.float32, (tokens, 2 * inter), dev)
+    grad_x, grad_gate_up, grad_down = torch.empty_like(x), torch.empty_like(gate_up), torch.empty_like(down)
+    scratch = torch.empty((lib.dpep_gated_ffn_backward_scratch_bytes(tokens, hidden, inter),), dtype=torch.uint8, device=dev)
+    grad_y, x, gate_up, down, kept = (_aligned(t) for t in (grad_y, x, gate_up, down, kept))
+    call = _Ffn(_address(gate_up), _address(down), _TYPES[x.dtype], hidden, inter)
+    with _on_device(dev):
+        status = lib.dpep_gated_ffn_backward(ctypes.byref(call), _ptr(grad_y), _ptr(x), _ptr(kept), tokens, _ptr(grad_x), _ptr(grad_gate_up), _ptr(grad_down),
+                                             _ptr(scratch), _stream(dev))
+    _lib.check(status, "gated_ffn_backward")
+    return grad_x, grad_gate_up, grad_down
+
+
+def quantize_tokens(x):
+    """(codes int8 [T,K], scales FP32 [T])."""
+    tokens, k = _require_rows("x", x, tuple(_TYPES), 16, _W8_MAX_K, _W8_MAX_ROWS)
+    codes = torch.empty((tokens, k), dtype=torch.int8, device=x.device)
+    scales = torch.empty((tokens,), dtype=torch.float32, device=x.device)
+    x = _aligned(x)
+    with _on_device(x.device):
+        status = _lib.load().dpep_quantize_tokens(_ptr(x), _TYPES[x.dtype], tokens, k, _ptr(codes), _ptr(scales), _stream(x.device))
+    _lib.check(status, "quantize_tokens")
+    return codes, scales
+
+
+def w8_matmul(x, codes, scales, dtype=None):
+    """x [T,K], or (codes int8 [T,K], scales FP32 [T]), times (codes int8 [N,K], scales FP32 [N]): [T,N] in `dtype`."""
+    if dtype is not None and dtype not in _TYPES:
+        raise ValueError("dtype must be FP32, BF16 or FP16")
+    n, k = _require_rows("codes", codes, (torch.int8,), 16, _W8_MAX_K, _W8_MAX_N)
+    if n == 0:
+        raise ValueError("codes must have a row")
+    dev = codes.device
+    _require("scales", scales, torch.float32, (n,), dev)
+    if isinstance(x, (tuple, list)):
+        if len(x) != 2:
+            raise ValueError("x must be a tensor or a pair of codes and scales")
+        rows, rows_k = _require_rows("x codes", x[0], (torch.int8,), 16, _W8_MAX_K, _W8_MAX_ROWS)
+        _require("x codes", x[0], torch.int8, None, dev)
+        _require("x scales", x[1], torch.float32, (rows,), dev)
+        dtype = torch.bfloat16 if dtype is None else dtype
+    else:
+        rows, rows_k = _require_rows("x", x, tuple(_TYPES), 16, _W8_MAX_K, _W8_MAX_ROWS)
+        _require("x", x, x.dtype, None, dev)
+        dtype = x.dtype if dtype is None else dtype
+    if rows_k != k:
+        raise ValueError(f"x must be [T, {k}] (got [{rows}, {rows_k}])")
+    x_codes, x_scales = x if isinstance(x, (tuple, list)) else quantize_tokens(x)
+    lib = _lib.load()
+    y = torch.empty((rows, n), dtype=dtype, device=dev)
+    scratch = torch.empty((lib.dpep_w8_matmul_scratch_bytes(rows, n, k),), dtype=torch.uint8, device=dev)
+    x_codes, codes = _aligned(x_codes), _aligned(codes)
+    call = _W8(_address(codes), _address(scales), n, k)
+    with _on_device(dev):
+        status = lib.dpep_w8_matmul(ctypes.byref(call), _ptr(x_codes), _ptr(x_scales), rows, _TYPES[dtype], _ptr(y), _ptr(scratch), _stream(dev))
+    _lib.check(status, "w8_matmul")
+    return y

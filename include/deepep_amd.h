@@ -445,6 +445,91 @@ size_t dpep_w4_experts_scratch_bytes(int num_tokens, int num_topk, int hidden, i
 int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const void* x, const void* topk_idx, int index_bytes, const float* topk_weights,
                     int num_tokens, int num_topk, int expert_begin, int num_local, void* y, void* scratch, void* stream);
 
+/* What every token passes through beside the routed experts: norm, dense gated block, products in 8-bit integers.  The reference has
+ * none of it.  "type" is DPEP_TYPE_*. */
+
+/* Root-mean-square norm of the rows, after the residual's addition.  s = x, or x + residual rounded to `type`;
+ * rstd = (mean of s^2 + eps)^-1/2;  v = s rstd weight, in fp32.
+ *   x, residual (or NULL), stream_out (s; needed with a residual, may be x or the residual, NULL without one), y (v rounded, or NULL) [T,H] of
+ *   `type`;  weight [H] of weight_type (`type` or fp32);  rstd fp32 [T] or NULL
+ *   quantize  v in 8 bits, each value rounded from fp32 once:
+ *     DPEP_QUANT_FP8    codes e4m3 [T,H], scales fp32 [T,ceil(H/128)]: as dpep_cast_to_fp8 (H a multiple of 16)
+ *     DPEP_QUANT_MXFP8  codes e4m3 [T,H], scales e8m0 bytes [T,H/32]: as dpep_mx_quant (H a multiple of 32)
+ *     DPEP_QUANT_INT8   codes int8 [T,H], scales fp32 [T]: as dpep_quantize_tokens (H a multiple of 16)
+ * H is a multiple of 8, at most DPEP_NORM_MAX_HIDDEN; pointers to rows are 16-byte aligned; T below 2^23.  Outputs overlap no input but for stream_out. */
+#define DPEP_NORM_MAX_HIDDEN 16384
+#define DPEP_NORM_MAX_TOKENS 0x7fffff
+#define DPEP_QUANT_NONE 0
+#define DPEP_QUANT_FP8 1
+#define DPEP_QUANT_MXFP8 2
+#define DPEP_QUANT_INT8 3
+typedef struct dpep_norm {
+    const void* x;
+    const void* residual;
+    const void* weight;
+    void* stream_out;
+    void* y;
+    float* rstd;
+    void* codes;
+    void* scales;
+    float eps;
+    int32_t type, weight_type, quantize, num_tokens, hidden;
+} dpep_norm;
+int dpep_rms_norm(const dpep_norm* n, void* stream);
+/* Its gradients, from that of y and (optional) that of s from elsewhere, with xh = s rstd and c the row's mean of grad_y weight xh:
+ *   grad_x = rstd (grad_y weight - xh c) + grad_stream, of x and of the residual alike;  grad_weight[h] = sum over t of grad_y xh, fp32
+ *   stream = s;  grad_x of `type` may be grad_y or grad_stream;  scratch dpep_rms_norm_backward_scratch_bytes, 16-byte aligned
+ * Sums are taken in an order that depends on the sizes alone. */
+typedef struct dpep_norm_gradients {
+    const void* grad_y;
+    const void* stream;
+    const void* weight;
+    const float* rstd;
+    const void* grad_stream;
+    void* grad_x;
+    float* grad_weight;
+    int32_t type, weight_type, num_tokens, hidden;
+} dpep_norm_gradients;
+size_t dpep_rms_norm_backward_scratch_bytes(int num_tokens, int hidden);
+int dpep_rms_norm_backward(const dpep_norm_gradients* g, void* scratch, void* stream);
+
+/* The gated feed-forward block y = (silu(x Wg^T) * (x Wu^T)) Wd^T.
+ *   gate_up [2I,H]: gate rows, then up rows;  down [H,I];  x, y [T,H]; all of `type` (BF16 or FP16), H and I multiples of 8 from 8 to
+ *   DPEP_FFN_MAX_DIM, rows 16-byte aligned
+ *   kept  fp32 [T,2I], the gate and up products for the backward, or NULL
+ * Sums in fp32; the rows between the products are rounded to `type`, as the matrix cores take them.  Outputs overlap no input. */
+#define DPEP_FFN_MAX_DIM 65536
+#define DPEP_FFN_MAX_TOKENS 0x1fffff
+typedef struct dpep_ffn {
+    const void* gate_up;
+    const void* down;
+    int32_t type, hidden, inter;
+} dpep_ffn;
+size_t dpep_gated_ffn_scratch_bytes(int num_tokens, int hidden, int inter);
+int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, float* kept, void* scratch, void* stream);
+/* Gradients of x and of both matrices (of `type`), from that of y. */
+size_t dpep_gated_ffn_backward_scratch_bytes(int num_tokens, int hidden, int inter);
+int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x, const float* kept, int num_tokens, void* grad_x, void* grad_gate_up,
+                            void* grad_down, void* scratch, void* stream);
+
+/* Tokens in 8-bit integers: scale = max(|x|) / 127 of the row (at least 1e-20 / 127), code = x * (127 / max(|x|)) rounded to nearest even.
+ *   x [T,K] of `type`, 16-byte aligned, K a multiple of 16;  codes int8 [T,K] 16-byte aligned;  scales fp32 [T]
+ * A row that holds a NaN gets a NaN for its scale, one that holds an infinity that. */
+int dpep_quantize_tokens(const void* x, int type, int num_tokens, int k, int8_t* codes, float* scales, void* stream);
+/* y[t,n] = x_scales[t] scales[n] sum_k x[t,k] codes[n,k]: integer sums, exact; scaled in fp32, rounded once to `type`.
+ *   codes int8 [N,K], x int8 [T,K]: 16-byte aligned, K a multiple of 16 up to DPEP_W8_MAX_K;  scales fp32 [N];  x_scales fp32 [T];  y [T,N]
+ *   overlaps no input;  scratch  dpep_w8_matmul_scratch_bytes, 16-byte aligned */
+#define DPEP_W8_MAX_K 65536
+#define DPEP_W8_MAX_N 0x1fffff
+#define DPEP_W8_MAX_ROWS 0x1fffff
+typedef struct dpep_w8 {
+    const int8_t* codes;
+    const float* scales;
+    int32_t n, k;
+} dpep_w8;
+size_t dpep_w8_matmul_scratch_bytes(int num_rows, int n, int k);
+int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int num_rows, int type, void* y, void* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
