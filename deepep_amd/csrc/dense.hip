@@ -124,83 +124,417 @@ struct Product {
     const void* b;
     int m, columns, k;
     Output out;
+    // how it is cut up: tiles, parts of k of `part_steps` steps, their sums
+    int m_tiles, n_tiles, parts, part_steps, pitch;
+    void* partial;
 };
 
-// ---- a tile of 64 x 64 at a time, operands staged value by value ----------------------------------------------------------------
-constexpr int kTile = 64, kStep = 64, kPitch = kStep + 16;
+// ---- large tiles on the matrix cores ------------------------------------------------------------------------------------------------
+// A workgroup of eight waves makes a tile of 64 kRows x 256 results (kRows = 4, 2 or 1), 128 bytes of k at a time ("step").  Both operands
+// go from memory to LDS without passing registers, each in two halves (rows of the tile 0 .. and 32 kRows ..; columns 0 .. and 128 ..; with kGated
+// the halves of B are the gate and the up rows of the same 128 columns).  A wave takes 16 kRows rows and 32 columns of each half, so that a step
+// is four products of a half of A with a half of B ("phases"): (0,0), (0,1), (1,1), (1,0).
+//
+// The waves w and w + 4 share a SIMD and run half a phase apart: while one multiplies, the other reads its operands' next fragments from LDS and asks
+// for half an operand of a later step.  A phase of a wave is [read, ask, wait, barrier, multiply, barrier], and waves 4 .. 7 pass one barrier
+// more at the start, waves 0 .. 3 at the end.
+//   Which half is asked for: in phase 0 B1 and in phase 1 A1 of step k + 1, in phase 2 A0 and in phase 3 B0 of step k + 2; there are two buffers, k odd and
+//   even.  Every wait leaves the four last halves outstanding, so that a half has four phases to arrive in.
+//   Read after write: a half is read in the phase that follows the wait which covers it (A0 and B0 are covered at the end of phase 3, B1 of phase 0, A1 of
+//   phase 1), and a barrier that all waves pass after their wait lies in between, for the later waves half a phase behind too.
+//   Write after read: A0 and B0 are read in phase 0 and overwritten from phase 2 and 3 on, B1 and A1 in phases 1 and 2 and from the next step's phase 0 and 1
+//   on.  The fragments that the later waves read in phase p are in their registers before they multiply, which is before the barrier that lets the earlier
+//   waves into phase p + 2.
+//
+// In LDS a row of 128 bytes of k holds its 16-byte pieces c at place c ^ key(row), so that eight lanes that read the same piece of eight rows find them in
+// different banks.  Operands that hold m or n contiguously lie in LDS as rows of k, 128 values wide, and are turned as they are read
+// (ds_read_tr); their pieces are spread by the row in the same way.
+//
+// The matrix instruction takes B as its first operand, so that a lane's four results are four columns of one row.  The columns of a pair of
+// instructions are dealt so that a lane ends up with eight next to one another: 16 bytes of 16-bit results.
+//
+// Rows, columns and values of k that are not there are read as zero (the loads' own bounds check).
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int rsrc __attribute__((ext_vector_type(4)));
 
-template <int kType, bool kTransA, bool kTransB, Finish kFinish>
-__global__ __launch_bounds__(256) void product_kernel(const Product p)
+constexpr int kThreads = 512;
+constexpr int kStepBytes = 128;
+constexpr int kColumns = 256, kHalfColumns = kColumns / 2;
+constexpr int kColumnBytes = kHalfColumns * kStepBytes;  // of half of B
+constexpr uint32_t kNowhere = 0x80000000u;
+
+template <int kLoads>
+__device__ __forceinline__ void wait_and_meet()
 {
-    using Value = std::conditional_t<kType == kInt8, int8_t, uint16_t>;
-    constexpr int kOfMfma = kType == kInt8 ? 64 : 32, kLane = kOfMfma / 4;  // values of k of an MFMA, of a lane
-    constexpr int kWide = kFinish == kGated ? kTile / 2 : kTile;            // columns of the tile
-    __shared__ __attribute__((aligned(16))) Value lds[2][kTile][kPitch];
-    __shared__ __attribute__((aligned(16))) float result[kTile][kTile + 4];
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    const int n_tiles = (p.columns + kWide - 1) / kWide;
-    const int m0 = blockIdx.x / n_tiles * kTile, n0 = blockIdx.x % n_tiles * kWide;
-    Sum<kType> acc[2][2] = {};
-    for (int k0 = 0; k0 < p.k; k0 += kStep) {
-        for (int i = tid; i < kTile * kStep; i += 256) {
-            {
-                const int row = kTransA ? i % kTile : i / kStep, at = kTransA ? i / kTile : i % kStep;
-                const bool live = m0 + row < p.m && k0 + at < p.k;
-                const size_t from = kTransA ? static_cast<size_t>(k0 + at) * p.m + m0 + row : static_cast<size_t>(m0 + row) * p.k + k0 + at;
-                lds[0][row][at] = live ? static_cast<const Value*>(p.a)[from] : Value{0};
-            }
-            {
-                const int row = kTransB ? i % kTile : i / kStep, at = kTransB ? i / kTile : i % kStep;
-                const int column = n0 + row % kWide;
-                const bool live = column < p.columns && k0 + at < p.k;
-                const size_t n = static_cast<size_t>(kFinish == kGated && row >= kWide ? p.columns : 0) + column;
-                const size_t from = kTransB ? static_cast<size_t>(k0 + at) * p.columns + n : n * p.k + k0 + at;
-                lds[1][row][at] = live ? static_cast<const Value*>(p.b)[from] : Value{0};
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int step = 0; step < kStep; step += kOfMfma)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int row = wave / 2 * 32 + i * 16 + lane % 16, column = wave % 2 * 32 + j * 16 + lane % 16, at = step + lane / 16 * kLane;
-                    acc[i][j] = multiply<kType>(*reinterpret_cast<const u32x4*>(&lds[1][column][at]), *reinterpret_cast<const u32x4*>(&lds[0][row][at]), acc[i][j]);
-                }
-        __syncthreads();
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void meet()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// 16 bytes a lane from an operand straight into LDS, lane after lane from `lds` on.
+__device__ __forceinline__ void load_to_lds(rsrc from, uint32_t offset, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
+}
+
+// Half an operand as the loads see it: where its next step begins, and how much there is from there on.
+struct Half {
+    uint64_t base;
+    long long bytes;  // of operands with k contiguous: up to the end of the last row
+    __device__ __forceinline__ rsrc of(long long records) const
+    {
+        const uint32_t size = records <= 0 ? 0u : static_cast<uint32_t>(records < 0x7fffffff ? records : 0x7fffffff);
+        return rsrc{__builtin_amdgcn_readfirstlane(static_cast<int>(base)), __builtin_amdgcn_readfirstlane(static_cast<int>(base >> 32)),
+                    __builtin_amdgcn_readfirstlane(static_cast<int>(size)), 0x00020000};
     }
+};
+
+// One operand of a tile: `kPer` loads a wave for each half of kRowsOfHalf rows (or columns).
+template <bool kTrans, int kRowsOfHalf, bool kPaired>
+struct Operand {
+    static constexpr int kPer = kRowsOfHalf >= 64 ? kRowsOfHalf / 64 : 1;
+    static constexpr bool kHalfWave = kRowsOfHalf == 32;
+    static constexpr int kBytes = kRowsOfHalf * kStepBytes;
+    Half half[2];
+    uint32_t offset[kPer], at[kPer];  // a lane's place in the half; its place in k (bytes)
+    long long stride;                 // bytes of a row in memory
+    int left;                         // bytes of k (rows of k where kTrans) that are left from the next step on
+    int across[2];                    // kTrans: bytes of a row of k that belong to the half and what follows it
+
+    static __device__ __forceinline__ int key(int row) { return kTrans ? (row & 3) << 2 : kPaired ? (row & 3) | ((row >> 3) & 1) << 2 : row & 7; }
+
+    // rows: of the operand's whole matrix; first[h]: its row (column) where half h begins; there[h]: rows (columns) from there on, at most as many as belong to it; k0, k: in values.
+    __device__ __forceinline__ void set(const void* matrix, int value_bytes, int rows, const int (&first)[2], const int (&there)[2], int k_all, int k0, int k, int wave, int lane)
+    {
+        const char* const p = static_cast<const char*>(matrix);
+        if constexpr (kTrans) {
+            stride = static_cast<long long>(rows) * value_bytes;
+            left = k - k0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) result[wave / 2 * 32 + i * 16 + lane % 16][wave % 2 * 32 + j * 16 + lane / 16 * 4 + e] = static_cast<float>(acc[i][j][e]);
-    __syncthreads();
-    for (int i = tid; i < kTile * kWide / 8; i += 256) {
-        const int row = i / (kWide / 8), at = i % (kWide / 8) * 8;
-        if (m0 + row >= p.m || n0 + at >= p.columns) continue;
-        float v[8];
-        load_wide(&result[row][at], v);
-        if constexpr (kFinish == kGated) {
-            float up[8];
-            load_wide(&result[row][kWide + at], up);
-            finish_gated<kType>(p.out, m0 + row, n0 + at, p.columns, v, up);
+            for (int h = 0; h < 2; ++h) {
+                half[h].base = reinterpret_cast<uint64_t>(p + static_cast<long long>(k0) * stride + static_cast<long long>(first[h]) * value_bytes);
+                across[h] = max(there[h], 0) * value_bytes;
+            }
         } else {
-            finish<kType, kFinish>(p.out, m0 + row, n0 + at, p.columns, v);
+            stride = static_cast<long long>(k_all) * value_bytes;
+            left = (k - k0) * value_bytes;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                half[h].base = reinterpret_cast<uint64_t>(p + first[h] * stride + static_cast<long long>(k0) * value_bytes);
+                half[h].bytes = there[h] <= 0 ? 0 : (there[h] - 1) * stride + left;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if constexpr (kTrans) {
+                const int row = (wave * kPer + i) * 4 + lane / 16, piece = lane % 16 ^ key(row);
+                at[i] = piece * 16;
+                offset[i] = static_cast<uint32_t>(row * stride) + piece * 16;
+            } else {
+                const int row = kHalfWave ? wave * 4 + lane / 8 : (wave * kPer + i) * 8 + lane / 8, piece = lane % 8 ^ key(row);
+                at[i] = piece * 16;
+                offset[i] = static_cast<uint32_t>(row * stride) + piece * 16;
+            }
         }
     }
+    // Ask for half h of the next step.
+    __device__ __forceinline__ void ask(int h, uint32_t lds, int wave, int lane) const
+    {
+        const rsrc from = half[h].of(kTrans ? (left <= 0 || across[h] <= 0 ? 0 : (min(left, 64) - 1) * stride + across[h]) : half[h].bytes);
+        const int limit = kTrans ? across[h] : left;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t place = static_cast<int>(at[i]) < limit ? offset[i] : kNowhere;
+            if constexpr (kHalfWave) {
+                if (lane < 32) load_to_lds(from, place, lds + wave * 512);
+            } else {
+                load_to_lds(from, place, lds + (wave * kPer + i) * 1024);
+            }
+        }
+    }
+    __device__ __forceinline__ void advance()
+    {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            half[h].base += kTrans ? 64 * stride : kStepBytes;
+            half[h].bytes -= kStepBytes;
+        }
+        left -= kTrans ? 64 : kStepBytes;
+    }
+};
+
+__device__ __forceinline__ s16x4 read_turned(const uint8_t* p)
+{
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+// 8 values of k of a lane, from rows of k at p and, four rows further, the other four.
+__device__ __forceinline__ u32x4 read_turned_pair(const uint8_t* p)
+{
+    const u32x2 a = __builtin_bit_cast(u32x2, read_turned(p)), b = __builtin_bit_cast(u32x2, read_turned(p + 4 * 256));
+    return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// Which piece of work a workgroup takes: workgroups go round the eight dies, each of which gets neighbouring tiles, in blocks of four tiles of rows, so that
+// its L2 serves the operands that its tiles share.
+struct Place {
+    int m, n, part;
+};
+__device__ __forceinline__ Place place_of(unsigned id, unsigned total, int m_tiles, int n_tiles)
+{
+    const unsigned die = id % 8, share = total / 8, more = total % 8;
+    const unsigned at = die * share + min(die, more) + id / 8;
+    const unsigned tiles = static_cast<unsigned>(m_tiles) * n_tiles, part = at / tiles, tile = at - part * tiles;
+    const unsigned block = 4u * n_tiles, which = tile / block, in = tile - which * block, high = min(4u, m_tiles - which * 4);
+    return {static_cast<int>(which * 4 + in % high), static_cast<int>(in / high), static_cast<int>(part)};
+}
+
+template <int kType, bool kTransA, bool kTransB, Finish kFinish, int kRows>
+__global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
+{
+    constexpr int kValue = kType == kInt8 ? 1 : 2, kValues = kStepBytes / kValue;  // bytes of a value, values of a step
+    constexpr int kTileRows = 64 * kRows, kHalfRows = kTileRows / 2, kWide = kFinish == kGated ? kHalfColumns : kColumns;
+    using A = Operand<kTransA, kHalfRows, false>;
+    using B = Operand<kTransB, kHalfColumns, true>;
+    constexpr int kAhead = 2 * A::kPer + 2 * B::kPer;
+    constexpr int kBuffer = 2 * A::kBytes + 2 * kColumnBytes;
+    static_assert(!kTransA || kRows == 4);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wave_row = wave / 4, wave_column = wave % 4;
+    const Place place = place_of(blockIdx.x, gridDim.x, p.m_tiles, p.n_tiles);
+    const int m0 = place.m * kTileRows, n0 = place.n * kWide;
+    const int k0 = min(p.k, place.part * p.part_steps * kValues), k1 = min(p.k, k0 + p.part_steps * kValues);
+    const int steps = (k1 - k0 + kValues - 1) / kValues;
+
+    A a;
+    B b;
+    {
+        const int first[2] = {m0, m0 + kHalfRows}, there[2] = {min(kHalfRows, p.m - m0), min(kHalfRows, p.m - m0 - kHalfRows)};
+        a.set(p.a, kValue, p.m, first, there, p.k, k0, k1, wave, lane);
+    }
+    {
+        const int second = kFinish == kGated ? p.columns + n0 : n0 + kHalfColumns, columns = p.columns - n0;
+        const int first[2] = {n0, second}, there[2] = {min(kHalfColumns, columns), min(kHalfColumns, kFinish == kGated ? columns : columns - kHalfColumns)};
+        b.set(p.b, kValue, p.columns, first, there, p.k, k0, k1, wave, lane);
+    }
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+    const auto a_at = [](int h) { return h * A::kBytes; };
+    const auto b_at = [](int h) { return 2 * A::kBytes + h * kColumnBytes; };
+
+    // Where a lane reads its fragments: [two places that the key tells apart].
+    int read_a[2], read_b[2];
+    {
+        const int r = lane % 16, group = lane / 16;
+        if constexpr (kTransA) {
+            const int row = 8 * group + r / 4, piece = wave_row * 8 + (r % 4) / 2;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) read_a[i] = row * 256 + ((piece + 4 * i) ^ A::key(row)) * 16 + (r % 2) * 8;
+        } else {
+            const int row = wave_row * 16 * kRows + r;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) read_a[i] = row * kStepBytes + ((4 * i + group) ^ A::key(row)) * 16;
+        }
+        if constexpr (kTransB) {
+            const int row = 8 * group + r / 4, piece = wave_column * 4 + r % 4;
+            read_b[0] = read_b[1] = row * 256 + (piece ^ B::key(row)) * 16;
+        } else {
+            const int row = wave_column * 32 + 8 * (r / 4) + r % 4;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) read_b[i] = row * kStepBytes + ((4 * i + group) ^ B::key(row)) * 16;
+        }
+    }
+    Sum<kType> acc[2][2][kRows][2] = {};  // [half of A][half of B][16 rows][of a pair of instructions]
+    u32x4 fa[kRows][2], fb[2][2][2];      // [.][half step], [half of B][of a pair][half step]
+    const auto read_rows = [&](const uint8_t* from) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if constexpr (kTransA) fa[i][s] = read_turned_pair(from + read_a[i / 2] + (i % 2) * 32 + s * 32 * 256);
+                else fa[i][s] = *reinterpret_cast<const u32x4*>(from + read_a[s] + i * 16 * kStepBytes);
+            }
+    };
+    const auto read_columns = [&](const uint8_t* from, int h) {
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if constexpr (kTransB) fb[h][f][s] = read_turned_pair(from + read_b[0] + f * 8 + s * 32 * 256);
+                else fb[h][f][s] = *reinterpret_cast<const u32x4*>(from + read_b[s] + f * 4 * kStepBytes);
+            }
+    };
+    const auto multiply_halves = [&](int ha, int hb) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int f = 0; f < 2; ++f) acc[ha][hb][i][f] = multiply<kType>(fb[hb][f][s], fa[i][s], acc[ha][hb][i][f]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+
+    a.ask(0, lds0 + a_at(0), wave, lane);
+    b.ask(0, lds0 + b_at(0), wave, lane);
+    b.ask(1, lds0 + b_at(1), wave, lane);
+    a.ask(1, lds0 + a_at(1), wave, lane);
+    a.advance();
+    b.advance();
+    a.ask(0, lds0 + kBuffer + a_at(0), wave, lane);
+    b.ask(0, lds0 + kBuffer + b_at(0), wave, lane);
+    wait_and_meet<kAhead>();
+    if (wave_row == 1) meet();
+    for (int k = 0, now = 0; k < steps; ++k, now ^= kBuffer) {
+        const uint8_t* const buffer = lds + now;
+        const uint32_t to = lds0 + now, to_other = lds0 + (now ^ kBuffer);
+        read_columns(buffer + b_at(0), 0);
+        read_rows(buffer + a_at(0));
+        b.ask(1, to_other + b_at(1), wave, lane);
+        wait_and_meet<kAhead>();
+        multiply_halves(0, 0);
+        meet();
+        read_columns(buffer + b_at(1), 1);
+        a.ask(1, to_other + a_at(1), wave, lane);
+        wait_and_meet<kAhead>();
+        multiply_halves(0, 1);
+        meet();
+        a.advance();
+        b.advance();
+        read_rows(buffer + a_at(1));
+        a.ask(0, to + a_at(0), wave, lane);
+        wait_and_meet<kAhead>();
+        multiply_halves(1, 1);
+        meet();
+        b.ask(0, to + b_at(0), wave, lane);
+        wait_and_meet<kAhead>();
+        multiply_halves(1, 0);
+        meet();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what was asked for past the end is in LDS before the workgroup gives it up)
+    if (wave_row == 0) meet();
+
+    const int column = n0 + wave_column * 32 + lane / 16 * 8;
+#pragma unroll
+    for (int ha = 0; ha < 2; ++ha)
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int m = m0 + ha * kHalfRows + wave_row * 16 * kRows + i * 16 + lane % 16;
+            if (m >= p.m) continue;
+            Sum<kType> v[2][2];
+#pragma unroll
+            for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+                for (int f = 0; f < 2; ++f) v[hb][f] = acc[ha][hb][i][f];
+            if (p.parts > 1) {
+                // Sums of a part of k, [part][m][columns, twice as many where kGated].
+                constexpr int kTimes = kFinish == kGated ? 2 : 1;
+                const size_t wide = static_cast<size_t>(kTimes) * p.pitch;
+                uint32_t* const row = static_cast<uint32_t*>(p.partial) + (static_cast<size_t>(place.part) * p.m + m) * wide;
+#pragma unroll
+                for (int hb = 0; hb < 2; ++hb) {
+                    const int n = kFinish == kGated ? column : column + hb * kHalfColumns;
+                    if (n >= p.columns) continue;
+                    u32x4* const to = reinterpret_cast<u32x4*>(row + (kFinish == kGated ? hb * static_cast<size_t>(p.pitch) : 0) + n);
+                    to[0] = __builtin_bit_cast(u32x4, v[hb][0]);
+                    to[1] = __builtin_bit_cast(u32x4, v[hb][1]);
+                }
+                continue;
+            }
+            float wide[2][8];
+#pragma unroll
+            for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) wide[hb][e] = static_cast<float>(v[hb][e / 4][e % 4]);
+            if constexpr (kFinish == kGated) {
+                if (column < p.columns) finish_gated<kType>(p.out, m, column, p.columns, wide[0], wide[1]);
+            } else {
+#pragma unroll
+                for (int hb = 0; hb < 2; ++hb) {
+                    const int n = column + hb * kHalfColumns;
+                    if (n < p.columns) finish<kType, kFinish>(p.out, m, n, p.columns, wide[hb]);
+                }
+            }
+        }
+}
+
+// The parts of k added up, and what becomes of the sums.
+template <int kType, Finish kFinish>
+__global__ __launch_bounds__(256) void join_kernel(const Product p)
+{
+    constexpr int kTimes = kFinish == kGated ? 2 : 1;
+    const size_t wide = static_cast<size_t>(kTimes) * p.pitch;
+    const int pieces = p.pitch / 8;
+    const size_t at = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    const size_t m = at / pieces;
+    const int n = static_cast<int>(at - m * pieces) * 8;
+    if (m >= static_cast<size_t>(p.m)) return;
+    float v[kTimes][8];
+#pragma unroll
+    for (int t = 0; t < kTimes; ++t) {
+        Sum<kType> sum[2] = {};
+        for (int part = 0; part < p.parts; ++part) {
+            const u32x4* const from = reinterpret_cast<const u32x4*>(static_cast<const uint32_t*>(p.partial) + (static_cast<size_t>(part) * p.m + m) * wide +
+                                                                     static_cast<size_t>(t) * p.pitch + n);
+            sum[0] += __builtin_bit_cast(Sum<kType>, from[0]);
+            sum[1] += __builtin_bit_cast(Sum<kType>, from[1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[t][e] = static_cast<float>(sum[e / 4][e % 4]);
+    }
+    if constexpr (kFinish == kGated) finish_gated<kType>(p.out, m, n, p.columns, v[0], v[1]);
+    else finish<kType, kFinish>(p.out, m, n, p.columns, v[0]);
+}
+
+// How a product is cut up.
+struct Cut {
+    int rows, m_tiles, n_tiles, parts, part_steps;
+    size_t bytes;  // of the parts' sums
+};
+Cut cut_of(int m, int columns, int k_bytes, bool gated, bool rows_fixed)
+{
+    const int wide = gated ? kHalfColumns : kColumns, steps = (k_bytes + kStepBytes - 1) / kStepBytes;
+    Cut c = {4, 0, (columns + wide - 1) / wide, 1, std::max(1, steps), 0};
+    if (!rows_fixed) c.rows = m <= 64 ? 1 : m <= 128 ? 2 : 4;
+    c.m_tiles = (m + 64 * c.rows - 1) / (64 * c.rows);
+    const long long tiles = static_cast<long long>(c.m_tiles) * c.n_tiles;
+    if (tiles < 128 && steps >= 8) {
+        c.parts = static_cast<int>(std::min<long long>({256 / tiles, steps / 4, 16}));
+        c.part_steps = (steps + c.parts - 1) / c.parts;
+        c.parts = (steps + c.part_steps - 1) / c.part_steps;
+    }
+    if (c.parts > 1) c.bytes = static_cast<size_t>(c.parts) * m * ((columns + 7) / 8 * 8) * (gated ? 2 : 1) * 4;
+    return c;
 }
 
 template <int kType, bool kTransA, bool kTransB, Finish kFinish>
-int launch(const Product& p, hipStream_t stream)
+int launch(Product p, void* partial, hipStream_t stream)
 {
     if (p.m == 0 || p.columns == 0) return DPEP_OK;
-    constexpr int kWide = kFinish == kGated ? kTile / 2 : kTile;
-    const long long tiles = static_cast<long long>((p.m + kTile - 1) / kTile) * ((p.columns + kWide - 1) / kWide);
-    DPEP_REQUIRE(tiles <= 0xffffff, "a product of %d x %d is too large", p.m, p.columns);
-    product_kernel<kType, kTransA, kTransB, kFinish><<<static_cast<unsigned>(tiles), 256, 0, stream>>>(p);
-    return launch_status("product");
+    const Cut c = cut_of(p.m, p.columns, p.k * (kType == kInt8 ? 1 : 2), kFinish == kGated, kTransA);
+    p.m_tiles = c.m_tiles;
+    p.n_tiles = c.n_tiles;
+    p.parts = c.parts;
+    p.part_steps = c.part_steps;
+    p.pitch = (p.columns + 7) / 8 * 8;
+    p.partial = partial;
+    const long long groups = static_cast<long long>(c.m_tiles) * c.n_tiles * c.parts;
+    DPEP_REQUIRE(groups <= 0x7fffff, "a product of %d x %d is too large", p.m, p.columns);
+    const dim3 grid(static_cast<unsigned>(groups));
+    if constexpr (!kTransA) {
+        if (c.rows == 1) tile_kernel<kType, false, kTransB, kFinish, 1><<<grid, kThreads, 0, stream>>>(p);
+        else if (c.rows == 2) tile_kernel<kType, false, kTransB, kFinish, 2><<<grid, kThreads, 0, stream>>>(p);
+        else tile_kernel<kType, false, kTransB, kFinish, 4><<<grid, kThreads, 0, stream>>>(p);
+    } else {
+        tile_kernel<kType, true, kTransB, kFinish, 4><<<grid, kThreads, 0, stream>>>(p);
+    }
+    if (int rc = launch_status("product"); rc != DPEP_OK || c.parts == 1) return rc;
+    const size_t pieces = static_cast<size_t>(p.m) * (p.pitch / 8);
+    join_kernel<kType, kFinish><<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream>>>(p);
+    return launch_status("product's parts");
 }
 
 int check_ffn(const dpep_ffn* f, const char* what, int tokens)
@@ -231,7 +565,8 @@ extern "C" {
 size_t dpep_gated_ffn_scratch_bytes(int num_tokens, int hidden, int inter)
 {
     if (num_tokens < 0 || hidden < 0 || inter < 0) return 0;
-    return whole(static_cast<size_t>(num_tokens) * inter * 2);
+    return whole(static_cast<size_t>(num_tokens) * inter * 2) +
+           std::max(cut_of(num_tokens, inter, hidden * 2, true, false).bytes, cut_of(num_tokens, hidden, inter * 2, false, false).bytes);
 }
 
 int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, float* kept, void* scratch, void* stream)
@@ -245,22 +580,25 @@ int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, fl
                      !overlap(kept, products, x, rows) && !overlap(kept, products, f->gate_up, 2 * half) && !overlap(kept, products, f->down, half),
                  "gated_ffn: an output overlaps an input");
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    void* const partial = static_cast<uint8_t*>(scratch) + whole(static_cast<size_t>(num_tokens) * f->inter * 2);
     return by_type(f->type, [&](auto type) {
         constexpr int kType = decltype(type)::value;
         Product p = {x, f->gate_up, num_tokens, f->inter, f->hidden, {}};
         p.out.c = scratch;
         p.out.kept = kept;
-        if (int rc = launch<kType, false, false, kGated>(p, s); rc != DPEP_OK) return rc;
+        if (int rc = launch<kType, false, false, kGated>(p, partial, s); rc != DPEP_OK) return rc;
         p = {scratch, f->down, num_tokens, f->hidden, f->inter, {}};
         p.out.c = y;
-        return launch<kType, false, false, kStore>(p, s);
+        return launch<kType, false, false, kStore>(p, partial, s);
     });
 }
 
 size_t dpep_gated_ffn_backward_scratch_bytes(int num_tokens, int hidden, int inter)
 {
     if (num_tokens < 0 || hidden < 0 || inter < 0) return 0;
-    return whole(static_cast<size_t>(num_tokens) * inter * 2) + whole(static_cast<size_t>(num_tokens) * inter * 4);
+    return whole(static_cast<size_t>(num_tokens) * inter * 2) + whole(static_cast<size_t>(num_tokens) * inter * 4) +
+           std::max(std::max(cut_of(num_tokens, inter, hidden * 2, false, false).bytes, cut_of(num_tokens, hidden, inter * 4, false, false).bytes),
+                    std::max(cut_of(2 * inter, hidden, num_tokens * 2, false, true).bytes, cut_of(hidden, inter, num_tokens * 2, false, true).bytes));
 }
 
 int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x, const float* kept, int num_tokens, void* grad_x, void* grad_gate_up,
@@ -282,29 +620,30 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
     const hipStream_t s = static_cast<hipStream_t>(stream);
     void* const h = scratch;
     void* const dz = static_cast<uint8_t*>(scratch) + whole(static_cast<size_t>(num_tokens) * f->inter * 2);
+    void* const partial = static_cast<uint8_t*>(dz) + whole(static_cast<size_t>(num_tokens) * f->inter * 4);
     return by_type(f->type, [&](auto type) {
         constexpr int kType = decltype(type)::value;
         Product p = {grad_y, f->down, num_tokens, f->inter, f->hidden, {}};
         p.out.c = dz;
         p.out.kept = const_cast<float*>(kept);
         p.out.h = h;
-        if (int rc = launch<kType, false, true, kGradient>(p, s); rc != DPEP_OK) return rc;
+        if (int rc = launch<kType, false, true, kGradient>(p, partial, s); rc != DPEP_OK) return rc;
         p = {dz, f->gate_up, num_tokens, f->hidden, 2 * f->inter, {}};
         p.out.c = grad_x;
-        if (int rc = launch<kType, false, true, kStore>(p, s); rc != DPEP_OK) return rc;
+        if (int rc = launch<kType, false, true, kStore>(p, partial, s); rc != DPEP_OK) return rc;
         p = {dz, x, 2 * f->inter, f->hidden, num_tokens, {}};
         p.out.c = grad_gate_up;
-        if (int rc = launch<kType, true, true, kStore>(p, s); rc != DPEP_OK) return rc;
+        if (int rc = launch<kType, true, true, kStore>(p, partial, s); rc != DPEP_OK) return rc;
         p = {grad_y, h, f->hidden, f->inter, num_tokens, {}};
         p.out.c = grad_down;
-        return launch<kType, true, true, kStore>(p, s);
+        return launch<kType, true, true, kStore>(p, partial, s);
     });
 }
 
 size_t dpep_w8_matmul_scratch_bytes(int num_rows, int n, int k)
 {
-    (void)num_rows, (void)n, (void)k;
-    return 0;
+    if (num_rows < 0 || n < 0 || k < 0) return 0;
+    return cut_of(num_rows, n, k, false, false).bytes;
 }
 
 int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int num_rows, int type, void* y, void* scratch, void* stream)
@@ -327,7 +666,7 @@ int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int
     p.out.row_scale = x_scales;
     p.out.column_scale = w->scales;
     p.out.type = type;
-    return launch<kInt8, false, false, kScaled>(p, static_cast<hipStream_t>(stream));
+    return launch<kInt8, false, false, kScaled>(p, scratch, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
