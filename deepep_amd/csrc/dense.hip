@@ -138,29 +138,30 @@ struct Product {
 // The waves w and w + 4 share a SIMD and run half a phase apart: while one multiplies, the other reads its operands' next fragments from LDS and asks
 // for half an operand of a later step.  A phase of a wave is [read, ask, wait, barrier, multiply, barrier], and waves 4 .. 7 pass one barrier
 // more at the start, waves 0 .. 3 at the end.
-//   Which half is asked for: in phase 0 B1 and in phase 1 A1 of step k + 1, in phase 2 A0 and in phase 3 B0 of step k + 2; there are two buffers, k odd and
-//   even.  Every wait leaves the four last halves outstanding, so that a half has four phases to arrive in.
-//   Read after write: a half is read in the phase that follows the wait which covers it (A0 and B0 are covered at the end of phase 3, B1 of phase 0, A1 of
-//   phase 1), and a barrier that all waves pass after their wait lies in between, for the later waves half a phase behind too.
-//   Write after read: A0 and B0 are read in phase 0 and overwritten from phase 2 and 3 on, B1 and A1 in phases 1 and 2 and from the next step's phase 0 and 1
-//   on.  The fragments that the later waves read in phase p are in their registers before they multiply, which is before the barrier that lets the earlier
-//   waves into phase p + 2.
+//   Which half is read: in phase 0 A0, in phase 1 B1, in phase 2 A1, in phase 3 the next step's B0 (into the registers of B1, so that the two sets of
+//   registers for B change places from step to step: the loop holds two steps).
+//   Which half is asked for: in phase 0 A1 of step k + 1, in phases 1, 2 and 3 B0, A0 and B1 of step k + 2; there are two buffers, k odd and even.  Every
+//   wait leaves the five last halves outstanding, so that a half has five phases to arrive in.
+//   Read after write: a half is read in the phase that follows the wait which covers it, the fifth after the one that asked; a barrier that all
+//   waves pass after their wait lies in between, for the later waves half a phase behind too.
+//   Write after read: a half's buffer is overwritten from the second phase after the one that read it on.  The fragments that the later waves read in
+//   phase p are in their registers before they multiply, which is before the barrier that lets the earlier waves into phase p + 2.
 //
 // In LDS a row of 128 bytes of k holds its 16-byte pieces c at place c ^ key(row), so that eight lanes that read the same piece of eight rows find them in
 // different banks.  Operands that hold m or n contiguously lie in LDS as rows of k, 128 values wide, and are turned as they are read
-// (ds_read_tr); their pieces are spread by the row in the same way.
+// (ds_read_tr: 16 lanes read four rows); their pieces are spread by the row so that 32 lanes, eight rows, meet no bank twice.
 //
 // The matrix instruction takes B as its first operand, so that a lane's four results are four columns of one row.  The columns of a pair of
 // instructions are dealt so that a lane ends up with eight next to one another: 16 bytes of 16-bit results.
 //
-// Rows, columns and values of k that are not there are read as zero (the loads' own bounds check).
+// Rows, columns and values of k that are not there are read as zero (the loads' own bounds check): a half's record ends with its last row, and pieces
+// behind the last column or, in the last step, behind the last k have an offset that is nowhere.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int rsrc __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 512;
 constexpr int kStepBytes = 128;
 constexpr int kColumns = 256, kHalfColumns = kColumns / 2;
-constexpr int kColumnBytes = kHalfColumns * kStepBytes;  // of half of B
 constexpr uint32_t kNowhere = 0x80000000u;
 
 template <int kLoads>
@@ -175,95 +176,99 @@ __device__ __forceinline__ void meet()
     asm volatile("s_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
-// 16 bytes a lane from an operand straight into LDS, lane after lane from `lds` on.
-__device__ __forceinline__ void load_to_lds(rsrc from, uint32_t offset, uint32_t lds)
+// 16 bytes a lane from an operand straight into LDS, lane after lane from base + kAt on.
+template <int kAt>
+__device__ __forceinline__ void load_to_lds(rsrc from, uint32_t offset, uint32_t base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(base), "n"(kAt), "v"(offset), "s"(from) : "memory", "scc");
+}
+// The same by the lower half of the wave's lanes, all of which are active.
+template <int kAt>
+__device__ __forceinline__ void load_half_to_lds(rsrc from, uint32_t offset, uint32_t base)
+{
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_mov_b32 exec_hi, 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 exec_hi, -1" ::"s"(base), "n"(kAt), "v"(offset), "s"(from)
+                 : "memory", "scc");
 }
 
-// Half an operand as the loads see it: where its next step begins, and how much there is from there on.
-struct Half {
-    uint64_t base;
-    long long bytes;  // of operands with k contiguous: up to the end of the last row
-    __device__ __forceinline__ rsrc of(long long records) const
-    {
-        const uint32_t size = records <= 0 ? 0u : static_cast<uint32_t>(records < 0x7fffffff ? records : 0x7fffffff);
-        return rsrc{__builtin_amdgcn_readfirstlane(static_cast<int>(base)), __builtin_amdgcn_readfirstlane(static_cast<int>(base >> 32)),
-                    __builtin_amdgcn_readfirstlane(static_cast<int>(size)), 0x00020000};
-    }
-};
-
-// One operand of a tile: `kPer` loads a wave for each half of kRowsOfHalf rows (or columns).
+// One operand of a tile as the loads see it: halves of kRowsOfHalf rows (or columns), kPer loads a wave each.
 template <bool kTrans, int kRowsOfHalf, bool kPaired>
 struct Operand {
     static constexpr int kPer = kRowsOfHalf >= 64 ? kRowsOfHalf / 64 : 1;
     static constexpr bool kHalfWave = kRowsOfHalf == 32;
     static constexpr int kBytes = kRowsOfHalf * kStepBytes;
-    Half half[2];
-    uint32_t offset[kPer], at[kPer];  // a lane's place in the half; its place in k (bytes)
-    long long stride;                 // bytes of a row in memory
-    int left;                         // bytes of k (rows of k where kTrans) that are left from the next step on
-    int across[2];                    // kTrans: bytes of a row of k that belong to the half and what follows it
+    uint64_t base[2];                            // where the halves' next step begins
+    int records[2];                              // and how many bytes there are
+    uint32_t offset[kTrans ? 2 : 1][kPer];       // a lane's place in a half (of each half, where the columns that are there make a difference)
+    uint64_t advance_bytes;
+    int left;                                    // values of k that are left from the next step on
 
-    static __device__ __forceinline__ int key(int row) { return kTrans ? (row & 3) << 2 : kPaired ? (row & 3) | ((row >> 3) & 1) << 2 : row & 7; }
+    static __device__ __forceinline__ int key(int row)
+    {
+        if constexpr (kTrans) return kPaired ? (row & 3) << 2 | (row >> 3 & 1) : (row & 3) << 2 | (row >> 3 & 1) << 1;
+        else return kPaired ? (row & 3) | (row >> 3 & 1) << 2 : row & 7;
+    }
+    // A lane's row of a half in load i, and its piece of that row.
+    static __device__ __forceinline__ int row_of(int i, int wave, int lane)
+    {
+        if constexpr (kTrans) return (wave * kPer + i) * 4 + lane / 16;
+        else return kHalfWave ? wave * 4 + lane / 8 : (wave * kPer + i) * 8 + lane / 8;
+    }
+    static __device__ __forceinline__ int piece_of(int i, int wave, int lane) { return (kTrans ? lane % 16 : lane % 8) ^ key(row_of(i, wave, lane)); }
 
-    // rows: of the operand's whole matrix; first[h]: its row (column) where half h begins; there[h]: rows (columns) from there on, at most as many as belong to it; k0, k: in values.
-    __device__ __forceinline__ void set(const void* matrix, int value_bytes, int rows, const int (&first)[2], const int (&there)[2], int k_all, int k0, int k, int wave, int lane)
+    // rows: of the operand's whole matrix; first[h]: its row (column) where half h begins; there[h]: rows (columns) from there on; k .. in values.
+    template <int kValue>
+    __device__ __forceinline__ void set(const void* matrix, int rows, const int (&first)[2], const int (&there)[2], int k_all, int k0, int k1, int wave, int lane)
     {
-        const char* const p = static_cast<const char*>(matrix);
-        if constexpr (kTrans) {
-            stride = static_cast<long long>(rows) * value_bytes;
-            left = k - k0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                half[h].base = reinterpret_cast<uint64_t>(p + static_cast<long long>(k0) * stride + static_cast<long long>(first[h]) * value_bytes);
-                across[h] = max(there[h], 0) * value_bytes;
-            }
-        } else {
-            stride = static_cast<long long>(k_all) * value_bytes;
-            left = (k - k0) * value_bytes;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                half[h].base = reinterpret_cast<uint64_t>(p + first[h] * stride + static_cast<long long>(k0) * value_bytes);
-                half[h].bytes = there[h] <= 0 ? 0 : (there[h] - 1) * stride + left;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if constexpr (kTrans) {
-                const int row = (wave * kPer + i) * 4 + lane / 16, piece = lane % 16 ^ key(row);
-                at[i] = piece * 16;
-                offset[i] = static_cast<uint32_t>(row * stride) + piece * 16;
-            } else {
-                const int row = kHalfWave ? wave * 4 + lane / 8 : (wave * kPer + i) * 8 + lane / 8, piece = lane % 8 ^ key(row);
-                at[i] = piece * 16;
-                offset[i] = static_cast<uint32_t>(row * stride) + piece * 16;
-            }
-        }
-    }
-    // Ask for half h of the next step.
-    __device__ __forceinline__ void ask(int h, uint32_t lds, int wave, int lane) const
-    {
-        const rsrc from = half[h].of(kTrans ? (left <= 0 || across[h] <= 0 ? 0 : (min(left, 64) - 1) * stride + across[h]) : half[h].bytes);
-        const int limit = kTrans ? across[h] : left;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const uint32_t place = static_cast<int>(at[i]) < limit ? offset[i] : kNowhere;
-            if constexpr (kHalfWave) {
-                if (lane < 32) load_to_lds(from, place, lds + wave * 512);
-            } else {
-                load_to_lds(from, place, lds + (wave * kPer + i) * 1024);
-            }
-        }
-    }
-    __device__ __forceinline__ void advance()
-    {
+        const long long stride = static_cast<long long>(kTrans ? rows : k_all) * kValue;
+        left = k1 - k0;
+        advance_bytes = kTrans ? (kStepBytes / kValue) * stride : kStepBytes;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            half[h].base += kTrans ? 64 * stride : kStepBytes;
-            half[h].bytes -= kStepBytes;
+            base[h] = reinterpret_cast<uint64_t>(matrix) + (kTrans ? k0 * stride + static_cast<long long>(first[h]) * kValue
+                                                                               : first[h] * stride + static_cast<long long>(k0) * kValue);
+            records[h] = there[h] <= 0 ? 0 : kTrans ? 0x7fffffff : static_cast<int>(min(there[h], kRowsOfHalf) * stride);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int piece = piece_of(i, wave, lane);
+                const uint32_t place = static_cast<uint32_t>(row_of(i, wave, lane) * stride) + piece * 16;
+                if constexpr (kTrans) offset[h][i] = piece * (16 / kValue) < there[h] ? place : kNowhere;
+                else offset[0][i] = place;
+            }
         }
-        left -= kTrans ? 64 : kStepBytes;
+        limit<kValue>(wave, lane);
+    }
+    // Where the next step is the last one or none: what lies behind the end of k is nowhere.
+    template <int kValue>
+    __device__ __forceinline__ void limit(int wave, int lane)
+    {
+        if (left >= kStepBytes / kValue) return;
+#pragma unroll
+        for (int h = 0; h < (kTrans ? 2 : 1); ++h)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if ((kTrans ? row_of(i, wave, lane) : piece_of(i, wave, lane) * (16 / kValue)) >= left) offset[h][i] = kNowhere;
+    }
+    // On to the next step, after both halves have been asked for.
+    template <int kValue>
+    __device__ __forceinline__ void advance(int wave, int lane)
+    {
+        base[0] += advance_bytes;
+        base[1] += advance_bytes;
+        left -= kStepBytes / kValue;
+        limit<kValue>(wave, lane);
+    }
+    // Ask for half kHalf of the next step, to kAt behind `lds`, the wave's own place in a half.
+    template <int kHalf, int kAt>
+    __device__ __forceinline__ void ask(uint32_t lds) const
+    {
+        const rsrc from = {static_cast<int>(base[kHalf]), static_cast<int>(base[kHalf] >> 32), records[kHalf], 0x00020000};
+        const uint32_t* const o = offset[kTrans ? kHalf : 0];
+        if constexpr (kHalfWave) {
+            load_half_to_lds<kAt>(from, o[0], lds);
+        } else {
+            load_to_lds<kAt>(from, o[0], lds);
+            if constexpr (kPer == 2) load_to_lds<kAt + 1024>(from, o[1], lds);
+        }
     }
 };
 
@@ -289,7 +294,9 @@ __device__ __forceinline__ Place place_of(unsigned id, unsigned total, int m_til
     const unsigned at = die * share + min(die, more) + id / 8;
     const unsigned tiles = static_cast<unsigned>(m_tiles) * n_tiles, part = at / tiles, tile = at - part * tiles;
     const unsigned block = 4u * n_tiles, which = tile / block, in = tile - which * block, high = min(4u, m_tiles - which * 4);
-    return {static_cast<int>(which * 4 + in % high), static_cast<int>(in / high), static_cast<int>(part)};
+    // (divisions leave the scalar registers; what follows from the place should not)
+    return {__builtin_amdgcn_readfirstlane(static_cast<int>(which * 4 + in % high)), __builtin_amdgcn_readfirstlane(static_cast<int>(in / high)),
+            __builtin_amdgcn_readfirstlane(static_cast<int>(part))};
 }
 
 template <int kType, bool kTransA, bool kTransB, Finish kFinish, int kRows>
@@ -299,10 +306,9 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
     constexpr int kTileRows = 64 * kRows, kHalfRows = kTileRows / 2, kWide = kFinish == kGated ? kHalfColumns : kColumns;
     using A = Operand<kTransA, kHalfRows, false>;
     using B = Operand<kTransB, kHalfColumns, true>;
-    constexpr int kAhead = 2 * A::kPer + 2 * B::kPer;
-    constexpr int kBuffer = 2 * A::kBytes + 2 * kColumnBytes;
+    constexpr int kAhead = 2 * A::kPer + 2 * B::kPer + std::min(A::kPer, B::kPer);  // the five last halves, whichever they are
     static_assert(!kTransA || kRows == 4);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * A::kBytes + 4 * B::kBytes];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wave_row = wave / 4, wave_column = wave % 4;
     const Place place = place_of(blockIdx.x, gridDim.x, p.m_tiles, p.n_tiles);
@@ -313,106 +319,121 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
     A a;
     B b;
     {
-        const int first[2] = {m0, m0 + kHalfRows}, there[2] = {min(kHalfRows, p.m - m0), min(kHalfRows, p.m - m0 - kHalfRows)};
-        a.set(p.a, kValue, p.m, first, there, p.k, k0, k1, wave, lane);
+        const int first[2] = {m0, m0 + kHalfRows}, there[2] = {p.m - m0, p.m - m0 - kHalfRows};
+        a.template set<kValue>(p.a, p.m, first, there, p.k, k0, k1, wave, lane);
     }
     {
         const int second = kFinish == kGated ? p.columns + n0 : n0 + kHalfColumns, columns = p.columns - n0;
-        const int first[2] = {n0, second}, there[2] = {min(kHalfColumns, columns), min(kHalfColumns, kFinish == kGated ? columns : columns - kHalfColumns)};
-        b.set(p.b, kValue, p.columns, first, there, p.k, k0, k1, wave, lane);
+        const int first[2] = {n0, second}, there[2] = {columns, kFinish == kGated ? columns : columns - kHalfColumns};
+        b.template set<kValue>(p.b, p.columns, first, there, p.k, k0, k1, wave, lane);
     }
+    // LDS: [half of A][buffer], [half of B][buffer], so that a lane's places in both buffers are within the reach of an instruction's own offset.
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
-    const auto a_at = [](int h) { return h * A::kBytes; };
-    const auto b_at = [](int h) { return 2 * A::kBytes + h * kColumnBytes; };
+    const uint32_t a_base = lds0 + wave * (A::kBytes / 8), b_base = lds0 + wave * (B::kBytes / 8);
+    constexpr auto a_at = [](int half, int buffer) { return (2 * half + buffer) * A::kBytes; };
+    constexpr auto b_at = [](int half, int buffer) { return 4 * A::kBytes + (2 * half + buffer) * B::kBytes; };
 
-    // Where a lane reads its fragments: [two places that the key tells apart].
-    int read_a[2], read_b[2];
+    // Where a lane reads its fragments: a place for each 16 rows (kTransA) or half step, as the key tells them apart.
+    constexpr int kPlaces = kTransA ? 4 : 2;
+    int read_a[kPlaces], read_b[2];
     {
         const int r = lane % 16, group = lane / 16;
         if constexpr (kTransA) {
             const int row = 8 * group + r / 4, piece = wave_row * 8 + (r % 4) / 2;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) read_a[i] = row * 256 + ((piece + 4 * i) ^ A::key(row)) * 16 + (r % 2) * 8;
+            for (int i = 0; i < kPlaces; ++i) read_a[i] = row * 256 + ((piece + 2 * i) ^ A::key(row)) * 16 + (r % 2) * 8;
         } else {
             const int row = wave_row * 16 * kRows + r;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) read_a[i] = row * kStepBytes + ((4 * i + group) ^ A::key(row)) * 16;
+            for (int i = 0; i < kPlaces; ++i) read_a[i] = row * kStepBytes + ((4 * i + group) ^ A::key(row)) * 16;
         }
         if constexpr (kTransB) {
+            // (of a pair of instructions the first takes the lower four columns of an even piece and the upper four of an odd one)
             const int row = 8 * group + r / 4, piece = wave_column * 4 + r % 4;
-            read_b[0] = read_b[1] = row * 256 + (piece ^ B::key(row)) * 16;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) read_b[i] = b_at(0, 0) + row * 256 + (piece ^ B::key(row)) * 16 + ((i ^ r) & 1) * 8;
         } else {
             const int row = wave_column * 32 + 8 * (r / 4) + r % 4;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) read_b[i] = row * kStepBytes + ((4 * i + group) ^ B::key(row)) * 16;
+            for (int i = 0; i < 2; ++i) read_b[i] = b_at(0, 0) + row * kStepBytes + ((4 * i + group) ^ B::key(row)) * 16;
         }
     }
     Sum<kType> acc[2][2][kRows][2] = {};  // [half of A][half of B][16 rows][of a pair of instructions]
-    u32x4 fa[kRows][2], fb[2][2][2];      // [.][half step], [half of B][of a pair][half step]
-    const auto read_rows = [&](const uint8_t* from) {
+    u32x4 fa[kRows][2], fb[2][2][2];      // [.][half step]; [set][of a pair][half step]
+    const auto read_rows = [&](auto half, auto buffer) {
+        constexpr int kAt = a_at(half, buffer);
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                if constexpr (kTransA) fa[i][s] = read_turned_pair(from + read_a[i / 2] + (i % 2) * 32 + s * 32 * 256);
-                else fa[i][s] = *reinterpret_cast<const u32x4*>(from + read_a[s] + i * 16 * kStepBytes);
+                if constexpr (kTransA) fa[i][s] = read_turned_pair(lds + read_a[i] + kAt + s * 32 * 256);
+                else fa[i][s] = *reinterpret_cast<const u32x4*>(lds + read_a[s] + kAt + i * 16 * kStepBytes);
             }
     };
-    const auto read_columns = [&](const uint8_t* from, int h) {
+    const auto read_columns = [&](auto half, auto buffer, auto set) {
+        constexpr int kAt = b_at(half, buffer) - b_at(0, 0);
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                if constexpr (kTransB) fb[h][f][s] = read_turned_pair(from + read_b[0] + f * 8 + s * 32 * 256);
-                else fb[h][f][s] = *reinterpret_cast<const u32x4*>(from + read_b[s] + f * 4 * kStepBytes);
+                if constexpr (kTransB) fb[set][f][s] = read_turned_pair(lds + read_b[f] + kAt + s * 32 * 256);
+                else fb[set][f][s] = *reinterpret_cast<const u32x4*>(lds + read_b[s] + kAt + f * 4 * kStepBytes);
             }
     };
-    const auto multiply_halves = [&](int ha, int hb) {
+    const auto multiply_halves = [&](auto ha, auto hb, auto set) {
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < kRows; ++i)
 #pragma unroll
-                for (int f = 0; f < 2; ++f) acc[ha][hb][i][f] = multiply<kType>(fb[hb][f][s], fa[i][s], acc[ha][hb][i][f]);
+                for (int f = 0; f < 2; ++f) acc[ha][hb][i][f] = multiply<kType>(fb[set][f][s], fa[i][s], acc[ha][hb][i][f]);
         __builtin_amdgcn_s_setprio(0);
     };
+    constexpr std::integral_constant<int, 0> c0;
+    constexpr std::integral_constant<int, 1> c1;
+    // A step whose operands lie in buffer `now`, with its B0 in the registers `set`; `now` and `set` change together.
+    const auto step = [&](auto now, auto other) {
+        read_rows(c0, now);
+        a.template ask<1, a_at(1, other)>(a_base);
+        a.template advance<kValue>(wave, lane);
+        wait_and_meet<kAhead>();
+        multiply_halves(c0, c0, now);
+        meet();
+        read_columns(c1, now, other);
+        b.template ask<0, b_at(0, now)>(b_base);
+        wait_and_meet<kAhead>();
+        multiply_halves(c0, c1, other);
+        meet();
+        read_rows(c1, now);
+        a.template ask<0, a_at(0, now)>(a_base);
+        wait_and_meet<kAhead>();
+        multiply_halves(c1, c1, other);
+        meet();
+        read_columns(c0, other, other);
+        b.template ask<1, b_at(1, now)>(b_base);
+        b.template advance<kValue>(wave, lane);
+        wait_and_meet<kAhead>();
+        multiply_halves(c1, c0, now);
+        meet();
+    };
 
-    a.ask(0, lds0 + a_at(0), wave, lane);
-    b.ask(0, lds0 + b_at(0), wave, lane);
-    b.ask(1, lds0 + b_at(1), wave, lane);
-    a.ask(1, lds0 + a_at(1), wave, lane);
-    a.advance();
-    b.advance();
-    a.ask(0, lds0 + kBuffer + a_at(0), wave, lane);
-    b.ask(0, lds0 + kBuffer + b_at(0), wave, lane);
+    b.template ask<0, b_at(0, 0)>(b_base);
+    a.template ask<0, a_at(0, 0)>(a_base);
+    b.template ask<1, b_at(1, 0)>(b_base);
+    a.template ask<1, a_at(1, 0)>(a_base);
+    a.template advance<kValue>(wave, lane);
+    b.template advance<kValue>(wave, lane);
+    b.template ask<0, b_at(0, 1)>(b_base);
+    a.template ask<0, a_at(0, 1)>(a_base);
+    b.template ask<1, b_at(1, 1)>(b_base);
+    b.template advance<kValue>(wave, lane);
     wait_and_meet<kAhead>();
+    read_columns(c0, c0, c0);
     if (wave_row == 1) meet();
-    for (int k = 0, now = 0; k < steps; ++k, now ^= kBuffer) {
-        const uint8_t* const buffer = lds + now;
-        const uint32_t to = lds0 + now, to_other = lds0 + (now ^ kBuffer);
-        read_columns(buffer + b_at(0), 0);
-        read_rows(buffer + a_at(0));
-        b.ask(1, to_other + b_at(1), wave, lane);
-        wait_and_meet<kAhead>();
-        multiply_halves(0, 0);
-        meet();
-        read_columns(buffer + b_at(1), 1);
-        a.ask(1, to_other + a_at(1), wave, lane);
-        wait_and_meet<kAhead>();
-        multiply_halves(0, 1);
-        meet();
-        a.advance();
-        b.advance();
-        read_rows(buffer + a_at(1));
-        a.ask(0, to + a_at(0), wave, lane);
-        wait_and_meet<kAhead>();
-        multiply_halves(1, 1);
-        meet();
-        b.ask(0, to + b_at(0), wave, lane);
-        wait_and_meet<kAhead>();
-        multiply_halves(1, 0);
-        meet();
+    for (int k = 0; k < steps; k += 2) {  // (an odd number of steps gets one of zeros: a way out between the two costs registers)
+        step(c0, c1);
+        step(c1, c0);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what was asked for past the end is in LDS before the workgroup gives it up)
     if (wave_row == 0) meet();
@@ -428,7 +449,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
-                for (int f = 0; f < 2; ++f) v[hb][f] = acc[ha][hb][i][f];
+                for (int f = 0; f < 2; ++f) v[hb][f] = kTransB && (lane / 16) % 2 == 1 ? acc[ha][hb][i][1 - f] : acc[ha][hb][i][f];
             if (p.parts > 1) {
                 // Sums of a part of k, [part][m][columns, twice as many where kGated].
                 constexpr int kTimes = kFinish == kGated ? 2 : 1;
