@@ -510,6 +510,112 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
     else finish<kType, kFinish>(p.out, m, n, p.columns, v[0]);
 }
 
+// ---- few rows: a stream of B ------------------------------------------------------------------------------------------------------
+// For up to 16 kBlocks rows of A the time is that of reading B, which goes from memory straight to registers, whole 128-byte lines: a load of a wave
+// covers a line of 8 rows of B, lane l piece l / 8 of row l % 8.  For the matrix instruction lanes l and l + 8 hold the same row's
+// pieces 2 g and 2 g + 1 (g = l / 16) in the place of two rows: multiplied by A's pieces 2 g its results 0 .. 7 are what the even pieces add to the eight
+// rows, by A's pieces 2 g + 1 results 8 .. 15 what the odd ones do, and the other halves are not looked at.  Twice the instructions, of which there is
+// no shortage here, instead of moving lines between lanes.
+//
+// A workgroup makes 16 rows of B (kGated: 8 of gate and their 8 of up); its eight waves take every eighth line of k and their sums meet in LDS.  A's pieces come from
+// the caches.  kAhead lines of a wave are under way at any time.
+constexpr int kStreamUnits = 2;  // of 8 rows of B
+constexpr int kStreamRows = 64;  // of A, at most
+template <int kType, Finish kFinish, int kBlocks>
+__global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void stream_kernel(const Product p)
+{
+    constexpr int kValue = kType == kInt8 ? 1 : 2, kWaves = kThreads / kWave, kAhead = kBlocks == 1 ? 4 : 3;
+    constexpr int kWide = kFinish == kGated ? 8 : 8 * kStreamUnits;  // columns of the result
+    __shared__ __attribute__((aligned(16))) uint32_t sums[kWaves][kStreamUnits][kBlocks][16][8];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int n0 = blockIdx.x * kWide, k_bytes = p.k * kValue, lines = (k_bytes + kStepBytes - 1) / kStepBytes;
+    const auto resource = [](const void* at, long long bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, static_cast<int>(min(bytes, 0x7fffffffll)), 0x00020000);
+    };
+    // (8 rows of B and 64 of A are less than 2^31 bytes)
+    __amdgpu_buffer_rsrc_t from_b[kStreamUnits];
+#pragma unroll
+    for (int u = 0; u < kStreamUnits; ++u) {
+        const int n = n0 + (kFinish == kGated ? 0 : 8 * u), there = min(8, p.columns - n);
+        const long long row = static_cast<long long>(kFinish == kGated && u == 1 ? p.columns : 0) + n;
+        from_b[u] = resource(static_cast<const char*>(p.b) + row * k_bytes, there <= 0 ? 0 : static_cast<long long>(there) * k_bytes);
+    }
+    const __amdgpu_buffer_rsrc_t from_a = resource(p.a, static_cast<long long>(p.m) * k_bytes);
+    const int at_b = lane % 8 * k_bytes + lane / 8 * 16, at_a = lane % 16 * k_bytes + lane / 16 * 32;
+    struct Line {
+        u32x4 b[kStreamUnits], a[kBlocks][2];
+    };
+    const auto load = [&](int line) {
+        Line l;
+        const int k = line * kStepBytes;
+        const bool live_b = k + lane / 8 * 16 < k_bytes;
+#pragma unroll
+        for (int u = 0; u < kStreamUnits; ++u)
+            l.b[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from_b[u], live_b ? static_cast<uint32_t>(at_b + k) : kNowhere, 0, 2));
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {
+                const bool live_a = k + lane / 16 * 32 + odd * 16 < k_bytes;
+                l.a[i][odd] = __builtin_bit_cast(
+                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(from_a, live_a ? static_cast<uint32_t>(at_a + i * 16 * k_bytes + k + odd * 16) : kNowhere, 0, 0));
+            }
+        return l;
+    };
+    Line ahead[kAhead];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) ahead[d] = load(wave + d * kWaves);
+    Sum<kType> acc[kStreamUnits][kBlocks][2] = {};
+    for (int line = wave; line < lines; line += kAhead * kWaves)
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) {
+            const Line now = ahead[d];
+            ahead[d] = load(line + (d + kAhead) * kWaves);
+#pragma unroll
+            for (int u = 0; u < kStreamUnits; ++u)
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                    for (int odd = 0; odd < 2; ++odd) acc[u][i][odd] = multiply<kType>(now.b[u], now.a[i][odd], acc[u][i][odd]);
+        }
+    // Lane (g, r) has results 4 g .. 4 g + 3 of row r of A: the even pieces' in groups 0 and 1, the odd ones' in groups 2 and 3.
+#pragma unroll
+    for (int u = 0; u < kStreamUnits; ++u)
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            Sum<kType> v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const auto odd = __shfl(acc[u][i][1][e], lane % 32 + 32);
+                v[e] = acc[u][i][0][e] + odd;
+            }
+            if (lane < 32) *reinterpret_cast<u32x4*>(&sums[wave][u][i][lane % 16][lane / 16 * 4]) = __builtin_bit_cast(u32x4, v);
+        }
+    __syncthreads();
+    constexpr int kTasks = kFinish == kGated ? 16 * kBlocks : 16 * kBlocks * kStreamUnits;
+    const int m = threadIdx.x % (16 * kBlocks), unit = threadIdx.x / (16 * kBlocks);
+    if (threadIdx.x >= kTasks || m >= p.m) return;
+    const auto total = [&](int u, float (&v)[8]) {
+        Sum<kType> sum[2] = {};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sum[h] += __builtin_bit_cast(Sum<kType>, *reinterpret_cast<const u32x4*>(&sums[w][u][m / 16][m % 16][4 * h]));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(sum[e / 4][e % 4]);
+    };
+    float v[8];
+    total(unit, v);
+    if constexpr (kFinish == kGated) {
+        float up[8];
+        total(1, up);
+        finish_gated<kType>(p.out, m, n0, p.columns, v, up);
+    } else {
+        const int n = n0 + 8 * unit;
+        if (n < p.columns) finish<kType, kFinish>(p.out, m, n, p.columns, v);
+    }
+}
+
 // How a product is cut up.
 struct Cut {
     int rows, m_tiles, n_tiles, parts, part_steps;
@@ -535,6 +641,16 @@ template <int kType, bool kTransA, bool kTransB, Finish kFinish>
 int launch(Product p, void* partial, hipStream_t stream)
 {
     if (p.m == 0 || p.columns == 0) return DPEP_OK;
+    if constexpr (!kTransA && !kTransB) {
+        if (p.m <= kStreamRows) {
+            constexpr int kWide = kFinish == kGated ? 8 : 8 * kStreamUnits;
+            const dim3 grid((p.columns + kWide - 1) / kWide);
+            if (p.m <= 16) stream_kernel<kType, kFinish, 1><<<grid, kThreads, 0, stream>>>(p);
+            else if (p.m <= 32) stream_kernel<kType, kFinish, 2><<<grid, kThreads, 0, stream>>>(p);
+            else stream_kernel<kType, kFinish, 4><<<grid, kThreads, 0, stream>>>(p);
+            return launch_status("product of few rows");
+        }
+    }
     const Cut c = cut_of(p.m, p.columns, p.k * (kType == kInt8 ? 1 : 2), kFinish == kGated, kTransA);
     p.m_tiles = c.m_tiles;
     p.n_tiles = c.n_tiles;
