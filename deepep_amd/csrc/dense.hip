@@ -68,6 +68,7 @@ struct Output {
     const float* row_scale;
     const float* column_scale;
     int type;           // of C where kScaled
+    bool whole;         // kScaled: rows are whole pieces of eight, aligned
 };
 
 __device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
@@ -108,12 +109,21 @@ __device__ __forceinline__ void finish(const Output& o, size_t m, int n, int col
     } else if constexpr (kFinish == kScaled) {
         const float row = o.row_scale[m];
         const size_t at = m * columns + n;
+        float y[8];
+        if (o.whole) {
+            load_wide(o.column_scale + n, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = v[i] * row * y[i];
+            if (o.type == DPEP_TYPE_F32) store_wide(static_cast<float*>(o.c) + at, y);
+            else *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(o.c) + at) = o.type == DPEP_TYPE_BF16 ? narrow8<DPEP_TYPE_BF16>(y) : narrow8<DPEP_TYPE_F16>(y);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (n + i >= columns) break;
-            const float y = v[i] * row * o.column_scale[n + i];
-            if (o.type == DPEP_TYPE_F32) static_cast<float*>(o.c)[at + i] = y;
-            else static_cast<uint16_t*>(o.c)[at + i] = static_cast<uint16_t>(o.type == DPEP_TYPE_BF16 ? f32_to_bf16(y) : pack_f16x2(y, 0.0f) & 0xffffu);
+            const float one = v[i] * row * o.column_scale[n + i];
+            if (o.type == DPEP_TYPE_F32) static_cast<float*>(o.c)[at + i] = one;
+            else static_cast<uint16_t*>(o.c)[at + i] = static_cast<uint16_t>(o.type == DPEP_TYPE_BF16 ? f32_to_bf16(one) : pack_f16x2(one, 0.0f) & 0xffffu);
         }
     }
 }
@@ -130,12 +140,11 @@ struct Product {
 };
 
 // ---- large tiles on the matrix cores ------------------------------------------------------------------------------------------------
-// A workgroup of eight waves makes a tile of 64 kRows x 256 results (kRows = 4, 2 or 1), 128 bytes of k at a time ("step").  Both operands
-// go from memory to LDS without passing registers, each in two halves (rows of the tile 0 .. and 32 kRows ..; columns 0 .. and 128 ..; with kGated
-// the halves of B are the gate and the up rows of the same 128 columns).  A wave takes 16 kRows rows and 32 columns of each half, so that a step
-// is four products of a half of A with a half of B ("phases"): (0,0), (0,1), (1,1), (1,0).
+// A workgroup of eight waves makes a tile of 256 x 256 results, or fewer, 128 bytes of k at a time ("step").  Both operands go from memory to LDS without
+// passing registers, each in two halves of rows (columns) of the tile; with kGated the halves of B are the gate and the up rows of the same
+// columns.  A wave takes 16 kRows rows and 32 columns of each half, so that a step is four products of a half of A with a half of B: (0,0), (0,1), (1,1), (1,0).
 //
-// The waves w and w + 4 share a SIMD and run half a phase apart: while one multiplies, the other reads its operands' next fragments from LDS and asks
+// Tiles of 256 x 256 take these one at a time ("phases").  The waves w and w + 4 share a SIMD and run half a phase apart: while one multiplies, the other reads its operands' next fragments from LDS and asks
 // for half an operand of a later step.  A phase of a wave is [read, ask, wait, barrier, multiply, barrier], and waves 4 .. 7 pass one barrier
 // more at the start, waves 0 .. 3 at the end.
 //   Which half is read: in phase 0 A0, in phase 1 B1, in phase 2 A1, in phase 3 the next step's B0 (into the registers of B1, so that the two sets of
@@ -161,7 +170,6 @@ typedef int rsrc __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 512;
 constexpr int kStepBytes = 128;
-constexpr int kColumns = 256, kHalfColumns = kColumns / 2;
 constexpr uint32_t kNowhere = 0x80000000u;
 
 template <int kLoads>
@@ -182,20 +190,12 @@ __device__ __forceinline__ void load_to_lds(rsrc from, uint32_t offset, uint32_t
 {
     asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(base), "n"(kAt), "v"(offset), "s"(from) : "memory", "scc");
 }
-// The same by the lower half of the wave's lanes, all of which are active.
-template <int kAt>
-__device__ __forceinline__ void load_half_to_lds(rsrc from, uint32_t offset, uint32_t base)
-{
-    asm volatile("s_add_u32 m0, %0, %1\n\ts_mov_b32 exec_hi, 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 exec_hi, -1" ::"s"(base), "n"(kAt), "v"(offset), "s"(from)
-                 : "memory", "scc");
-}
-
 // One operand of a tile as the loads see it: halves of kRowsOfHalf rows (or columns), kPer loads a wave each.
 template <bool kTrans, int kRowsOfHalf, bool kPaired>
 struct Operand {
-    static constexpr int kPer = kRowsOfHalf >= 64 ? kRowsOfHalf / 64 : 1;
-    static constexpr bool kHalfWave = kRowsOfHalf == 32;
+    static constexpr int kPer = kRowsOfHalf / 64;
     static constexpr int kBytes = kRowsOfHalf * kStepBytes;
+    static_assert(kRowsOfHalf == 128 || kRowsOfHalf == 64);
     uint64_t base[2];                            // where the halves' next step begins
     int records[2];                              // and how many bytes there are
     uint32_t offset[kTrans ? 2 : 1][kPer];       // a lane's place in a half (of each half, where the columns that are there make a difference)
@@ -204,16 +204,17 @@ struct Operand {
 
     static __device__ __forceinline__ int key(int row)
     {
-        if constexpr (kTrans) return kPaired ? (row & 3) << 2 | (row >> 3 & 1) : (row & 3) << 2 | (row >> 3 & 1) << 1;
+        if constexpr (kTrans && kRowsOfHalf == 128) return kPaired ? (row & 3) << 2 | (row >> 3 & 1) : (row & 3) << 2 | (row >> 3 & 1) << 1;
+        else if constexpr (kTrans) return kPaired ? (row >> 1 & 1) << 2 | (row >> 3 & 1) : (row >> 3 & 1) << 2 | (row >> 1 & 1) << 1;
         else return kPaired ? (row & 3) | (row >> 3 & 1) << 2 : row & 7;
     }
     // A lane's row of a half in load i, and its piece of that row.
     static __device__ __forceinline__ int row_of(int i, int wave, int lane)
     {
-        if constexpr (kTrans) return (wave * kPer + i) * 4 + lane / 16;
-        else return kHalfWave ? wave * 4 + lane / 8 : (wave * kPer + i) * 8 + lane / 8;
+        if constexpr (kTrans) return (wave * kPer + i) * (512 / kRowsOfHalf) + lane / (kRowsOfHalf / 8);
+        else return (wave * kPer + i) * 8 + lane / 8;
     }
-    static __device__ __forceinline__ int piece_of(int i, int wave, int lane) { return (kTrans ? lane % 16 : lane % 8) ^ key(row_of(i, wave, lane)); }
+    static __device__ __forceinline__ int piece_of(int i, int wave, int lane) { return (kTrans ? lane % (kRowsOfHalf / 8) : lane % 8) ^ key(row_of(i, wave, lane)); }
 
     // rows: of the operand's whole matrix; first[h]: its row (column) where half h begins; there[h]: rows (columns) from there on; k .. in values.
     template <int kValue>
@@ -263,12 +264,8 @@ struct Operand {
     {
         const rsrc from = {static_cast<int>(base[kHalf]), static_cast<int>(base[kHalf] >> 32), records[kHalf], 0x00020000};
         const uint32_t* const o = offset[kTrans ? kHalf : 0];
-        if constexpr (kHalfWave) {
-            load_half_to_lds<kAt>(from, o[0], lds);
-        } else {
-            load_to_lds<kAt>(from, o[0], lds);
-            if constexpr (kPer == 2) load_to_lds<kAt + 1024>(from, o[1], lds);
-        }
+        load_to_lds<kAt>(from, o[0], lds);
+        if constexpr (kPer == 2) load_to_lds<kAt + 1024>(from, o[1], lds);
     }
 };
 
@@ -276,10 +273,11 @@ __device__ __forceinline__ s16x4 read_turned(const uint8_t* p)
 {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
 }
-// 8 values of k of a lane, from rows of k at p and, four rows further, the other four.
+// 8 values of k of a lane, from rows of k at p and, four rows of kBytes further, the other four.
+template <int kBytes>
 __device__ __forceinline__ u32x4 read_turned_pair(const uint8_t* p)
 {
-    const u32x2 a = __builtin_bit_cast(u32x2, read_turned(p)), b = __builtin_bit_cast(u32x2, read_turned(p + 4 * 256));
+    const u32x2 a = __builtin_bit_cast(u32x2, read_turned(p)), b = __builtin_bit_cast(u32x2, read_turned(p + 4 * kBytes));
     return u32x4{a[0], a[1], b[0], b[1]};
 }
 
@@ -299,49 +297,53 @@ __device__ __forceinline__ Place place_of(unsigned id, unsigned total, int m_til
             __builtin_amdgcn_readfirstlane(static_cast<int>(part))};
 }
 
-template <int kType, bool kTransA, bool kTransB, Finish kFinish, int kRows>
+// Tiles of 256 x 256, in two buffers, or of 128 x 128 in a ring of five.
+template <bool kLarge>
+struct Shape {
+    static constexpr int kTile = kLarge ? 256 : 128, kHalf = kTile / 2;
+    static constexpr int kWavesN = kLarge ? 4 : 2, kRows = kLarge ? 4 : 1;  // waves across the columns, 32 of each half a wave; 16s of rows of each half a wave
+    static constexpr int kStage = 4 * kHalf * kStepBytes, kStages = kLarge ? 2 : 5;
+};
+
+template <int kType, bool kTransA, bool kTransB, Finish kFinish, bool kLarge>
 __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
 {
+    using S = Shape<kLarge>;
     constexpr int kValue = kType == kInt8 ? 1 : 2, kValues = kStepBytes / kValue;  // bytes of a value, values of a step
-    constexpr int kTileRows = 64 * kRows, kHalfRows = kTileRows / 2, kWide = kFinish == kGated ? kHalfColumns : kColumns;
-    using A = Operand<kTransA, kHalfRows, false>;
-    using B = Operand<kTransB, kHalfColumns, true>;
-    constexpr int kAhead = 2 * A::kPer + 2 * B::kPer + std::min(A::kPer, B::kPer);  // the five last halves, whichever they are
-    static_assert(!kTransA || kRows == 4);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * A::kBytes + 4 * B::kBytes];
+    constexpr int kHalf = S::kHalf, kRows = S::kRows, kWide = kFinish == kGated ? kHalf : 2 * kHalf;
+    using A = Operand<kTransA, kHalf, false>;
+    using B = Operand<kTransB, kHalf, true>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kStages * S::kStage];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int wave_row = wave / 4, wave_column = wave % 4;
+    const int wave_row = wave / S::kWavesN, wave_column = wave % S::kWavesN;
     const Place place = place_of(blockIdx.x, gridDim.x, p.m_tiles, p.n_tiles);
-    const int m0 = place.m * kTileRows, n0 = place.n * kWide;
+    const int m0 = place.m * 2 * kHalf, n0 = place.n * kWide;
     const int k0 = min(p.k, place.part * p.part_steps * kValues), k1 = min(p.k, k0 + p.part_steps * kValues);
     const int steps = (k1 - k0 + kValues - 1) / kValues;
 
     A a;
     B b;
     {
-        const int first[2] = {m0, m0 + kHalfRows}, there[2] = {p.m - m0, p.m - m0 - kHalfRows};
+        const int first[2] = {m0, m0 + kHalf}, there[2] = {p.m - m0, p.m - m0 - kHalf};
         a.template set<kValue>(p.a, p.m, first, there, p.k, k0, k1, wave, lane);
     }
     {
-        const int second = kFinish == kGated ? p.columns + n0 : n0 + kHalfColumns, columns = p.columns - n0;
-        const int first[2] = {n0, second}, there[2] = {columns, kFinish == kGated ? columns : columns - kHalfColumns};
+        const int second = kFinish == kGated ? p.columns + n0 : n0 + kHalf, columns = p.columns - n0;
+        const int first[2] = {n0, second}, there[2] = {columns, kFinish == kGated ? columns : columns - kHalf};
         b.template set<kValue>(p.b, p.columns, first, there, p.k, k0, k1, wave, lane);
     }
-    // LDS: [half of A][buffer], [half of B][buffer], so that a lane's places in both buffers are within the reach of an instruction's own offset.
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
     const uint32_t a_base = lds0 + wave * (A::kBytes / 8), b_base = lds0 + wave * (B::kBytes / 8);
-    constexpr auto a_at = [](int half, int buffer) { return (2 * half + buffer) * A::kBytes; };
-    constexpr auto b_at = [](int half, int buffer) { return 4 * A::kBytes + (2 * half + buffer) * B::kBytes; };
 
     // Where a lane reads its fragments: a place for each 16 rows (kTransA) or half step, as the key tells them apart.
-    constexpr int kPlaces = kTransA ? 4 : 2;
+    constexpr int kPlaces = kTransA ? kRows : 2, kBytesK = 2 * kHalf;  // (bytes of a row of k)
     int read_a[kPlaces], read_b[2];
     {
         const int r = lane % 16, group = lane / 16;
         if constexpr (kTransA) {
-            const int row = 8 * group + r / 4, piece = wave_row * 8 + (r % 4) / 2;
+            const int row = 8 * group + r / 4, piece = wave_row * 2 * kRows + (r % 4) / 2;
 #pragma unroll
-            for (int i = 0; i < kPlaces; ++i) read_a[i] = row * 256 + ((piece + 2 * i) ^ A::key(row)) * 16 + (r % 2) * 8;
+            for (int i = 0; i < kPlaces; ++i) read_a[i] = row * kBytesK + ((piece + 2 * i) ^ A::key(row)) * 16 + (r % 2) * 8;
         } else {
             const int row = wave_row * 16 * kRows + r;
 #pragma unroll
@@ -351,99 +353,147 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
             // (of a pair of instructions the first takes the lower four columns of an even piece and the upper four of an odd one)
             const int row = 8 * group + r / 4, piece = wave_column * 4 + r % 4;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) read_b[i] = b_at(0, 0) + row * 256 + (piece ^ B::key(row)) * 16 + ((i ^ r) & 1) * 8;
+            for (int i = 0; i < 2; ++i) read_b[i] = row * kBytesK + (piece ^ B::key(row)) * 16 + ((i ^ r) & 1) * 8;
         } else {
             const int row = wave_column * 32 + 8 * (r / 4) + r % 4;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) read_b[i] = b_at(0, 0) + row * kStepBytes + ((4 * i + group) ^ B::key(row)) * 16;
+            for (int i = 0; i < 2; ++i) read_b[i] = row * kStepBytes + ((4 * i + group) ^ B::key(row)) * 16;
         }
     }
     Sum<kType> acc[2][2][kRows][2] = {};  // [half of A][half of B][16 rows][of a pair of instructions]
-    u32x4 fa[kRows][2], fb[2][2][2];      // [.][half step]; [set][of a pair][half step]
-    const auto read_rows = [&](auto half, auto buffer) {
-        constexpr int kAt = a_at(half, buffer);
+    const auto read_rows = [&](int at, u32x4 (&f)[kRows][2]) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                if constexpr (kTransA) fa[i][s] = read_turned_pair(lds + read_a[i] + kAt + s * 32 * 256);
-                else fa[i][s] = *reinterpret_cast<const u32x4*>(lds + read_a[s] + kAt + i * 16 * kStepBytes);
+                if constexpr (kTransA) f[i][s] = read_turned_pair<kBytesK>(lds + read_a[i] + at + s * 32 * kBytesK);
+                else f[i][s] = *reinterpret_cast<const u32x4*>(lds + read_a[s] + at + i * 16 * kStepBytes);
             }
     };
-    const auto read_columns = [&](auto half, auto buffer, auto set) {
-        constexpr int kAt = b_at(half, buffer) - b_at(0, 0);
+    const auto read_columns = [&](int at, u32x4 (&f)[2][2]) {
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                if constexpr (kTransB) fb[set][f][s] = read_turned_pair(lds + read_b[f] + kAt + s * 32 * 256);
-                else fb[set][f][s] = *reinterpret_cast<const u32x4*>(lds + read_b[s] + kAt + f * 4 * kStepBytes);
+                if constexpr (kTransB) f[i][s] = read_turned_pair<kBytesK>(lds + read_b[i] + at + s * 32 * kBytesK);
+                else f[i][s] = *reinterpret_cast<const u32x4*>(lds + read_b[s] + at + i * 4 * kStepBytes);
             }
     };
-    const auto multiply_halves = [&](auto ha, auto hb, auto set) {
-        __builtin_amdgcn_s_setprio(1);
+    const auto multiply_halves = [&](Sum<kType> (&sum)[kRows][2], const u32x4 (&fa)[kRows][2], const u32x4 (&fb)[2][2]) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < kRows; ++i)
 #pragma unroll
-                for (int f = 0; f < 2; ++f) acc[ha][hb][i][f] = multiply<kType>(fb[set][f][s], fa[i][s], acc[ha][hb][i][f]);
-        __builtin_amdgcn_s_setprio(0);
+                for (int f = 0; f < 2; ++f) sum[i][f] = multiply<kType>(fb[f][s], fa[i][s], sum[i][f]);
     };
     constexpr std::integral_constant<int, 0> c0;
     constexpr std::integral_constant<int, 1> c1;
-    // A step whose operands lie in buffer `now`, with its B0 in the registers `set`; `now` and `set` change together.
-    const auto step = [&](auto now, auto other) {
-        read_rows(c0, now);
-        a.template ask<1, a_at(1, other)>(a_base);
+
+    if constexpr (kLarge) {
+        constexpr int kAhead = 10;  // the five last halves, whichever they are
+        // LDS: [half of A][buffer], [half of B][buffer], so that a lane's places in both buffers are within the reach of an instruction's own offset.
+        constexpr auto a_at = [](int half, int buffer) { return (2 * half + buffer) * A::kBytes; };
+        constexpr auto b_at = [](int half, int buffer) { return 4 * A::kBytes + (2 * half + buffer) * B::kBytes; };
+#pragma unroll
+        for (int i = 0; i < 2; ++i) read_b[i] += b_at(0, 0);
+        u32x4 fa[kRows][2], fb[2][2][2];  // [.][half step]; [set][of a pair][half step]
+        const auto multiply_phase = [&](Sum<kType> (&sum)[kRows][2], const u32x4 (&columns)[2][2]) {
+            __builtin_amdgcn_s_setprio(1);
+            multiply_halves(sum, fa, columns);
+            __builtin_amdgcn_s_setprio(0);
+            meet();
+        };
+        // A step whose operands lie in buffer `now`, with its B0 in the registers `now`.
+        const auto step = [&](auto now, auto other) {
+            read_rows(a_at(0, now), fa);
+            a.template ask<1, a_at(1, other)>(a_base);
+            a.template advance<kValue>(wave, lane);
+            wait_and_meet<kAhead>();
+            multiply_phase(acc[0][0], fb[now]);
+            read_columns(b_at(1, now) - b_at(0, 0), fb[other]);
+            b.template ask<0, b_at(0, now)>(b_base);
+            wait_and_meet<kAhead>();
+            multiply_phase(acc[0][1], fb[other]);
+            read_rows(a_at(1, now), fa);
+            a.template ask<0, a_at(0, now)>(a_base);
+            wait_and_meet<kAhead>();
+            multiply_phase(acc[1][1], fb[other]);
+            read_columns(b_at(0, other) - b_at(0, 0), fb[other]);
+            b.template ask<1, b_at(1, now)>(b_base);
+            b.template advance<kValue>(wave, lane);
+            wait_and_meet<kAhead>();
+            multiply_phase(acc[1][0], fb[now]);
+        };
+        b.template ask<0, b_at(0, 0)>(b_base);
+        a.template ask<0, a_at(0, 0)>(a_base);
+        b.template ask<1, b_at(1, 0)>(b_base);
+        a.template ask<1, a_at(1, 0)>(a_base);
         a.template advance<kValue>(wave, lane);
-        wait_and_meet<kAhead>();
-        multiply_halves(c0, c0, now);
-        meet();
-        read_columns(c1, now, other);
-        b.template ask<0, b_at(0, now)>(b_base);
-        wait_and_meet<kAhead>();
-        multiply_halves(c0, c1, other);
-        meet();
-        read_rows(c1, now);
-        a.template ask<0, a_at(0, now)>(a_base);
-        wait_and_meet<kAhead>();
-        multiply_halves(c1, c1, other);
-        meet();
-        read_columns(c0, other, other);
-        b.template ask<1, b_at(1, now)>(b_base);
+        b.template advance<kValue>(wave, lane);
+        b.template ask<0, b_at(0, 1)>(b_base);
+        a.template ask<0, a_at(0, 1)>(a_base);
+        b.template ask<1, b_at(1, 1)>(b_base);
         b.template advance<kValue>(wave, lane);
         wait_and_meet<kAhead>();
-        multiply_halves(c1, c0, now);
-        meet();
-    };
-
-    b.template ask<0, b_at(0, 0)>(b_base);
-    a.template ask<0, a_at(0, 0)>(a_base);
-    b.template ask<1, b_at(1, 0)>(b_base);
-    a.template ask<1, a_at(1, 0)>(a_base);
-    a.template advance<kValue>(wave, lane);
-    b.template advance<kValue>(wave, lane);
-    b.template ask<0, b_at(0, 1)>(b_base);
-    a.template ask<0, a_at(0, 1)>(a_base);
-    b.template ask<1, b_at(1, 1)>(b_base);
-    b.template advance<kValue>(wave, lane);
-    wait_and_meet<kAhead>();
-    read_columns(c0, c0, c0);
-    if (wave_row == 1) meet();
-    for (int k = 0; k < steps; k += 2) {  // (an odd number of steps gets one of zeros: a way out between the two costs registers)
-        step(c0, c1);
-        step(c1, c0);
+        read_columns(0, fb[0]);
+        if (wave >= 4) meet();
+        for (int k = 0; k < steps; k += 2) {  // (an odd number of steps gets one of zeros: a way out between the two costs registers)
+            step(c0, c1);
+            step(c1, c0);
+        }
+        if (wave < 4) meet();
+    } else {
+        // A ring of kStages steps: while a step is multiplied, the next one's fragments are read and the step kStages - 1 further on is asked for, into the place of
+        // the one before, whose fragments are in every wave's registers by the barrier.
+        constexpr int kLoads = 4, kStages = S::kStages;  // loads of a wave for a step
+        const auto ask = [&](int stage) {
+            const uint32_t to = stage * S::kStage;
+            a.template ask<0, 0>(a_base + to);
+            a.template ask<1, A::kBytes>(a_base + to);
+            b.template ask<0, 2 * A::kBytes>(b_base + to);
+            b.template ask<1, 2 * A::kBytes + B::kBytes>(b_base + to);
+            a.template advance<kValue>(wave, lane);
+            b.template advance<kValue>(wave, lane);
+        };
+        u32x4 fa[2][2][kRows][2], fb[2][2][2][2];  // [set][half][.][half step]
+        const auto read = [&](int stage, auto set) {
+            const int at = stage * S::kStage;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                read_rows(at + h * A::kBytes, fa[set][h]);
+                read_columns(at + 2 * A::kBytes + h * B::kBytes, fb[set][h]);
+            }
+        };
+        int reading = 1, asking = kStages - 1;  // stages
+        const auto step = [&](auto now, auto other) {
+            wait_and_meet<(kStages - 3) * kLoads>();
+            read(reading, other);
+            ask(asking);
+            reading = reading + 1 == kStages ? 0 : reading + 1;
+            asking = asking + 1 == kStages ? 0 : asking + 1;
+#pragma unroll
+            for (int ha = 0; ha < 2; ++ha)
+#pragma unroll
+                for (int hb = 0; hb < 2; ++hb) multiply_halves(acc[ha][hb], fa[now][ha], fb[now][hb]);
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) ask(i);
+        wait_and_meet<(kStages - 2) * kLoads>();
+        read(0, c0);
+        for (int k = 0; k < steps; k += 2) {
+            step(c0, c1);
+            if (k + 1 < steps) step(c1, c0);
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what was asked for past the end is in LDS before the workgroup gives it up)
-    if (wave_row == 0) meet();
 
     const int column = n0 + wave_column * 32 + lane / 16 * 8;
 #pragma unroll
     for (int ha = 0; ha < 2; ++ha)
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int m = m0 + ha * kHalfRows + wave_row * 16 * kRows + i * 16 + lane % 16;
+            const int m = m0 + ha * kHalf + wave_row * 16 * kRows + i * 16 + lane % 16;
             if (m >= p.m) continue;
             Sum<kType> v[2][2];
 #pragma unroll
@@ -457,7 +507,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
                 uint32_t* const row = static_cast<uint32_t*>(p.partial) + (static_cast<size_t>(place.part) * p.m + m) * wide;
 #pragma unroll
                 for (int hb = 0; hb < 2; ++hb) {
-                    const int n = kFinish == kGated ? column : column + hb * kHalfColumns;
+                    const int n = kFinish == kGated ? column : column + hb * kHalf;
                     if (n >= p.columns) continue;
                     u32x4* const to = reinterpret_cast<u32x4*>(row + (kFinish == kGated ? hb * static_cast<size_t>(p.pitch) : 0) + n);
                     to[0] = __builtin_bit_cast(u32x4, v[hb][0]);
@@ -475,7 +525,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
             } else {
 #pragma unroll
                 for (int hb = 0; hb < 2; ++hb) {
-                    const int n = column + hb * kHalfColumns;
+                    const int n = column + hb * kHalf;
                     if (n < p.columns) finish<kType, kFinish>(p.out, m, n, p.columns, wide[hb]);
                 }
             }
@@ -497,6 +547,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
 #pragma unroll
     for (int t = 0; t < kTimes; ++t) {
         Sum<kType> sum[2] = {};
+#pragma unroll 4
         for (int part = 0; part < p.parts; ++part) {
             const u32x4* const from = reinterpret_cast<const u32x4*>(static_cast<const uint32_t*>(p.partial) + (static_cast<size_t>(part) * p.m + m) * wide +
                                                                      static_cast<size_t>(t) * p.pitch + n);
@@ -520,7 +571,6 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
 // A workgroup makes 16 rows of B (kGated: 8 of gate and their 8 of up); its eight waves take every eighth line of k and their sums meet in LDS.  A's pieces come from
 // the caches.  kAhead lines of a wave are under way at any time.
 constexpr int kStreamUnits = 2;  // of 8 rows of B
-constexpr int kStreamRows = 64;  // of A, at most
 template <int kType, Finish kFinish, int kBlocks>
 __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void stream_kernel(const Product p)
 {
@@ -528,7 +578,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void stream_kernel(
     constexpr int kWide = kFinish == kGated ? 8 : 8 * kStreamUnits;  // columns of the result
     __shared__ __attribute__((aligned(16))) uint32_t sums[kWaves][kStreamUnits][kBlocks][16][8];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int n0 = blockIdx.x * kWide, k_bytes = p.k * kValue, lines = (k_bytes + kStepBytes - 1) / kStepBytes;
+    const int n0 = blockIdx.x * kWide, m0 = blockIdx.y * 16 * kBlocks, rows = min(16 * kBlocks, p.m - m0), k_bytes = p.k * kValue, lines = (k_bytes + kStepBytes - 1) / kStepBytes;
     const auto resource = [](const void* at, long long bytes) {
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, static_cast<int>(min(bytes, 0x7fffffffll)), 0x00020000);
     };
@@ -540,7 +590,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void stream_kernel(
         const long long row = static_cast<long long>(kFinish == kGated && u == 1 ? p.columns : 0) + n;
         from_b[u] = resource(static_cast<const char*>(p.b) + row * k_bytes, there <= 0 ? 0 : static_cast<long long>(there) * k_bytes);
     }
-    const __amdgpu_buffer_rsrc_t from_a = resource(p.a, static_cast<long long>(p.m) * k_bytes);
+    const __amdgpu_buffer_rsrc_t from_a = resource(static_cast<const char*>(p.a) + static_cast<long long>(m0) * k_bytes, static_cast<long long>(rows) * k_bytes);
     const int at_b = lane % 8 * k_bytes + lane / 8 * 16, at_a = lane % 16 * k_bytes + lane / 16 * 32;
     struct Line {
         u32x4 b[kStreamUnits], a[kBlocks][2];
@@ -594,7 +644,7 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void stream_kernel(
     __syncthreads();
     constexpr int kTasks = kFinish == kGated ? 16 * kBlocks : 16 * kBlocks * kStreamUnits;
     const int m = threadIdx.x % (16 * kBlocks), unit = threadIdx.x / (16 * kBlocks);
-    if (threadIdx.x >= kTasks || m >= p.m) return;
+    if (threadIdx.x >= kTasks || m >= rows) return;
     const auto total = [&](int u, float (&v)[8]) {
         Sum<kType> sum[2] = {};
 #pragma unroll
@@ -609,49 +659,63 @@ __global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void stream_kernel(
     if constexpr (kFinish == kGated) {
         float up[8];
         total(1, up);
-        finish_gated<kType>(p.out, m, n0, p.columns, v, up);
+        finish_gated<kType>(p.out, m0 + m, n0, p.columns, v, up);
     } else {
         const int n = n0 + 8 * unit;
-        if (n < p.columns) finish<kType, kFinish>(p.out, m, n, p.columns, v);
+        if (n < p.columns) finish<kType, kFinish>(p.out, m0 + m, n, p.columns, v);
     }
 }
 
-// How a product is cut up.
+// How a product is cut up: a stream of B, or tiles of 256 or 128, and k into parts whose sums another kernel adds up.
+enum Way { kStream, kSmall, kLargeTiles };
 struct Cut {
-    int rows, m_tiles, n_tiles, parts, part_steps;
+    Way way;
+    int m_tiles, n_tiles, parts, part_steps;
     size_t bytes;  // of the parts' sums
 };
-Cut cut_of(int m, int columns, int k_bytes, bool gated, bool rows_fixed)
+// The quickest by what tiles were measured to take on 256 compute units: a step of a large tile 1.5 us with all of them at work, of a small one 0.58, 5 and 4 us
+// around a tile's steps; joining parts 3.5 us and their sums at 4 bytes / ps.  A streaming workgroup, 16 rows of B and up to 64 of A, reads both at 31 bytes / ns.
+Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
 {
-    const int wide = gated ? kHalfColumns : kColumns, steps = (k_bytes + kStepBytes - 1) / kStepBytes;
-    Cut c = {4, 0, (columns + wide - 1) / wide, 1, std::max(1, steps), 0};
-    if (!rows_fixed) c.rows = m <= 64 ? 1 : m <= 128 ? 2 : 4;
-    c.m_tiles = (m + 64 * c.rows - 1) / (64 * c.rows);
-    const long long tiles = static_cast<long long>(c.m_tiles) * c.n_tiles;
-    if (tiles < 128 && steps >= 8) {
-        c.parts = static_cast<int>(std::min<long long>({256 / tiles, steps / 4, 16}));
-        c.part_steps = (steps + c.parts - 1) / c.parts;
-        c.parts = (steps + c.part_steps - 1) / c.part_steps;
+    const int steps = std::max(1, (k_bytes + kStepBytes - 1) / kStepBytes), times = gated ? 2 : 1;
+    Cut best = {};
+    double least = 0;
+    if (!turned) {
+        const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64, rows = m <= 16 ? m : m <= 32 ? 32 : 64;
+        const double rounds = static_cast<double>((static_cast<long long>(m_tiles) * n_tiles + 255) / 256);
+        best = {kStream, m_tiles, n_tiles, 1, steps, 0};
+        least = 4 + rounds * (16 + rows) * static_cast<double>(k_bytes) / 31000;
     }
-    if (c.parts > 1) c.bytes = static_cast<size_t>(c.parts) * m * ((columns + 7) / 8 * 8) * (gated ? 2 : 1) * 4;
-    return c;
+    for (const Way way : {kSmall, kLargeTiles}) {
+        const bool large = way == kLargeTiles;
+        const int tile = large ? 256 : 128, wide = tile / times;
+        const int m_tiles = (m + tile - 1) / tile, n_tiles = (columns + wide - 1) / wide;
+        for (int wanted = 1; wanted <= 16; ++wanted) {
+            const int part_steps = (steps + wanted - 1) / wanted, parts = (steps + part_steps - 1) / part_steps;
+            if (parts != wanted) continue;
+            const double rounds = static_cast<double>((static_cast<long long>(m_tiles) * n_tiles * parts + 255) / 256);
+            const size_t bytes = parts == 1 ? 0 : static_cast<size_t>(parts) * m * ((columns + 7) / 8 * 8) * times * 4;
+            const double us = rounds * (large ? 5 + 1.5 * part_steps : 4 + 0.58 * part_steps) + (parts == 1 ? 0 : 3.5 + 2e-6 * static_cast<double>(bytes) / 4);
+            if (best.parts == 0 || us < least) best = {way, m_tiles, n_tiles, parts, part_steps, bytes}, least = us;
+        }
+    }
+    return best;
 }
 
 template <int kType, bool kTransA, bool kTransB, Finish kFinish>
 int launch(Product p, void* partial, hipStream_t stream)
 {
     if (p.m == 0 || p.columns == 0) return DPEP_OK;
+    const Cut c = cut_of(p.m, p.columns, p.k * (kType == kInt8 ? 1 : 2), kFinish == kGated, kTransA || kTransB);
     if constexpr (!kTransA && !kTransB) {
-        if (p.m <= kStreamRows) {
-            constexpr int kWide = kFinish == kGated ? 8 : 8 * kStreamUnits;
-            const dim3 grid((p.columns + kWide - 1) / kWide);
+        if (c.way == kStream) {
+            const dim3 grid(c.n_tiles, c.m_tiles);
             if (p.m <= 16) stream_kernel<kType, kFinish, 1><<<grid, kThreads, 0, stream>>>(p);
             else if (p.m <= 32) stream_kernel<kType, kFinish, 2><<<grid, kThreads, 0, stream>>>(p);
             else stream_kernel<kType, kFinish, 4><<<grid, kThreads, 0, stream>>>(p);
             return launch_status("product of few rows");
         }
     }
-    const Cut c = cut_of(p.m, p.columns, p.k * (kType == kInt8 ? 1 : 2), kFinish == kGated, kTransA);
     p.m_tiles = c.m_tiles;
     p.n_tiles = c.n_tiles;
     p.parts = c.parts;
@@ -661,13 +725,8 @@ int launch(Product p, void* partial, hipStream_t stream)
     const long long groups = static_cast<long long>(c.m_tiles) * c.n_tiles * c.parts;
     DPEP_REQUIRE(groups <= 0x7fffff, "a product of %d x %d is too large", p.m, p.columns);
     const dim3 grid(static_cast<unsigned>(groups));
-    if constexpr (!kTransA) {
-        if (c.rows == 1) tile_kernel<kType, false, kTransB, kFinish, 1><<<grid, kThreads, 0, stream>>>(p);
-        else if (c.rows == 2) tile_kernel<kType, false, kTransB, kFinish, 2><<<grid, kThreads, 0, stream>>>(p);
-        else tile_kernel<kType, false, kTransB, kFinish, 4><<<grid, kThreads, 0, stream>>>(p);
-    } else {
-        tile_kernel<kType, true, kTransB, kFinish, 4><<<grid, kThreads, 0, stream>>>(p);
-    }
+    if (c.way == kLargeTiles) tile_kernel<kType, kTransA, kTransB, kFinish, true><<<grid, kThreads, 0, stream>>>(p);
+    else tile_kernel<kType, kTransA, kTransB, kFinish, false><<<grid, kThreads, 0, stream>>>(p);
     if (int rc = launch_status("product"); rc != DPEP_OK || c.parts == 1) return rc;
     const size_t pieces = static_cast<size_t>(p.m) * (p.pitch / 8);
     join_kernel<kType, kFinish><<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream>>>(p);
@@ -734,7 +793,7 @@ size_t dpep_gated_ffn_backward_scratch_bytes(int num_tokens, int hidden, int int
 {
     if (num_tokens < 0 || hidden < 0 || inter < 0) return 0;
     return whole(static_cast<size_t>(num_tokens) * inter * 2) + whole(static_cast<size_t>(num_tokens) * inter * 4) +
-           std::max(std::max(cut_of(num_tokens, inter, hidden * 2, false, false).bytes, cut_of(num_tokens, hidden, inter * 4, false, false).bytes),
+           std::max(std::max(cut_of(num_tokens, inter, hidden * 2, false, true).bytes, cut_of(num_tokens, hidden, inter * 4, false, true).bytes),
                     std::max(cut_of(2 * inter, hidden, num_tokens * 2, false, true).bytes, cut_of(hidden, inter, num_tokens * 2, false, true).bytes));
 }
 
@@ -803,6 +862,7 @@ int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int
     p.out.row_scale = x_scales;
     p.out.column_scale = w->scales;
     p.out.type = type;
+    p.out.whole = w->n % 8 == 0 && aligned16(y) && aligned16(w->scales);
     return launch<kInt8, false, false, kScaled>(p, scratch, static_cast<hipStream_t>(stream));
 }
 
