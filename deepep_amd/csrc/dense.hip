@@ -136,6 +136,7 @@ struct Product {
     Output out;
     // how it is cut up: tiles, parts of k of `part_steps` steps, their sums
     int m_tiles, n_tiles, parts, part_steps, pitch;
+    int turned_a;  // A holds m contiguously (where the kernel does not say so)
     void* partial;
 };
 
@@ -144,17 +145,15 @@ struct Product {
 // passing registers, each in two halves of rows (columns) of the tile; with kGated the halves of B are the gate and the up rows of the same
 // columns.  A wave takes 16 kRows rows and 32 columns of each half, so that a step is four products of a half of A with a half of B: (0,0), (0,1), (1,1), (1,0).
 //
-// Tiles of 256 x 256 take these one at a time ("phases").  The waves w and w + 4 share a SIMD and run half a phase apart: while one multiplies, the other reads its operands' next fragments from LDS and asks
-// for half an operand of a later step.  A phase of a wave is [read, ask, wait, barrier, multiply, barrier], and waves 4 .. 7 pass one barrier
-// more at the start, waves 0 .. 3 at the end.
-//   Which half is read: in phase 0 A0, in phase 1 B1, in phase 2 A1, in phase 3 the next step's B0 (into the registers of B1, so that the two sets of
-//   registers for B change places from step to step: the loop holds two steps).
-//   Which half is asked for: in phase 0 A1 of step k + 1, in phases 1, 2 and 3 B0, A0 and B1 of step k + 2; there are two buffers, k odd and even.  Every
-//   wait leaves the five last halves outstanding, so that a half has five phases to arrive in.
-//   Read after write: a half is read in the phase that follows the wait which covers it, the fifth after the one that asked; a barrier that all
-//   waves pass after their wait lies in between, for the later waves half a phase behind too.
-//   Write after read: a half's buffer is overwritten from the second phase after the one that read it on.  The fragments that the later waves read in
-//   phase p are in their registers before they multiply, which is before the barrier that lets the earlier waves into phase p + 2.
+// Tiles of 256 x 256 take these two at a time ("phases").  The waves w and w + 4 share a SIMD and run half a phase apart: while one multiplies, the other reads the
+// fragments of its next phase from LDS and asks for halves of later steps.  A phase of a wave is [read, ask, wait, barrier, multiply, barrier], and waves
+// 4 .. 7 pass one barrier more at the start, waves 0 .. 3 at the end.
+//   Phase 0 reads A0, B0 and B1 and asks for A1 of step k + 1, phase 1 reads A1 and asks for A0, B0 and B1 of step k + 2, into the place of step k's; there are two
+//   buffers.  A wait covers what was asked for more than two phases ago (8 loads of a wave are later), and the wave's own reads.
+//   Read after write: what a phase reads was asked for two phases before, every wave has waited for it one phase before, and a barrier that all waves pass after
+//   that lies in between.
+//   Write after read: a half is overwritten from the phase after the one that read it on, and a wave passes the barrier of its reading phase only when
+//   its fragments are in its registers.
 //
 // In LDS a row of 128 bytes of k holds its 16-byte pieces c at place c ^ key(row), so that eight lanes that read the same piece of eight rows find them in
 // different banks.  Operands that hold m or n contiguously lie in LDS as rows of k, 128 values wide, and are turned as they are read
@@ -172,10 +171,11 @@ constexpr int kThreads = 512;
 constexpr int kStepBytes = 128;
 constexpr uint32_t kNowhere = 0x80000000u;
 
+// For all loads but the last kLoads and for what was read from LDS, and for the other waves.
 template <int kLoads>
 __device__ __forceinline__ void wait_and_meet()
 {
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
 __device__ __forceinline__ void meet()
@@ -306,17 +306,16 @@ struct Shape {
 };
 
 template <int kType, bool kTransA, bool kTransB, Finish kFinish, bool kLarge>
-__global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
+__device__ __forceinline__ void make_tile(const Product& p, unsigned id, unsigned total, uint8_t* lds)
 {
     using S = Shape<kLarge>;
     constexpr int kValue = kType == kInt8 ? 1 : 2, kValues = kStepBytes / kValue;  // bytes of a value, values of a step
     constexpr int kHalf = S::kHalf, kRows = S::kRows, kWide = kFinish == kGated ? kHalf : 2 * kHalf;
     using A = Operand<kTransA, kHalf, false>;
     using B = Operand<kTransB, kHalf, true>;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kStages * S::kStage];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wave_row = wave / S::kWavesN, wave_column = wave % S::kWavesN;
-    const Place place = place_of(blockIdx.x, gridDim.x, p.m_tiles, p.n_tiles);
+    const Place place = place_of(id, total, p.m_tiles, p.n_tiles);
     const int m0 = place.m * 2 * kHalf, n0 = place.n * kWide;
     const int k0 = min(p.k, place.part * p.part_steps * kValues), k1 = min(p.k, k0 + p.part_steps * kValues);
     const int steps = (k1 - k0 + kValues - 1) / kValues;
@@ -391,52 +390,47 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
     constexpr std::integral_constant<int, 1> c1;
 
     if constexpr (kLarge) {
-        constexpr int kAhead = 10;  // the five last halves, whichever they are
         // LDS: [half of A][buffer], [half of B][buffer], so that a lane's places in both buffers are within the reach of an instruction's own offset.
         constexpr auto a_at = [](int half, int buffer) { return (2 * half + buffer) * A::kBytes; };
         constexpr auto b_at = [](int half, int buffer) { return 4 * A::kBytes + (2 * half + buffer) * B::kBytes; };
 #pragma unroll
         for (int i = 0; i < 2; ++i) read_b[i] += b_at(0, 0);
-        u32x4 fa[kRows][2], fb[2][2][2];  // [.][half step]; [set][of a pair][half step]
-        const auto multiply_phase = [&](Sum<kType> (&sum)[kRows][2], const u32x4 (&columns)[2][2]) {
+        u32x4 fa[kRows][2], fb[2][2][2];  // [.][half step]; [half][of a pair][half step]
+        const auto multiply_phase = [&](auto half, auto first, auto second) {
             __builtin_amdgcn_s_setprio(1);
-            multiply_halves(sum, fa, columns);
+            multiply_halves(acc[half][first], fa, fb[first]);
+            multiply_halves(acc[half][second], fa, fb[second]);
             __builtin_amdgcn_s_setprio(0);
             meet();
         };
-        // A step whose operands lie in buffer `now`, with its B0 in the registers `now`.
+        // A step whose operands lie in buffer `now`.
         const auto step = [&](auto now, auto other) {
+            read_columns(b_at(0, now) - b_at(0, 0), fb[0]);
             read_rows(a_at(0, now), fa);
+            read_columns(b_at(1, now) - b_at(0, 0), fb[1]);
             a.template ask<1, a_at(1, other)>(a_base);
             a.template advance<kValue>(wave, lane);
-            wait_and_meet<kAhead>();
-            multiply_phase(acc[0][0], fb[now]);
-            read_columns(b_at(1, now) - b_at(0, 0), fb[other]);
-            b.template ask<0, b_at(0, now)>(b_base);
-            wait_and_meet<kAhead>();
-            multiply_phase(acc[0][1], fb[other]);
+            wait_and_meet<8>();
+            multiply_phase(c0, c0, c1);
             read_rows(a_at(1, now), fa);
             a.template ask<0, a_at(0, now)>(a_base);
-            wait_and_meet<kAhead>();
-            multiply_phase(acc[1][1], fb[other]);
-            read_columns(b_at(0, other) - b_at(0, 0), fb[other]);
+            b.template ask<0, b_at(0, now)>(b_base);
             b.template ask<1, b_at(1, now)>(b_base);
             b.template advance<kValue>(wave, lane);
-            wait_and_meet<kAhead>();
-            multiply_phase(acc[1][0], fb[now]);
+            wait_and_meet<8>();
+            multiply_phase(c1, c1, c0);
         };
-        b.template ask<0, b_at(0, 0)>(b_base);
         a.template ask<0, a_at(0, 0)>(a_base);
+        b.template ask<0, b_at(0, 0)>(b_base);
         b.template ask<1, b_at(1, 0)>(b_base);
         a.template ask<1, a_at(1, 0)>(a_base);
         a.template advance<kValue>(wave, lane);
         b.template advance<kValue>(wave, lane);
-        b.template ask<0, b_at(0, 1)>(b_base);
         a.template ask<0, a_at(0, 1)>(a_base);
+        b.template ask<0, b_at(0, 1)>(b_base);
         b.template ask<1, b_at(1, 1)>(b_base);
         b.template advance<kValue>(wave, lane);
-        wait_and_meet<kAhead>();
-        read_columns(0, fb[0]);
+        wait_and_meet<8>();
         if (wave >= 4) meet();
         for (int k = 0; k < steps; k += 2) {  // (an odd number of steps gets one of zeros: a way out between the two costs registers)
             step(c0, c1);
@@ -530,6 +524,31 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
                 }
             }
         }
+}
+
+template <int kType, bool kTransA, bool kTransB, Finish kFinish, bool kLarge>
+__global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<kLarge>::kStages * Shape<kLarge>::kStage];
+    make_tile<kType, kTransA, kTransB, kFinish, kLarge>(p, blockIdx.x, gridDim.x, lds);
+}
+
+// Three products that do not wait for one another in one launch: workgroups of the next fill up the compute units that the last tiles of one leave idle.
+// B holds n contiguously in all of them, A m in some.
+// (What is picked out of the arguments by a computed index is whole words at whole words' distances: a byte for each product among them made
+// the compiler take addresses that are no multiples of four into scalar loads, which ignore the lowest two bits of each part of an address.)
+struct Products {
+    Product of[3];
+    unsigned begin[4];  // a product's first workgroup
+};
+template <int kType, bool kLarge>
+__global__ __launch_bounds__(kThreads, 2) void products_kernel(const Products p)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<kLarge>::kStages * Shape<kLarge>::kStage];
+    const int which = blockIdx.x < p.begin[1] ? 0 : blockIdx.x < p.begin[2] ? 1 : 2;
+    const unsigned id = blockIdx.x - p.begin[which], total = p.begin[which + 1] - p.begin[which];
+    if (p.of[which].turned_a != 0) make_tile<kType, true, true, kStore, kLarge>(p.of[which], id, total, lds);
+    else make_tile<kType, false, true, kStore, kLarge>(p.of[which], id, total, lds);
 }
 
 // The parts of k added up, and what becomes of the sums.
@@ -672,19 +691,19 @@ struct Cut {
     Way way;
     int m_tiles, n_tiles, parts, part_steps;
     size_t bytes;  // of the parts' sums
+    double us;
 };
 // The quickest by what tiles were measured to take on 256 compute units: a step of a large tile 1.5 us with all of them at work, of a small one 0.58, 5 and 4 us
 // around a tile's steps; joining parts 3.5 us and their sums at 4 bytes / ps.  A streaming workgroup, 16 rows of B and up to 64 of A, reads both at 31 bytes / ns.
+inline double tile_us(bool large, int steps) { return large ? 5 + 1.5 * steps : 4 + 0.58 * steps; }
 Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
 {
     const int steps = std::max(1, (k_bytes + kStepBytes - 1) / kStepBytes), times = gated ? 2 : 1;
     Cut best = {};
-    double least = 0;
     if (!turned) {
         const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64, rows = m <= 16 ? m : m <= 32 ? 32 : 64;
         const double rounds = static_cast<double>((static_cast<long long>(m_tiles) * n_tiles + 255) / 256);
-        best = {kStream, m_tiles, n_tiles, 1, steps, 0};
-        least = 4 + rounds * (16 + rows) * static_cast<double>(k_bytes) / 31000;
+        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 4 + rounds * (16 + rows) * static_cast<double>(k_bytes) / 31000};
     }
     for (const Way way : {kSmall, kLargeTiles}) {
         const bool large = way == kLargeTiles;
@@ -695,8 +714,8 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
             if (parts != wanted) continue;
             const double rounds = static_cast<double>((static_cast<long long>(m_tiles) * n_tiles * parts + 255) / 256);
             const size_t bytes = parts == 1 ? 0 : static_cast<size_t>(parts) * m * ((columns + 7) / 8 * 8) * times * 4;
-            const double us = rounds * (large ? 5 + 1.5 * part_steps : 4 + 0.58 * part_steps) + (parts == 1 ? 0 : 3.5 + 2e-6 * static_cast<double>(bytes) / 4);
-            if (best.parts == 0 || us < least) best = {way, m_tiles, n_tiles, parts, part_steps, bytes}, least = us;
+            const double us = rounds * tile_us(large, part_steps) + (parts == 1 ? 0 : 3.5 + 2e-6 * static_cast<double>(bytes) / 4);
+            if (best.parts == 0 || us < best.us) best = {way, m_tiles, n_tiles, parts, part_steps, bytes, us};
         }
     }
     return best;
@@ -731,6 +750,52 @@ int launch(Product p, void* partial, hipStream_t stream)
     const size_t pieces = static_cast<size_t>(p.m) * (p.pitch / 8);
     join_kernel<kType, kFinish><<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream>>>(p);
     return launch_status("product's parts");
+}
+
+// Three products (of 16-bit values, results stored, no part of another's operands), together if that is quicker than one after the other.
+template <int kType>
+int launch_three(Product (&products)[3], void* partial, hipStream_t stream)
+{
+    double apart = 0;
+    for (const Product& p : products) apart += cut_of(p.m, p.columns, p.k * 2, false, true).us;
+    std::sort(products, products + 3, [](const Product& a, const Product& b) { return a.k > b.k; });  // (long tiles first, short ones fill up)
+    Products best = {};
+    double least = apart;
+    bool best_large = false;
+    for (int large = 0; large < 2; ++large) {
+        const int tile = large ? 256 : 128;
+        Products now = {};
+        double work = 0, longest = 0;
+        long long begin = 0;
+        for (int i = 0; i < 3; ++i) {
+            Product p = products[i];
+            p.m_tiles = (p.m + tile - 1) / tile;
+            p.n_tiles = (p.columns + tile - 1) / tile;
+            p.parts = 1;
+            p.part_steps = std::max(1, (p.k * 2 + kStepBytes - 1) / kStepBytes);
+            const double us = tile_us(large != 0, p.part_steps);
+            const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+            work += static_cast<double>(tiles) * us;
+            longest = std::max(longest, us);
+            now.of[i] = p;
+            now.begin[i] = static_cast<unsigned>(begin);
+            begin += tiles;
+        }
+        now.begin[3] = static_cast<unsigned>(begin);
+        // the last tiles, short ones, end half of their time apart
+        const double us = std::max(longest, work / 256 + tile_us(large != 0, now.of[2].part_steps) / 2);
+        if (begin <= 0x7fffff && us < least) best = now, least = us, best_large = large != 0;
+    }
+    if (best.begin[3] != 0) {
+        if (best_large) products_kernel<kType, true><<<best.begin[3], kThreads, 0, stream>>>(best);
+        else products_kernel<kType, false><<<best.begin[3], kThreads, 0, stream>>>(best);
+        return launch_status("products");
+    }
+    for (const Product& p : products) {
+        const int rc = p.turned_a != 0 ? launch<kType, true, true, kStore>(p, partial, stream) : launch<kType, false, true, kStore>(p, partial, stream);
+        if (rc != DPEP_OK) return rc;
+    }
+    return DPEP_OK;
 }
 
 int check_ffn(const dpep_ffn* f, const char* what, int tokens)
@@ -824,15 +889,14 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
         p.out.kept = const_cast<float*>(kept);
         p.out.h = h;
         if (int rc = launch<kType, false, true, kGradient>(p, partial, s); rc != DPEP_OK) return rc;
-        p = {dz, f->gate_up, num_tokens, f->hidden, 2 * f->inter, {}};
-        p.out.c = grad_x;
-        if (int rc = launch<kType, false, true, kStore>(p, partial, s); rc != DPEP_OK) return rc;
-        p = {dz, x, 2 * f->inter, f->hidden, num_tokens, {}};
-        p.out.c = grad_gate_up;
-        if (int rc = launch<kType, true, true, kStore>(p, partial, s); rc != DPEP_OK) return rc;
-        p = {grad_y, h, f->hidden, f->inter, num_tokens, {}};
-        p.out.c = grad_down;
-        return launch<kType, true, true, kStore>(p, partial, s);
+        Product products[3] = {{dz, f->gate_up, num_tokens, f->hidden, 2 * f->inter, {}},
+                               {dz, x, 2 * f->inter, f->hidden, num_tokens, {}},
+                               {grad_y, h, f->hidden, f->inter, num_tokens, {}}};
+        products[0].out.c = grad_x;
+        products[1].out.c = grad_gate_up;
+        products[2].out.c = grad_down;
+        products[1].turned_a = products[2].turned_a = 1;
+        return launch_three<kType>(products, partial, s);
     });
 }
 

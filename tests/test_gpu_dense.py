@@ -70,6 +70,22 @@ def test_backward(tokens, hidden, inter, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("tokens,hidden,inter", [(4096, 1024, 1032), (2100, 2056, 1536)])
+def test_many_tokens(tokens, hidden, inter):
+    """Sizes at which the products take their largest tiles, and the three of the backward pass a launch together."""
+    from deepep_amd import dense
+
+    x, gate_up, down, grad_y = _make(tokens, hidden, inter, "bf16")
+    y, kept = dense.gated_ffn(x, gate_up, down, keep=True)
+    want = od.ffn(*_wide(x, gate_up, down), "bf16")
+    _check(y, want["y"], want["y_off"])
+    got = dense.gated_ffn_backward(grad_y, x, gate_up, down, kept)
+    for grad, (value, bound) in zip(got, od.ffn_backward(*_wide(grad_y, x, gate_up, down), "bf16")):
+        _check(grad, value, bound)
+    for a, b in zip(got, dense.gated_ffn_backward(grad_y, x, gate_up, down, kept)):
+        assert torch.equal(a, b)
+
+
 def test_gradients_match_differences():
     """The change of a loss along a direction, from the block itself in half precision, against its gradients: to 2 %, what two outputs rounded to 2^-11 leave of a
     difference of a tenth of them."""
