@@ -75,19 +75,42 @@ __device__ __forceinline__ void load_weight(const void* weight, bool wide, int a
     else widen<kType>(load_raw<kType>(weight, at), w);
 }
 
-// Sum and maximum over the wave, in a fixed order; the result is in every lane.
+// Sum and maximum over lanes in a fixed order, by moves between the lanes' registers (an LDS permute a step costs 50 ns and more).
+template <int kMove, int kRowMask = 0xf>
+__device__ __forceinline__ uint32_t moved(uint32_t v)
+{
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kMove, kRowMask, 0xf, false));
+}
+template <int kMove, int kRowMask = 0xf>
+__device__ __forceinline__ float add_moved(float v)
+{
+    return v + __uint_as_float(moved<kMove, kRowMask>(__float_as_uint(v)));
+}
+// Of the wave; in every lane.
 __device__ __forceinline__ float wave_sum(float v)
 {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    v = add_moved<0x111>(v);  // row_shr:1, 2, 4, 8
+    v = add_moved<0x112>(v);
+    v = add_moved<0x114>(v);
+    v = add_moved<0x118>(v);
+    v = add_moved<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v = add_moved<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), 63)));
 }
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes)
+// Of 4, 16 or 64 lanes next to one another; in each of them.
+template <int kLanes>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1)
-        if (d < lanes) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d)));
-    return v;
+    static_assert(kLanes == 4 || kLanes == 16 || kLanes == 64);
+    v = max(v, moved<0xb1>(v));  // quad_perm:[1,0,3,2], [2,3,0,1]
+    v = max(v, moved<0x4e>(v));
+    if constexpr (kLanes == 4) return v;
+    v = max(v, moved<0x124>(v));  // row_ror:4, 8
+    v = max(v, moved<0x128>(v));
+    if constexpr (kLanes == 16) return v;
+    v = max(v, moved<0x142, 0xa>(v));
+    v = max(v, moved<0x143, 0xc>(v));
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 // The same over a workgroup.  `shared`: a word for each wave; the caller keeps two uses of it apart.
 template <int kThreads>
@@ -106,7 +129,7 @@ __device__ __forceinline__ float block_sum(float v, float* shared)
 template <int kThreads>
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* shared)
 {
-    v = lanes_max(v, kWave);
+    v = lanes_max<kWave>(v);
     if constexpr (kThreads > kWave) {
         if (threadIdx.x % kWave == 0) shared[threadIdx.x / kWave] = v;
         __syncthreads();
@@ -202,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const dpep_norm p)
         if (live && p.y != nullptr) store_raw<kType>(p.y, row + at, narrow<kType>(v[c]));
         if (p.quantize == DPEP_QUANT_FP8) {
             if (c * kThreads * kVec >= hidden) continue;  // (the same for all lanes)
-            const uint32_t block = lanes_max(live ? magnitude(v[c]) : 0u, 16);
+            const uint32_t block = lanes_max<16>(live ? magnitude(v[c]) : 0u);
             const float m = __uint_as_float(max(block, __float_as_uint(1e-4f)));
             const float inverse = (1.0f / m) * 448.0f;
             if (!live) continue;
@@ -214,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const dpep_norm p)
             if (at % 128 == 0) static_cast<float*>(p.scales)[static_cast<size_t>(blockIdx.x) * ((hidden + 127) / 128) + at / 128] = m / 448.0f;
         } else if (p.quantize == DPEP_QUANT_MXFP8) {
             if (c * kThreads * kVec >= hidden) continue;
-            const int byte = mx_scale_byte(__uint_as_float(lanes_max(live ? magnitude(v[c]) : 0u, 4)));
+            const int byte = mx_scale_byte(__uint_as_float(lanes_max<4>(live ? magnitude(v[c]) : 0u)));
             if (!live) continue;
             u32x2 codes;
 #pragma unroll
@@ -258,56 +281,71 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* x, int
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------------
-// A workgroup takes rows blockIdx.x, + gridDim.x, ...; its share of grad_weight stays in registers and leaves as one row of `partial`.
+// A workgroup takes rows blockIdx.x, + gridDim.x, ...; the weight and its share of grad_weight stay in registers, and the next row is under way while
+// one is worked on (without that a row's loads, its sum over the workgroup and its stores follow one another).  The share leaves as one row of
+// `partial`.
 template <int kThreads, int kChunks, int kType>
 __global__ __launch_bounds__(kThreads) void norm_backward_kernel(const dpep_norm_gradients p, float* partial)
 {
     __shared__ float sums[2][kThreads / kWave];
     const int tid = threadIdx.x, hidden = p.hidden;
-    float gw[kChunks][kVec] = {};
-    int turn = 0;
-    for (int t = blockIdx.x; t < p.num_tokens; t += gridDim.x, turn ^= 1) {
-        const size_t row = static_cast<size_t>(t) * hidden;
-        const float rstd = p.rstd[t];
+    struct Row {
         Raw<kType> g[kChunks], s[kChunks], more[kChunks];
+        float rstd;
+    };
+    const auto load = [&](int t) {
+        Row r;
+        const size_t row = static_cast<size_t>(t) * hidden;
+        r.rstd = p.rstd[t];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
             const int at = (c * kThreads + tid) * kVec;
             if (at >= hidden) continue;
-            g[c] = load_raw<kType>(p.grad_y, row + at);
-            s[c] = load_raw<kType>(p.stream, row + at);
-            if (p.grad_stream != nullptr) more[c] = load_raw<kType>(p.grad_stream, row + at);
+            r.g[c] = load_raw<kType>(p.grad_y, row + at);
+            r.s[c] = load_raw<kType>(p.stream, row + at);
+            if (p.grad_stream != nullptr) r.more[c] = load_raw<kType>(p.grad_stream, row + at);
         }
+        return r;
+    };
+    Row next = load(blockIdx.x);  // (there are no more workgroups than rows)
+    float gw[kChunks][kVec] = {}, w[kChunks][kVec];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int at = (c * kThreads + tid) * kVec;
+        if (at < hidden) load_weight<kType>(p.weight, p.weight_type == DPEP_TYPE_F32, at, w[c]);
+    }
+    int turn = 0;
+    for (int t = blockIdx.x; t < p.num_tokens; t += gridDim.x, turn ^= 1) {
+        const Row now = next;
+        if (t < p.num_tokens - static_cast<int>(gridDim.x)) next = load(t + gridDim.x);
         float sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-            const int at = (c * kThreads + tid) * kVec;
-            if (at >= hidden) continue;
-            float w[kVec], gv[kVec], sv[kVec];
-            load_weight<kType>(p.weight, p.weight_type == DPEP_TYPE_F32, at, w);
-            widen<kType>(g[c], gv);
-            widen<kType>(s[c], sv);
+            if ((c * kThreads + tid) * kVec >= hidden) continue;
+            float gv[kVec], sv[kVec];
+            widen<kType>(now.g[c], gv);
+            widen<kType>(now.s[c], sv);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                const float hat = sv[i] * rstd, gh = gv[i] * hat;
+                const float hat = sv[i] * now.rstd, gh = gv[i] * hat;
                 gw[c][i] += gh;
-                sum += gh * w[i];
+                sum += gh * w[c][i];
             }
         }
         const float mean = block_sum<kThreads>(sum, sums[turn]) / static_cast<float>(hidden);
+        const size_t row = static_cast<size_t>(t) * hidden;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
             const int at = (c * kThreads + tid) * kVec;
             if (at >= hidden) continue;
-            float w[kVec], gv[kVec], sv[kVec], out[kVec];
-            load_weight<kType>(p.weight, p.weight_type == DPEP_TYPE_F32, at, w);
-            widen<kType>(g[c], gv);
-            widen<kType>(s[c], sv);
+            float gv[kVec], sv[kVec], out[kVec];
+            widen<kType>(now.g[c], gv);
+            widen<kType>(now.s[c], sv);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) out[i] = rstd * (gv[i] * w[i] - sv[i] * rstd * mean);
+            for (int i = 0; i < kVec; ++i) out[i] = now.rstd * (gv[i] * w[c][i] - sv[i] * now.rstd * mean);
             if (p.grad_stream != nullptr) {
                 float mv[kVec];
-                widen<kType>(more[c], mv);
+                widen<kType>(now.more[c], mv);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) out[i] += mv[i];
             }
@@ -321,33 +359,44 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(const dpep_norm
     }
 }
 
-// Columns of `partial` [rows,H] added up, 64 columns a workgroup of 16 waves.
+// Columns of `partial` [rows,H] added up, 64 columns a workgroup: 64 rows at a time, four columns a lane.
 __global__ __launch_bounds__(1024) void sum_partial_kernel(const float* partial, int rows, int hidden, float* out)
 {
-    __shared__ float part[16][kWave];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, column = blockIdx.x * kWave + lane;
-    float sum = 0.0f;
-    if (column < hidden) {
+    __shared__ __attribute__((aligned(16))) float part[64][64];
+    const int first = threadIdx.x / 16, at = threadIdx.x % 16 * 4, column = blockIdx.x * 64 + at;
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (column < hidden) {  // (H is a multiple of 8)
 #pragma unroll 8
-        for (int r = wave; r < rows; r += 16) sum += partial[static_cast<size_t>(r) * hidden + column];
+        for (int r = first; r < rows; r += 64) sum += *reinterpret_cast<const f32x4*>(partial + static_cast<size_t>(r) * hidden + column);
     }
-    part[wave][lane] = sum;
+    *reinterpret_cast<f32x4*>(&part[first][at]) = sum;
     __syncthreads();
-    if (wave != 0 || column >= hidden) return;
-    sum = 0.0f;
+    // 16 threads a column, four rows each, then the 16 of them in turn.
+    const int mine = threadIdx.x / 16, group = threadIdx.x % 16;
+    float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) sum += part[w][lane];
-    out[column] = sum;
+    for (int i = 0; i < 4; ++i) v += part[group * 4 + i][mine];
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    if (group == 0 && blockIdx.x * 64 + mine < hidden) out[blockIdx.x * 64 + mine] = v;
 }
 
-constexpr int kBackwardGroups = 512;
+// Workgroups of the backward, one to a compute unit: each row of `partial` is written and read again (16384 rows of 7168, both directions: 342 us with 256,
+// 354 with 512; 777 of 2880: 16.6 and 19.1).
+constexpr int kBackwardGroups = 256;
 inline int backward_groups(int tokens) { return std::min(tokens, kBackwardGroups); }
 
-// The kernel for a row of `hidden` values: f(threads, chunks).
+// The kernel for rows of `hidden` values: f(threads, chunks).  Few rows leave the machine empty and each is as quick as its longest thread; of many, four
+// pieces a thread keep more loads under way.
 template <class F>
-void by_hidden(int hidden, F f)
+void by_hidden(int tokens, int hidden, F f)
 {
-    if (hidden <= 64 * kVec) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    if (tokens <= 256 && hidden > 256 * kVec) {
+        if (hidden <= 512 * kVec) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 1>{});
+        else if (hidden <= 1024 * kVec) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 1>{});
+        else f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+    } else if (hidden <= 64 * kVec) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
     else if (hidden <= 256 * kVec) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
     else if (hidden <= 512 * kVec) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
     else if (hidden <= 1024 * kVec) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
@@ -405,7 +454,7 @@ int dpep_rms_norm(const dpep_norm* n, void* stream)
                      !overlap(n->stream_out, rows, n->weight, of_weight),
                  "rms_norm: stream_out overlaps an input");
     by_type(n->type, [&](auto type) {
-        by_hidden(n->hidden, [&](auto threads, auto chunks) {
+        by_hidden(n->num_tokens, n->hidden, [&](auto threads, auto chunks) {
             norm_kernel<decltype(threads)::value, decltype(chunks)::value, decltype(type)::value>
                 <<<n->num_tokens, decltype(threads)::value, 0, static_cast<hipStream_t>(stream)>>>(*n);
         });
@@ -437,14 +486,18 @@ int dpep_rms_norm_backward(const dpep_norm_gradients* g, void* scratch, void* st
                          !overlap(g->grad_weight, g->hidden * 4ull, scratch, groups * (g->hidden * 4ull)),
                      "rms_norm_backward: grad_x overlaps an input");
         by_type(g->type, [&](auto type) {
-            by_hidden(g->hidden, [&](auto threads, auto chunks) {
-                norm_backward_kernel<decltype(threads)::value, decltype(chunks)::value, decltype(type)::value>
-                    <<<groups, decltype(threads)::value, 0, s>>>(*g, static_cast<float*>(scratch));
-            });
+            constexpr int kType = decltype(type)::value;
+            float* const partial = static_cast<float*>(scratch);
+            const int hidden = g->hidden;
+            if (hidden <= 64 * kVec) norm_backward_kernel<64, 1, kType><<<groups, 64, 0, s>>>(*g, partial);
+            else if (hidden <= 256 * kVec) norm_backward_kernel<256, 1, kType><<<groups, 256, 0, s>>>(*g, partial);
+            else if (hidden <= 512 * kVec) norm_backward_kernel<512, 1, kType><<<groups, 512, 0, s>>>(*g, partial);
+            else if (hidden <= 1024 * kVec) norm_backward_kernel<512, 2, kType><<<groups, 512, 0, s>>>(*g, partial);
+            else norm_backward_kernel<1024, 2, kType><<<groups, 1024, 0, s>>>(*g, partial);
         });
         if (int rc = launch_status("rms_norm_backward"); rc != DPEP_OK) return rc;
     }
-    sum_partial_kernel<<<(g->hidden + kWave - 1) / kWave, 1024, 0, s>>>(static_cast<const float*>(scratch), groups, g->hidden, g->grad_weight);
+    sum_partial_kernel<<<(g->hidden + 63) / 64, 1024, 0, s>>>(static_cast<const float*>(scratch), groups, g->hidden, g->grad_weight);
     return launch_status("rms_norm_backward");
 }
 

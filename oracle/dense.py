@@ -30,8 +30,8 @@ def norm_backward(g, s, weight, eps, grad_stream=None):
     if grad_stream is not None:
         grad, size = grad + grad_stream, size + np.abs(grad_stream)
     each = np.abs(g * hat).sum(axis=0)
-    # (a column is summed over the rows of a workgroup, then 32 times 16 workgroups)
-    return grad, 4 * NORM_SLACK * size, (g * hat).sum(axis=0), (NORM_SLACK + (len(s) / 512 + 64) * EPS32) * each
+    # (a column is summed over the rows of a workgroup, one of up to 256, then over those)
+    return grad, 4 * NORM_SLACK * size, (g * hat).sum(axis=0), (NORM_SLACK + (len(s) / 256 + 64) * EPS32) * each
 
 
 def fp8_blocks(v):
