@@ -462,14 +462,28 @@ __device__ __forceinline__ void make_tile(const Product& p, unsigned id, unsigne
         int reading = 1, asking = kStages - 1;  // stages
         const auto step = [&](auto now, auto other) {
             wait_and_meet<(kStages - 3) * kLoads>();
-            read(reading, other);
-            ask(asking);
+            const int at = reading * S::kStage;
+            const uint32_t to = asking * S::kStage;
+            read_rows(at, fa[other][0]);
+            multiply_halves(acc[0][0], fa[now][0], fb[now][0]);
+            a.template ask<0, 0>(a_base + to);
+            __builtin_amdgcn_sched_barrier(0);
+            read_columns(at + 2 * A::kBytes, fb[other][0]);
+            multiply_halves(acc[0][1], fa[now][0], fb[now][1]);
+            b.template ask<0, 2 * A::kBytes>(b_base + to);
+            __builtin_amdgcn_sched_barrier(0);
+            read_columns(at + 2 * A::kBytes + B::kBytes, fb[other][1]);
+            multiply_halves(acc[1][1], fa[now][1], fb[now][1]);
+            b.template ask<1, 2 * A::kBytes + B::kBytes>(b_base + to);
+            __builtin_amdgcn_sched_barrier(0);
+            read_rows(at + A::kBytes, fa[other][1]);
             reading = reading + 1 == kStages ? 0 : reading + 1;
             asking = asking + 1 == kStages ? 0 : asking + 1;
-#pragma unroll
-            for (int ha = 0; ha < 2; ++ha)
-#pragma unroll
-                for (int hb = 0; hb < 2; ++hb) multiply_halves(acc[ha][hb], fa[now][ha], fb[now][hb]);
+            multiply_halves(acc[1][0], fa[now][1], fb[now][0]);
+            a.template ask<1, A::kBytes>(a_base + to);
+            a.template advance<kValue>(wave, lane);
+            b.template advance<kValue>(wave, lane);
+            __builtin_amdgcn_sched_barrier(0);
         };
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) ask(i);
@@ -581,106 +595,106 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
 }
 
 // ---- few rows: a stream of B ------------------------------------------------------------------------------------------------------
-// For up to 16 kBlocks rows of A the time is that of reading B, which goes from memory straight to registers, whole 128-byte lines: a load of a wave
-// covers a line of 8 rows of B, lane l piece l / 8 of row l % 8.  For the matrix instruction lanes l and l + 8 hold the same row's
-// pieces 2 g and 2 g + 1 (g = l / 16) in the place of two rows: multiplied by A's pieces 2 g its results 0 .. 7 are what the even pieces add to the eight
-// rows, by A's pieces 2 g + 1 results 8 .. 15 what the odd ones do, and the other halves are not looked at.  Twice the instructions, of which there is
-// no shortage here, instead of moving lines between lanes.
-//
-// A workgroup makes 16 rows of B (kGated: 8 of gate and their 8 of up); its eight waves take every eighth line of k and their sums meet in LDS.  A's pieces come from
-// the caches.  kAhead lines of a wave are under way at any time.
-constexpr int kStreamUnits = 2;  // of 8 rows of B
-template <int kType, Finish kFinish, int kBlocks>
-__global__ __launch_bounds__(kThreads, kBlocks == 1 ? 4 : 2) void stream_kernel(const Product p)
+// For few rows of A the time is that of reading B.  A workgroup makes 16 columns (kGated: 8 of gate and the same 8 of up) for up to 16 kBlocks rows; its eight waves take
+// every eighth line of 128 bytes of k, and their sums meet in LDS at the end.  Each wave has a ring of its own in LDS, into which its lines of B and A
+// go straight from memory, 8 rows of whole lines a load, and waits for nobody else on the way.  (Read to registers in the matrix instruction's own order a load of
+// A touches 64 lines instead of 8: 64 rows of 7168, 4096 columns took 37 us by that.)
+template <int kType, Finish kFinish, int kBlocks, int kStages>
+__global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
 {
-    constexpr int kValue = kType == kInt8 ? 1 : 2, kWaves = kThreads / kWave, kAhead = kBlocks == 1 ? 4 : 3;
-    constexpr int kWide = kFinish == kGated ? 8 : 8 * kStreamUnits;  // columns of the result
-    __shared__ __attribute__((aligned(16))) uint32_t sums[kWaves][kStreamUnits][kBlocks][16][8];
+    constexpr int kValue = kType == kInt8 ? 1 : 2, kWaves = kThreads / kWave;
+    constexpr int kLoads = 2 + 2 * kBlocks, kStage = kLoads * 1024;  // of a wave for a line
+    constexpr int kWide = kFinish == kGated ? 8 : 16;                // columns of the result
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves * kStages * kStage];
+    static_assert(sizeof(lds) >= kWaves * kBlocks * 1024);
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int n0 = blockIdx.x * kWide, m0 = blockIdx.y * 16 * kBlocks, rows = min(16 * kBlocks, p.m - m0), k_bytes = p.k * kValue, lines = (k_bytes + kStepBytes - 1) / kStepBytes;
-    const auto resource = [](const void* at, long long bytes) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, static_cast<int>(min(bytes, 0x7fffffffll)), 0x00020000);
-    };
-    // (8 rows of B and 64 of A are less than 2^31 bytes)
-    __amdgpu_buffer_rsrc_t from_b[kStreamUnits];
+    const int n0 = blockIdx.x * kWide, m0 = blockIdx.y * 16 * kBlocks, rows = min(16 * kBlocks, p.m - m0);
+    const int k_bytes = p.k * kValue, lines = (k_bytes + kStepBytes - 1) / kStepBytes;
+    // 8 rows a load; what lies behind a load's last row is read as zero.  (8 rows are less than 2^31 bytes.)
+    uint64_t base[kLoads];
+    int records[kLoads];
 #pragma unroll
-    for (int u = 0; u < kStreamUnits; ++u) {
-        const int n = n0 + (kFinish == kGated ? 0 : 8 * u), there = min(8, p.columns - n);
-        const long long row = static_cast<long long>(kFinish == kGated && u == 1 ? p.columns : 0) + n;
-        from_b[u] = resource(static_cast<const char*>(p.b) + row * k_bytes, there <= 0 ? 0 : static_cast<long long>(there) * k_bytes);
+    for (int j = 0; j < kLoads; ++j) {
+        const int n = n0 + (kFinish == kGated ? 0 : 8 * j), row = j < 2 ? (kFinish == kGated && j == 1 ? p.columns : 0) + n : m0 + (j - 2) * 8;
+        const int there = min(8, j < 2 ? p.columns - n : rows - (j - 2) * 8);
+        base[j] = reinterpret_cast<uint64_t>(j < 2 ? p.b : p.a) + static_cast<uint64_t>(row) * k_bytes;
+        records[j] = __builtin_amdgcn_readfirstlane(max(there, 0)) * k_bytes;  // (a number between two bounds comes from a vector instruction)
     }
-    const __amdgpu_buffer_rsrc_t from_a = resource(static_cast<const char*>(p.a) + static_cast<long long>(m0) * k_bytes, static_cast<long long>(rows) * k_bytes);
-    const int at_b = lane % 8 * k_bytes + lane / 8 * 16, at_a = lane % 16 * k_bytes + lane / 16 * 32;
-    struct Line {
-        u32x4 b[kStreamUnits], a[kBlocks][2];
-    };
-    const auto load = [&](int line) {
-        Line l;
-        const int k = line * kStepBytes;
-        const bool live_b = k + lane / 8 * 16 < k_bytes;
-#pragma unroll
-        for (int u = 0; u < kStreamUnits; ++u)
-            l.b[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from_b[u], live_b ? static_cast<uint32_t>(at_b + k) : kNowhere, 0, 2));
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-            for (int odd = 0; odd < 2; ++odd) {
-                const bool live_a = k + lane / 16 * 32 + odd * 16 < k_bytes;
-                l.a[i][odd] = __builtin_bit_cast(
-                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(from_a, live_a ? static_cast<uint32_t>(at_a + i * 16 * k_bytes + k + odd * 16) : kNowhere, 0, 0));
-            }
-        return l;
-    };
-    Line ahead[kAhead];
-#pragma unroll
-    for (int d = 0; d < kAhead; ++d) ahead[d] = load(wave + d * kWaves);
-    Sum<kType> acc[kStreamUnits][kBlocks][2] = {};
-    for (int line = wave; line < lines; line += kAhead * kWaves)
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d) {
-            const Line now = ahead[d];
-            ahead[d] = load(line + (d + kAhead) * kWaves);
-#pragma unroll
-            for (int u = 0; u < kStreamUnits; ++u)
-#pragma unroll
-                for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-                    for (int odd = 0; odd < 2; ++odd) acc[u][i][odd] = multiply<kType>(now.b[u], now.a[i][odd], acc[u][i][odd]);
+    // Lane l loads a piece of row l / 8, which lies in LDS where the pieces of eight rows that are read together meet no bank twice.
+    const int piece = lane % 8 ^ lane / 8;
+    uint32_t at = wave * kStepBytes + piece * 16;  // in k, bytes
+    const uint32_t row_at = lane / 8 * k_bytes;
+    const uint32_t mine = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + wave * kStages * kStage;
+    const auto from = [&](int j) { return rsrc{static_cast<int>(base[j]), static_cast<int>(base[j] >> 32), records[j], 0x00020000}; };
+    const auto ask = [&](int stage) {
+        const uint32_t place = at < static_cast<uint32_t>(k_bytes) ? row_at + at : kNowhere, to = mine + stage * kStage;
+        load_to_lds<0>(from(0), place, to);
+        load_to_lds<1024>(from(1), place, to);
+        load_to_lds<2048>(from(2), place, to);
+        load_to_lds<3072>(from(3), place, to);
+        if constexpr (kBlocks >= 2) {
+            load_to_lds<4096>(from(4), place, to);
+            load_to_lds<5120>(from(5), place, to);
         }
-    // Lane (g, r) has results 4 g .. 4 g + 3 of row r of A: the even pieces' in groups 0 and 1, the odd ones' in groups 2 and 3.
-#pragma unroll
-    for (int u = 0; u < kStreamUnits; ++u)
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-            Sum<kType> v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const auto odd = __shfl(acc[u][i][1][e], lane % 32 + 32);
-                v[e] = acc[u][i][0][e] + odd;
-            }
-            if (lane < 32) *reinterpret_cast<u32x4*>(&sums[wave][u][i][lane % 16][lane / 16 * 4]) = __builtin_bit_cast(u32x4, v);
+        if constexpr (kBlocks >= 4) {
+            load_to_lds<6144>(from(6), place, to);
+            load_to_lds<7168>(from(7), place, to);
+            load_to_lds<8192>(from(8), place, to);
+            load_to_lds<9216>(from(9), place, to);
         }
+        at += kWaves * kStepBytes;
+    };
+    int read_at[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) read_at[s] = wave * kStages * kStage + lane % 16 * kStepBytes + ((4 * s + lane / 16) ^ (lane & 7)) * 16;
+    Sum<kType> acc[kBlocks] = {};
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) ask(i);
+    int stage = 0;
+    for (int line = wave; line < lines; line += kWaves) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
+        u32x4 b[2], a[kBlocks][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            b[s] = *reinterpret_cast<const u32x4*>(lds + read_at[s] + stage * kStage);
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) a[i][s] = *reinterpret_cast<const u32x4*>(lds + read_at[s] + stage * kStage + 2048 * (i + 1));
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the stage is read, and may be asked for again)
+        __builtin_amdgcn_sched_barrier(0);
+        ask(stage);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) acc[i] = multiply<kType>(b[s], a[i][s], acc[i]);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    constexpr int kTasks = kFinish == kGated ? 16 * kBlocks : 16 * kBlocks * kStreamUnits;
-    const int m = threadIdx.x % (16 * kBlocks), unit = threadIdx.x / (16 * kBlocks);
-    if (threadIdx.x >= kTasks || m >= rows) return;
-    const auto total = [&](int u, float (&v)[8]) {
+    // Lane (g, r) has results 4 g .. 4 g + 3 of row r: sums[wave][block][row][16].
+    uint32_t(*const sums)[kBlocks][16][16] = reinterpret_cast<uint32_t(*)[kBlocks][16][16]>(lds);
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) *reinterpret_cast<u32x4*>(&sums[wave][i][lane % 16][lane / 16 * 4]) = __builtin_bit_cast(u32x4, acc[i]);
+    __syncthreads();
+    const int m = threadIdx.x % (16 * kBlocks), octet = threadIdx.x / (16 * kBlocks);
+    if (octet >= (kFinish == kGated ? 1 : 2) || m >= rows) return;
+    const auto total = [&](int o, float (&v)[8]) {
         Sum<kType> sum[2] = {};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) sum[h] += __builtin_bit_cast(Sum<kType>, *reinterpret_cast<const u32x4*>(&sums[w][u][m / 16][m % 16][4 * h]));
+            for (int h = 0; h < 2; ++h) sum[h] += __builtin_bit_cast(Sum<kType>, *reinterpret_cast<const u32x4*>(&sums[w][m / 16][m % 16][8 * o + 4 * h]));
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(sum[e / 4][e % 4]);
     };
     float v[8];
-    total(unit, v);
+    total(octet, v);
     if constexpr (kFinish == kGated) {
         float up[8];
         total(1, up);
         finish_gated<kType>(p.out, m0 + m, n0, p.columns, v, up);
     } else {
-        const int n = n0 + 8 * unit;
+        const int n = n0 + 8 * octet;
         if (n < p.columns) finish<kType, kFinish>(p.out, m0 + m, n, p.columns, v);
     }
 }
@@ -694,16 +708,17 @@ struct Cut {
     double us;
 };
 // The quickest by what tiles were measured to take on 256 compute units: a step of a large tile 1.5 us with all of them at work, of a small one 0.58, 5 and 4 us
-// around a tile's steps; joining parts 3.5 us and their sums at 4 bytes / ps.  A streaming workgroup, 16 rows of B and up to 64 of A, reads both at 31 bytes / ns.
+// around a tile's steps; joining parts 3.5 us and their sums at 4 bytes / ps.  A stream takes 3 us,
+// what its workgroups read of B and of up to 64 rows of A, in rounds of 256, at 62 bytes / ns, and 0.4 of the time of reading B from memory.
 inline double tile_us(bool large, int steps) { return large ? 5 + 1.5 * steps : 4 + 0.58 * steps; }
 Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
 {
     const int steps = std::max(1, (k_bytes + kStepBytes - 1) / kStepBytes), times = gated ? 2 : 1;
     Cut best = {};
     if (!turned) {
-        const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64, rows = m <= 16 ? m : m <= 32 ? 32 : 64;
-        const double rounds = static_cast<double>((static_cast<long long>(m_tiles) * n_tiles + 255) / 256);
-        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 4 + rounds * (16 + rows) * static_cast<double>(k_bytes) / 31000};
+        const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64;
+        const double rounds = std::max(1.0, static_cast<double>(n_tiles) * m_tiles / 256), read = static_cast<double>(16 + std::min(m, 64)) * k_bytes;
+        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 3 + rounds * read / 62e3 + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
     }
     for (const Way way : {kSmall, kLargeTiles}) {
         const bool large = way == kLargeTiles;
@@ -729,9 +744,11 @@ int launch(Product p, void* partial, hipStream_t stream)
     if constexpr (!kTransA && !kTransB) {
         if (c.way == kStream) {
             const dim3 grid(c.n_tiles, c.m_tiles);
-            if (p.m <= 16) stream_kernel<kType, kFinish, 1><<<grid, kThreads, 0, stream>>>(p);
-            else if (p.m <= 32) stream_kernel<kType, kFinish, 2><<<grid, kThreads, 0, stream>>>(p);
-            else stream_kernel<kType, kFinish, 4><<<grid, kThreads, 0, stream>>>(p);
+            // (rings of two stages leave room for a second workgroup)
+            if (p.m <= 16 && c.n_tiles <= 256) stream_kernel<kType, kFinish, 1, 5><<<grid, kThreads, 0, stream>>>(p);
+            else if (p.m <= 16) stream_kernel<kType, kFinish, 1, 2><<<grid, kThreads, 0, stream>>>(p);
+            else if (p.m <= 32) stream_kernel<kType, kFinish, 2, 3><<<grid, kThreads, 0, stream>>>(p);
+            else stream_kernel<kType, kFinish, 4, 2><<<grid, kThreads, 0, stream>>>(p);
             return launch_status("product of few rows");
         }
     }
