@@ -304,18 +304,22 @@ __device__ __forceinline__ Place place_of(unsigned id, unsigned total, int m_til
             __builtin_amdgcn_readfirstlane(static_cast<int>(part))};
 }
 
-// Tiles of 256 x 256, in two buffers, or of 128 x 128 in a ring of five.
-template <bool kLarge>
+// How a product is made: by a stream of B, or by tiles of 128 x 128 in a ring of five stages, the same in two stages, which leave room for a second workgroup on a
+// compute unit, or 256 x 256 in two.
+enum Way { kStream, kRing, kPairs, kLargeTiles };
+template <Way kWay>
 struct Shape {
+    static constexpr bool kLarge = kWay == kLargeTiles;
     static constexpr int kTile = kLarge ? 256 : 128, kHalf = kTile / 2;
     static constexpr int kWavesN = kLarge ? 4 : 2, kRows = kLarge ? 4 : 1;  // waves across the columns, 32 of each half a wave; 16s of rows of each half a wave
-    static constexpr int kStage = 4 * kHalf * kStepBytes, kStages = kLarge ? 2 : 5;
+    static constexpr int kStage = 4 * kHalf * kStepBytes, kStages = kWay == kRing ? 5 : 2;
+    static constexpr int kWavesOfSimd = kWay == kPairs ? 4 : 2;
 };
 
-template <int kType, bool kTransA, bool kTransB, Finish kFinish, bool kLarge>
+template <int kType, bool kTransA, bool kTransB, Finish kFinish, Way kWay>
 __device__ __forceinline__ void make_tile(const Product& p, unsigned id, unsigned total, uint8_t* lds)
 {
-    using S = Shape<kLarge>;
+    using S = Shape<kWay>;
     constexpr int kValue = kType == kInt8 ? 1 : 2, kValues = kStepBytes / kValue;  // bytes of a value, values of a step
     constexpr int kHalf = S::kHalf, kRows = S::kRows, kWide = kFinish == kGated ? kHalf : 2 * kHalf;
     using A = Operand<kTransA, kHalf, false>;
@@ -396,7 +400,7 @@ __device__ __forceinline__ void make_tile(const Product& p, unsigned id, unsigne
     constexpr std::integral_constant<int, 0> c0;
     constexpr std::integral_constant<int, 1> c1;
 
-    if constexpr (kLarge) {
+    if constexpr (S::kLarge) {
         // LDS: [half of A][buffer], [half of B][buffer], so that a lane's places in both buffers are within the reach of an instruction's own offset.
         constexpr auto a_at = [](int half, int buffer) { return (2 * half + buffer) * A::kBytes; };
         constexpr auto b_at = [](int half, int buffer) { return 4 * A::kBytes + (2 * half + buffer) * B::kBytes; };
@@ -444,6 +448,40 @@ __device__ __forceinline__ void make_tile(const Product& p, unsigned id, unsigne
             step(c1, c0);
         }
         if (wave < 4) meet();
+    } else if constexpr (kWay == kPairs) {
+        // While a step is read and multiplied the next one is asked for, into the place of the one before; the other workgroup of the compute unit has the matrix
+        // cores while this one waits, and goes on while it begins or ends a tile.
+        u32x4 fa[2][kRows][2], fb[2][2][2];  // [half][.][half step]
+        const auto step = [&](int at, uint32_t to) {
+            wait_and_meet<0>();
+            read_rows(at, fa[0]);
+            read_columns(at + 2 * A::kBytes, fb[0]);
+            a.template ask<0, 0>(a_base + to);
+            read_columns(at + 2 * A::kBytes + B::kBytes, fb[1]);
+            b.template ask<0, 2 * A::kBytes>(b_base + to);
+            read_rows(at + A::kBytes, fa[1]);
+            b.template ask<1, 2 * A::kBytes + B::kBytes>(b_base + to);
+            a.template ask<1, A::kBytes>(a_base + to);
+            a.template advance<kValue>(wave, lane);
+            b.template advance<kValue>(wave, lane);
+            __builtin_amdgcn_s_setprio(1);
+            multiply_halves(acc[0][0], fa[0], fb[0]);
+            multiply_halves(acc[0][1], fa[0], fb[1]);
+            multiply_halves(acc[1][1], fa[1], fb[1]);
+            multiply_halves(acc[1][0], fa[1], fb[0]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        a.template ask<0, 0>(a_base);
+        b.template ask<0, 2 * A::kBytes>(b_base);
+        b.template ask<1, 2 * A::kBytes + B::kBytes>(b_base);
+        a.template ask<1, A::kBytes>(a_base);
+        a.template advance<kValue>(wave, lane);
+        b.template advance<kValue>(wave, lane);
+        for (int k = 0; k < steps; k += 2) {
+            step(0, S::kStage);
+            if (k + 1 < steps) step(S::kStage, 0);
+        }
     } else {
         // A ring of kStages steps: while a step is multiplied, the next one's fragments are read and the step kStages - 1 further on is asked for, into the place of
         // the one before, whose fragments are in every wave's registers by the barrier.
@@ -547,11 +585,11 @@ __device__ __forceinline__ void make_tile(const Product& p, unsigned id, unsigne
         }
 }
 
-template <int kType, bool kTransA, bool kTransB, Finish kFinish, bool kLarge>
-__global__ __launch_bounds__(kThreads, 2) void tile_kernel(const Product p)
+template <int kType, bool kTransA, bool kTransB, Finish kFinish, Way kWay>
+__global__ __launch_bounds__(kThreads, Shape<kWay>::kWavesOfSimd) void tile_kernel(const Product p)
 {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<kLarge>::kStages * Shape<kLarge>::kStage];
-    make_tile<kType, kTransA, kTransB, kFinish, kLarge>(p, blockIdx.x, gridDim.x, lds);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<kWay>::kStages * Shape<kWay>::kStage];
+    make_tile<kType, kTransA, kTransB, kFinish, kWay>(p, blockIdx.x, gridDim.x, lds);
 }
 
 // Three products that do not wait for one another in one launch: workgroups of the next fill up the compute units that the last tiles of one leave idle.
@@ -562,14 +600,14 @@ struct Products {
     Product of[3];
     unsigned begin[4];  // a product's first workgroup
 };
-template <int kType, bool kLarge>
-__global__ __launch_bounds__(kThreads, 2) void products_kernel(const Products p)
+template <int kType, Way kWay>
+__global__ __launch_bounds__(kThreads, Shape<kWay>::kWavesOfSimd) void products_kernel(const Products p)
 {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<kLarge>::kStages * Shape<kLarge>::kStage];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Shape<kWay>::kStages * Shape<kWay>::kStage];
     const int which = blockIdx.x < p.begin[1] ? 0 : blockIdx.x < p.begin[2] ? 1 : 2;
     const unsigned id = blockIdx.x - p.begin[which], total = p.begin[which + 1] - p.begin[which];
-    if (p.of[which].turned_a != 0) make_tile<kType, true, true, kStore, kLarge>(p.of[which], id, total, lds);
-    else make_tile<kType, false, true, kStore, kLarge>(p.of[which], id, total, lds);
+    if (p.of[which].turned_a != 0) make_tile<kType, true, true, kStore, kWay>(p.of[which], id, total, lds);
+    else make_tile<kType, false, true, kStore, kWay>(p.of[which], id, total, lds);
 }
 
 // The parts of k added up, and what becomes of the sums.
@@ -706,18 +744,27 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
     }
 }
 
-// How a product is cut up: a stream of B, or tiles of 256 or 128, and k into parts whose sums another kernel adds up.
-enum Way { kStream, kSmall, kLargeTiles };
+// How a product is cut up, k into parts whose sums another kernel adds up.
 struct Cut {
     Way way;
     int m_tiles, n_tiles, parts, part_steps;
     size_t bytes;  // of the parts' sums
     double us;
 };
-// The quickest by what tiles were measured to take on 256 compute units: a step of a large tile 1.5 us with all of them at work, of a small one 0.58, 5 and 4 us
-// around a tile's steps; joining parts 3.5 us and their sums at 4 bytes / ps.  A stream takes 3 us,
-// what its workgroups read of B and of up to 64 rows of A, in rounds of 256, at 62 bytes / ns, and 0.4 of the time of reading B from memory.
-inline double tile_us(bool large, int steps) { return large ? 5 + 1.5 * steps : 4 + 0.58 * steps; }
+// The quickest by what was measured on 256 compute units.  Where all of them are at work a step of a large tile takes 1.5 us, of one in the ring 0.58, and of two that share a
+// compute unit 0.92, with 5, 4 and 4.5 us around a tile's steps; a last round of pairs with no more than one tile a compute unit takes 0.7 of a whole one.  So
+// pairs win from one to about two and a half tiles of 128 a compute unit, and where k is short (8-bit integers, 400 tiles, 23 steps: 31 us by the ring, 25 by pairs, 39 by large tiles; 256 tiles, 56
+// steps: 34, 43, 67; 1024 tiles, 56 steps: 126, 108, 88).
+// Joining parts takes 3.5 us, and 2 ps for each of the 4-byte sums, written and read.  A stream takes 3 us, what its workgroups read of B
+// and of up to 64 rows of A, in rounds of 256, at 62 bytes / ns, and 0.4 of the time of reading B from memory.
+inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 5 + 1.5 * steps : way == kRing ? 4 + 0.58 * steps : 4.5 + 0.92 * steps; }
+inline int at_once(Way way) { return way == kPairs ? 512 : 256; }
+inline double rounds_of(Way way, long long tiles)
+{
+    const long long whole = tiles / at_once(way), rest = tiles % at_once(way);
+    if (rest == 0) return static_cast<double>(whole);
+    return static_cast<double>(whole) + (way != kPairs ? 1.0 : 0.7 + 0.3 * static_cast<double>(std::max(0ll, rest - 256)) / 256);
+}
 Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
 {
     const int steps = std::max(1, (k_bytes + kStepBytes - 1) / kStepBytes), times = gated ? 2 : 1;
@@ -727,16 +774,15 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
         const double rounds = std::max(1.0, static_cast<double>(n_tiles) * m_tiles / 256), read = static_cast<double>(16 + std::min(m, 64)) * k_bytes;
         best = {kStream, m_tiles, n_tiles, 1, steps, 0, 3 + rounds * read / 62e3 + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
     }
-    for (const Way way : {kSmall, kLargeTiles}) {
-        const bool large = way == kLargeTiles;
-        const int tile = large ? 256 : 128, wide = tile / times;
+    for (const Way way : {kRing, kPairs, kLargeTiles}) {
+        const int tile = way == kLargeTiles ? 256 : 128, wide = tile / times;
         const int m_tiles = (m + tile - 1) / tile, n_tiles = (columns + wide - 1) / wide;
         for (int wanted = 1; wanted <= 16; ++wanted) {
             const int part_steps = (steps + wanted - 1) / wanted, parts = (steps + part_steps - 1) / part_steps;
             if (parts != wanted) continue;
-            const double rounds = static_cast<double>((static_cast<long long>(m_tiles) * n_tiles * parts + 255) / 256);
+            const double rounds = rounds_of(way, static_cast<long long>(m_tiles) * n_tiles * parts);
             const size_t bytes = parts == 1 ? 0 : static_cast<size_t>(parts) * m * ((columns + 7) / 8 * 8) * times * 4;
-            const double us = rounds * tile_us(large, part_steps) + (parts == 1 ? 0 : 3.5 + 2e-6 * static_cast<double>(bytes) / 4);
+            const double us = rounds * tile_us(way, part_steps) + (parts == 1 ? 0 : 3.5 + 0.5e-6 * static_cast<double>(bytes));
             if (best.parts == 0 || us < best.us) best = {way, m_tiles, n_tiles, parts, part_steps, bytes, us};
         }
     }
@@ -768,51 +814,81 @@ int launch(Product p, void* partial, hipStream_t stream)
     const long long groups = static_cast<long long>(c.m_tiles) * c.n_tiles * c.parts;
     DPEP_REQUIRE(groups <= 0x7fffff, "a product of %d x %d is too large", p.m, p.columns);
     const dim3 grid(static_cast<unsigned>(groups));
-    if (c.way == kLargeTiles) tile_kernel<kType, kTransA, kTransB, kFinish, true><<<grid, kThreads, 0, stream>>>(p);
-    else tile_kernel<kType, kTransA, kTransB, kFinish, false><<<grid, kThreads, 0, stream>>>(p);
+    if (c.way == kLargeTiles) tile_kernel<kType, kTransA, kTransB, kFinish, kLargeTiles><<<grid, kThreads, 0, stream>>>(p);
+    else if (c.way == kPairs) tile_kernel<kType, kTransA, kTransB, kFinish, kPairs><<<grid, kThreads, 0, stream>>>(p);
+    else tile_kernel<kType, kTransA, kTransB, kFinish, kRing><<<grid, kThreads, 0, stream>>>(p);
     if (int rc = launch_status("product"); rc != DPEP_OK || c.parts == 1) return rc;
     const size_t pieces = static_cast<size_t>(p.m) * (p.pitch / 8);
     join_kernel<kType, kFinish><<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream>>>(p);
     return launch_status("product's parts");
 }
 
-// Three products (of 16-bit values, results stored, no part of another's operands), together if that is quicker than one after the other.
+// When `slots` that take tiles as they get free are done with the tiles of three products, tiles[i] of us[i] each, one product after the other.
+double done_after(int slots, const long long (&tiles)[3], const double (&us)[3])
+{
+    double free_at[8] = {};  // groups of slots that get free together, at most one more for each product begun: the first group's rest and those moved on
+    int slots_of[8] = {slots}, groups = 1;
+    double end = 0;
+    for (int i = 0; i < 3; ++i) {
+        long long left = tiles[i];
+        if (left == 0) continue;
+        const long long rounds = std::max(0ll, left / slots - 2);  // (every slot takes these)
+        for (int g = 0; g < groups; ++g) free_at[g] += static_cast<double>(rounds) * us[i];
+        left -= rounds * slots;
+        while (left > 0) {
+            const int first = static_cast<int>(std::min_element(free_at, free_at + groups) - free_at);
+            const int taken = static_cast<int>(std::min<long long>(left, slots_of[first]));
+            const double then = free_at[first] + us[i];
+            if (taken < slots_of[first]) {
+                slots_of[first] -= taken;
+                free_at[groups] = then;
+                slots_of[groups++] = taken;
+            } else {
+                free_at[first] = then;
+            }
+            left -= taken;
+        }
+    }
+    for (int g = 0; g < groups; ++g) end = std::max(end, free_at[g]);
+    return end;
+}
+
+// Three products (of 16-bit values, results stored, no part of another's operands), together if that is quicker than one after the other with 4 us for a launch.
+// (8192 tokens, 4096 and 2048 values: 605 us with the product before them together in large tiles, 690 apart; 2048 tokens, 2048 and 1024: 72 in large tiles, 80 in pairs, 83 in the
+// ring, 86 apart; 16000, 640 and 160: 127 in the ring, 69 apart, with k in parts.)
 template <int kType>
 int launch_three(Product (&products)[3], void* partial, hipStream_t stream)
 {
-    double apart = 0;
-    for (const Product& p : products) apart += cut_of(p.m, p.columns, p.k * 2, false, true).us;
+    double least = 8;
+    for (const Product& p : products) least += cut_of(p.m, p.columns, p.k * 2, false, true).us;
     std::sort(products, products + 3, [](const Product& a, const Product& b) { return a.k > b.k; });  // (long tiles first, short ones fill up)
     Products best = {};
-    double least = apart;
-    bool best_large = false;
-    for (int large = 0; large < 2; ++large) {
-        const int tile = large ? 256 : 128;
+    Way best_way = kRing;
+    for (const Way way : {kRing, kPairs, kLargeTiles}) {
+        const int tile = way == kLargeTiles ? 256 : 128;
         Products now = {};
-        double work = 0, longest = 0;
-        long long begin = 0;
+        long long tiles[3], begin = 0;
+        double us[3];
         for (int i = 0; i < 3; ++i) {
             Product p = products[i];
             p.m_tiles = (p.m + tile - 1) / tile;
             p.n_tiles = (p.columns + tile - 1) / tile;
             p.parts = 1;
             p.part_steps = std::max(1, (p.k * 2 + kStepBytes - 1) / kStepBytes);
-            const double us = tile_us(large != 0, p.part_steps);
-            const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-            work += static_cast<double>(tiles) * us;
-            longest = std::max(longest, us);
+            us[i] = tile_us(way, p.part_steps);
+            tiles[i] = static_cast<long long>(p.m_tiles) * p.n_tiles;
             now.of[i] = p;
             now.begin[i] = static_cast<unsigned>(begin);
-            begin += tiles;
+            begin += tiles[i];
         }
         now.begin[3] = static_cast<unsigned>(begin);
-        // the last tiles, short ones, end half of their time apart
-        const double us = std::max(longest, work / 256 + tile_us(large != 0, now.of[2].part_steps) / 2);
-        if (begin <= 0x7fffff && us < least) best = now, least = us, best_large = large != 0;
+        const double done = done_after(at_once(way), tiles, us) * (way == kPairs && begin <= 256 ? 0.7 : 1.0);
+        if (begin <= 0x7fffff && done < least) best = now, least = done, best_way = way;
     }
     if (best.begin[3] != 0) {
-        if (best_large) products_kernel<kType, true><<<best.begin[3], kThreads, 0, stream>>>(best);
-        else products_kernel<kType, false><<<best.begin[3], kThreads, 0, stream>>>(best);
+        if (best_way == kLargeTiles) products_kernel<kType, kLargeTiles><<<best.begin[3], kThreads, 0, stream>>>(best);
+        else if (best_way == kPairs) products_kernel<kType, kPairs><<<best.begin[3], kThreads, 0, stream>>>(best);
+        else products_kernel<kType, kRing><<<best.begin[3], kThreads, 0, stream>>>(best);
         return launch_status("products");
     }
     for (const Product& p : products) {
