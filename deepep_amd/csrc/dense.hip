@@ -195,7 +195,7 @@ __device__ __forceinline__ void meet()
 template <int kAt>
 __device__ __forceinline__ void load_to_lds(rsrc from, uint32_t offset, uint32_t base)
 {
-    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(base), "n"(kAt), "v"(offset), "s"(from) : "memory", "scc");
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(base), "n"(kAt), "v"(offset), "s"(from) : "memory", "scc", "m0");
 }
 // One operand of a tile as the loads see it: halves of kRowsOfHalf rows (or columns), kPer loads a wave each.
 template <bool kTrans, int kRowsOfHalf, bool kPaired>
