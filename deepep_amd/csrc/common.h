@@ -36,6 +36,22 @@ inline bool overlap(const void* a, size_t bytes_a, const void* b, size_t bytes_b
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return a != nullptr && b != nullptr && x < y + bytes_b && y < x + bytes_a;
 }
+struct Span {
+    const void* p;
+    size_t bytes;
+};
+// What is written (scratch is) overlaps nothing that is read, nor one another.
+template <size_t kWritten, size_t kRead>
+inline bool apart(const Span (&written)[kWritten], const Span (&read)[kRead])
+{
+    for (size_t i = 0; i < kWritten; ++i) {
+        for (const Span& r : read)
+            if (overlap(written[i].p, written[i].bytes, r.p, r.bytes)) return false;
+        for (size_t j = 0; j < i; ++j)
+            if (overlap(written[i].p, written[i].bytes, written[j].p, written[j].bytes)) return false;
+    }
+    return true;
+}
 
 struct Workspace {
     uint32_t magic;

@@ -54,7 +54,8 @@ __device__ __forceinline__ void load_wide(const float* from, float (&v)[8])
     for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
 }
 
-// What becomes of results.  Each takes eight of them next to one another in a row; columns are a multiple of eight but for those of kScaled.
+// What becomes of results.  Sums are in 32 bits until here.  h and dz are rounded to the operands' type, once each from 32 bits, because the matrix cores take 16-bit
+// operands in the next product; what the backward needs of the products, g and u, is kept in FP32, so that dz is off by its own rounding alone.  Each takes eight of them next to one another in a row; columns are a multiple of eight but for those of kScaled.
 enum Finish {
     kStore,     // C rounded to the operands' type
     kGated,     // columns of gate and up together: h, and the products where they are kept
@@ -62,7 +63,7 @@ enum Finish {
     kScaled,    // 8-bit integers' sums with the scales of row and column
 };
 struct Output {
-    void* c;            // [M, ldc]
+    void* c;            // [M, N], of kGradient dz [M, 2 N]
     float* kept;        // [M, 2 N]: gate, then up
     void* h;            // kGradient: [M, N]
     const float* row_scale;
@@ -168,6 +169,9 @@ struct Product {
 //
 // The matrix instruction takes B as its first operand, so that a lane's four results are four columns of one row.  The columns of a pair of
 // instructions are dealt so that a lane ends up with eight next to one another: 16 bytes of 16-bit results.
+//
+// 8192 tokens, 7168 and 2048 values, BF16: 372 us for the gated product (1.29 PFLOP/s), 211 for the second (1.14), 213 for dh, 880 for the three of the backward
+// (1.37); 8192 x 4096 of 7168 in 8-bit integers: 184 (2.6 POP/s).  Power bounds these: the clock falls to 1.7 GHz, and inputs of zeros take 0.83 of the time.
 //
 // Rows, columns and values of k that are not there are read as zero (the loads' own bounds check): a half's record ends with its last row, and pieces
 // behind the last column or, in the last step, behind the last k have an offset that is nowhere.
@@ -483,6 +487,9 @@ __device__ __forceinline__ void make_tile(const Product& p, unsigned id, unsigne
             if (k + 1 < steps) step(S::kStage, 0);
         }
     } else {
+        // What bounds this is L1: with the products left out a workgroup takes as long, with the reads from LDS left out too, without the loads 0.8 of it.  Some 100 lines of
+        // 128 bytes are under way a compute unit, however far ahead they are asked for, and come after 670 cycles in the mean (512 tokens, 7168 to 2 x
+        // 2048: 40 us, 14 TB/s from L2).
         // A ring of kStages steps: while a step is multiplied, the next one's fragments are read and the step kStages - 1 further on is asked for, into the place of
         // the one before, whose fragments are in every wave's registers by the barrier.
         constexpr int kLoads = 4, kStages = S::kStages;  // loads of a wave for a step
@@ -644,6 +651,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
 // every eighth line of 128 bytes of k, and their sums meet in LDS at the end.  Each wave has a ring of its own in LDS, into which its lines of B and A
 // go straight from memory, 8 rows of whole lines a load, and waits for nobody else on the way.  (Read to registers in the matrix instruction's own order a load of
 // A touches 64 lines instead of 8: 64 rows of 7168, 4096 columns took 37 us by that.)
+// One token: 7168 to 2 x 2048 in BF16 (59 MB) 12.0 us, 2048 to 7168 (29 MB) 8.4, 7168 to 4096 in 8 bits (29 MB) 7.6, where an empty kernel takes 2 to 3.
 template <int kType, Finish kFinish, int kBlocks, int kStages>
 __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
 {
@@ -790,10 +798,9 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
 }
 
 template <int kType, bool kTransA, bool kTransB, Finish kFinish>
-int launch(Product p, void* partial, hipStream_t stream)
+int launch(Product p, const Cut& c, void* partial, hipStream_t stream)
 {
     if (p.m == 0 || p.columns == 0) return DPEP_OK;
-    const Cut c = cut_of(p.m, p.columns, p.k * (kType == kInt8 ? 1 : 2), kFinish == kGated, kTransA || kTransB);
     if constexpr (!kTransA && !kTransB) {
         if (c.way == kStream) {
             const dim3 grid(c.n_tiles, c.m_tiles);
@@ -857,11 +864,12 @@ double done_after(int slots, const long long (&tiles)[3], const double (&us)[3])
 // (8192 tokens, 4096 and 2048 values: 605 us with the product before them together in large tiles, 690 apart; 2048 tokens, 2048 and 1024: 72 in large tiles, 80 in pairs, 83 in the
 // ring, 86 apart; 16000, 640 and 160: 127 in the ring, 69 apart, with k in parts.)
 template <int kType>
-int launch_three(Product (&products)[3], void* partial, hipStream_t stream)
+int launch_three(const Product (&products)[3], const Cut (&cuts)[3], void* partial, hipStream_t stream)
 {
     double least = 8;
-    for (const Product& p : products) least += cut_of(p.m, p.columns, p.k * 2, false, true).us;
-    std::sort(products, products + 3, [](const Product& a, const Product& b) { return a.k > b.k; });  // (long tiles first, short ones fill up)
+    for (const Cut& c : cuts) least += c.us;
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return products[a].k > products[b].k; });  // (long tiles first, short ones fill up)
     Products best = {};
     Way best_way = kRing;
     for (const Way way : {kRing, kPairs, kLargeTiles}) {
@@ -870,7 +878,7 @@ int launch_three(Product (&products)[3], void* partial, hipStream_t stream)
         long long tiles[3], begin = 0;
         double us[3];
         for (int i = 0; i < 3; ++i) {
-            Product p = products[i];
+            Product p = products[order[i]];
             p.m_tiles = (p.m + tile - 1) / tile;
             p.n_tiles = (p.columns + tile - 1) / tile;
             p.parts = 1;
@@ -891,8 +899,9 @@ int launch_three(Product (&products)[3], void* partial, hipStream_t stream)
         else products_kernel<kType, kRing><<<best.begin[3], kThreads, 0, stream>>>(best);
         return launch_status("products");
     }
-    for (const Product& p : products) {
-        const int rc = p.turned_a != 0 ? launch<kType, true, true, kStore>(p, partial, stream) : launch<kType, false, true, kStore>(p, partial, stream);
+    for (int i = 0; i < 3; ++i) {
+        const int rc = products[i].turned_a != 0 ? launch<kType, true, true, kStore>(products[i], cuts[i], partial, stream)
+                                                 : launch<kType, false, true, kStore>(products[i], cuts[i], partial, stream);
         if (rc != DPEP_OK) return rc;
     }
     return DPEP_OK;
@@ -910,6 +919,29 @@ int check_ffn(const dpep_ffn* f, const char* what, int tokens)
 }
 inline size_t whole(size_t bytes) { return (bytes + 255) & ~static_cast<size_t>(255); }
 
+// How a block's products are cut up, and its scratch: the rows between the products, then the parts' sums of one product at a time.
+struct ForwardCuts {
+    Cut gate_up, down;
+    size_t scratch;
+    ForwardCuts(int tokens, int hidden, int inter)
+        : gate_up(cut_of(tokens, inter, hidden * 2, true, false)),
+          down(cut_of(tokens, hidden, inter * 2, false, false)),
+          scratch(whole(static_cast<size_t>(tokens) * inter * 2) + std::max(gate_up.bytes, down.bytes))
+    {
+    }
+};
+struct BackwardCuts {
+    Cut rows, three[3];  // dh; dx, dWgu, dWd
+    size_t scratch;
+    BackwardCuts(int tokens, int hidden, int inter)
+        : rows(cut_of(tokens, inter, hidden * 2, false, true)),
+          three{cut_of(tokens, hidden, inter * 4, false, true), cut_of(2 * inter, hidden, tokens * 2, false, true), cut_of(hidden, inter, tokens * 2, false, true)},
+          scratch(whole(static_cast<size_t>(tokens) * inter * 2) + whole(static_cast<size_t>(tokens) * inter * 4) +
+                  std::max(std::max(rows.bytes, three[0].bytes), std::max(three[1].bytes, three[2].bytes)))
+    {
+    }
+};
+
 template <class F>
 int by_type(int type, F f)
 {
@@ -925,9 +957,7 @@ extern "C" {
 
 size_t dpep_gated_ffn_scratch_bytes(int num_tokens, int hidden, int inter)
 {
-    if (num_tokens < 0 || hidden < 0 || inter < 0) return 0;
-    return whole(static_cast<size_t>(num_tokens) * inter * 2) +
-           std::max(cut_of(num_tokens, inter, hidden * 2, true, false).bytes, cut_of(num_tokens, hidden, inter * 2, false, false).bytes);
+    return num_tokens < 0 || hidden < 0 || inter < 0 ? 0 : ForwardCuts(num_tokens, hidden, inter).scratch;
 }
 
 int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, float* kept, void* scratch, void* stream)
@@ -937,9 +967,10 @@ int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, fl
     DPEP_REQUIRE(x != nullptr && y != nullptr && scratch != nullptr && aligned16(x) && aligned16(y) && aligned16(kept) && aligned16(scratch),
                  "gated_ffn: a NULL or misaligned buffer");
     const size_t rows = static_cast<size_t>(num_tokens) * f->hidden * 2, half = static_cast<size_t>(f->hidden) * f->inter * 2, products = static_cast<size_t>(num_tokens) * f->inter * 8;
-    DPEP_REQUIRE(!overlap(y, rows, x, rows) && !overlap(y, rows, f->gate_up, 2 * half) && !overlap(y, rows, f->down, half) && !overlap(y, rows, kept, products) &&
-                     !overlap(kept, products, x, rows) && !overlap(kept, products, f->gate_up, 2 * half) && !overlap(kept, products, f->down, half),
-                 "gated_ffn: an output overlaps an input");
+    const ForwardCuts cuts(num_tokens, f->hidden, f->inter);
+    const Span written[] = {{y, rows}, {kept, products}, {scratch, cuts.scratch}};
+    const Span read[] = {{x, rows}, {f->gate_up, 2 * half}, {f->down, half}};
+    DPEP_REQUIRE(apart(written, read), "gated_ffn: an output or scratch overlaps an input or one another");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     void* const partial = static_cast<uint8_t*>(scratch) + whole(static_cast<size_t>(num_tokens) * f->inter * 2);
     return by_type(f->type, [&](auto type) {
@@ -947,19 +978,16 @@ int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, fl
         Product p = {x, f->gate_up, num_tokens, f->inter, f->hidden, {}};
         p.out.c = scratch;
         p.out.kept = kept;
-        if (int rc = launch<kType, false, false, kGated>(p, partial, s); rc != DPEP_OK) return rc;
+        if (int rc = launch<kType, false, false, kGated>(p, cuts.gate_up, partial, s); rc != DPEP_OK) return rc;
         p = {scratch, f->down, num_tokens, f->hidden, f->inter, {}};
         p.out.c = y;
-        return launch<kType, false, false, kStore>(p, partial, s);
+        return launch<kType, false, false, kStore>(p, cuts.down, partial, s);
     });
 }
 
 size_t dpep_gated_ffn_backward_scratch_bytes(int num_tokens, int hidden, int inter)
 {
-    if (num_tokens < 0 || hidden < 0 || inter < 0) return 0;
-    return whole(static_cast<size_t>(num_tokens) * inter * 2) + whole(static_cast<size_t>(num_tokens) * inter * 4) +
-           std::max(std::max(cut_of(num_tokens, inter, hidden * 2, false, true).bytes, cut_of(num_tokens, hidden, inter * 4, false, true).bytes),
-                    std::max(cut_of(2 * inter, hidden, num_tokens * 2, false, true).bytes, cut_of(hidden, inter, num_tokens * 2, false, true).bytes));
+    return num_tokens < 0 || hidden < 0 || inter < 0 ? 0 : BackwardCuts(num_tokens, hidden, inter).scratch;
 }
 
 int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x, const float* kept, int num_tokens, void* grad_x, void* grad_gate_up,
@@ -971,13 +999,12 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
                                      aligned16(kept) && aligned16(grad_x) && aligned16(scratch)),
                  "gated_ffn_backward: a NULL or misaligned buffer");
     const size_t rows = static_cast<size_t>(num_tokens) * f->hidden * 2, half = static_cast<size_t>(f->hidden) * f->inter * 2, products = static_cast<size_t>(num_tokens) * f->inter * 8;
-    const struct { const void* p; size_t bytes; } inputs[] = {{grad_y, rows}, {x, rows}, {kept, products}, {f->gate_up, 2 * half}, {f->down, half}},
-                                                  outputs[] = {{grad_x, rows}, {grad_gate_up, 2 * half}, {grad_down, half}};
-    for (const auto& out : outputs) {
-        for (const auto& in : inputs) DPEP_REQUIRE(!overlap(out.p, out.bytes, in.p, in.bytes), "gated_ffn_backward: an output overlaps an input");
-        for (const auto& other : outputs)
-            DPEP_REQUIRE(&out == &other || !overlap(out.p, out.bytes, other.p, other.bytes), "gated_ffn_backward: two outputs overlap");
-    }
+    const Span read[] = {{grad_y, rows}, {x, rows}, {kept, products}, {f->gate_up, 2 * half}, {f->down, half}};
+    const Span outputs[] = {{grad_x, rows}, {grad_gate_up, 2 * half}, {grad_down, half}};
+    const BackwardCuts cuts(num_tokens, f->hidden, f->inter);
+    const Span aside[] = {{scratch, cuts.scratch}};
+    DPEP_REQUIRE(apart(outputs, {Span{nullptr, 0}}), "gated_ffn_backward: two outputs overlap");
+    DPEP_REQUIRE(apart(outputs, read) && apart(aside, read) && apart(aside, outputs), "gated_ffn_backward: an output or scratch overlaps an input or one another");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     void* const h = scratch;
     void* const dz = static_cast<uint8_t*>(scratch) + whole(static_cast<size_t>(num_tokens) * f->inter * 2);
@@ -988,7 +1015,7 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
         p.out.c = dz;
         p.out.kept = const_cast<float*>(kept);
         p.out.h = h;
-        if (int rc = launch<kType, false, true, kGradient>(p, partial, s); rc != DPEP_OK) return rc;
+        if (int rc = launch<kType, false, true, kGradient>(p, cuts.rows, partial, s); rc != DPEP_OK) return rc;
         Product products[3] = {{dz, f->gate_up, num_tokens, f->hidden, 2 * f->inter, {}},
                                {dz, x, 2 * f->inter, f->hidden, num_tokens, {}},
                                {grad_y, h, f->hidden, f->inter, num_tokens, {}}};
@@ -996,7 +1023,7 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
         products[1].out.c = grad_gate_up;
         products[2].out.c = grad_down;
         products[1].turned_a = products[2].turned_a = 1;
-        return launch_three<kType>(products, partial, s);
+        return launch_three<kType>(products, cuts.three, partial, s);
     });
 }
 
@@ -1016,17 +1043,18 @@ int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int
     DPEP_REQUIRE(w->codes != nullptr && w->scales != nullptr && aligned16(w->codes), "w8_matmul: a NULL or misaligned matrix");
     if (num_rows == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && x_scales != nullptr && y != nullptr && aligned16(x), "w8_matmul: a NULL or misaligned buffer");
-    DPEP_REQUIRE(scratch != nullptr || dpep_w8_matmul_scratch_bytes(num_rows, w->n, w->k) == 0, "w8_matmul: scratch is NULL");
+    const Cut cut = cut_of(num_rows, w->n, w->k, false, false);
+    DPEP_REQUIRE(scratch != nullptr || cut.bytes == 0, "w8_matmul: scratch is NULL");
     const size_t results = static_cast<size_t>(num_rows) * w->n * (type == DPEP_TYPE_F32 ? 4 : 2);
-    DPEP_REQUIRE(!overlap(y, results, x, static_cast<size_t>(num_rows) * w->k) && !overlap(y, results, x_scales, num_rows * 4ull) &&
-                     !overlap(y, results, w->codes, static_cast<size_t>(w->n) * w->k) && !overlap(y, results, w->scales, w->n * 4ull),
-                 "w8_matmul: y overlaps an input");
+    const Span written[] = {{y, results}, {scratch, cut.bytes}};
+    const Span read[] = {{x, static_cast<size_t>(num_rows) * w->k}, {x_scales, num_rows * 4ull}, {w->codes, static_cast<size_t>(w->n) * w->k}, {w->scales, w->n * 4ull}};
+    DPEP_REQUIRE(apart(written, read), "w8_matmul: y or scratch overlaps an input or one another");
     Product p = {x, w->codes, num_rows, w->n, w->k, {}};
     p.out.c = y;
     p.out.row_scale = x_scales;
     p.out.column_scale = w->scales;
     p.out.type = type;
-    return launch<kInt8, false, false, kScaled>(p, scratch, static_cast<hipStream_t>(stream));
+    return launch<kInt8, false, false, kScaled>(p, cut, scratch, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

