@@ -760,9 +760,9 @@ struct Cut {
     double us;
 };
 // The quickest by what was measured on 256 compute units.  Where all of them are at work a step of a large tile takes 1.5 us, of one in the ring 0.58, and of two that share a
-// compute unit 0.92, with 5, 4 and 4.5 us around a tile's steps; a last round of pairs with no more than one tile a compute unit takes 0.7 of a whole one.  So
-// pairs win from one to about two and a half tiles of 128 a compute unit, and where k is short (8-bit integers, 400 tiles, 23 steps: 31 us by the ring, 25 by pairs, 39 by large tiles; 256 tiles, 56
-// steps: 34, 43, 67; 1024 tiles, 56 steps: 126, 108, 88).
+// compute unit 0.92, with 5, 4 and 4.5 us around a tile's steps; a last round of pairs takes 0.75 of a whole one with no more than one tile a compute unit, 0.85 and up
+// with more.  So pairs win from one to about two and a half tiles of 128 a compute unit, and where k is short (8-bit integers, 400 tiles, 23 steps: 31 us by the
+// ring, 25 by pairs, 39 by large tiles; 256 tiles, 56 steps: 34, 43, 67; 1024 tiles, 56 steps: 126, 108, 88).
 // Joining parts takes 3.5 us, and 2 ps for each of the 4-byte sums, written and read.  A stream takes 3 us, what its workgroups read of B
 // and of up to 64 rows of A, in rounds of 256, at 62 bytes / ns, and 0.4 of the time of reading B from memory.
 inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 5 + 1.5 * steps : way == kRing ? 4 + 0.58 * steps : 4.5 + 0.92 * steps; }
@@ -771,7 +771,7 @@ inline double rounds_of(Way way, long long tiles)
 {
     const long long whole = tiles / at_once(way), rest = tiles % at_once(way);
     if (rest == 0) return static_cast<double>(whole);
-    return static_cast<double>(whole) + (way != kPairs ? 1.0 : 0.7 + 0.3 * static_cast<double>(std::max(0ll, rest - 256)) / 256);
+    return static_cast<double>(whole) + (way != kPairs ? 1.0 : rest <= 256 ? 0.75 : 0.7 + 0.3 * static_cast<double>(rest) / 512);
 }
 Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
 {
@@ -890,7 +890,7 @@ int launch_three(const Product (&products)[3], const Cut (&cuts)[3], void* parti
             begin += tiles[i];
         }
         now.begin[3] = static_cast<unsigned>(begin);
-        const double done = done_after(at_once(way), tiles, us) * (way == kPairs && begin <= 256 ? 0.7 : 1.0);
+        const double done = done_after(at_once(way), tiles, us) * (way == kPairs && begin <= 256 ? 0.75 : 1.0);
         if (begin <= 0x7fffff && done < least) best = now, least = done, best_way = way;
     }
     if (best.begin[3] != 0) {
