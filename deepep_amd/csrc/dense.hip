@@ -684,7 +684,7 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
         load_to_lds<0>(from(0), place, to);
         load_to_lds<1024>(from(1), place, to);
         load_to_lds<2048>(from(2), place, to);
-        load_to_lds<3072>(from(3), place, to);
+        load_to_lds<3 * 1024>(from(3), place, to);
         if constexpr (kBlocks >= 2) {
             load_to_lds<4096>(from(4), place, to);
             load_to_lds<5120>(from(5), place, to);

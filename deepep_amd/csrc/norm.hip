@@ -238,7 +238,8 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const dpep_norm p)
             if (at % 128 == 0) static_cast<float*>(p.scales)[static_cast<size_t>(blockIdx.x) * ((hidden + 127) / 128) + at / 128] = m / 448.0f;
         } else if (p.quantize == DPEP_QUANT_MXFP8) {
             if (c * kThreads * kVec >= hidden) continue;
-            const int byte = mx_scale_byte(__uint_as_float(lanes_max<4>(live ? magnitude(v[c]) : 0u)));
+            const uint32_t block = lanes_max<4>(live ? magnitude(v[c]) : 0u);
+            const int byte = block >= 0x7f800000u ? 255 : mx_scale_byte(__uint_as_float(block));  // (255 is the format's NaN)
             if (!live) continue;
             u32x2 codes;
 #pragma unroll

@@ -454,7 +454,8 @@ int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const
  *   `type`;  weight [H] of weight_type (`type` or fp32);  rstd fp32 [T] or NULL
  *   quantize  v in 8 bits, each value rounded from fp32 once:
  *     DPEP_QUANT_FP8    codes e4m3 [T,H], scales fp32 [T,ceil(H/128)]: as dpep_cast_to_fp8 (H a multiple of 16)
- *     DPEP_QUANT_MXFP8  codes e4m3 [T,H], scales e8m0 bytes [T,H/32]: as dpep_mx_quant (H a multiple of 32)
+ *     DPEP_QUANT_MXFP8  codes e4m3 [T,H], scales e8m0 bytes [T,H/32]: as dpep_mx_quant (H a multiple of 32), and the scale NaN (255) for a
+ *                       block of 32 that holds a NaN or an infinity
  *     DPEP_QUANT_INT8   codes int8 [T,H], scales fp32 [T]: as dpep_quantize_tokens (H a multiple of 16)
  * H is a multiple of 8, at most DPEP_NORM_MAX_HIDDEN; pointers to rows are 16-byte aligned; T below 2^23.  Outputs overlap no input but for stream_out, nor
  * one another. */

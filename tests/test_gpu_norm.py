@@ -163,6 +163,21 @@ def test_rows_that_are_not_finite_stay_in_their_rows():
         assert torch.isnan(got.y[2, 9]) and not torch.isfinite(got.scales[2]).all()
 
 
+def test_blocks_that_are_not_finite_have_a_scale_that_is_none():
+    from deepep_amd import dense
+
+    rng = np.random.default_rng(15)
+    x, w = _rows(rng, 4, 256, "bf16"), _weight(rng, 256, "bf16")
+    want = dense.rms_norm(x, w, quantize="mxfp8")
+    x[1, 7], x[2, 41] = float("nan"), float("-inf")
+    got = dense.rms_norm(x, w, quantize="mxfp8")
+    for row in (0, 3):
+        assert torch.equal(got.codes[row].view(torch.uint8), want.codes[row].view(torch.uint8)) and torch.equal(got.scales[row], want.scales[row])
+    assert (got.scales[1] == 255).all()
+    # (an infinity's norm makes zeros of the other values and a NaN of it)
+    assert got.scales[2, 1] == 255 and (got.scales[2] == 255).sum() == 1
+
+
 def test_views_and_unaligned_rows():
     """Rows that start at an odd element are taken by way of a copy; rows that are not contiguous are refused."""
     from deepep_amd import dense
