@@ -144,3 +144,23 @@ def test_mega_moe_takes_the_norms_codes():
         assert mm.relative_frobenius(y.float().cpu().numpy(), want) <= 2e-2
     finally:
         buf.destroy()
+
+
+def test_inference_mode_and_leaves(block):
+    """The same results in inference mode, of inference tensors, and of leaves that want gradients (none are recorded)."""
+    from deepep_amd import dense, w8
+
+    block.quantize()
+    x, residual = _rows(17, 6).cuda(), _rows(18, 6).cuda()
+    want = block.decode(x, residual)
+    y, kept = dense.gated_ffn(x, block.shared_gate_up, block.shared_down, keep=True)
+    grads = dense.gated_ffn_backward(residual, x, block.shared_gate_up, block.shared_down, kept)
+    with torch.inference_mode():
+        got = block.decode(x.clone(), residual.clone())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(w8.matmul(x.clone(), block.shared_8[0]), w8.matmul(x, block.shared_8[0]))
+        again = dense.gated_ffn_backward(residual.clone(), x.clone(), block.shared_gate_up, block.shared_down, kept.clone())
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+    leaves = [t.clone().requires_grad_(True) for t in (x, block.shared_gate_up, block.shared_down)]
+    out = dense.gated_ffn(*leaves)
+    assert torch.equal(out, y) and not out.requires_grad
