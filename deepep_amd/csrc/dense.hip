@@ -632,7 +632,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
 #pragma unroll
     for (int t = 0; t < kTimes; ++t) {
         Sum<kType> sum[2] = {};
-#pragma unroll 4
+#pragma unroll 8
         for (int part = 0; part < p.parts; ++part) {
             const u32x4* const from = reinterpret_cast<const u32x4*>(static_cast<const uint32_t*>(p.partial) + (static_cast<size_t>(part) * p.m + m) * wide +
                                                                      static_cast<size_t>(t) * p.pitch + n);
@@ -765,7 +765,7 @@ struct Cut {
 // ring, 25 by pairs, 39 by large tiles; 256 tiles, 56 steps: 34, 43, 67; 1024 tiles, 56 steps: 126, 108, 88).
 // Joining parts takes 3.5 us, and 2 ps for each of the 4-byte sums, written and read.  A stream takes 3 us, what its workgroups read of B
 // and of up to 64 rows of A, in rounds of 256, at 62 bytes / ns, and 0.4 of the time of reading B from memory.
-inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 5 + 1.5 * steps : way == kRing ? 4 + 0.58 * steps : 4.5 + 0.92 * steps; }
+inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 10 + 1.45 * steps : way == kRing ? 4 + 0.58 * steps : 4.5 + 0.92 * steps; }
 inline int at_once(Way way) { return way == kPairs ? 512 : 256; }
 inline double rounds_of(Way way, long long tiles)
 {
@@ -790,7 +790,7 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
             if (parts != wanted) continue;
             const double rounds = rounds_of(way, static_cast<long long>(m_tiles) * n_tiles * parts);
             const size_t bytes = parts == 1 ? 0 : static_cast<size_t>(parts) * m * ((columns + 7) / 8 * 8) * times * 4;
-            const double us = rounds * tile_us(way, part_steps) + (parts == 1 ? 0 : 3.5 + 0.5e-6 * static_cast<double>(bytes));
+            const double us = rounds * tile_us(way, part_steps) + (parts == 1 ? 0 : 3.5 + 0.2 * parts + 0.5e-6 * static_cast<double>(bytes));
             if (best.parts == 0 || us < best.us) best = {way, m_tiles, n_tiles, parts, part_steps, bytes, us};
         }
     }
