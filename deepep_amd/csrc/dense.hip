@@ -7,6 +7,7 @@
 // All of them are products C[m,n] = sum_k A(m,k) B(n,k) of operands that hold k or m / n contiguously, with something done to a
 // result before it is stored.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -647,19 +648,20 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
 }
 
 // ---- few rows: a stream of B ------------------------------------------------------------------------------------------------------
-// For few rows of A the time is that of reading B.  A workgroup makes 16 columns (kGated: 8 of gate and the same 8 of up) for up to 16 kBlocks rows; its eight waves take
+// For few rows of A the time is that of reading B.  A workgroup makes kGroups times 16 columns (kGated: 8 of gate and the same 8 of up) for up to 16 kBlocks rows; its eight waves take
 // every eighth line of 128 bytes of k, and their sums meet in LDS at the end.  Each wave has a ring of its own in LDS, into which its lines of B and A
 // go straight from memory, 8 rows of whole lines a load, and waits for nobody else on the way.  (Read to registers in the matrix instruction's own order a load of
 // A touches 64 lines instead of 8: 64 rows of 7168, 4096 columns took 37 us by that.)
 // One token: 7168 to 2 x 2048 in BF16 (59 MB) 12.0 us, 2048 to 7168 (29 MB) 8.4, 7168 to 4096 in 8 bits (29 MB) 7.6, where an empty kernel takes 2 to 3.
-template <int kType, Finish kFinish, int kBlocks, int kStages>
+template <int kType, Finish kFinish, int kGroups, int kBlocks, int kStages>
 __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
 {
     constexpr int kValue = kType == kInt8 ? 1 : 2, kWaves = kThreads / kWave;
-    constexpr int kLoads = 2 + 2 * kBlocks, kStage = kLoads * 1024;  // of a wave for a line
-    constexpr int kWide = kFinish == kGated ? 8 : 16;                // columns of the result
+    constexpr int kLoadsB = 2 * kGroups, kLoads = kLoadsB + 2 * kBlocks, kStage = kLoads * 1024;  // of a wave for a line
+    constexpr int kWide = kGroups * (kFinish == kGated ? 8 : 16);                                 // columns of the result
+    static_assert(kLoads >= 4 && kLoads <= 10);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves * kStages * kStage];
-    static_assert(sizeof(lds) >= kWaves * kBlocks * 1024);
+    static_assert(sizeof(lds) >= kWaves * kGroups * kBlocks * 1024);
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n0 = blockIdx.x * kWide, m0 = blockIdx.y * 16 * kBlocks, rows = min(16 * kBlocks, p.m - m0);
     const int k_bytes = p.k * kValue, lines = (k_bytes + kStepBytes - 1) / kStepBytes;
@@ -668,9 +670,10 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
     int records[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-        const int n = n0 + (kFinish == kGated ? 0 : 8 * j), row = j < 2 ? (kFinish == kGated && j == 1 ? p.columns : 0) + n : m0 + (j - 2) * 8;
-        const int there = min(8, j < 2 ? p.columns - n : rows - (j - 2) * 8);
-        base[j] = reinterpret_cast<uint64_t>(j < 2 ? p.b : p.a) + static_cast<uint64_t>(row) * k_bytes;
+        const bool of_b = j < kLoadsB;
+        const int n = n0 + 8 * (kFinish == kGated ? j / 2 : j), in_a = (j - kLoadsB) * 8;
+        const int row = of_b ? (kFinish == kGated && j % 2 == 1 ? p.columns : 0) + n : m0 + in_a, there = min(8, of_b ? p.columns - n : rows - in_a);
+        base[j] = reinterpret_cast<uint64_t>(of_b ? p.b : p.a) + static_cast<uint64_t>(row) * k_bytes;
         records[j] = __builtin_amdgcn_readfirstlane(max(there, 0)) * k_bytes;  // (a number between two bounds comes from a vector instruction)
     }
     // Lane l loads a piece of row l / 8, which lies in LDS where the pieces of eight rows that are read together meet no bank twice.
@@ -685,13 +688,15 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
         load_to_lds<1024>(from(1), place, to);
         load_to_lds<2048>(from(2), place, to);
         load_to_lds<3 * 1024>(from(3), place, to);
-        if constexpr (kBlocks >= 2) {
+        if constexpr (kLoads >= 6) {
             load_to_lds<4096>(from(4), place, to);
             load_to_lds<5120>(from(5), place, to);
         }
-        if constexpr (kBlocks >= 4) {
+        if constexpr (kLoads >= 8) {
             load_to_lds<6144>(from(6), place, to);
             load_to_lds<7168>(from(7), place, to);
+        }
+        if constexpr (kLoads >= 10) {
             load_to_lds<8192>(from(8), place, to);
             load_to_lds<9216>(from(9), place, to);
         }
@@ -700,18 +705,19 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
     int read_at[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) read_at[s] = wave * kStages * kStage + lane % 16 * kStepBytes + ((4 * s + lane / 16) ^ (lane & 7)) * 16;
-    Sum<kType> acc[kBlocks] = {};
+    Sum<kType> acc[kGroups][kBlocks] = {};
 #pragma unroll
     for (int i = 0; i < kStages; ++i) ask(i);
     int stage = 0;
     for (int line = wave; line < lines; line += kWaves) {
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
-        u32x4 b[2], a[kBlocks][2];
+        u32x4 b[kGroups][2], a[kBlocks][2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            b[s] = *reinterpret_cast<const u32x4*>(lds + read_at[s] + stage * kStage);
 #pragma unroll
-            for (int i = 0; i < kBlocks; ++i) a[i][s] = *reinterpret_cast<const u32x4*>(lds + read_at[s] + stage * kStage + 2048 * (i + 1));
+            for (int g = 0; g < kGroups; ++g) b[g][s] = *reinterpret_cast<const u32x4*>(lds + read_at[s] + stage * kStage + 2048 * g);
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) a[i][s] = *reinterpret_cast<const u32x4*>(lds + read_at[s] + stage * kStage + 2048 * (kGroups + i));
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the stage is read, and may be asked for again)
         __builtin_amdgcn_sched_barrier(0);
@@ -720,35 +726,41 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < kBlocks; ++i) acc[i] = multiply<kType>(b[s], a[i][s], acc[i]);
+            for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i) acc[g][i] = multiply<kType>(b[g][s], a[i][s], acc[g][i]);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    // Lane (g, r) has results 4 g .. 4 g + 3 of row r: sums[wave][block][row][16].
-    uint32_t(*const sums)[kBlocks][16][16] = reinterpret_cast<uint32_t(*)[kBlocks][16][16]>(lds);
+    // Lane (q, r) has results 4 q .. 4 q + 3 of row r: sums[wave][group][block][row][16].
+    uint32_t(*const sums)[kGroups][kBlocks][16][16] = reinterpret_cast<uint32_t(*)[kGroups][kBlocks][16][16]>(lds);
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) *reinterpret_cast<u32x4*>(&sums[wave][i][lane % 16][lane / 16 * 4]) = __builtin_bit_cast(u32x4, acc[i]);
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) *reinterpret_cast<u32x4*>(&sums[wave][g][i][lane % 16][lane / 16 * 4]) = __builtin_bit_cast(u32x4, acc[g][i]);
     __syncthreads();
     const int m = threadIdx.x % (16 * kBlocks), octet = threadIdx.x / (16 * kBlocks);
-    if (octet >= (kFinish == kGated ? 1 : 2) || m >= rows) return;
-    const auto total = [&](int o, float (&v)[8]) {
+    if (octet >= kWide / 8 || m >= rows) return;
+    const auto total = [&](int group, int o, float (&v)[8]) {
         Sum<kType> sum[2] = {};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) sum[h] += __builtin_bit_cast(Sum<kType>, *reinterpret_cast<const u32x4*>(&sums[w][m / 16][m % 16][8 * o + 4 * h]));
+            for (int h = 0; h < 2; ++h) sum[h] += __builtin_bit_cast(Sum<kType>, *reinterpret_cast<const u32x4*>(&sums[w][group][m / 16][m % 16][8 * o + 4 * h]));
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(sum[e / 4][e % 4]);
     };
+    const int n = n0 + 8 * octet;
+    if (n >= p.columns) return;
     float v[8];
-    total(octet, v);
     if constexpr (kFinish == kGated) {
         float up[8];
-        total(1, up);
-        finish_gated<kType>(p.out, m0 + m, n0, p.columns, v, up);
+        total(octet, 0, v);
+        total(octet, 1, up);
+        finish_gated<kType>(p.out, m0 + m, n, p.columns, v, up);
     } else {
-        const int n = n0 + 8 * octet;
-        if (n < p.columns) finish<kType, kFinish>(p.out, m0 + m, n, p.columns, v);
+        total(octet / 2, octet % 2, v);
+        finish<kType, kFinish>(p.out, m0 + m, n, p.columns, v);
     }
 }
 
@@ -763,9 +775,13 @@ struct Cut {
 // compute unit 0.92, with 5, 4 and 4.5 us around a tile's steps; a last round of pairs takes 0.75 of a whole one with no more than one tile a compute unit, 0.85 and up
 // with more.  So pairs win from one to about two and a half tiles of 128 a compute unit, and where k is short (8-bit integers, 400 tiles, 23 steps: 31 us by the
 // ring, 25 by pairs, 39 by large tiles; 256 tiles, 56 steps: 34, 43, 67; 1024 tiles, 56 steps: 126, 108, 88).
-// Joining parts takes 3.5 us, and 2 ps for each of the 4-byte sums, written and read.  A stream takes 3 us, what its workgroups read of B
-// and of up to 64 rows of A, in rounds of 256, at 62 bytes / ns, and 0.4 of the time of reading B from memory.
+// Joining parts takes 3.5 us and 0.2 a part, and 2 ps for each of the 4-byte sums, written and read.  A round of 256 workgroups of a stream takes 3 us and what one
+// reads of B and of up to 64 rows of A, at 62 bytes / ns; beside that counts 0.4 of the time of reading B from memory.
 inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 10 + 1.45 * steps : way == kRing ? 4 + 0.58 * steps : 4.5 + 0.92 * steps; }
+// Groups of 16 columns of a stream's workgroup.  Two read A half as often: for more tiles than compute units, and for up to 16 rows if they then fit one round; above that, two
+// workgroups on a compute unit, with rings of two stages, end more evenly.  (16-bit, 14 rows of 6544 to 2 x 3304 and back, 413 and 409 tiles: 36 us by twos, 40 by ones; 24 rows, 7168
+// to 2 x 2048: 27, 30; 8-bit, 3 rows of 15440 to 9681, 606 tiles: 42, 34.)
+inline int stream_groups(int m, int n_tiles) { return n_tiles <= 256 || m > 32 || (m <= 16 && n_tiles > 512) ? 1 : 2; }
 inline int at_once(Way way) { return way == kPairs ? 512 : 256; }
 inline double rounds_of(Way way, long long tiles)
 {
@@ -778,9 +794,10 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
     const int steps = std::max(1, (k_bytes + kStepBytes - 1) / kStepBytes), times = gated ? 2 : 1;
     Cut best = {};
     if (!turned) {
-        const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64;
-        const double rounds = std::max(1.0, static_cast<double>(n_tiles) * m_tiles / 256), read = static_cast<double>(16 + std::min(m, 64)) * k_bytes;
-        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 3 + rounds * read / 62e3 + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
+        const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64, groups = stream_groups(m, n_tiles);
+        const double workgroups = static_cast<double>((n_tiles + groups - 1) / groups) * m_tiles, read = static_cast<double>(16 * groups + std::min(m, 64)) * k_bytes / 62e3;
+        const double rounds = m <= 16 && groups == 1 ? 3 + std::max(1.0, workgroups / 256) * read : std::ceil(workgroups / 256) * (3 + read);
+        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 0.5 + rounds + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
     }
     for (const Way way : {kRing, kPairs, kLargeTiles}) {
         const int tile = way == kLargeTiles ? 256 : 128, wide = tile / times;
@@ -803,12 +820,14 @@ int launch(Product p, const Cut& c, void* partial, hipStream_t stream)
     if (p.m == 0 || p.columns == 0) return DPEP_OK;
     if constexpr (!kTransA && !kTransB) {
         if (c.way == kStream) {
-            const dim3 grid(c.n_tiles, c.m_tiles);
-            // (rings of two stages leave room for a second workgroup)
-            if (p.m <= 16 && c.n_tiles <= 256) stream_kernel<kType, kFinish, 1, 5><<<grid, kThreads, 0, stream>>>(p);
-            else if (p.m <= 16) stream_kernel<kType, kFinish, 1, 2><<<grid, kThreads, 0, stream>>>(p);
-            else if (p.m <= 32) stream_kernel<kType, kFinish, 2, 3><<<grid, kThreads, 0, stream>>>(p);
-            else stream_kernel<kType, kFinish, 4, 2><<<grid, kThreads, 0, stream>>>(p);
+            const int groups = stream_groups(p.m, c.n_tiles);
+            const dim3 grid((c.n_tiles + groups - 1) / groups, c.m_tiles);
+            if (p.m <= 16 && groups == 2) stream_kernel<kType, kFinish, 2, 1, 3><<<grid, kThreads, 0, stream>>>(p);
+            else if (p.m <= 16 && c.n_tiles <= 256) stream_kernel<kType, kFinish, 1, 1, 5><<<grid, kThreads, 0, stream>>>(p);
+            else if (p.m <= 16) stream_kernel<kType, kFinish, 1, 1, 2><<<grid, kThreads, 0, stream>>>(p);
+            else if (p.m <= 32 && groups == 2) stream_kernel<kType, kFinish, 2, 2, 2><<<grid, kThreads, 0, stream>>>(p);
+            else if (p.m <= 32) stream_kernel<kType, kFinish, 1, 2, 3><<<grid, kThreads, 0, stream>>>(p);
+            else stream_kernel<kType, kFinish, 1, 4, 2><<<grid, kThreads, 0, stream>>>(p);
             return launch_status("product of few rows");
         }
     }
