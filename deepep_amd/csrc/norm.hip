@@ -262,8 +262,38 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const dpep_norm p)
     }
 }
 
-// ---- tokens in 8-bit integers, rows of any length ----------------------------------------------------------------------------------
-// Two passes over a row, which the second finds in the L2 (rows of up to 65536 values do not fit a workgroup's registers).  100 FP16 rows of 2880: 3.0 us.
+// ---- tokens in 8-bit integers -----------------------------------------------------------------------------------------------------
+// A row in a workgroup's registers, as in the norm.  100 FP16 rows of 2880: 3.0 us.
+template <int kThreads, int kChunks, int kType>
+__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* x, int k, uint8_t* codes, float* scales)
+{
+    __shared__ uint32_t tops[kThreads / kWave];
+    const size_t row = static_cast<size_t>(blockIdx.x) * k;
+    Raw<kType> raw[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int at = (c * kThreads + static_cast<int>(threadIdx.x)) * kVec;
+        if (at < k) raw[c] = load_raw<kType>(x, row + at);
+    }
+    uint32_t largest = 0;
+    float v[kVec];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        if ((c * kThreads + static_cast<int>(threadIdx.x)) * kVec >= k) continue;
+        widen<kType>(raw[c], v);
+        largest = max(largest, magnitude(v));
+    }
+    const TokenScale token(block_max<kThreads>(largest, tops));
+    if (threadIdx.x == 0) scales[blockIdx.x] = token.scale;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int at = (c * kThreads + static_cast<int>(threadIdx.x)) * kVec;
+        if (at >= k) continue;
+        widen<kType>(raw[c], v);
+        *reinterpret_cast<u32x2*>(codes + row + at) = token.codes(v);
+    }
+}
+// Rows that do not fit: two passes, of which the second finds the row in the L2 (4380 BF16 rows of 14736: 52 us by two passes, 31 by one).
 template <int kType>
 __global__ __launch_bounds__(256) void quantize_tokens_kernel(const void* x, int k, uint8_t* codes, float* scales)
 {
@@ -385,10 +415,15 @@ __global__ __launch_bounds__(1024) void sum_partial_kernel(const float* partial,
     if (group == 0 && blockIdx.x * 64 + mine < hidden) out[blockIdx.x * 64 + mine] = v;
 }
 
-// Workgroups of the backward, one to a compute unit: each row of `partial` is written and read again (16384 rows of 7168, both directions: 342 us with 256,
-// 354 with 512; 777 of 2880: 16.6 and 19.1).
-constexpr int kBackwardGroups = 256;
-inline int backward_groups(int tokens) { return std::min(tokens, kBackwardGroups); }
+// Workgroups of the backward.  More of them have more loads under way, but each writes a row of `partial` that is read again: one to a compute unit for long rows, two
+// for rows of up to 4096 values, four for up to 1024, and four rows each at least (BF16, us with 256, 512 and 1024 workgroups: 9240 rows of 1024 33, 22, 20; of 2144 37, 29, 33; of
+// 4096 46, 44, 48; of 7168 79, 82, 86; 777 of 2880 10.9, 12.1, 15).
+inline int backward_groups(int tokens, int hidden)
+{
+    int groups = hidden <= 1024 ? 1024 : hidden <= 4096 ? 512 : 256;
+    while (groups > 256 && tokens < 4 * groups) groups /= 2;
+    return std::min(tokens, groups);
+}
 
 // The kernel for rows of `hidden` values: f(threads, chunks).  Few rows leave the machine empty and each is as quick as its longest thread; of many, four
 // pieces a thread keep more loads under way.
@@ -466,7 +501,7 @@ int dpep_rms_norm(const dpep_norm* n, void* stream)
 size_t dpep_rms_norm_backward_scratch_bytes(int num_tokens, int hidden)
 {
     if (num_tokens < 0 || hidden < 0) return 0;
-    return static_cast<size_t>(backward_groups(num_tokens)) * hidden * 4;
+    return static_cast<size_t>(backward_groups(num_tokens, hidden)) * hidden * 4;
 }
 
 int dpep_rms_norm_backward(const dpep_norm_gradients* g, void* scratch, void* stream)
@@ -475,7 +510,7 @@ int dpep_rms_norm_backward(const dpep_norm_gradients* g, void* scratch, void* st
     if (int rc = check_rows("rms_norm_backward", g->type, g->weight_type, g->num_tokens, g->hidden); rc != DPEP_OK) return rc;
     DPEP_REQUIRE(g->weight != nullptr && g->grad_weight != nullptr, "rms_norm_backward: a NULL buffer");
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const int groups = backward_groups(g->num_tokens);
+    const int groups = backward_groups(g->num_tokens, g->hidden);
     if (groups > 0) {
         DPEP_REQUIRE(g->grad_y != nullptr && g->stream != nullptr && g->rstd != nullptr && g->grad_x != nullptr && scratch != nullptr, "rms_norm_backward: a NULL buffer");
         DPEP_REQUIRE(aligned16(g->grad_y) && aligned16(g->stream) && aligned16(g->weight) && aligned16(g->grad_stream) && aligned16(g->grad_x) && aligned16(scratch),
@@ -511,8 +546,14 @@ int dpep_quantize_tokens(const void* x, int type, int num_tokens, int k, int8_t*
     const size_t cells = static_cast<size_t>(num_tokens) * k, rows = cells * bytes_of(type);
     const Span written[] = {{codes, cells}, {scales, num_tokens * 4ull}}, read[] = {{x, rows}};
     DPEP_REQUIRE(apart(written, read), "quantize_tokens: an output overlaps x or the other output");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    uint8_t* const to = reinterpret_cast<uint8_t*>(codes);
     by_type(type, [&](auto t) {
-        quantize_tokens_kernel<decltype(t)::value><<<num_tokens, 256, 0, static_cast<hipStream_t>(stream)>>>(x, k, reinterpret_cast<uint8_t*>(codes), scales);
+        if (k <= DPEP_NORM_MAX_HIDDEN)
+            by_hidden(num_tokens, k, [&](auto threads, auto chunks) {
+                quantize_rows_kernel<decltype(threads)::value, decltype(chunks)::value, decltype(t)::value><<<num_tokens, decltype(threads)::value, 0, s>>>(x, k, to, scales);
+            });
+        else quantize_tokens_kernel<decltype(t)::value><<<num_tokens, 256, 0, s>>>(x, k, to, scales);
     });
     return launch_status("quantize_tokens");
 }
