@@ -652,7 +652,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p)
 // every eighth line of 128 bytes of k, and their sums meet in LDS at the end.  Each wave has a ring of its own in LDS, into which its lines of B and A
 // go straight from memory, 8 rows of whole lines a load, and waits for nobody else on the way.  (Read to registers in the matrix instruction's own order a load of
 // A touches 64 lines instead of 8: 64 rows of 7168, 4096 columns took 37 us by that.)
-// One token: 7168 to 2 x 2048 in BF16 (59 MB) 12.0 us, 2048 to 7168 (29 MB) 8.4, 7168 to 4096 in 8 bits (29 MB) 7.6, where an empty kernel takes 2 to 3.
+// One token: 7168 to 2 x 2048 in BF16 (59 MB) 12.0 us, 2048 to 7168 (29 MB) 7.3, 7168 to 4096 in 8 bits (29 MB) 7.6, where an empty kernel takes 2 to 3.
 template <int kType, Finish kFinish, int kGroups, int kBlocks, int kStages>
 __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
 {

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const dpep_norm p)
 }
 
 // ---- tokens in 8-bit integers -----------------------------------------------------------------------------------------------------
-// A row in a workgroup's registers, as in the norm.  100 FP16 rows of 2880: 3.0 us.
+// A row in a workgroup's registers, as in the norm.  100 FP16 rows of 2880: 2.6 us.
 template <int kThreads, int kChunks, int kType>
 __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const void* x, int k, uint8_t* codes, float* scales)
 {
