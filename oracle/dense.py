@@ -30,7 +30,7 @@ def norm_backward(g, s, weight, eps, grad_stream=None):
     if grad_stream is not None:
         grad, size = grad + grad_stream, size + np.abs(grad_stream)
     each = np.abs(g * hat).sum(axis=0)
-    # (a column is summed over the rows of a workgroup, one of up to 256, then over those)
+    # (a column is summed over the rows of a workgroup, of which there are 256 to 1024 if there are as many rows, then over those: 64 at a time)
     return grad, 4 * NORM_SLACK * size, (g * hat).sum(axis=0), (NORM_SLACK + (len(s) / 256 + 64) * EPS32) * each
 
 

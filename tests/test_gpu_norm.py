@@ -135,6 +135,22 @@ def test_gradients(tokens, hidden, dtype, weight, residual):
     assert torch.equal(grad_x, again[0]) and torch.equal(grad_w, again[1])
 
 
+@pytest.mark.parametrize("tokens,hidden,dtype", [(1300, 2056, "bf16"), (2050, 2880, "fp16"), (2100, 264, "bf16"), (4100, 4096, "bf16"), (4099, 1024, "fp32"), (9001, 512, "bf16"), (20000, 72, "fp16")])
+def test_gradients_of_many_rows(tokens, hidden, dtype):
+    """Sizes that take more workgroups than compute units, with all numbers of rows to one."""
+    from deepep_amd import dense
+
+    x, w, _, rng = _make(tokens, hidden, dtype, "fp32", False)
+    normed = dense.rms_norm(x, w, eps=EPS)
+    g = _rows(rng, tokens, hidden, dtype)
+    grad_x, grad_w = dense.rms_norm_backward(g, normed.stream, w, normed.rstd)
+    want, bound, want_w, bound_w = od.norm_backward(_wide(g), _wide(x), _wide(w), EPS)
+    _check(grad_x, want, bound, dtype)
+    _check(grad_w, want_w, bound_w, "fp32")
+    again = dense.rms_norm_backward(g, normed.stream, w, normed.rstd)
+    assert torch.equal(grad_x, again[0]) and torch.equal(grad_w, again[1])
+
+
 def test_no_rows():
     from deepep_amd import dense, w8
 

@@ -66,6 +66,22 @@ def test_tokens(rows, k, dtype):
     assert (np.abs(codes.double().cpu().numpy() - target) <= 0.5 + 8 * od.EPS32 * 127).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,k", [(1, 512), (300, 512), (300, 528), (2, 2064), (257, 2048), (257, 4112), (300, 8192), (300, 8208), (3, 16384), (260, 16384), (3, 16400), (300, 20000)])
+def test_tokens_of_all_widths(rows, k, dtype):
+    """Rows in a workgroup's registers, in each number of pieces, and rows that do not fit."""
+    from deepep_amd import w8
+
+    rng = np.random.default_rng(rows * 7 + k)
+    x = torch.from_numpy(rng.normal(size=(rows, k)) * (0.1 + rng.random((rows, 1)))).to(DTYPES[dtype]).cuda()
+    x[-1, -1] = 7.5  # a row's largest value in its last place
+    codes, scales = w8.quantize_tokens(x)
+    target, want = od.tokens(x.double().cpu().numpy())
+    assert (np.abs(scales.double().cpu().numpy() - want) <= 2 * od.EPS32 * want).all()
+    assert (np.abs(codes.double().cpu().numpy() - target) <= 0.5 + 8 * od.EPS32 * 127).all()
+    assert codes[-1, -1] == 127
+
+
 @pytest.mark.parametrize("rows", [1, 12, 40, 300])
 def test_wide_rows_are_quantised_in_the_call(rows):
     from deepep_amd import w8
