@@ -782,6 +782,7 @@ inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 10 + 1.4
 // workgroups on a compute unit, with rings of two stages, end more evenly.  (16-bit, 14 rows of 6544 to 2 x 3304 and back, 413 and 409 tiles: 36 us by twos, 40 by ones; 24 rows, 7168
 // to 2 x 2048: 27, 30; 8-bit, 3 rows of 15440 to 9681, 606 tiles: 42, 34.)
 inline int stream_groups(int m, int n_tiles) { return n_tiles <= 256 || m > 32 || (m <= 16 && n_tiles > 512) ? 1 : 2; }
+inline double join_us(int parts, size_t bytes) { return 3.5 + 0.2 * parts + 0.5e-6 * static_cast<double>(bytes); }
 inline int at_once(Way way) { return way == kPairs ? 512 : 256; }
 inline double rounds_of(Way way, long long tiles)
 {
@@ -807,13 +808,32 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
             if (parts != wanted) continue;
             const double rounds = rounds_of(way, static_cast<long long>(m_tiles) * n_tiles * parts);
             const size_t bytes = parts == 1 ? 0 : static_cast<size_t>(parts) * m * ((columns + 7) / 8 * 8) * times * 4;
-            const double us = rounds * tile_us(way, part_steps) + (parts == 1 ? 0 : 3.5 + 0.2 * parts + 0.5e-6 * static_cast<double>(bytes));
+            const double us = rounds * tile_us(way, part_steps) + (parts == 1 ? 0 : join_us(parts, bytes));
             if (best.parts == 0 || us < best.us) best = {way, m_tiles, n_tiles, parts, part_steps, bytes, us};
         }
     }
     return best;
 }
 
+inline Product cut_up(Product p, const Cut& c, void* partial)
+{
+    p.m_tiles = c.m_tiles;
+    p.n_tiles = c.n_tiles;
+    p.parts = c.parts;
+    p.part_steps = c.part_steps;
+    p.pitch = (p.columns + 7) / 8 * 8;
+    p.partial = partial;
+    return p;
+}
+// The sums of a product's parts, if it has any.
+template <int kType, Finish kFinish>
+int join(const Product& p, hipStream_t stream)
+{
+    const size_t pieces = static_cast<size_t>(p.m) * (p.pitch / 8);
+    if (p.parts == 1 || pieces == 0) return DPEP_OK;
+    join_kernel<kType, kFinish><<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream>>>(p);
+    return launch_status("product's parts");
+}
 template <int kType, bool kTransA, bool kTransB, Finish kFinish>
 int launch(Product p, const Cut& c, void* partial, hipStream_t stream)
 {
@@ -831,22 +851,15 @@ int launch(Product p, const Cut& c, void* partial, hipStream_t stream)
             return launch_status("product of few rows");
         }
     }
-    p.m_tiles = c.m_tiles;
-    p.n_tiles = c.n_tiles;
-    p.parts = c.parts;
-    p.part_steps = c.part_steps;
-    p.pitch = (p.columns + 7) / 8 * 8;
-    p.partial = partial;
+    p = cut_up(p, c, partial);
     const long long groups = static_cast<long long>(c.m_tiles) * c.n_tiles * c.parts;
     DPEP_REQUIRE(groups <= 0x7fffff, "a product of %d x %d is too large", p.m, p.columns);
     const dim3 grid(static_cast<unsigned>(groups));
     if (c.way == kLargeTiles) tile_kernel<kType, kTransA, kTransB, kFinish, kLargeTiles><<<grid, kThreads, 0, stream>>>(p);
     else if (c.way == kPairs) tile_kernel<kType, kTransA, kTransB, kFinish, kPairs><<<grid, kThreads, 0, stream>>>(p);
     else tile_kernel<kType, kTransA, kTransB, kFinish, kRing><<<grid, kThreads, 0, stream>>>(p);
-    if (int rc = launch_status("product"); rc != DPEP_OK || c.parts == 1) return rc;
-    const size_t pieces = static_cast<size_t>(p.m) * (p.pitch / 8);
-    join_kernel<kType, kFinish><<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream>>>(p);
-    return launch_status("product's parts");
+    if (int rc = launch_status("product"); rc != DPEP_OK) return rc;
+    return join<kType, kFinish>(p, stream);
 }
 
 // When `slots` that take tiles as they get free are done with the tiles of three products, tiles[i] of us[i] each, one product after the other.
@@ -879,50 +892,87 @@ double done_after(int slots, const long long (&tiles)[3], const double (&us)[3])
     return end;
 }
 
-// Three products (of 16-bit values, results stored, no part of another's operands), together if that is quicker than one after the other with 4 us for a launch.
+// Three products of 16-bit values without a part of another's operands: together in one launch, long tiles first and short ones to fill up, if that is quicker than one after
+// the other with 4 us for a launch; a product of long k may be split there too.
 // (8192 tokens, 4096 and 2048 values: 605 us with the product before them together in large tiles, 690 apart; 2048 tokens, 2048 and 1024: 72 in large tiles, 80 in pairs, 83 in the
-// ring, 86 apart; 16000, 640 and 160: 127 in the ring, 69 apart, with k in parts.)
-template <int kType>
-int launch_three(const Product (&products)[3], const Cut (&cuts)[3], void* partial, hipStream_t stream)
-{
-    double least = 8;
-    for (const Cut& c : cuts) least += c.us;
+// ring, 86 apart; 16000, 640 and 160: 127 in the ring, 69 apart, with k in parts; 6175, 912 and 240, both directions:
+// 95 without parts, 75 with.)
+struct Together {
+    bool quicker = false;
+    Way way = kRing;
     int order[3] = {0, 1, 2};
-    std::sort(order, order + 3, [&](int a, int b) { return products[a].k > products[b].k; });  // (long tiles first, short ones fill up)
-    Products best = {};
-    Way best_way = kRing;
-    for (const Way way : {kRing, kPairs, kLargeTiles}) {
-        const int tile = way == kLargeTiles ? 256 : 128;
-        Products now = {};
-        long long tiles[3], begin = 0;
-        double us[3];
-        for (int i = 0; i < 3; ++i) {
-            Product p = products[order[i]];
-            p.m_tiles = (p.m + tile - 1) / tile;
-            p.n_tiles = (p.columns + tile - 1) / tile;
-            p.parts = 1;
-            p.part_steps = std::max(1, (p.k * 2 + kStepBytes - 1) / kStepBytes);
-            us[i] = tile_us(way, p.part_steps);
-            tiles[i] = static_cast<long long>(p.m_tiles) * p.n_tiles;
-            now.of[i] = p;
-            now.begin[i] = static_cast<unsigned>(begin);
-            begin += tiles[i];
+    Cut cuts[3] = {};  // of the products, by their own number
+    size_t bytes = 0;  // of the parts' sums of all
+};
+Together together_of(const int (&m)[3], const int (&columns)[3], const int (&k)[3], const Cut (&apart)[3])
+{
+    Together best;
+    double least = 8 + apart[0].us + apart[1].us + apart[2].us;
+    for (const Way way : {kRing, kPairs, kLargeTiles})
+        for (const int most : {1 << 30, 64, 32, 16, 8}) {  // steps of a part
+            const int tile = way == kLargeTiles ? 256 : 128;
+            Together now;
+            now.way = way;
+            double joins = 0;
+            bool cut = false;
+            for (int i = 0; i < 3; ++i) {
+                Cut& c = now.cuts[i];
+                const int steps = std::max(1, (k[i] * 2 + kStepBytes - 1) / kStepBytes), wanted = std::min(16, (steps - 1) / most + 1);
+                c.m_tiles = (m[i] + tile - 1) / tile;
+                c.n_tiles = (columns[i] + tile - 1) / tile;
+                c.part_steps = (steps + wanted - 1) / wanted;
+                c.parts = (steps + c.part_steps - 1) / c.part_steps;
+                c.bytes = c.parts == 1 ? 0 : static_cast<size_t>(c.parts) * m[i] * ((columns[i] + 7) / 8 * 8) * 4;
+                if (c.parts == 1 || m[i] == 0) continue;
+                cut = true;
+                joins += join_us(c.parts, c.bytes);
+                now.bytes += c.bytes;
+            }
+            if (most != 1 << 30 && !cut) continue;
+            std::sort(now.order, now.order + 3, [&](int x, int y) { return now.cuts[x].part_steps > now.cuts[y].part_steps; });
+            long long tiles[3], all = 0;
+            double us[3];
+            for (int i = 0; i < 3; ++i) {
+                const Cut& c = now.cuts[now.order[i]];
+                tiles[i] = static_cast<long long>(c.m_tiles) * c.n_tiles * c.parts;
+                us[i] = tile_us(way, c.part_steps);
+                all += tiles[i];
+            }
+            const double done = joins + done_after(at_once(way), tiles, us) * (way == kPairs && all <= 256 ? 0.75 : 1.0);
+            if (all <= 0x7fffff && done < least) {
+                least = done;
+                best = now;
+                best.quicker = true;
+            }
         }
-        now.begin[3] = static_cast<unsigned>(begin);
-        const double done = done_after(at_once(way), tiles, us) * (way == kPairs && begin <= 256 ? 0.75 : 1.0);
-        if (begin <= 0x7fffff && done < least) best = now, least = done, best_way = way;
+    return best;
+}
+
+template <int kType>
+int launch_three(const Product (&products)[3], const Cut (&apart)[3], const Together& together, void* partial, hipStream_t stream)
+{
+    if (!together.quicker) {
+        for (int i = 0; i < 3; ++i) {
+            const int rc = products[i].turned_a != 0 ? launch<kType, true, true, kStore>(products[i], apart[i], partial, stream)
+                                                     : launch<kType, false, true, kStore>(products[i], apart[i], partial, stream);
+            if (rc != DPEP_OK) return rc;
+        }
+        return DPEP_OK;
     }
-    if (best.begin[3] != 0) {
-        if (best_way == kLargeTiles) products_kernel<kType, kLargeTiles><<<best.begin[3], kThreads, 0, stream>>>(best);
-        else if (best_way == kPairs) products_kernel<kType, kPairs><<<best.begin[3], kThreads, 0, stream>>>(best);
-        else products_kernel<kType, kRing><<<best.begin[3], kThreads, 0, stream>>>(best);
-        return launch_status("products");
-    }
+    Products all = {};
+    uint8_t* sums = static_cast<uint8_t*>(partial);
     for (int i = 0; i < 3; ++i) {
-        const int rc = products[i].turned_a != 0 ? launch<kType, true, true, kStore>(products[i], cuts[i], partial, stream)
-                                                 : launch<kType, false, true, kStore>(products[i], cuts[i], partial, stream);
-        if (rc != DPEP_OK) return rc;
+        const Cut& c = together.cuts[together.order[i]];
+        Product& p = all.of[i] = cut_up(products[together.order[i]], c, sums);
+        sums += c.bytes;
+        all.begin[i + 1] = all.begin[i] + static_cast<unsigned>(p.m_tiles) * p.n_tiles * p.parts;
     }
+    if (together.way == kLargeTiles) products_kernel<kType, kLargeTiles><<<all.begin[3], kThreads, 0, stream>>>(all);
+    else if (together.way == kPairs) products_kernel<kType, kPairs><<<all.begin[3], kThreads, 0, stream>>>(all);
+    else products_kernel<kType, kRing><<<all.begin[3], kThreads, 0, stream>>>(all);
+    if (int rc = launch_status("products"); rc != DPEP_OK) return rc;
+    for (const Product& p : all.of)
+        if (int rc = join<kType, kStore>(p, stream); rc != DPEP_OK) return rc;
     return DPEP_OK;
 }
 
@@ -950,13 +1000,15 @@ struct ForwardCuts {
     }
 };
 struct BackwardCuts {
-    Cut rows, three[3];  // dh; dx, dWgu, dWd
+    Cut rows, three[3];  // dh; dx, dWgu, dWd, apart
+    Together together;
     size_t scratch;
     BackwardCuts(int tokens, int hidden, int inter)
         : rows(cut_of(tokens, inter, hidden * 2, false, true)),
           three{cut_of(tokens, hidden, inter * 4, false, true), cut_of(2 * inter, hidden, tokens * 2, false, true), cut_of(hidden, inter, tokens * 2, false, true)},
+          together(together_of({tokens, 2 * inter, hidden}, {hidden, hidden, inter}, {2 * inter, tokens, tokens}, three)),
           scratch(whole(static_cast<size_t>(tokens) * inter * 2) + whole(static_cast<size_t>(tokens) * inter * 4) +
-                  std::max(std::max(rows.bytes, three[0].bytes), std::max(three[1].bytes, three[2].bytes)))
+                  std::max(rows.bytes, together.quicker ? together.bytes : std::max(three[0].bytes, std::max(three[1].bytes, three[2].bytes))))
     {
     }
 };
@@ -1042,7 +1094,7 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
         products[1].out.c = grad_gate_up;
         products[2].out.c = grad_down;
         products[1].turned_a = products[2].turned_a = 1;
-        return launch_three<kType>(products, cuts.three, partial, s);
+        return launch_three<kType>(products, cuts.three, cuts.together, partial, s);
     });
 }
 

@@ -31,7 +31,7 @@ def _check(got, want, bound):
 
 SIZES = [  # tokens, hidden, inter
     (3, 4104, 2056), (16, 4504, 2312), (20, 4104, 2064), (40, 4104, 2064), (250, 2088, 1000), (500, 4104, 1032), (1001, 2888, 1400), (1500, 1032, 1408), (1600, 640, 160),
-    (16000, 640, 160), (2047, 2056, 1016), (16000, 128, 4104), (4090, 4072, 2040), (8100, 4040, 2008),
+    (16000, 640, 160), (2047, 2056, 1016), (16000, 128, 4104), (103, 296, 4552), (590, 984, 3592), (6175, 912, 240), (36, 5848, 1928), (4090, 4072, 2040), (8100, 4040, 2008),
 ]
 
 
