@@ -72,7 +72,7 @@ struct Output {
     int type;           // of C where kScaled
 };
 
-// 1 / (1 + 2^(-g log2 e)) by the machine's own power and reciprocal, each good to a step: off by some (|g| share + 2) 2^-24, while h and dz are rounded to 2^-8 or 2^-11.  (The library's exponential
+// 1 / (1 + 2^(-g log2 e)) by the machine's own power and reciprocal, each good to a step: off by some (|g| (1 - share) + 2) 2^-24 of it, while h and dz are rounded to 2^-8 or 2^-11.  (The library's exponential
 // and division are some 25 instructions a value: dh of 2048 tokens, 2048 and 1024 values 25.6 us with them, 24.1 so.)
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g)); }
 
