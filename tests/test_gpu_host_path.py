@@ -3,6 +3,7 @@ and outgrown by it, row-major payloads that walk past their grid, the routing co
 handles that leave the native path, and memory that is handed out again behind asynchronous calls."""
 
 import ctypes
+import os
 import threading
 import time
 
@@ -636,6 +637,41 @@ def test_other_python_threads_run_while_a_dispatch_waits_for_its_row_count():
         assert let_in >= 15
     finally:
         stop.set()
+        thread.join(timeout=60)
+        buffer.destroy()
+
+
+def test_a_thread_on_the_same_cpu_runs_while_a_dispatch_waits():
+    """The wait for the row count polls; a thread that it lets in runs even if it has no other CPU than the one that polls."""
+    x, _ = _batch(64, 256, 2, 3)
+    idx = torch.stack([torch.randperm(8)[:2] for _ in range(64)]).cuda()
+    xd = x.cuda()
+    buffer = _buffer(num_bytes=4 << 20)
+    turns, stop = [0], threading.Event()
+    allowed = os.sched_getaffinity(0)
+    one = {min(allowed)}
+
+    def other():
+        os.sched_setaffinity(0, one)
+        while not stop.is_set():
+            turns[0] += 1
+
+    thread = threading.Thread(target=other)
+    try:
+        buffer.dispatch(xd, topk_idx=idx, num_experts=8)
+        os.sched_setaffinity(0, one)
+        thread.start()
+        let_in = 0
+        for _ in range(20):
+            torch.cuda.synchronize()
+            torch.cuda._sleep(40_000)
+            before = turns[0]
+            buffer.dispatch(xd, topk_idx=idx, num_experts=8)
+            let_in += turns[0] > before
+        assert let_in >= 10
+    finally:
+        stop.set()
+        os.sched_setaffinity(0, allowed)
         thread.join(timeout=60)
         buffer.destroy()
 
