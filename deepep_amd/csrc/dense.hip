@@ -1117,7 +1117,7 @@ int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int
     if (num_rows == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && x_scales != nullptr && y != nullptr && aligned16(x), "w8_matmul: a NULL or misaligned buffer");
     const Cut cut = cut_of(num_rows, w->n, w->k, false, false);
-    DPEP_REQUIRE(scratch != nullptr || cut.bytes == 0, "w8_matmul: scratch is NULL");
+    DPEP_REQUIRE(cut.bytes == 0 || (scratch != nullptr && aligned16(scratch)), "w8_matmul: scratch is NULL or misaligned");
     const size_t results = static_cast<size_t>(num_rows) * w->n * (type == DPEP_TYPE_F32 ? 4 : 2);
     const Span written[] = {{y, results}, {scratch, cut.bytes}};
     const Span read[] = {{x, static_cast<size_t>(num_rows) * w->k}, {x_scales, num_rows * 4ull}, {w->codes, static_cast<size_t>(w->n) * w->k}, {w->scales, w->n * 4ull}};

@@ -521,7 +521,7 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
 int dpep_quantize_tokens(const void* x, int type, int num_tokens, int k, int8_t* codes, float* scales, void* stream);
 /* y[t,n] = x_scales[t] scales[n] sum_k x[t,k] codes[n,k]: integer sums, exact; scaled in fp32, rounded once to `type`.
  *   codes int8 [N,K], x int8 [T,K]: 16-byte aligned, K a multiple of 16 up to DPEP_W8_MAX_K;  scales fp32 [N];  x_scales fp32 [T];  y [T,N];
- *   scratch  dpep_w8_matmul_scratch_bytes;  y and scratch overlap no input, nor one another */
+ *   scratch  dpep_w8_matmul_scratch_bytes, 16-byte aligned;  y and scratch overlap no input, nor one another */
 #define DPEP_W8_MAX_K 65536
 #define DPEP_W8_MAX_N 0x1fffff
 #define DPEP_W8_MAX_ROWS 0x1fffff

@@ -214,6 +214,16 @@ def test_c_abi_refuses_what_overlaps():
     _refused(lib.dpep_quantize_tokens(at, 1, 4, 32, 2 * at, 2 * at + 64, None), "other output")
 
 
+def test_c_abi_refuses_scratch_that_is_not_aligned():
+    """The parts' sums are stored and read 16 bytes at a time."""
+    lib, far = _lib.load(), 1 << 30  # (no call below reaches memory)
+    w = ops._W8(1 << 20, 3 << 20, 300, 16384)
+    assert lib.dpep_w8_matmul_scratch_bytes(300, 300, 16384) > 0
+    for off in (1, 4, 8):
+        _refused(lib.dpep_w8_matmul(ctypes.byref(w), far, 2 * far, 300, 1, 3 * far, 4 * far + off, None), "scratch is NULL or misaligned")
+    _refused(lib.dpep_w8_matmul(ctypes.byref(w), far, 2 * far, 300, 1, 3 * far, None, None), "scratch is NULL or misaligned")
+
+
 def test_quantize_rounds_to_half_a_step():
     gen = torch.Generator().manual_seed(0)
     w = torch.randn(5, 48, generator=gen)
