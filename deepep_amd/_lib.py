@@ -74,6 +74,7 @@ SIGNATURES = {
     "dpep_gated_ffn_backward": (_I, (_P, _P, _P, _P, _I, _P, _P, _P, _P, _P)),
     "dpep_quantize_tokens": (_I, (_P, _I, _I, _I, _P, _P, _P)),
     "dpep_w8_matmul_scratch_bytes": (_Z, (_I, _I, _I)),
+    "dpep_product_choices": (_I, (_I, _I, _I, _I, _P)),
     "dpep_w8_matmul": (_I, (_P, _P, _P, _I, _I, _P, _P, _P)),
 }
 

@@ -766,6 +766,8 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const Product p)
     }
 }
 
+constexpr long long kMostWorkgroups = 0x7fffff;  // of kThreads: a grid has less than 2^32 threads
+
 // How a product is cut up, k into parts whose sums another kernel adds up.
 struct Cut {
     Way way;
@@ -784,6 +786,16 @@ inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 10 + 1.4
 // workgroups on a compute unit, with rings of two stages, end more evenly.  (16-bit, 14 rows of 6544 to 2 x 3304 and back, 413 and 409 tiles: 36 us by twos, 40 by ones; 24 rows, 7168
 // to 2 x 2048: 27, 30; 8-bit, 3 rows of 15440 to 9681, 606 tiles: 42, 34.)
 inline int stream_groups(int m, int n_tiles) { return n_tiles <= 256 || m > 32 || (m <= 16 && n_tiles > 512) ? 1 : 2; }
+struct Stream {
+    int groups, blocks, stages;
+};
+inline Stream stream_of(int m, int n_tiles)
+{
+    const int groups = stream_groups(m, n_tiles);
+    if (m <= 16) return {groups, 1, groups == 2 ? 3 : n_tiles <= 256 ? 5 : 2};
+    if (m <= 32) return {groups, 2, groups == 2 ? 2 : 3};
+    return {1, 4, 2};
+}
 inline double join_us(int parts, size_t bytes) { return 3.5 + 0.2 * parts + 0.5e-6 * static_cast<double>(bytes); }
 inline int at_once(Way way) { return way == kPairs ? 512 : 256; }
 inline double rounds_of(Way way, long long tiles)
@@ -807,8 +819,9 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
         const int m_tiles = (m + tile - 1) / tile, n_tiles = (columns + wide - 1) / wide;
         for (int wanted = 1; wanted <= 16; ++wanted) {
             const int part_steps = (steps + wanted - 1) / wanted, parts = (steps + part_steps - 1) / part_steps;
-            if (parts != wanted) continue;
-            const double rounds = rounds_of(way, static_cast<long long>(m_tiles) * n_tiles * parts);
+            const long long workgroups = static_cast<long long>(m_tiles) * n_tiles * parts;
+            if (parts != wanted || workgroups > kMostWorkgroups) continue;
+            const double rounds = rounds_of(way, workgroups);
             const size_t bytes = parts == 1 ? 0 : static_cast<size_t>(parts) * m * ((columns + 7) / 8 * 8) * times * 4;
             const double us = rounds * tile_us(way, part_steps) + (parts == 1 ? 0 : join_us(parts, bytes));
             if (best.parts == 0 || us < best.us) best = {way, m_tiles, n_tiles, parts, part_steps, bytes, us};
@@ -842,21 +855,19 @@ int launch(Product p, const Cut& c, void* partial, hipStream_t stream)
     if (p.m == 0 || p.columns == 0) return DPEP_OK;
     if constexpr (!kTransA && !kTransB) {
         if (c.way == kStream) {
-            const int groups = stream_groups(p.m, c.n_tiles);
-            const dim3 grid((c.n_tiles + groups - 1) / groups, c.m_tiles);
-            if (p.m <= 16 && groups == 2) stream_kernel<kType, kFinish, 2, 1, 3><<<grid, kThreads, 0, stream>>>(p);
-            else if (p.m <= 16 && c.n_tiles <= 256) stream_kernel<kType, kFinish, 1, 1, 5><<<grid, kThreads, 0, stream>>>(p);
-            else if (p.m <= 16) stream_kernel<kType, kFinish, 1, 1, 2><<<grid, kThreads, 0, stream>>>(p);
-            else if (p.m <= 32 && groups == 2) stream_kernel<kType, kFinish, 2, 2, 2><<<grid, kThreads, 0, stream>>>(p);
-            else if (p.m <= 32) stream_kernel<kType, kFinish, 1, 2, 3><<<grid, kThreads, 0, stream>>>(p);
+            const Stream shape = stream_of(p.m, c.n_tiles);
+            const dim3 grid((c.n_tiles + shape.groups - 1) / shape.groups, c.m_tiles);
+            if (shape.blocks == 1 && shape.groups == 2) stream_kernel<kType, kFinish, 2, 1, 3><<<grid, kThreads, 0, stream>>>(p);
+            else if (shape.blocks == 1 && shape.stages == 5) stream_kernel<kType, kFinish, 1, 1, 5><<<grid, kThreads, 0, stream>>>(p);
+            else if (shape.blocks == 1) stream_kernel<kType, kFinish, 1, 1, 2><<<grid, kThreads, 0, stream>>>(p);
+            else if (shape.blocks == 2 && shape.groups == 2) stream_kernel<kType, kFinish, 2, 2, 2><<<grid, kThreads, 0, stream>>>(p);
+            else if (shape.blocks == 2) stream_kernel<kType, kFinish, 1, 2, 3><<<grid, kThreads, 0, stream>>>(p);
             else stream_kernel<kType, kFinish, 1, 4, 2><<<grid, kThreads, 0, stream>>>(p);
             return launch_status("product of few rows");
         }
     }
     p = cut_up(p, c, partial);
-    const long long groups = static_cast<long long>(c.m_tiles) * c.n_tiles * c.parts;
-    DPEP_REQUIRE(groups <= 0x7fffff, "a product of %d x %d is too large", p.m, p.columns);
-    const dim3 grid(static_cast<unsigned>(groups));
+    const dim3 grid(static_cast<unsigned>(c.m_tiles) * c.n_tiles * c.parts);
     if (c.way == kLargeTiles) tile_kernel<kType, kTransA, kTransB, kFinish, kLargeTiles><<<grid, kThreads, 0, stream>>>(p);
     else if (c.way == kPairs) tile_kernel<kType, kTransA, kTransB, kFinish, kPairs><<<grid, kThreads, 0, stream>>>(p);
     else tile_kernel<kType, kTransA, kTransB, kFinish, kRing><<<grid, kThreads, 0, stream>>>(p);
@@ -941,7 +952,7 @@ Together together_of(const int (&m)[3], const int (&columns)[3], const int (&k)[
                 all += tiles[i];
             }
             const double done = joins + done_after(at_once(way), tiles, us) * (way == kPairs && all <= 256 ? 0.75 : 1.0);
-            if (all <= 0x7fffff && done < least) {
+            if (all <= kMostWorkgroups && done < least) {
                 least = done;
                 best = now;
                 best.quicker = true;
@@ -1015,6 +1026,27 @@ struct BackwardCuts {
     }
 };
 
+// Sizes of a block that its entry points take.
+inline bool block_fits(int tokens, int hidden, int inter)
+{
+    const auto dim = [](int d) { return d >= 8 && d % 8 == 0 && d <= DPEP_FFN_MAX_DIM; };
+    return tokens >= 0 && tokens <= DPEP_FFN_MAX_TOKENS && dim(hidden) && dim(inter);
+}
+inline bool product_fits(int rows, int n, int k)
+{
+    return rows >= 0 && rows <= DPEP_W8_MAX_ROWS && n >= 1 && n <= DPEP_W8_MAX_N && k >= 16 && k % 16 == 0 && k <= DPEP_W8_MAX_K &&
+           (rows + 255ll) / 256 * ((n + 255ll) / 256) <= kMostWorkgroups;
+}
+inline dpep_product_choice choice_of(const Cut& c, int m, bool together)
+{
+    dpep_product_choice choice = {c.way, c.parts, 0, 0, 0, together, static_cast<int64_t>(c.m_tiles) * c.n_tiles * c.parts};
+    if (c.way != kStream) return choice;
+    const Stream shape = stream_of(m, c.n_tiles);
+    choice.stream_groups = shape.groups, choice.stream_blocks = shape.blocks, choice.stream_stages = shape.stages;
+    choice.workgroups = static_cast<int64_t>((c.n_tiles + shape.groups - 1) / shape.groups) * c.m_tiles;
+    return choice;
+}
+
 template <class F>
 int by_type(int type, F f)
 {
@@ -1030,7 +1062,7 @@ extern "C" {
 
 size_t dpep_gated_ffn_scratch_bytes(int num_tokens, int hidden, int inter)
 {
-    return num_tokens < 0 || hidden < 0 || inter < 0 ? 0 : ForwardCuts(num_tokens, hidden, inter).scratch;
+    return block_fits(num_tokens, hidden, inter) ? ForwardCuts(num_tokens, hidden, inter).scratch : 0;
 }
 
 int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, float* kept, void* scratch, void* stream)
@@ -1060,7 +1092,7 @@ int dpep_gated_ffn(const dpep_ffn* f, const void* x, int num_tokens, void* y, fl
 
 size_t dpep_gated_ffn_backward_scratch_bytes(int num_tokens, int hidden, int inter)
 {
-    return num_tokens < 0 || hidden < 0 || inter < 0 ? 0 : BackwardCuts(num_tokens, hidden, inter).scratch;
+    return block_fits(num_tokens, hidden, inter) ? BackwardCuts(num_tokens, hidden, inter).scratch : 0;
 }
 
 int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x, const float* kept, int num_tokens, void* grad_x, void* grad_gate_up,
@@ -1100,10 +1132,33 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
     });
 }
 
+int dpep_product_choices(int operation, int rows, int a, int b, dpep_product_choice* choices)
+{
+    DPEP_REQUIRE(choices != nullptr, "product_choices: choices is NULL");
+    DPEP_REQUIRE(operation >= DPEP_PRODUCTS_FFN && operation <= DPEP_PRODUCTS_W8, "product_choices: operation=%d is not one of DPEP_PRODUCTS_*", operation);
+    DPEP_REQUIRE(operation == DPEP_PRODUCTS_W8 ? product_fits(rows, a, b) : block_fits(rows, a, b), "product_choices: %d, %d and %d are not taken", rows, a, b);
+    if (operation == DPEP_PRODUCTS_W8) {
+        choices[0] = choice_of(cut_of(rows, a, b, false, false), rows, false);
+        return 1;
+    }
+    if (operation == DPEP_PRODUCTS_FFN) {
+        const ForwardCuts cuts(rows, a, b);
+        choices[0] = choice_of(cuts.gate_up, rows, false);
+        choices[1] = choice_of(cuts.down, rows, false);
+        return 2;
+    }
+    const BackwardCuts cuts(rows, a, b);
+    choices[0] = choice_of(cuts.rows, rows, false);
+    for (int i = 0; i < 3; ++i) {
+        choices[1 + i] = choice_of(cuts.together.quicker ? cuts.together.cuts[i] : cuts.three[i], rows, cuts.together.quicker);
+        if (cuts.together.quicker) choices[1 + i].way = cuts.together.way;
+    }
+    return 4;
+}
+
 size_t dpep_w8_matmul_scratch_bytes(int num_rows, int n, int k)
 {
-    if (num_rows < 0 || n < 0 || k < 0) return 0;
-    return cut_of(num_rows, n, k, false, false).bytes;
+    return product_fits(num_rows, n, k) ? cut_of(num_rows, n, k, false, false).bytes : 0;
 }
 
 int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int num_rows, int type, void* y, void* scratch, void* stream)
@@ -1113,6 +1168,7 @@ int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int
     DPEP_REQUIRE(w->k >= 16 && w->k % 16 == 0 && w->k <= DPEP_W8_MAX_K, "w8_matmul: K=%d is not a multiple of 16 in [16, %d]", w->k, DPEP_W8_MAX_K);
     DPEP_REQUIRE(w->n >= 1 && w->n <= DPEP_W8_MAX_N, "w8_matmul: N=%d is not in [1, %d]", w->n, DPEP_W8_MAX_N);
     DPEP_REQUIRE(num_rows >= 0 && num_rows <= DPEP_W8_MAX_ROWS, "w8_matmul: T=%d is not in [0, %d]", num_rows, DPEP_W8_MAX_ROWS);
+    DPEP_REQUIRE(product_fits(num_rows, w->n, w->k), "w8_matmul: T=%d times N=%d is too large", num_rows, w->n);
     DPEP_REQUIRE(w->codes != nullptr && w->scales != nullptr && aligned16(w->codes), "w8_matmul: a NULL or misaligned matrix");
     if (num_rows == 0) return DPEP_OK;
     DPEP_REQUIRE(x != nullptr && x_scales != nullptr && y != nullptr && aligned16(x), "w8_matmul: a NULL or misaligned buffer");

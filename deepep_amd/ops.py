@@ -980,3 +980,21 @@ def w8_matmul(x, codes, scales, dtype=None):
         status = lib.dpep_w8_matmul(ctypes.byref(call), _ptr(x_codes), _ptr(x_scales), rows, _TYPES[dtype], _ptr(y), _ptr(scratch), _stream(dev))
     _lib.check(status, "w8_matmul")
     return y
+
+
+class _ProductChoice(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("way", "parts", "stream_groups", "stream_blocks", "stream_stages", "together")] + [("workgroups", ctypes.c_int64)]
+
+
+PRODUCT_WAYS = ("stream", "ring", "pairs", "large")
+_PRODUCTS = {"ffn": 0, "ffn_backward": 1, "w8": 2}  # DPEP_PRODUCTS_*
+
+
+def product_choices(operation: str, rows: int, a: int, b: int):
+    """How calls of these sizes make their products: dicts of ``way`` (of ``PRODUCT_WAYS``), ``parts`` of k, ``stream`` (groups, blocks, stages; or None), ``together`` and
+    ``workgroups``.  ``operation``: ``"ffn"`` (rows, H, I: gate and up, then down), ``"ffn_backward"`` (dh, then the gradients of x, gate_up and down) or ``"w8"`` (rows, N, K).  Host arithmetic only."""
+    made = (_ProductChoice * 4)()
+    count = _lib.load().dpep_product_choices(_PRODUCTS[operation], rows, a, b, made)
+    _lib.check(min(count, 0), "product_choices")
+    return [dict(way=PRODUCT_WAYS[c.way], parts=c.parts, stream=(c.stream_groups, c.stream_blocks, c.stream_stages) if c.way == 0 else None, together=bool(c.together),
+                 workgroups=c.workgroups) for c in made[:count]]

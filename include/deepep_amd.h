@@ -521,7 +521,8 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
 int dpep_quantize_tokens(const void* x, int type, int num_tokens, int k, int8_t* codes, float* scales, void* stream);
 /* y[t,n] = x_scales[t] scales[n] sum_k x[t,k] codes[n,k]: integer sums, exact; scaled in fp32, rounded once to `type`.
  *   codes int8 [N,K], x int8 [T,K]: 16-byte aligned, K a multiple of 16 up to DPEP_W8_MAX_K;  scales fp32 [N];  x_scales fp32 [T];  y [T,N];
- *   scratch  dpep_w8_matmul_scratch_bytes, 16-byte aligned;  y and scratch overlap no input, nor one another */
+ *   scratch  dpep_w8_matmul_scratch_bytes, 16-byte aligned;  y and scratch overlap no input, nor one another
+ * ceil(T/256) ceil(N/256) is below 2^23 (results of 550 G and more do not fit the card). */
 #define DPEP_W8_MAX_K 65536
 #define DPEP_W8_MAX_N 0x1fffff
 #define DPEP_W8_MAX_ROWS 0x1fffff
@@ -532,6 +533,22 @@ typedef struct dpep_w8 {
 } dpep_w8;
 size_t dpep_w8_matmul_scratch_bytes(int num_rows, int n, int k);
 int dpep_w8_matmul(const dpep_w8* w, const int8_t* x, const float* x_scales, int num_rows, int type, void* y, void* scratch, void* stream);
+
+/* How calls of these sizes make their products, for tests and diagnosis.  Host arithmetic only.
+ *   operation  DPEP_PRODUCTS_FFN: of rows, a = H and b = I, the gate and up product and the down product;  _FFN_BACKWARD: dh, then the gradients of x, gate_up and
+ *              down;  _W8: of rows, a = N and b = K, one
+ *   choices    room for 4.  Returns how many there are, or an error below zero */
+#define DPEP_PRODUCTS_FFN 0
+#define DPEP_PRODUCTS_FFN_BACKWARD 1
+#define DPEP_PRODUCTS_W8 2
+typedef struct dpep_product_choice {
+    int32_t way;      /* 0 a stream of the matrix, tiles of 128 in a ring (1) or two workgroups to a compute unit (2), tiles of 256 (3) */
+    int32_t parts;    /* of k; where there are more than one another kernel adds up their sums */
+    int32_t stream_groups, stream_blocks, stream_stages; /* of a stream: groups of 16 columns and blocks of 16 rows of a workgroup, stages of its rings */
+    int32_t together; /* in one launch with the other two */
+    int64_t workgroups;
+} dpep_product_choice;
+int dpep_product_choices(int operation, int rows, int a, int b, dpep_product_choice* choices);
 
 #ifdef __cplusplus
 }

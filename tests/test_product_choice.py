@@ -1,0 +1,40 @@
+"""How the gated block's and the 8-bit products are cut up (host arithmetic, no GPU needed)."""
+
+import ctypes
+
+import pytest
+
+from deepep_amd import _lib, ops
+
+MOST_WORKGROUPS = 0x7FFFFF  # of 512 threads
+
+
+@pytest.mark.parametrize("operation,sizes", [
+    ("ffn", (2097151, 8, 32768)), ("ffn", (2097151, 8, 65536)), ("ffn", (2097151, 65536, 8)), ("ffn", (2097151, 65536, 65536)), ("ffn", (1, 65536, 65536)),
+    ("ffn_backward", (2097151, 8, 65536)), ("ffn_backward", (2097151, 65536, 8)), ("ffn_backward", (2097151, 65536, 65536)),
+    ("w8", (2097151, 131072, 16)), ("w8", (2097151, 131072, 65536)), ("w8", (1, 2097151, 65536)), ("w8", (261888, 2097151, 16)),
+])
+def test_cuts_of_the_largest_sizes_can_be_launched(operation, sizes):
+    choices = ops.product_choices(operation, *sizes)
+    together = [c for c in choices if c["together"]]
+    assert all(c["workgroups"] <= MOST_WORKGROUPS for c in choices) and sum(c["workgroups"] for c in together) <= MOST_WORKGROUPS
+
+
+def test_products_that_cannot_be_launched_are_refused():
+    lib, at = _lib.load(), 1 << 20  # (no call below reaches memory)
+    w = ops._W8(at, at, 2097151, 16)
+    assert lib.dpep_w8_matmul(ctypes.byref(w), at, at, 2097151, 1, at, at, None) == -1
+    assert "too large" in lib.dpep_last_error().decode()
+    assert lib.dpep_w8_matmul_scratch_bytes(2097151, 2097151, 16) == 0
+
+
+def test_sizes_that_no_call_takes():
+    lib = _lib.load()
+    for bad in (("ffn", 1, 12, 8), ("ffn", 1, 8, 65544), ("ffn_backward", -1, 8, 8), ("ffn", 1 << 21, 8, 8), ("w8", 1, 0, 16), ("w8", 1, 8, 24), ("w8", 1 << 21, 8, 16)):
+        with pytest.raises(ValueError, match="product_choices"):
+            ops.product_choices(*bad)
+    assert lib.dpep_product_choices(0, 1, 8, 8, None) == -1 and lib.dpep_product_choices(3, 1, 8, 8, ctypes.byref((ops._ProductChoice * 4)())) == -1
+    for bad in ((-1, 8, 8), (1 << 21, 8, 8), (1, 1 << 30, 8), (1, 8, 0x7FFFFFF8)):
+        assert lib.dpep_gated_ffn_scratch_bytes(*bad) == 0 and lib.dpep_gated_ffn_backward_scratch_bytes(*bad) == 0
+    for bad in ((-1, 8, 16), (1, 1 << 30, 16), (1, 8, 0x7FFFFFF0)):
+        assert lib.dpep_w8_matmul_scratch_bytes(*bad) == 0
