@@ -149,13 +149,14 @@ __device__ __forceinline__ uint32_t magnitude(const float (&v)[kVec])
     return m;
 }
 
-// 8 codes of a token's values, given the largest magnitude of the token.
+// 8 codes of a token's values, given the largest magnitude of the token.  Beside an infinity, whose own inverse is zero and would make a NaN of it, the others are zeros:
+// 2^-130 takes it to 127 with its sign and the largest finite number to 1/4.
 struct TokenScale {
     float inverse, scale;
     __device__ __forceinline__ explicit TokenScale(uint32_t largest)
     {
         const float m = __uint_as_float(max(largest, __float_as_uint(1e-20f)));
-        inverse = (1.0f / m) * 127.0f;
+        inverse = largest == 0x7f800000u ? 0x1p-130f : (1.0f / m) * 127.0f;
         scale = m / 127.0f;
     }
     __device__ __forceinline__ u32x2 codes(const float (&v)[kVec]) const

@@ -517,7 +517,7 @@ int dpep_gated_ffn_backward(const dpep_ffn* f, const void* grad_y, const void* x
 
 /* Tokens in 8-bit integers: scale = max(|x|) / 127 of the row (at least 1e-20 / 127), code = x * (127 / max(|x|)) rounded to nearest even.
  *   x [T,K] of `type`, 16-byte aligned, K a multiple of 16;  codes int8 [T,K] 16-byte aligned;  scales fp32 [T]
- * A row that holds a NaN gets a NaN for its scale, one that holds an infinity that. */
+ * A row that holds a NaN gets a NaN for its scale; one that holds infinities gets infinity, 127 with their sign for their codes and 0 for the others'. */
 int dpep_quantize_tokens(const void* x, int type, int num_tokens, int k, int8_t* codes, float* scales, void* stream);
 /* y[t,n] = x_scales[t] scales[n] sum_k x[t,k] codes[n,k]: integer sums, exact; scaled in fp32, rounded once to `type`.
  *   codes int8 [N,K], x int8 [T,K]: 16-byte aligned, K a multiple of 16 up to DPEP_W8_MAX_K;  scales fp32 [N];  x_scales fp32 [T];  y [T,N];

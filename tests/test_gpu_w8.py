@@ -122,6 +122,23 @@ def test_rows_that_are_not_finite():
     assert torch.isfinite(y[0]).all() and torch.isnan(y[1]).all() and not torch.isfinite(y[2]).any()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("k", [64, 2064, 20000])
+def test_infinities_keep_their_sign(dtype, k):
+    from deepep_amd import w8
+
+    most = torch.finfo(DTYPES[dtype]).max
+    x = torch.full((4, k), most, dtype=DTYPES[dtype], device="cuda")
+    x[0, 5], x[1, k - 1], x[2, 5], x[2, 6] = float("inf"), -float("inf"), float("inf"), -float("inf")
+    x[3, 5] = float("nan")
+    codes, scales = w8.quantize_tokens(x)
+    want = torch.zeros(3, k, dtype=torch.int8)
+    want[0, 5], want[1, k - 1], want[2, 5], want[2, 6] = 127, -127, 127, -127
+    assert torch.equal(codes[:3].cpu(), want) and (scales[:3] == float("inf")).all() and torch.isnan(scales[3])
+    y = w8.matmul((codes, scales), w8.W8Weights(torch.ones(8, k, dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda")))
+    assert (y[0] == float("inf")).all() and (y[1] == -float("inf")).all() and torch.isnan(y[2:]).all()
+
+
 def test_no_rows():
     from deepep_amd import w8
 
