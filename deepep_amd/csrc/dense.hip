@@ -72,8 +72,10 @@ struct Output {
     int type;           // of C where kScaled
 };
 
-// 1 / (1 + 2^(-g log2 e)) by the machine's own power and reciprocal, each good to a step: off by some (|g| (1 - share) + 2) 2^-24 of it, while h and dz are rounded to 2^-8 or 2^-11.  (The library's exponential
-// and division are some 25 instructions a value: dh of 2048 tokens, 2048 and 1024 values 25.6 us with them, 24.1 so.)
+// 1 / (1 + 2^(-g log2 e)) by the machine's own power and reciprocal, each good to a whole step, which is up to 2 x 2^-24 of a value.  The power's argument is off by 1.23 x 2^-24 of
+// itself (its rounding, and that of the constant), so that the share is off by up to ((1.23 |g| + 2) (1 - share) + 3) 2^-24 of it, and is 0 below 2^-126: some 8 x 2^-24 from g = -2 on, 1.23 |g| + 5
+// far below, while h and dz are rounded to 2^-8 or 2^-11.  (The library's exponential and division, off by a step or two, are some 25 instructions a value: dh of 2048 tokens, 2048 and
+// 1024 values 25.6 us with them, 24.1 so.)
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g)); }
 
 template <int kType>

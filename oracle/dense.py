@@ -63,6 +63,29 @@ def _silu(g):
     return g * share, share
 
 
+def _share_off(g, share):
+    """What the share may be off by in 32 bits, as 1 / (1 + 2^(-g log2 e)) with a power and a reciprocal that are good to a whole step (2 half steps, relative): the power's argument
+    is off by the half step of its product and 0.224 of one of the constant, 1.23 |g| half steps of the power, and the power by 2 more; these count by the power's share (1 - share)
+    of the sum, which is rounded once; the reciprocal 2.  What falls below 2^-126 may be lost."""
+    return ((1.23 * np.abs(g) + 2.0) * (1.0 - share) + 3.0) * EPS32 * share + 2.0**-126
+
+
+def h_off(g, u):
+    """What h = (g share) u may be off by in 32 bits, g and u exact: the share's, and two products."""
+    silu, share = _silu(g)
+    return np.abs(g * u) * _share_off(g, share) + 2 * EPS32 * np.abs(silu * u)
+
+
+def dz_off(dh, g, u):
+    """The same of dg = ((dh u) share) (1 + g (1 - share)) and du = (dh g) share: with w = 1 + q, q = g (1 - share), the share's where it is a factor, and three products; w's, which are
+    |g| times the share's, the rounding of 1 - share and of q, and that of the sum."""
+    silu, share = _silu(g)
+    q = g * (1.0 - share)
+    off, w = _share_off(g, share), np.abs(1.0 + q)
+    dg = np.abs(dh * u) * (w * (off + 3 * EPS32 * share) + (share + off) * (np.abs(g) * off + 2 * EPS32 * np.abs(q) + EPS32 * w))
+    return dg, np.abs(dh * g) * off + 2 * EPS32 * np.abs(dh * silu)
+
+
 def ffn(x, gate_up, down, dtype):
     """dict of y, its bound, and what a backward pass needs of the intermediate values."""
     inter = down.shape[1]
@@ -72,11 +95,11 @@ def ffn(x, gate_up, down, dtype):
     silu, share = _silu(g)
     h = silu * u
     # silu's slope is at most 1.1
-    h_off = 1.1 * g_off * (np.abs(u) + u_off) + np.abs(silu) * u_off + 8 * EPS32 * np.abs(h)
-    h_off = h_off + HALF[dtype] * (np.abs(h) + h_off) + TINY[dtype]
+    off = 1.1 * g_off * (np.abs(u) + u_off) + np.abs(silu) * u_off + h_off(g, u)
+    off = off + HALF[dtype] * (np.abs(h) + off) + TINY[dtype]
     y = h @ down.T
-    y_off = h_off @ np.abs(down).T + _sum_bound(inter, (np.abs(h) + h_off) @ np.abs(down).T)
-    return dict(y=y, y_off=y_off + HALF[dtype] * (np.abs(y) + y_off) + TINY[dtype], z=z, z_off=z_off, g=g, u=u, g_off=g_off, u_off=u_off, h=h, h_off=h_off, silu=silu,
+    y_off = off @ np.abs(down).T + _sum_bound(inter, (np.abs(h) + off) @ np.abs(down).T)
+    return dict(y=y, y_off=y_off + HALF[dtype] * (np.abs(y) + y_off) + TINY[dtype], z=z, z_off=z_off, g=g, u=u, g_off=g_off, u_off=u_off, h=h, h_off=off, silu=silu,
                 share=share)
 
 
@@ -89,15 +112,16 @@ def ffn_backward(grad_y, x, gate_up, down, dtype):
     dg, du = dh * f["u"] * slope, dh * f["silu"]
     size, u_size = np.abs(dh) + dh_off, np.abs(f["u"]) + f["u_off"]
     # silu's slope is at most 1.1 and its change at most 0.5
-    dg_off = 1.1 * (dh_off * u_size + size * f["u_off"]) + 0.5 * size * u_size * f["g_off"] + 16 * EPS32 * np.abs(dh * f["u"]) * 1.1
-    du_off = dh_off * np.abs(f["silu"]) + 1.1 * size * f["g_off"] + 16 * EPS32 * np.abs(du)
-    dz, dz_off = np.concatenate([dg, du], axis=1), np.concatenate([dg_off, du_off], axis=1)
-    dz_off = dz_off + HALF[dtype] * (np.abs(dz) + dz_off) + TINY[dtype]
+    own = dz_off(size, f["g"], u_size)
+    dg_off = 1.1 * (dh_off * u_size + size * f["u_off"]) + 0.5 * size * u_size * f["g_off"] + own[0]
+    du_off = dh_off * np.abs(f["silu"]) + 1.1 * size * f["g_off"] + own[1]
+    dz, off = np.concatenate([dg, du], axis=1), np.concatenate([dg_off, du_off], axis=1)
+    off = off + HALF[dtype] * (np.abs(dz) + off) + TINY[dtype]
 
     def product(a, b, a_off, b_off, k):
         value, size = a @ b, (np.abs(a) + a_off) @ (np.abs(b) + b_off)
-        off = size - np.abs(a) @ np.abs(b) + _sum_bound(k, size)
-        return value, off + HALF[dtype] * (np.abs(value) + off) + TINY[dtype]
+        all_off = size - np.abs(a) @ np.abs(b) + _sum_bound(k, size)
+        return value, all_off + HALF[dtype] * (np.abs(value) + all_off) + TINY[dtype]
 
     zero = 0.0
-    return [product(dz, gate_up, dz_off, zero, dz.shape[1]), product(dz.T, x, dz_off.T, zero, len(x)), product(grad_y.T, f["h"], zero, f["h_off"], len(x))]
+    return [product(dz, gate_up, off, zero, dz.shape[1]), product(dz.T, x, off.T, zero, len(x)), product(grad_y.T, f["h"], zero, f["h_off"], len(x))]

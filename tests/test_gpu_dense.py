@@ -138,6 +138,35 @@ def test_large_gates_saturate():
     assert (grads[1][4:8] == 0).all() and (grads[1][12:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tokens", [1, 200])
+def test_gates_of_all_sizes(tokens, dtype):
+    """The activation and its gradients by themselves: products of one term each, which are exact, so that what is off is the 32-bit arithmetic between them (more for large gates) and one
+    rounding to 16 bits."""
+    from deepep_amd import dense
+
+    size = 512
+    rng = np.random.default_rng(tokens)
+    gates = np.concatenate([-np.linspace(5, 80, 300), np.linspace(-5, 80, size - 300)])
+    rounded = lambda v: torch.from_numpy(v).to(DTYPES[dtype]).cuda()  # noqa: E731
+    x = torch.zeros(tokens, size, dtype=DTYPES[dtype], device="cuda")
+    x[0, 0] = 1
+    gate_up = torch.zeros(2 * size, size, dtype=DTYPES[dtype], device="cuda")
+    gate_up[:size, 0], gate_up[size:, 0] = rounded(gates), rounded(rng.normal(size=size) * np.exp(np.clip(-gates, 0, 60) if dtype == "bf16" else 0 * gates))
+    down = torch.eye(size, dtype=DTYPES[dtype], device="cuda")
+    grad_y = torch.zeros_like(x)
+    grad_y[0] = rounded(rng.normal(size=size))
+    y, kept = dense.gated_ffn(x, gate_up, down, keep=True)
+    assert torch.equal(kept[0], gate_up[:, 0].float()) and not kept[1:].any() and not y[1:].any()
+    _, grad_gate_up, _ = dense.gated_ffn_backward(grad_y, x, gate_up, down, kept)
+    g, u, dh = _wide(gate_up[:size, 0], gate_up[size:, 0], grad_y[0])
+    share = 1 / (1 + np.exp(-g))
+    dg, du = dh * u * share * (1 + g * (1 - share)), dh * g * share
+    for got, want, off in ((y[0], g * share * u, od.h_off(g, u)), (grad_gate_up[:size, 0], dg, od.dz_off(dh, g, u)[0]), (grad_gate_up[size:, 0], du, od.dz_off(dh, g, u)[1])):
+        assert (off <= 0.1 * od.HALF[dtype] * np.abs(want) + od.HALF[dtype] ** 2).all()  # (and says something)
+        _check(got, want, off + od.HALF[dtype] * (np.abs(want) + off) + od.TINY[dtype])
+
+
 @pytest.mark.parametrize("tokens", [1, 20, 200])
 def test_nothing_is_written_past_the_rows(tokens):
     """Results in the middle of larger buffers, through the C-ABI: what lies around them stays as it was."""
