@@ -417,7 +417,7 @@ __global__ __launch_bounds__(1024) void sum_partial_kernel(const float* partial,
 }
 
 // Workgroups of the backward.  More of them have more loads under way, but each writes a row of `partial` that is read again: one to a compute unit for long rows, two
-// for rows of up to 4096 values, four for up to 1024, and four rows each at least (BF16, us with 256, 512 and 1024 workgroups: 9240 rows of 1024 33, 22, 20; of 2144 37, 29, 33; of
+// for rows of up to 4096 values, four for up to 1024, more than one only where each then has four rows or more; up to 256 rows take a workgroup each (BF16, us with 256, 512 and 1024 workgroups: 9240 rows of 1024 33, 22, 20; of 2144 37, 29, 33; of
 // 4096 46, 44, 48; of 7168 79, 82, 86; 777 of 2880 10.9, 12.1, 15).
 inline int backward_groups(int tokens, int hidden)
 {
