@@ -37,7 +37,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     x, residual [T,H] FP32, BF16 or FP16, H a multiple of 8 up to 16384; weight [H] in x's type or FP32.  ``quantize``, from FP32 values:
     ``"fp8"`` codes float8_e4m3fn [T,H] and FP32 scales [T, ceil(H/128)], as ``ElasticBuffer.dispatch`` takes them (H a multiple of 16);
     ``"mxfp8"`` codes float8_e4m3fn and e8m0 bytes uint8 [T,H/32], as ``fp8_fp4_mega_moe`` takes them (H a multiple of 32);
-    ``"int8"`` codes int8 and FP32 scales [T], as ``w8.matmul`` takes them (H a multiple of 16).  ``output=False``: y is not stored."""
+    ``"int8"`` codes int8 and FP32 scales [T], as ``w8.matmul`` takes them (H a multiple of 16).  ``output=False``: y is not stored.
+
+    Squares are added up in FP32: values from 1.8e19 / sqrt(H) on, whose sum passes its range, are normed to 0."""
     done = _lib.host().rms_norm(x, weight, residual, eps, quantize, output)  # the ordinary call, made natively
     if done is None:
         done = ops.rms_norm(x, weight, residual, eps, quantize, output)

@@ -457,6 +457,8 @@ int dpep_w4_experts(const dpep_w4* gate_up, const dpep_w4* down, int type, const
  *     DPEP_QUANT_MXFP8  codes e4m3 [T,H], scales e8m0 bytes [T,H/32]: as dpep_mx_quant (H a multiple of 32), and the scale NaN (255) for a
  *                       block of 32 that holds a NaN or an infinity
  *     DPEP_QUANT_INT8   codes int8 [T,H], scales fp32 [T]: as dpep_quantize_tokens (H a multiple of 16)
+ * The squares are added up in fp32: a row whose sum passes its range (values of 1.8e19 / sqrt(H) and more) has rstd 0 and v 0, one whose mean square is below
+ * it and eps 0 an infinite rstd; what is not finite in a row stays in that row's results.
  * H is a multiple of 8, at most DPEP_NORM_MAX_HIDDEN; pointers to rows are 16-byte aligned; T below 2^23.  Outputs overlap no input but for stream_out, nor
  * one another. */
 #define DPEP_NORM_MAX_HIDDEN 16384

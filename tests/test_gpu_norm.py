@@ -179,6 +179,22 @@ def test_rows_that_are_not_finite_stay_in_their_rows():
         assert torch.isnan(got.y[2, 9]) and not torch.isfinite(got.scales[2]).all()
 
 
+def test_squares_that_pass_the_range_of_32_bits():
+    """As documented: a row whose squares' sum overflows is normed to zeros with rstd 0, and no other row knows of it."""
+    from deepep_amd import dense
+
+    rng = np.random.default_rng(16)
+    x, w = _rows(rng, 3, 256, "fp32"), _weight(rng, 256, "fp32")
+    want = dense.rms_norm(x, w)
+    x[1] = 1e20
+    got = dense.rms_norm(x, w)
+    assert got.rstd[1] == 0 and not got.y[1].any()
+    for row in (0, 2):
+        assert torch.equal(got.y[row], want.y[row])
+    grad_x, _ = dense.rms_norm_backward(x.sign(), x, w, got.rstd)
+    assert torch.isfinite(grad_x).all()
+
+
 def test_blocks_that_are_not_finite_have_a_scale_that_is_none():
     from deepep_amd import dense
 
