@@ -612,6 +612,8 @@ struct Products {
     Product of[3];
     unsigned begin[4];  // a product's first workgroup
 };
+static_assert(std::is_same_v<decltype(Product::turned_a), int> && sizeof(Product) % 8 == 0 && sizeof(Products) == 3 * sizeof(Product) + 4 * sizeof(unsigned),
+              "what is picked by a computed index is whole words, and nothing lies beside the products and their begins");
 template <int kType, Way kWay>
 __global__ __launch_bounds__(kThreads, Shape<kWay>::kWavesOfSimd) void products_kernel(const Products p)
 {
