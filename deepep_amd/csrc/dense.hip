@@ -784,7 +784,7 @@ struct Cut {
 // with more.  So pairs win from one to about two and a half tiles of 128 a compute unit, and where k is short (8-bit integers, 400 tiles, 23 steps: 31 us by the
 // ring, 25 by pairs, 39 by large tiles; 256 tiles, 56 steps: 34, 43, 67; 1024 tiles, 56 steps: 126, 108, 88).
 // Joining parts takes 3.5 us and 0.2 a part, and 2 ps for each of the 4-byte sums, written and read.  A round of 256 workgroups of a stream takes 3 us and what one
-// reads of B and of up to 64 rows of A, at 62 bytes / ns; beside that counts 0.4 of the time of reading B from memory.
+// reads of B and of up to 64 rows of A, at 62 bytes / ns; beside that count 0.4 us for each 256 workgroups (8-bit, 6 rows of 432 to 62901: 22.9 us by 3932 short ones, 9.9 by pairs) and 0.4 of the time of reading B from memory.
 inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 10 + 1.45 * steps : way == kRing ? 4 + 0.58 * steps : 4.5 + 0.92 * steps; }
 // Groups of 16 columns of a stream's workgroup.  Two read A half as often: for more tiles than compute units, and for up to 16 rows if they then fit one round; above that, two
 // workgroups on a compute unit, with rings of two stages, end more evenly.  (16-bit, 14 rows of 6544 to 2 x 3304 and back, 413 and 409 tiles: 36 us by twos, 40 by ones; 24 rows, 7168
@@ -802,6 +802,14 @@ inline Stream stream_of(int m, int n_tiles)
 }
 inline double join_us(int parts, size_t bytes) { return 3.5 + 0.2 * parts + 0.5e-6 * static_cast<double>(bytes); }
 inline int at_once(Way way) { return way == kPairs ? 512 : 256; }
+// No tiles are quicker than memory, which gives 5.4 MB / us where every place for a workgroup is taken, and as much less as the rounds leave free, to half of it.  (The steps' costs above are those of operands
+// that L2 holds for many tiles; of few rows every byte of B comes from memory.  8-bit, 4 rows of 28672 to 8192: 59 us by the pairs that the steps alone would choose, 43 by a stream; 1 row of 4096
+// to 128256 114 and 95; 16-bit, 8 rows of 18432 to 7168 156 and 138.  975 products of 1 to 400 rows, every way timed: the chosen one is 1.6 % above the quickest in the mean, 3.3 without this.)
+inline double memory_us(Way way, long long workgroups, double bytes)
+{
+    const double rounds = static_cast<double>(workgroups) / at_once(way);
+    return workgroups == 0 ? 0 : bytes / 5.4e6 * std::min(2.0, std::ceil(rounds) / rounds);
+}
 inline double rounds_of(Way way, long long tiles)
 {
     const long long whole = tiles / at_once(way), rest = tiles % at_once(way);
@@ -811,12 +819,13 @@ inline double rounds_of(Way way, long long tiles)
 Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
 {
     const int steps = std::max(1, (k_bytes + kStepBytes - 1) / kStepBytes), times = gated ? 2 : 1;
+    const double needed = (static_cast<double>(columns) * times + m) * k_bytes + 2.0 * m * columns;  // both operands and 16-bit results
     Cut best = {};
     if (!turned) {
         const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64, groups = stream_groups(m, n_tiles);
         const double workgroups = static_cast<double>((n_tiles + groups - 1) / groups) * m_tiles, read = static_cast<double>(16 * groups + std::min(m, 64)) * k_bytes / 62e3;
         const double rounds = m <= 16 && groups == 1 ? 3 + std::max(1.0, workgroups / 256) * read : std::ceil(workgroups / 256) * (3 + read);
-        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 0.5 + rounds + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
+        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 0.5 + rounds + 0.4 * workgroups / 256 + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
     }
     for (const Way way : {kRing, kPairs, kLargeTiles}) {
         const int tile = way == kLargeTiles ? 256 : 128, wide = tile / times;
@@ -827,7 +836,7 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
             if (parts != wanted || workgroups > kMostWorkgroups) continue;
             const double rounds = rounds_of(way, workgroups);
             const size_t bytes = parts == 1 ? 0 : static_cast<size_t>(parts) * m * ((columns + 7) / 8 * 8) * times * 4;
-            const double us = rounds * tile_us(way, part_steps) + (parts == 1 ? 0 : join_us(parts, bytes));
+            const double us = std::max(rounds * tile_us(way, part_steps), memory_us(way, workgroups, needed + bytes)) + (parts == 1 ? 0 : join_us(parts, bytes));
             if (best.parts == 0 || us < best.us) best = {way, m_tiles, n_tiles, parts, part_steps, bytes, us};
         }
     }
@@ -948,14 +957,15 @@ Together together_of(const int (&m)[3], const int (&columns)[3], const int (&k)[
             if (most != 1 << 30 && !cut) continue;
             std::sort(now.order, now.order + 3, [&](int x, int y) { return now.cuts[x].part_steps > now.cuts[y].part_steps; });
             long long tiles[3], all = 0;
-            double us[3];
+            double us[3], bytes = static_cast<double>(now.bytes);
             for (int i = 0; i < 3; ++i) {
                 const Cut& c = now.cuts[now.order[i]];
                 tiles[i] = static_cast<long long>(c.m_tiles) * c.n_tiles * c.parts;
                 us[i] = tile_us(way, c.part_steps);
                 all += tiles[i];
+                bytes += 2.0 * ((static_cast<double>(m[i]) + columns[i]) * k[i] + static_cast<double>(m[i]) * columns[i]);
             }
-            const double done = joins + done_after(at_once(way), tiles, us) * (way == kPairs && all <= 256 ? 0.75 : 1.0);
+            const double done = joins + std::max(done_after(at_once(way), tiles, us) * (way == kPairs && all <= 256 ? 0.75 : 1.0), memory_us(way, all, bytes));
             if (all <= kMostWorkgroups && done < least) {
                 least = done;
                 best = now;

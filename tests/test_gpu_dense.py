@@ -243,6 +243,27 @@ def test_two_streams_at_once():
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
+def test_two_streams_at_once_backward():
+    """The three products in one launch, on two streams with a scratch of each."""
+    from deepep_amd import dense, ops
+
+    assert all(c["together"] for c in ops.product_choices("ffn_backward", 700, 1032, 256)[1:]) and ops.product_choices("ffn_backward", 700, 1032, 256)[0]["parts"] > 1
+    sets = []
+    for seed in (1, 2):
+        x, gate_up, down, grad_y = _make(700, 1032, 256, "bf16", seed)
+        sets.append((grad_y, x, gate_up, down, dense.gated_ffn(x, gate_up, down, keep=True)[1]))
+    want = [dense.gated_ffn_backward(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(dense.gated_ffn_backward(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for grads in got[i] for a, b in zip(grads, want[i]))
+
+
 def test_unaligned_rows_and_parameters():
     from deepep_amd import dense
 

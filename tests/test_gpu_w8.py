@@ -169,6 +169,26 @@ def test_captured_products_replay(rows):
         assert torch.equal(y, want)
 
 
+def test_two_streams_at_once():
+    """k in parts, whose sums are scratch of each call, and rows quantised in the call."""
+    from deepep_amd import ops, w8
+
+    assert ops.product_choices("w8", 300, 40, 16384)[0]["parts"] > 1
+    gen = torch.Generator().manual_seed(4)
+    rows = [torch.randn(300, 16384, generator=gen).bfloat16().cuda() for _ in range(2)]
+    weights = w8.W8Weights(*_make(1, 40, 16384)[1])
+    want = [w8.matmul(x, weights) for x in rows]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in rows], [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(w8.matmul(rows[i], weights))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
 def test_matrix_quantised_once():
     from deepep_amd import w8
 

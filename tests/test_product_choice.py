@@ -20,6 +20,20 @@ def test_cuts_of_the_largest_sizes_can_be_launched(operation, sizes):
     assert all(c["workgroups"] <= MOST_WORKGROUPS for c in choices) and sum(c["workgroups"] for c in together) <= MOST_WORKGROUPS
 
 
+@pytest.mark.parametrize("operation,sizes,ways", [
+    # few rows on large matrices: nothing but the reading of the matrix counts
+    ("ffn", (1, 8192, 28672), ["stream", "stream"]), ("ffn", (4, 7168, 18432), ["stream", "stream"]), ("w8", (1, 128256, 4096), ["stream"]), ("w8", (4, 8192, 28672), ["stream"]),
+    # and many short workgroups their own starts
+    ("w8", (6, 62901, 432), ["pairs"]), ("ffn", (3, 280, 14928), ["pairs", "stream"]),
+    # what the rules were measured at before
+    ("ffn", (1, 7168, 2048), ["stream", "stream"]), ("ffn", (33, 2880, 1408), ["stream", "stream"]), ("ffn", (512, 7168, 2048), ["ring", "ring"]),
+    ("ffn", (8192, 7168, 2048), ["large", "large"]), ("ffn_backward", (8192, 7168, 2048), ["large"] * 4), ("ffn_backward", (1000, 2880, 1408), ["ring", "pairs", "pairs", "pairs"]),
+    ("w8", (1, 4096, 7168), ["stream"]), ("w8", (100, 1407, 2880), ["stream"]), ("w8", (8192, 4096, 7168), ["large"]),
+])
+def test_ways_of_known_sizes(operation, sizes, ways):
+    assert [c["way"] for c in ops.product_choices(operation, *sizes)] == ways
+
+
 def test_products_that_cannot_be_launched_are_refused():
     lib, at = _lib.load(), 1 << 20  # (no call below reaches memory)
     w = ops._W8(at, at, 2097151, 16)
