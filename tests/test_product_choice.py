@@ -1,10 +1,13 @@
 """How the gated block's and the 8-bit products are cut up (host arithmetic, no GPU needed)."""
 
 import ctypes
+import math
+import random
 
 import pytest
 
 from deepep_amd import _lib, ops
+from tests import test_gpu_dense, test_gpu_dense_choices, test_gpu_dense_ways, test_gpu_w8
 
 MOST_WORKGROUPS = 0x7FFFFF  # of 512 threads
 
@@ -52,3 +55,31 @@ def test_sizes_that_no_call_takes():
         assert lib.dpep_gated_ffn_scratch_bytes(*bad) == 0 and lib.dpep_gated_ffn_backward_scratch_bytes(*bad) == 0
     for bad in ((-1, 8, 16), (1, 1 << 30, 16), (1, 8, 0x7FFFFFF0)):
         assert lib.dpep_w8_matmul_scratch_bytes(*bad) == 0
+
+
+_PRODUCTS = {"ffn": ("gate and up", "down"), "ffn_backward": ("dh", "dx", "dw", "dw"), "w8": ("codes",)}
+
+
+def _made(operation, sizes):
+    """What of the kernels a call takes: which product, way, shape of its stream, k whole or in parts, alone or with the two others."""
+    return {(product, c["way"], c["stream"], c["parts"] > 1, c["together"]) for product, c in zip(_PRODUCTS[operation], ops.product_choices(operation, *sizes))}
+
+
+def _parameters(test, names):
+    return next(mark.args[1] for mark in test.pytestmark if mark.name == "parametrize" and mark.args[0] == names)
+
+
+def test_the_gpu_tests_sizes_take_every_way_there_is():
+    blocks = (test_gpu_dense.SIZES + _parameters(test_gpu_dense.test_many_tokens, "tokens,hidden,inter") + test_gpu_dense_ways.SIZES + test_gpu_dense_choices.SIZES)
+    codes = test_gpu_w8.SIZES + _parameters(test_gpu_dense_ways.test_codes, "rows,n,k") + test_gpu_dense_choices.CODES
+    tested = set().union(*(_made(operation, sizes) for sizes in blocks for operation in ("ffn", "ffn_backward")), *(_made("w8", sizes) for sizes in codes))
+    rng, reached = random.Random(3), {}
+    log = lambda low, high: int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))  # noqa: E731
+    for _ in range(60000):
+        operation = rng.choice(sorted(_PRODUCTS))
+        sizes = (log(1, 20000), log(1, 200000), log(1, 4096) * 16) if operation == "w8" else (log(1, 20000), log(1, 3600) * 8, log(1, 3600) * 8)
+        if sizes[1] * sizes[2] < 1.5e9 and sizes[0] * max(sizes[1:]) < 1e9:
+            for made in _made(operation, sizes):
+                reached.setdefault(made, (operation, sizes))
+    assert len(reached) > 50
+    assert not {made: sizes for made, sizes in reached.items() if made not in tested}
