@@ -151,6 +151,36 @@ def test_gradients_of_many_rows(tokens, hidden, dtype):
     assert torch.equal(grad_x, again[0]) and torch.equal(grad_w, again[1])
 
 
+@pytest.mark.parametrize("tokens,hidden,dtype,weight,residual", [
+    (300, 1000, "bf16", "fp32", True), (257, 2048, "fp32", "fp32", False), (300, 5024, "fp16", "fp16", True), (260, 8192, "fp32", "fp32", True), (300, 8208, "bf16", "bf16", False),
+    (257, 12320, "fp16", "fp32", True), (258, 16384, "bf16", "fp32", True), (257, 16384, "fp32", "fp32", False)])
+def test_many_rows_of_all_widths(tokens, hidden, dtype, weight, residual):
+    """More rows than compute units, in each number of pieces a thread: the norm, its codes and its gradients."""
+    from deepep_amd import dense
+
+    x, w, r, rng = _make(tokens, hidden, dtype, weight, residual)
+    got = dense.rms_norm(x, w, r, eps=EPS)
+    v, rstd = od.norm(_wide(got.stream), _wide(w), EPS)
+    _check(got.rstd, rstd, od.NORM_SLACK * rstd, "fp32")
+    _check(got.y, v, od.NORM_SLACK * np.abs(v), dtype)
+    slack = 2 * od.NORM_SLACK
+    if hidden % 16 == 0:
+        coded = dense.rms_norm(x, w, r, eps=EPS, quantize="fp8")
+        assert torch.equal(coded.y, got.y)
+        target, scales = od.fp8_blocks(v)
+        _check(coded.scales, scales, slack * scales, "fp32")
+        assert (np.abs(_wide(coded.codes.float()) - target) <= od.e4m3_bound(target) * (1 + 1e-9) + slack * np.abs(target)).all()
+        coded = dense.rms_norm(x, w, r, eps=EPS, quantize="int8", output=False)
+        target, scales = od.tokens(v)
+        _check(coded.scales, scales, slack * scales, "fp32")
+        assert (np.abs(_wide(coded.codes) - target) <= 0.5 + slack * 127).all()
+    g = _rows(rng, tokens, hidden, dtype)
+    grad_x, grad_w = dense.rms_norm_backward(g, got.stream, w, got.rstd)
+    want, bound, want_w, bound_w = od.norm_backward(_wide(g), _wide(got.stream), _wide(w), EPS)
+    _check(grad_x, want, bound, dtype)
+    _check(grad_w, want_w, bound_w, "fp32")
+
+
 def test_no_rows():
     from deepep_amd import dense, w8
 
