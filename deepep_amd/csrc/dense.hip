@@ -784,7 +784,8 @@ struct Cut {
 // with more.  So pairs win from one to about two and a half tiles of 128 a compute unit, and where k is short (8-bit integers, 400 tiles, 23 steps: 31 us by the
 // ring, 25 by pairs, 39 by large tiles; 256 tiles, 56 steps: 34, 43, 67; 1024 tiles, 56 steps: 126, 108, 88).
 // Joining parts takes 3.5 us and 0.2 a part, and 2 ps for each of the 4-byte sums, written and read.  A round of 256 workgroups of a stream takes 3 us and what one
-// reads of B and of up to 64 rows of A, at 62 bytes / ns; beside that count 0.4 us for each 256 workgroups (8-bit, 6 rows of 432 to 62901: 22.9 us by 3932 short ones, 9.9 by pairs) and 0.4 of the time of reading B from memory.
+// reads of B and of up to 64 rows of A, at 62 bytes / ns; up to 16 rows, whose rounds run into one another, 3 us once and 0.35 for each 256 workgroups (8-bit, 6 rows of 432 to 62901: 22.9 us by 3932 short
+// ones, 9.9 by pairs).  Beside that counts 0.4 of the time of reading B from memory.
 inline double tile_us(Way way, int steps) { return way == kLargeTiles ? 10 + 1.45 * steps : way == kRing ? 4 + 0.58 * steps : 4.5 + 0.92 * steps; }
 // Groups of 16 columns of a stream's workgroup.  Two read A half as often: for more tiles than compute units, and for up to 16 rows if they then fit one round; above that, two
 // workgroups on a compute unit, with rings of two stages, end more evenly.  (16-bit, 14 rows of 6544 to 2 x 3304 and back, 413 and 409 tiles: 36 us by twos, 40 by ones; 24 rows, 7168
@@ -802,13 +803,14 @@ inline Stream stream_of(int m, int n_tiles)
 }
 inline double join_us(int parts, size_t bytes) { return 3.5 + 0.2 * parts + 0.5e-6 * static_cast<double>(bytes); }
 inline int at_once(Way way) { return way == kPairs ? 512 : 256; }
-// No tiles are quicker than memory, which gives 5.4 MB / us where every place for a workgroup is taken, and as much less as the rounds leave free, to half of it.  (The steps' costs above are those of operands
+// No tiles are quicker than memory, which gives 5.8 MB / us, 2 us after the start, where every place for a workgroup is taken, and as much less as the rounds leave free, to half of it.  (The steps' costs above are those of operands
 // that L2 holds for many tiles; of few rows every byte of B comes from memory.  8-bit, 4 rows of 28672 to 8192: 59 us by the pairs that the steps alone would choose, 43 by a stream; 1 row of 4096
-// to 128256 114 and 95; 16-bit, 8 rows of 18432 to 7168 156 and 138.  975 products of 1 to 400 rows, every way timed: the chosen one is 1.6 % above the quickest in the mean, 3.3 without this.)
+// to 128256 114 and 95; 16-bit, 8 rows of 18432 to 7168 156 and 138.  1975 products of 1 to 2500 rows, every way timed: the chosen one is 1.8 % above the quickest in the mean; without this and the cost of a stream's
+// workgroups 3.5.)
 inline double memory_us(Way way, long long workgroups, double bytes)
 {
     const double rounds = static_cast<double>(workgroups) / at_once(way);
-    return workgroups == 0 ? 0 : bytes / 5.4e6 * std::min(2.0, std::ceil(rounds) / rounds);
+    return workgroups == 0 ? 0 : 2 + bytes / 5.8e6 * std::min(2.0, std::ceil(rounds) / rounds);
 }
 inline double rounds_of(Way way, long long tiles)
 {
@@ -824,8 +826,8 @@ Cut cut_of(int m, int columns, int k_bytes, bool gated, bool turned)
     if (!turned) {
         const int n_tiles = (columns * times + 15) / 16, m_tiles = (m + 63) / 64, groups = stream_groups(m, n_tiles);
         const double workgroups = static_cast<double>((n_tiles + groups - 1) / groups) * m_tiles, read = static_cast<double>(16 * groups + std::min(m, 64)) * k_bytes / 62e3;
-        const double rounds = m <= 16 && groups == 1 ? 3 + std::max(1.0, workgroups / 256) * read : std::ceil(workgroups / 256) * (3 + read);
-        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 0.5 + rounds + 0.4 * workgroups / 256 + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
+        const double rounds = m <= 16 && groups == 1 ? 3 + std::max(1.0, workgroups / 256) * read + 0.35 * workgroups / 256 : std::ceil(workgroups / 256) * (3 + read);
+        best = {kStream, m_tiles, n_tiles, 1, steps, 0, 0.5 + rounds + 0.4 * columns * times * static_cast<double>(k_bytes) / 5.5e6};
     }
     for (const Way way : {kRing, kPairs, kLargeTiles}) {
         const int tile = way == kLargeTiles ? 256 : 128, wide = tile / times;

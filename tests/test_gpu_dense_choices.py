@@ -12,7 +12,7 @@ SIZES = [  # tokens, hidden, inter
     (77, 1544, 1304), (67, 8, 4392),  # pairs, k in parts: gate and up; down
     (2360, 8936, 896), (2476, 7672, 1928), (7078, 584, 7296),  # tiles of 256, k in parts: gate and up; dh; down
     (8460, 400, 912), (7235, 136, 1512), (2500, 264, 136),  # the backward's three together, of 256 and of 128, k in parts
-    (1682, 3608, 904), (16226, 192, 1400),  # apart, k whole: pairs and ring
+    (1682, 3608, 904), (16226, 192, 1400), (14714, 240, 3104),  # apart, k whole: pairs and ring
     (14249, 56, 1752), (18852, 328, 2184), (3078, 624, 5832), (3511, 960, 8112), (14685, 392, 3680),  # apart, k in parts: ring, pairs, tiles of 256
 ]
 CODES = [(3, 8360, 176), (1, 33000, 4096), (65, 3, 7776), (140, 4500, 7184), (5582, 727, 18688)]  # rows, n, k

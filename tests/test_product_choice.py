@@ -27,7 +27,7 @@ def test_cuts_of_the_largest_sizes_can_be_launched(operation, sizes):
     # few rows on large matrices: nothing but the reading of the matrix counts
     ("ffn", (1, 8192, 28672), ["stream", "stream"]), ("ffn", (4, 7168, 18432), ["stream", "stream"]), ("w8", (1, 128256, 4096), ["stream"]), ("w8", (4, 8192, 28672), ["stream"]),
     # and many short workgroups their own starts
-    ("w8", (6, 62901, 432), ["pairs"]), ("ffn", (3, 280, 14928), ["pairs", "stream"]),
+    ("w8", (6, 62901, 432), ["pairs"]), ("ffn", (6, 264, 28176), ["pairs", "stream"]),
     # what the rules were measured at before
     ("ffn", (1, 7168, 2048), ["stream", "stream"]), ("ffn", (33, 2880, 1408), ["stream", "stream"]), ("ffn", (512, 7168, 2048), ["ring", "ring"]),
     ("ffn", (8192, 7168, 2048), ["large", "large"]), ("ffn_backward", (8192, 7168, 2048), ["large"] * 4), ("ffn_backward", (1000, 2880, 1408), ["ring", "pairs", "pairs", "pairs"]),
